@@ -205,6 +205,18 @@ int gsq_gdn_seq(const void* qkv, int64_t qkv_stride, const void* z, int64_t z_st
                 int64_t seq, int64_t key_heads, int64_t value_heads, int64_t head_k_dim, int64_t head_v_dim,
                 int64_t conv_kernel, float eps, int dtype, void* stream);
 
+/* gsq_gdn_seq over a tree of `seq` (at most 64) drafted tokens: token t follows token parents[t] < t, or the
+ * cached ones (-1), in its convolution window and in the recurrence; parents int32 on the device,
+ * n_trees = 1 or batch rows of seq. Outputs as gsq_gdn_seq over each token's path gives them (float32
+ * sums in another order); the states are only read: the tokens that are kept go through gsq_gdn_seq
+ * afterwards. A batch row whose parents are not such gets NaN outputs; a value that is not finite makes the
+ * outputs of its token's path and of those that follow it NaN, in the heads it belongs to. */
+int gsq_gdn_tree(const void* qkv, int64_t qkv_stride, const void* z, int64_t z_stride, const void* ab, int64_t ab_stride,
+                 const void* conv_state, const void* conv_w, const float* ssm_a, const float* dt_bias,
+                 const float* rec_state, const void* norm_w, const int32_t* parents, int64_t n_trees, void* out,
+                 int64_t out_stride, int64_t batch, int64_t seq, int64_t key_heads, int64_t value_heads,
+                 int64_t head_k_dim, int64_t head_v_dim, int64_t conv_kernel, float eps, int dtype, void* stream);
+
 /* One new token of gated grouped-query attention for `batch` rows (replaces the attention of a
  * full-attention layer at decode, qwen35.py's mlx-lm attention): per query head h (kv head
  * h / (heads / kv_heads)), q = round(rms_norm(q) * q_norm_w) from the q half of qg's head
@@ -247,6 +259,44 @@ int gsq_attn_seq_split(const void* qg, int64_t qg_stride, const void* k, int64_t
                        void* k_cache, void* v_cache, const int64_t* pos, void* out, int64_t out_stride, void* q_work,
                        float* work, int64_t chunk, int64_t batch, int64_t seq, int64_t heads, int64_t kv_heads,
                        int64_t head_dim, int64_t rotary_dim, int64_t max_len, float eps, int dtype, void* stream);
+
+/* ---- an 8-bit K/V cache ----
+ * For the same gated attention: bytes [batch, kv_heads, max_len, head_dim] and float32 scales [batch,
+ * kv_heads, max_len] for K and for V. A row x is held as s = max|x| / 127 (rounded to float32; NaN if a
+ * value of x is not finite) and u = 128 + rint(x / s) (s = 0: 128), and stands for (u - 128) s.
+ * pos: n_pos (1 or batch) int64 on the device, the position of each batch row's first new token; with
+ * parents (int32 on the device, n_trees = 1 or batch rows of seq <= 64) the seq tokens are drafted as a
+ * tree: token t follows token parents[t] < t, or the cached tokens (-1). A batch row whose tokens do
+ * not all lie inside the cache, or whose parents are not such, gets NaN outputs and keeps its cache.
+ * fp16 or bf16; head_dim 64, 128 or 256; rows b * seq + t of qg, k, v, q and out, strides in elements. */
+
+/* q and k (qg, k as for gsq_attn_seq) RMS-normalized per head and rotated at their positions (*pos + t; in
+ * a tree *pos + depth), q rounded once into q [batch, seq, heads, head_dim]; k and v quantised into
+ * position *pos + t of the caches. Caches and q 16-byte aligned. */
+int gsq_kv8_write(const void* qg, int64_t qg_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                  const void* q_norm_w, const void* k_norm_w, const double* inv_freq, uint8_t* k_cache, uint8_t* v_cache,
+                  float* k_scale, float* v_scale, const int64_t* pos, int64_t n_pos, const int32_t* parents,
+                  int64_t n_trees, void* q, int64_t batch, int64_t seq, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                  int64_t rotary_dim, int64_t max_len, float eps, int dtype, void* stream);
+
+/* The values (u - 128) s of positions start .. start + n - 1 of `heads` (batch * kv_heads) caches, in float32
+ * and rounded to dtype (GSQ_F32 / GSQ_F16 / GSQ_BF16), into k and v [heads, n, head_dim]; head_dim a multiple of 16; caches, k
+ * and v 16-byte aligned. */
+int gsq_kv8_read(const uint8_t* k_cache, const uint8_t* v_cache, const float* k_scale, const float* v_scale, void* k,
+                 void* v, int64_t heads, int64_t max_len, int64_t start, int64_t n, int64_t head_dim, int dtype,
+                 void* stream);
+
+/* out = round(softmax(q K^T / sqrt(head_dim)) V * sigmoid(gate)) per head, gates in qg; token t attends to
+ * positions 0 .. *pos + t, in a tree to 0 .. *pos - 1, its ancestors and itself. splits > 1: the
+ * positions are shared out over that many workgroups for each tile of rows (at most 65535), whose sums
+ * meet in work (batch * heads * seq * splits * (head_dim + 2) floats) and are combined by a second
+ * kernel; work is not used with splits = 1. Caches, work and rows of q 16-byte aligned, rows of qg and
+ * out 8-byte aligned. */
+int gsq_attn_kv8(const void* q, int64_t q_stride, const void* qg, int64_t qg_stride, const uint8_t* k_cache,
+                 const uint8_t* v_cache, const float* k_scale, const float* v_scale, const int64_t* pos, int64_t n_pos,
+                 const int32_t* parents, int64_t n_trees, void* out, int64_t out_stride, float* work, int64_t splits,
+                 int64_t batch, int64_t seq, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_len, int dtype,
+                 void* stream);
 
 /* Message of the last failed call on this thread ("" if none). */
 const char* gsq_last_error(void);

@@ -33,7 +33,11 @@ hipError_t launch_add_rms_norm(int dt, void* x, const void* delta, const void* w
 hipError_t launch_swiglu(int dt, const void* gu, void* out, int64_t rows, int n, hipStream_t s);
 hipError_t launch_gdn_step(int dt, const GdnArgs& a, hipStream_t s);
 hipError_t launch_gdn_seq(int dt, const GdnArgs& a, hipStream_t s);
+hipError_t launch_gdn_tree(int dt, const GdnTreeArgs& a, hipStream_t s);
 hipError_t launch_attn_seq(bool bf16, const AttnSeqArgs& a, hipStream_t s);
+hipError_t launch_kv8_write(bool bf16, const Kv8WriteArgs& a, hipStream_t s);
+hipError_t launch_kv8_read(int dt, const Kv8ReadArgs& a, hipStream_t s);
+hipError_t launch_attn_kv8(bool bf16, const Kv8AttnArgs& a, hipStream_t s);
 hipError_t launch_attn_decode(int dt, const AttnArgs& a, hipStream_t s);
 int qmv_table_bytes(int qt);
 int build_qmv_table(int qt, const uint16_t* grid16, const uint8_t* ksigns, std::vector<uint8_t>& out);
@@ -786,6 +790,126 @@ int gsq_attn_seq_split(const void* qg, int64_t qg_stride, const void* k, int64_t
   a.rd = (int)rotary_dim; a.L = (int)max_len; a.eps = eps;
   hipError_t e = launch_attn_seq(dtype == GSQ_BF16, a, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return fail(GSQ_E_HIP, "attn_seq launch: %s", hipGetErrorString(e));
+  return GSQ_OK;
+}
+
+int gsq_gdn_tree(const void* qkv, int64_t qkv_stride, const void* z, int64_t z_stride, const void* ab, int64_t ab_stride,
+                 const void* conv_state, const void* conv_w, const float* ssm_a, const float* dt_bias,
+                 const float* rec_state, const void* norm_w, const int32_t* parents, int64_t n_trees, void* out,
+                 int64_t out_stride, int64_t batch, int64_t seq, int64_t key_heads, int64_t value_heads,
+                 int64_t head_k_dim, int64_t head_v_dim, int64_t conv_kernel, float eps, int dtype, void* stream) {
+  if (dtype != GSQ_F32 && dtype != GSQ_F16 && dtype != GSQ_BF16) return fail(GSQ_E_TYPE, "unsupported dtype code %d", dtype);
+  if (batch < 0 || batch > 65535) return fail(GSQ_E_VALUE, "batch must be 0..65535");
+  if (seq < 0 || seq > 64) return fail(GSQ_E_VALUE, "a tree holds at most 64 tokens");
+  if (batch == 0 || seq == 0) return GSQ_OK;
+  if (key_heads <= 0 || value_heads <= 0 || value_heads % key_heads || value_heads > 65535)
+    return fail(GSQ_E_VALUE, "value heads must be a positive multiple of key heads (at most 65535)");
+  if (head_k_dim <= 0 || head_k_dim > 128 || head_k_dim % 4) return fail(GSQ_E_VALUE, "key head dim must be a multiple of 4 up to 128");
+  if (head_v_dim <= 0 || head_v_dim % 64 || head_v_dim > 256) return fail(GSQ_E_VALUE, "value head dim must be 64, 128, 192 or 256");
+  if (conv_kernel < 2 || conv_kernel > 8) return fail(GSQ_E_VALUE, "convolution kernel must be 2..8");
+  if (n_trees != 1 && n_trees != batch) return fail(GSQ_E_VALUE, "one tree, or one for each batch row");
+  if (!qkv || !z || !ab || !conv_state || !conv_w || !ssm_a || !dt_bias || !rec_state || !norm_w || !parents || !out)
+    return fail(GSQ_E_VALUE, "NULL pointer");
+  if (!(eps >= 0.f)) return fail(GSQ_E_VALUE, "eps must be >= 0");
+  GdnTreeArgs a;
+  a.qkv = qkv; a.z = z; a.ab = ab; a.conv = conv_state; a.conv_w = conv_w; a.ssm_a = ssm_a; a.dt_bias = dt_bias;
+  a.rec = rec_state; a.norm_w = norm_w; a.parents = parents; a.out = out;
+  a.qkv_stride = qkv_stride; a.z_stride = z_stride; a.ab_stride = ab_stride; a.out_stride = out_stride;
+  a.parents_stride = n_trees > 1 ? seq : 0;
+  a.B = (int)batch; a.S = (int)seq; a.Hk = (int)key_heads; a.Hv = (int)value_heads; a.dk = (int)head_k_dim;
+  a.dv = (int)head_v_dim; a.K = (int)conv_kernel; a.eps = eps;
+  hipError_t e = launch_gdn_tree(dtype, a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(GSQ_E_HIP, "gdn_tree launch: %s", hipGetErrorString(e));
+  return GSQ_OK;
+}
+
+// What the calls on an 8-bit cache share: head layout, lengths, positions and parents.
+static int check_kv8(int64_t batch, int64_t seq, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_len,
+                     int64_t n_pos, const int32_t* parents, int64_t n_trees) {
+  if (kv_heads <= 0 || heads <= 0 || heads % kv_heads || heads > 65535)
+    return fail(GSQ_E_VALUE, "heads must be a positive multiple of kv heads (at most 65535)");
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256) return fail(GSQ_E_VALUE, "head dim must be 64, 128 or 256");
+  if (max_len <= 0 || max_len >= (1ll << 31) - 64) return fail(GSQ_E_VALUE, "invalid cache length");
+  if (seq > max_len) return fail(GSQ_E_VALUE, "%lld tokens do not fit a cache of %lld", (long long)seq, (long long)max_len);
+  if (seq * heads >= (1ll << 31)) return fail(GSQ_E_VALUE, "too many query rows");
+  if (n_pos != 1 && n_pos != batch) return fail(GSQ_E_VALUE, "one position, or one for each batch row");
+  if (parents && seq > 64) return fail(GSQ_E_VALUE, "a tree holds at most 64 tokens");
+  if (parents && n_trees != 1 && n_trees != batch) return fail(GSQ_E_VALUE, "one tree, or one for each batch row");
+  return GSQ_OK;
+}
+
+int gsq_kv8_write(const void* qg, int64_t qg_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                  const void* q_norm_w, const void* k_norm_w, const double* inv_freq, uint8_t* k_cache, uint8_t* v_cache,
+                  float* k_scale, float* v_scale, const int64_t* pos, int64_t n_pos, const int32_t* parents,
+                  int64_t n_trees, void* q, int64_t batch, int64_t seq, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                  int64_t rotary_dim, int64_t max_len, float eps, int dtype, void* stream) {
+  if (dtype != GSQ_F16 && dtype != GSQ_BF16) return fail(GSQ_E_TYPE, "unsupported dtype code %d", dtype);
+  if (batch < 0 || batch > 65535 || seq < 0) return fail(GSQ_E_VALUE, "batch must be 0..65535, seq not negative");
+  if (batch == 0 || seq == 0) return GSQ_OK;
+  if (int rc = check_kv8(batch, seq, heads, kv_heads, head_dim, max_len, n_pos, parents, n_trees)) return rc;
+  if (rotary_dim < 0 || rotary_dim > head_dim || rotary_dim % 2) return fail(GSQ_E_VALUE, "invalid rotary dim");
+  if (!qg || !k || !v || !q_norm_w || !k_norm_w || (!inv_freq && rotary_dim) || !k_cache || !v_cache || !k_scale ||
+      !v_scale || !pos || !q)
+    return fail(GSQ_E_VALUE, "NULL pointer");
+  if ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache) | reinterpret_cast<uintptr_t>(q)) & 15)
+    return fail(GSQ_E_VALUE, "k_cache, v_cache and q must be 16-byte aligned");
+  if (!(eps >= 0.f)) return fail(GSQ_E_VALUE, "eps must be >= 0");
+  Kv8WriteArgs a;
+  a.qg = qg; a.k = k; a.v = v; a.q_norm_w = q_norm_w; a.k_norm_w = k_norm_w; a.inv_freq = inv_freq;
+  a.kc = k_cache; a.vc = v_cache; a.ks = k_scale; a.vs = v_scale; a.pos = pos; a.parents = parents; a.q = q;
+  a.qg_stride = qg_stride; a.k_stride = k_stride; a.v_stride = v_stride;
+  a.pos_stride = n_pos > 1; a.parents_stride = n_trees > 1 ? seq : 0; a.L = max_len;
+  a.B = (int)batch; a.S = (int)seq; a.H = (int)heads; a.Hkv = (int)kv_heads; a.hd = (int)head_dim;
+  a.rd = (int)rotary_dim; a.eps = eps;
+  hipError_t e = launch_kv8_write(dtype == GSQ_BF16, a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(GSQ_E_HIP, "kv8_write launch: %s", hipGetErrorString(e));
+  return GSQ_OK;
+}
+
+int gsq_kv8_read(const uint8_t* k_cache, const uint8_t* v_cache, const float* k_scale, const float* v_scale, void* k,
+                 void* v, int64_t heads, int64_t max_len, int64_t start, int64_t n, int64_t head_dim, int dtype,
+                 void* stream) {
+  if (dtype != GSQ_F32 && dtype != GSQ_F16 && dtype != GSQ_BF16) return fail(GSQ_E_TYPE, "unsupported dtype code %d", dtype);
+  if (heads < 0 || max_len < 0 || n < 0 || start < 0 || start > max_len || n > max_len - start)
+    return fail(GSQ_E_VALUE, "rows %lld .. + %lld of a cache of %lld", (long long)start, (long long)n, (long long)max_len);
+  if (head_dim <= 0 || head_dim % 16 || head_dim > 65536) return fail(GSQ_E_VALUE, "head dim must be a multiple of 16");
+  if (heads == 0 || n == 0) return GSQ_OK;
+  if (heads >= (1ll << 31) || max_len >= (1ll << 31)) return fail(GSQ_E_VALUE, "invalid cache shape");
+  if (!k_cache || !v_cache || !k_scale || !v_scale || !k || !v) return fail(GSQ_E_VALUE, "NULL pointer");
+  if ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache) | reinterpret_cast<uintptr_t>(k) |
+       reinterpret_cast<uintptr_t>(v)) & 15)
+    return fail(GSQ_E_VALUE, "caches and outputs must be 16-byte aligned");
+  Kv8ReadArgs a;
+  a.kc = k_cache; a.vc = v_cache; a.ks = k_scale; a.vs = v_scale; a.k = k; a.v = v;
+  a.L = max_len; a.start = start; a.n = n; a.heads = heads; a.hd = (int)head_dim;
+  hipError_t e = launch_kv8_read(dtype, a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(GSQ_E_HIP, "kv8_read launch: %s", hipGetErrorString(e));
+  return GSQ_OK;
+}
+
+int gsq_attn_kv8(const void* q, int64_t q_stride, const void* qg, int64_t qg_stride, const uint8_t* k_cache,
+                 const uint8_t* v_cache, const float* k_scale, const float* v_scale, const int64_t* pos, int64_t n_pos,
+                 const int32_t* parents, int64_t n_trees, void* out, int64_t out_stride, float* work, int64_t splits,
+                 int64_t batch, int64_t seq, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_len, int dtype,
+                 void* stream) {
+  if (dtype != GSQ_F16 && dtype != GSQ_BF16) return fail(GSQ_E_TYPE, "unsupported dtype code %d", dtype);
+  if (batch < 0 || batch > 65535 || seq < 0) return fail(GSQ_E_VALUE, "batch must be 0..65535, seq not negative");
+  if (batch == 0 || seq == 0) return GSQ_OK;
+  if (int rc = check_kv8(batch, seq, heads, kv_heads, head_dim, max_len, n_pos, parents, n_trees)) return rc;
+  if (splits < 1 || splits > 65535 || (splits > 1 && !work)) return fail(GSQ_E_VALUE, "1..65535 splits, with work for more than one");
+  if (!q || !qg || !k_cache || !v_cache || !k_scale || !v_scale || !pos || !out) return fail(GSQ_E_VALUE, "NULL pointer");
+  if ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache) | reinterpret_cast<uintptr_t>(q) |
+       reinterpret_cast<uintptr_t>(work)) & 15 || q_stride % 8)
+    return fail(GSQ_E_VALUE, "k_cache, v_cache, work and rows of q must be 16-byte aligned");
+  if (((reinterpret_cast<uintptr_t>(qg) | reinterpret_cast<uintptr_t>(out)) & 7) || qg_stride % 4 || out_stride % 4)
+    return fail(GSQ_E_VALUE, "rows of qg and out must be 8-byte aligned");
+  Kv8AttnArgs a;
+  a.q = q; a.qg = qg; a.kc = k_cache; a.vc = v_cache; a.ks = k_scale; a.vs = v_scale; a.pos = pos; a.parents = parents;
+  a.out = out; a.part = work; a.q_stride = q_stride; a.qg_stride = qg_stride; a.out_stride = out_stride;
+  a.pos_stride = n_pos > 1; a.parents_stride = n_trees > 1 ? seq : 0; a.L = max_len;
+  a.B = (int)batch; a.S = (int)seq; a.H = (int)heads; a.Hkv = (int)kv_heads; a.hd = (int)head_dim; a.nsplit = (int)splits;
+  hipError_t e = launch_attn_kv8(dtype == GSQ_BF16, a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(GSQ_E_HIP, "attn_kv8 launch: %s", hipGetErrorString(e));
   return GSQ_OK;
 }
 

@@ -142,6 +142,25 @@ struct GdnArgs {
   float eps;
 };
 
+// Arguments of the GatedDeltaNet of a tree of S drafted tokens (gsq_gdn_tree; kernel in
+// gsq_gdn_tree.hip): rows b * S + t of qkv, z, ab and out; the states are only read.
+struct GdnTreeArgs {
+  const void* qkv;
+  const void* z;
+  const void* ab;     // 2 Hv values per row: a, then b
+  const void* conv;   // [B, K-1, conv_dim]
+  const void* conv_w;  // [conv_dim, K]
+  const float* ssm_a;  // [Hv]
+  const float* dt_bias;  // [Hv]
+  const float* rec;    // [B, Hv, dk, dv]
+  const void* norm_w;  // [dv]
+  const int32_t* parents;  // row bb's at bb * parents_stride
+  void* out;
+  int64_t qkv_stride, z_stride, ab_stride, out_stride, parents_stride;
+  int B, S, Hk, Hv, dk, dv, K;
+  float eps;
+};
+
 // Arguments of one single-token gated attention (gsq_attn_decode; kernel in gsq_model.hip).
 struct AttnArgs {
   const void* qg;   // [B] rows of H * 2hd: per head q then gate (row stride qg_stride)
@@ -184,6 +203,56 @@ struct AttnSeqArgs {
   // [B, H, S, nsplit] rows of hd floats, then as many (maximum, sum) pairs; nsplit 1: unused
   float* part = nullptr;
   int chunk = 0, nsplit = 1;
+};
+
+// Arguments of the operators on an 8-bit K/V cache (kernels in gsq_kv8.hip): bytes [B, Hkv, L, hd] and
+// float32 scales [B, Hkv, L]. Row bb's first new token is at position pos[bb * pos_stride]; tokens of a
+// tree have parents[bb * parents_stride + t] < t (-1: the cached tokens), null: a sequence. Rows
+// b * S + t of q, qg, k, v and out, strides in elements.
+struct Kv8WriteArgs {
+  const void* qg;  // rows of H * 2hd: per head q then gate
+  const void* k;   // rows of Hkv * hd
+  const void* v;
+  const void* q_norm_w;  // [hd]
+  const void* k_norm_w;
+  const double* inv_freq;  // [rd / 2]
+  uint8_t* kc;
+  uint8_t* vc;
+  float* ks;
+  float* vs;
+  const int64_t* pos;
+  const int32_t* parents;
+  void* q;  // [B, S, H, hd]: normalized, rotated queries
+  int64_t qg_stride, k_stride, v_stride, pos_stride, parents_stride, L;
+  int B, S, H, Hkv, hd, rd;
+  float eps;
+};
+
+struct Kv8ReadArgs {
+  const uint8_t* kc;
+  const uint8_t* vc;
+  const float* ks;
+  const float* vs;
+  void* k;  // [heads, n, hd]
+  void* v;
+  int64_t L, start, n;
+  int64_t heads;  // B * Hkv
+  int hd;
+};
+
+struct Kv8AttnArgs {
+  const void* q;   // rows of H * hd
+  const void* qg;  // rows of H * 2hd (the gates)
+  const uint8_t* kc;
+  const uint8_t* vc;
+  const float* ks;
+  const float* vs;
+  const int64_t* pos;
+  const int32_t* parents;
+  void* out;    // rows of H * hd
+  float* part;  // nsplit > 1: [B, Hkv, S * H / Hkv, nsplit] rows of hd floats, then (maximum, sum) pairs
+  int64_t q_stride, qg_stride, out_stride, pos_stride, parents_stride, L;
+  int B, S, H, Hkv, hd, nsplit;
 };
 
 // A kernel's raised dynamic LDS limit (one static object per kernel): a function attribute belongs to

@@ -12,37 +12,9 @@
 #include <type_traits>
 
 #include "gsq_common.h"
+#include "gsq_elem.h"
 
 namespace gsq {
-
-enum { MD_F32 = 0, MD_F16 = 1, MD_BF16 = 2 };
-
-template <int DT> struct Elem;
-template <> struct Elem<MD_F32> {
-  using T = float;
-  __device__ static float ld(const T* p) { return *p; }
-  __device__ static T mk(float v) { return v; }
-};
-template <> struct Elem<MD_F16> {
-  using T = _Float16;
-  __device__ static float ld(const T* p) { return (float)*p; }
-  __device__ static T mk(float v) { return (_Float16)v; }
-};
-template <> struct Elem<MD_BF16> {
-  using T = uint16_t;
-  __device__ static float ld(const T* p) { return __builtin_bit_cast(float, (uint32_t)*p << 16); }
-  __device__ static T mk(float v) { return (uint16_t)f32_to_bf16_bits(v); }
-};
-
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
-}
-
-// Workgroup barrier that waits for this wave's LDS operations only: global loads issued before
-// it stay in flight. The kernels here exchange data between threads through LDS only.
-__device__ __forceinline__ void lds_sync() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // sum of v over the block (blockDim.x a multiple of 64, at most 1024); every thread gets it
 __device__ __forceinline__ float block_sum(float v, float* red) {
@@ -70,8 +42,6 @@ __device__ __forceinline__ float4 block_sum4(float4 v, float4* red) {
   }
   return s;
 }
-
-__device__ __forceinline__ float silu_f(float x) { return x / (1.f + expf(-x)); }
 
 // ---- residual add + RMSNorm ------------------------------------------------------------
 // Row r: if delta, x[r] = round(x[r] + delta[r]) (written back); y[r] = round(x[r] / rms * w).
