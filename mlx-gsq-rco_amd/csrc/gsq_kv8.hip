@@ -9,6 +9,7 @@
 // normalized and rotated values before any rounding to 16 bits.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cfloat>
 #include <cstdint>
 #include <type_traits>
@@ -249,260 +250,261 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8ReadArgs a) {
 
 // ---- attention -----------------------------------------------------------------------------------
 // Rows of a KV head: its rep = heads / kv_heads query heads of every token, row t rep + r for head r of
-// token t. A workgroup takes 16 NT rows of one (batch row, KV head) and a run of 32-position blocks;
-// its four waves take the blocks in turn, each with a softmax of its own, and are merged at the end.
+// token t. Two kernels share the arithmetic: attn_kv8_rows_kernel for few rows, attn_kv8_tile_kernel for
+// many.
 //
 //  * Products on fp16 MFMAs, transposed: S^T = K Q^T puts a row (query) on each lane column, lane % 16,
-//    and positions 16 b + 4 (lane / 16) + e of the block on its registers, which is the layout of the B
+//    and positions 16 b + 4 (lane / 16) + e of a block of 32 on its registers, which is the layout of the B
 //    operand of O^T = V^T P^T: probabilities never leave their lane.
-//  * Bytes are exact in fp16, so K and V cost no rounding; the scale of a K row multiplies its scores, that
-//    of a V row its probabilities. bf16 queries are scaled to fp16 by a power of two for each row:
-//    their 8 bits fit, and what falls below 2^-38 of the row's largest cannot be seen in float32 sums.
-//  * K and V go from memory to registers in 16-byte pieces and are expanded there: no LDS, no barrier
-//    in the loop. For K the dims of a product's step are those a lane's piece holds (any order of dims
-//    gives the same sum); for V a lane holds hd / 16 neighbouring dims of 8 positions, and dim d of a
-//    lane's run belongs to output tile d.
+//  * A byte u with a zero byte above it is the fp16 (subnormal) number u 2^-24, which the matrix cores
+//    take as it is: one v_perm expands two bytes, and K and V cost no rounding. What the 128 in u adds
+//    is known: -128 sum(q) starts the score's accumulator, and a product with a constant row sums the
+//    weights of V, whose 128-fold leaves the outputs every kBiasBlocks blocks (so that float32 sums of
+//    a long context are not those of numbers a hundred times their size).
+//  * The scale of a K row multiplies its scores, that of a V row its probabilities. bf16 queries are
+//    scaled to fp16 by a power of two for each row: their 8 bits fit, and what falls below 2^-38 of the
+//    row's largest cannot be seen in float32 sums.
+//  * K's dims may be taken in any order (the sum is the same): those of a product's step are what a lane's
+//    16 bytes hold. V's are spread so that a lane's piece of a row is PW neighbouring dims, each of
+//    another output tile, and two rows give a pair of one tile's operand by one v_perm.
 //  * The reference of the exponent moves only when a score passes it by 2^kLazy, for all rows of the
 //    wave at once: mostly no rescaling and no exchange between lanes in the loop.
 //  * A weight (probability times V scale, 2^kPScale over the largest V scale met) is at most 2^(2 kLazy +
 //    kPScale) = 2^15 and held in fp16: for bf16 outputs in one value (11 bits, eight times finer than the
 //    output's own rounding), for fp16 outputs in two (22 bits, down to 2^-25 of the unit), as one would
 //    add an error as large as the output's rounding.
-constexpr int kLazy = 3;
+constexpr float kLazy = 3.f;
 constexpr float kPScale = 9.f;
-
-// bytes of a dword pair as fp16 (u - 128): v_perm puts 0x64 above a byte, which is 1024 + u in fp16
-__device__ __forceinline__ uint32_t bytes_f16(uint32_t hi, uint32_t lo, uint32_t sel) {
-  const uint32_t w = __builtin_amdgcn_perm(hi, lo, sel) | 0x64006400u;
-  return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, w) + (f16x2){(_Float16)-1152.f, (_Float16)-1152.f});
-}
+constexpr int kBiasBlocks = 32;  // blocks between two subtractions of 128 times the weights
 
 __device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// blocks of 32 positions that rows up to token t see, and those of a split
+// v, as a value that nothing is known about: what is formed from it is formed there, not kept in a register
+// through the loop around it
+__device__ __forceinline__ int anew(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+// eight bytes as an operand of u 2^-24
+__device__ __forceinline__ u32x4 bytes8(uint32_t w0, uint32_t w1) {
+  return (u32x4){__builtin_amdgcn_perm(0, w0, 0x0C010C00), __builtin_amdgcn_perm(0, w0, 0x0C030C02),
+                 __builtin_amdgcn_perm(0, w1, 0x0C010C00), __builtin_amdgcn_perm(0, w1, 0x0C030C02)};
+}
+// byte i of two dwords as a pair
+__device__ __forceinline__ uint32_t byte_pair(uint32_t second, uint32_t first, int i) {
+  return __builtin_amdgcn_perm(second, first, 0x0C000C00u | (uint32_t)((4 + i) << 16) | (uint32_t)i);
+}
+
+// blocks of 32 positions that rows up to token t see
 __device__ __forceinline__ int kv8_blocks(int64_t pos, int t) { return (int)((pos + t) / 32) + 1; }
 
-template <bool BF, int HD, int NT>
-__global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) attn_kv8_kernel(Kv8AttnArgs a) {
-  using E = E16<BF>;
-  constexpr int KS = HD / 32, KL = HD / 64, VB = HD / 16, RT = 16 * NT;  // VB: dims (bytes) of a lane, output tiles
-  constexpr bool QREG = NT <= 2;
-  constexpr int TERMS = BF ? 1 : 2;  // fp16 values that hold a weight
-  constexpr int VW = VB / 4;  // dwords of a lane's V piece
-  typedef uint32_t vpiece __attribute__((ext_vector_type(VW)));
-  extern __shared__ __attribute__((aligned(16))) uint8_t kv8_lds[];
-  // queries in operand order (16 bytes per lane, step and tile), row factors, scales of a wave's block;
-  // the merge of the waves takes the same memory afterwards
-  u32x4* const qs = reinterpret_cast<u32x4*>(kv8_lds);
-  float* const rowc_s = reinterpret_cast<float*>(kv8_lds + RT * HD * 2);
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  float* const sc = rowc_s + RT + wave * 64;
-  const int g = lane >> 4, c = lane & 15;
-  const int rep = a.H / a.Hkv, R = a.S * rep, ntile = (R + RT - 1) / RT;
-  const int kvh = blockIdx.x % a.Hkv, rest = blockIdx.x / a.Hkv, z = rest % a.nsplit, tile = ntile - 1 - rest / a.nsplit;
-  const int bb = blockIdx.y, r0 = tile * RT;
-  const int64_t* const posp = a.pos + (int64_t)bb * a.pos_stride;
-  const int32_t* const parents = a.parents ? a.parents + (int64_t)bb * a.parents_stride : nullptr;
-  // rows r0 .. of this KV head in q, qg and out
-  auto row_at = [&](int r, int64_t stride, int width) {
+// What a workgroup is asked to do: 16 NT rows of one (batch row, KV head), positions of one split.
+template <int RT>
+struct Kv8Task {
+  const int64_t* posp;
+  const int32_t* parents;
+  int rep, R, kvh, z, bb, r0, tfirst, tlast, blk0, blk1;
+  int64_t pos, base;
+  __device__ explicit Kv8Task(const Kv8AttnArgs& a) {
+    rep = a.H / a.Hkv;
+    R = a.S * rep;
+    const int ntile = (R + RT - 1) / RT;
+    kvh = blockIdx.x % a.Hkv;  // consecutive workgroups: other KV heads, then other splits of the same rows
+    const int rest = blockIdx.x / a.Hkv;
+    z = rest % a.nsplit;
+    r0 = (ntile - 1 - rest / a.nsplit) * RT;  // the last rows see most: first
+    bb = blockIdx.y;
+    posp = a.pos + (int64_t)bb * a.pos_stride;
+    parents = a.parents ? a.parents + (int64_t)bb * a.parents_stride : nullptr;
+    base = ((int64_t)bb * a.Hkv + kvh) * a.L;
+    tfirst = r0 / rep;
+    tlast = min(r0 + RT - 1, R - 1) / rep;
+  }
+  // the blocks of this split; false if there are none
+  __device__ bool blocks(const Kv8AttnArgs& a) {
+    pos = posp[0];
+    const int nblk = kv8_blocks(pos, tlast), per = (nblk + a.nsplit - 1) / a.nsplit;
+    blk0 = z * per;
+    blk1 = min(nblk, blk0 + per);
+    return blk0 < blk1;
+  }
+  // row r of this KV head in q, qg and out
+  __device__ int64_t row_at(const Kv8AttnArgs& a, int r, int64_t stride, int width) const {
     const int t = r / rep;
     return ((int64_t)bb * a.S + t) * stride + (int64_t)(kvh * rep + r - t * rep) * width;
-  };
-  if (row_invalid(posp, a.L, a.S, parents)) {
-    if (a.nsplit == 1)
-      for (int i = tid; i < RT * HD; i += 256)
-        if (r0 + i / HD < R)
-          static_cast<uint16_t*>(a.out)[row_at(r0 + i / HD, a.out_stride, HD) + i % HD] = E::mk(__builtin_nanf(""));
-    return;
   }
-  const int64_t pos = posp[0];
-  const int tfirst = r0 / rep, tlast = min(r0 + RT - 1, R - 1) / rep;
-  const int nblk = kv8_blocks(pos, tlast), per = (nblk + a.nsplit - 1) / a.nsplit;
-  const int blk0 = z * per, blk1 = min(nblk, blk0 + per);
-  if (blk0 >= blk1) return;  // the merge knows
-  const int64_t base = ((int64_t)bb * a.Hkv + kvh) * a.L;
-  const int64_t klast = pos + tlast;  // last position any row sees
+};
 
-  u32x4 kr[2][KL];
-  vpiece vr[8];
-  auto load_k = [&](int blk) {  // positions past the last repeat it
-    const int64_t j0 = (int64_t)blk * 32;
-    const int left = (int)min(klast - j0, (int64_t)31);
-    const uint8_t* p = a.kc + (base + j0) * HD + 16 * g;
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int s = 0; s < KL; ++s)
-        kr[b][s] = *reinterpret_cast<const u32x4*>(p + min(16 * b + c, left) * HD + 64 * s);
-  };
-  auto load_v = [&](int blk) {
-    const int64_t j0 = (int64_t)blk * 32;
-    const int left = (int)min(klast - j0, (int64_t)31);
-    const uint8_t* p = a.vc + (base + j0) * HD + VB * c;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      vr[i] = *reinterpret_cast<const vpiece*>(p + min(16 * (i >> 2) + 4 * g + (i & 3), left) * HD);
-  };
-  float scv = 0.f;  // lane l < 32: K scale of position l of the block; else V scale of l - 32
-  auto load_s = [&](int blk) {
-    const int64_t j0 = (int64_t)blk * 32;
-    const int left = (int)min(klast - j0, (int64_t)31);
-    scv = (lane < 32 ? a.ks : a.vs)[base + j0 + min(lane & 31, left)];
-  };
-  int blk = blk0 + wave;
-  if (blk < blk1) {
-    load_k(blk);
-    load_v(blk);
-    load_s(blk);
-  }
-  // queries to LDS in operand order: HD / 8 threads a row, 8 values each
-  {
-    constexpr int TR = HD / 8;  // threads a row: 8, 16 or 32
+// NaN outputs of a batch row that is not served
+template <bool BF, int HD, int RT>
+__device__ __forceinline__ void kv8_nan_rows(const Kv8AttnArgs& a, const Kv8Task<RT>& w) {
+  if (a.nsplit == 1)  // else the merge writes them
+    for (int i = threadIdx.x; i < RT * HD; i += blockDim.x)
+      if (w.r0 + i / HD < w.R)
+        static_cast<uint16_t*>(a.out)[w.row_at(a, w.r0 + i / HD, a.out_stride, HD) + i % HD] = E16<BF>::mk(__builtin_nanf(""));
+}
+
+// Queries of the task to LDS in operand order (16 bytes per lane, step and 16-row tile), with each row's
+// factor (2^24 over its power of two) and bias; HD / 8 threads a row. All threads of the workgroup.
+template <bool BF, int HD, int RT>
+__device__ __forceinline__ void kv8_stage_q(const Kv8AttnArgs& a, const Kv8Task<RT>& k, u32x4* qs, float* rowc_s, float* bias_s) {
+  using E = E16<BF>;
+  constexpr int TR = HD / 8, KS = HD / 32;
 #pragma unroll 1
-    for (int i = tid; i < RT * TR; i += 256) {
-      const int r = i / TR, o = i % TR;  // octet o: dims 8 o .. + 7
-      u32x4 w = {0, 0, 0, 0};
-      if (r0 + r < R)
-        w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + row_at(r0 + r, a.q_stride, HD) + 8 * o);
-      float cr = 1.f;
-      if constexpr (BF) {
-        float v[8], mx = 0.f;
+  for (int i = threadIdx.x; i < RT * TR; i += blockDim.x) {
+    const int r = i / TR, o = i % TR;  // octet o: dims 8 o .. + 7
+    u32x4 w = {0, 0, 0, 0};
+    if (k.r0 + r < k.R)
+      w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + k.row_at(a, k.r0 + r, a.q_stride, HD) + 8 * o);
+    float v[8], sum = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          v[e] = E::ld((uint16_t)(w[e >> 1] >> (16 * (e & 1))));
-          mx = fmaxf(mx, fabsf(v[e]));
-        }
+    for (int e = 0; e < 8; ++e) v[e] = E::ld((uint16_t)(w[e >> 1] >> (16 * (e & 1))));
+    int ex = 0;
+    if constexpr (BF) {
+      float mx = 0.f;
 #pragma unroll
-        for (int x = 1; x < TR; x <<= 1) mx = fmaxf(mx, __shfl_xor(mx, x, 64));
-        int ex = 0;
-        if (mx > 0.f && mx <= FLT_MAX) ex = 14 - ilogbf(mx);
-        cr = ldexpf(1.f, -ex);
+      for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(v[e]));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = pack_h2(ldexpf(v[2 * e], ex), ldexpf(v[2 * e + 1], ex));
-      }
-      // dims 64 s + 16 g + 8 h: step 2 s + h of lane group g
-      const int s = o >> 3, gg = (o >> 1) & 3, ks = 2 * s + (o & 1);
-      qs[((r >> 4) * KS + ks) * 64 + 16 * gg + (r & 15)] = w;
-      if (o == 0) rowc_s[r] = cr;
+      for (int x = 1; x < TR; x <<= 1) mx = fmaxf(mx, __shfl_xor(mx, x, 64));
+      if (mx > 0.f && mx <= FLT_MAX) ex = 14 - ilogbf(mx);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = ldexpf(v[e], ex);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = pack_h2(v[2 * e], v[2 * e + 1]);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum += v[e];
+#pragma unroll
+    for (int x = 1; x < TR; x <<= 1) sum += __shfl_xor(sum, x, 64);
+    // dims 64 s + 16 g + 8 h: step 2 s + h of lane group g
+    const int ks = 2 * (o >> 3) + (o & 1);
+    qs[((r >> 4) * KS + ks) * 64 + 16 * ((o >> 1) & 3) + (r & 15)] = w;
+    if (o == 0) {
+      rowc_s[r] = ldexpf(1.f, 24 - ex);
+      bias_s[r] = -sum * 0x1p-17f;
     }
   }
-  __syncthreads();
-  u32x4 qf[QREG ? NT : 1][QREG ? KS : 1];
-  if constexpr (QREG) {
+}
+
+// The softmax and the sums of a wave's 16 NT rows over the blocks it has seen.
+template <bool BF, int HD, int NT>
+struct Kv8Rows {
+  static constexpr int VB = HD / 16, TERMS = BF ? 1 : 2;  // output tiles; fp16 values that hold a weight
+  float rowc[NT], bias[NT], m[NT], l[NT];
+  bool unset[NT];  // the row has seen no position yet: m is 0
+  bool pending;    // some row of the wave is unset
+  float vref, vunit;  // largest V scale met (the weights' unit), and 2^kPScale over it
+  f32x4 acc[NT][VB], wsum[NT];  // wsum: 128 times the weights, in acc's unit
+
+  __device__ void init(const float* rowc_s, const float* bias_s) {
+    pending = true;
+    vref = 0x1p-100f;
+    vunit = exp2_raw(kPScale + 100.f);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      rowc[n] = rowc_s[16 * n];
+      bias[n] = bias_s[16 * n];
+      m[n] = l[n] = 0.f;
+      unset[n] = true;
+      wsum[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < VB; ++i) acc[n][i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    }
+  }
+  // factor of K's scales: fp16 queries need none of their own
+  __device__ static float key_factor() { return 1.44269504088896340736f / sqrtf((float)HD) * (BF ? 1.f : 0x1p24f); }
+
+  // Scales (ks, vs) of one position a lane, as the sums take them. A V row that is not finite makes the scores of
+  // its position NaN and has no weight, so that it does not reach the rows that do not see it (0 x NaN
+  // would).
+  __device__ void scales(float& ks, float& vs) {
+    const bool fine = fabsf(vs) <= FLT_MAX;
+    ks = fine ? ks * key_factor() : __builtin_nanf("");
+    vs = fine ? vs : 0.f;
+    if (__any(vs > vref * 8.f)) {
+      float x = vs;
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o, 64));
+      const float f = vref / x;
+      vref = x;
+      vunit = exp2_raw(kPScale) / x;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        wsum[n] *= f;
+#pragma unroll
+        for (int i = 0; i < VB; ++i) acc[n][i] *= f;
+      }
+    }
+    vs *= vunit;
+  }
+
+  // scores s of a block from position j0 on to weights pf; ks4, vs4: scales() of this lane's positions; rows
+  // r0 + lane % 16 + 16 n; masked: some position may lie behind a row's token, or off its path
+  template <int RT>
+  __device__ void weights(const Kv8AttnArgs& a, const Kv8Task<RT>& k, int r0, int64_t j0, bool masked, uint64_t paths,
+                          f32x4 (&s)[NT][2], const f32x4 (&ks4)[2], const f32x4 (&vs4)[2], u32x4 (&pf)[TERMS][NT]) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int s = 0; s < KS; ++s) qf[n][s] = qs[(n * KS + s) * 64 + lane];
-  }
-  float rowc[NT], m[NT], l[NT];
-  int tok[NT];
-  uint64_t path[NT];
-  const uint64_t paths = parents ? tree_path(parents, a.S) : 0;
+      for (int b = 0; b < 2; ++b)
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    rowc[n] = rowc_s[16 * n + c];
-    m[n] = -FLT_MAX;
-    l[n] = 0.f;
-    tok[n] = min(r0 + 16 * n + c, R - 1) / rep;
-    path[n] = __shfl((uint32_t)paths, tok[n], 64) | ((uint64_t)__shfl((uint32_t)(paths >> 32), tok[n], 64) << 32);
-  }
-  f32x4 acc[NT][VB];
+        for (int e = 0; e < 4; ++e)
+          s[n][b][e] = __builtin_fmaf(BF ? s[n][b][e] * rowc[n] : s[n][b][e], ks4[b][e], -m[n]);
+    if (masked) {
+      const int node0 = (int)max(min(j0 - k.pos, (int64_t)1 << 30), -((int64_t)1 << 30)) + 4 * g;  // negative: cached positions
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int i = 0; i < VB; ++i) acc[n][i] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  float vref = 0x1p-100f;  // largest V scale met (the probabilities' unit)
-  const float c_ = 1.44269504088896340736f / sqrtf((float)HD);
-
-  for (; blk < blk1; blk += 4) {
-    const bool more = blk + 4 < blk1;
-    // scales of the block's positions to the lanes that hold them
-    sc[lane] = lane < 32 ? scv * c_ : scv;
-    __builtin_amdgcn_wave_barrier();
-    f32x4 ks4[2], vs4[2];
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      ks4[b] = *reinterpret_cast<const f32x4*>(sc + 16 * b + 4 * g);
-      vs4[b] = *reinterpret_cast<const f32x4*>(sc + 32 + 16 * b + 4 * g);
-    }
-    __builtin_amdgcn_wave_barrier();
-    if (more) load_s(blk + 4);
-    f32x4 s[NT][2];
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n) s[n][b] = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int st = 0; st < KS; ++st) {
-        const uint32_t w0 = kr[b][st >> 1][2 * (st & 1)], w1 = kr[b][st >> 1][2 * (st & 1) + 1];
-        const u32x4 kf = {bytes_f16(0, w0, 0x0C010C00), bytes_f16(0, w0, 0x0C030C02), bytes_f16(0, w1, 0x0C010C00),
-                          bytes_f16(0, w1, 0x0C030C02)};
-#pragma unroll
-        for (int n = 0; n < NT; ++n) s[n][b] = mma16(kf, QREG ? qf[QREG ? n : 0][QREG ? st : 0] : qs[(n * KS + st) * 64 + lane], s[n][b]);
-      }
-    }
-    if (more) load_k(blk + 4);
-    // positions behind a row's token, or off its path
-    const int64_t j0 = (int64_t)blk * 32;
-    if (parents ? j0 + 31 >= pos : j0 + 31 > pos + tfirst) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n) {
+        const int tok = min(r0 + 16 * n + c, k.R - 1) / k.rep;
+        uint64_t path = 0;
+        if (k.parents) path = __shfl((uint32_t)paths, tok, 64) | ((uint64_t)__shfl((uint32_t)(paths >> 32), tok, 64) << 32);
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int64_t node = j0 + 16 * b + 4 * g + e - pos;  // negative: a cached position
-            const bool see = parents ? node < 0 || (node < 64 && ((path[n] >> (node & 63)) & 1)) : node <= tok[n];
-            s[n][b][e] = see ? s[n][b][e] * ks4[b][e] * (BF ? rowc[n] : 1.f) : -INFINITY;
+            const int node = node0 + 16 * b + e;
+            const bool see = node <= tok && (!k.parents || node < 0 || ((path >> (node & 63)) & 1));
+            s[n][b][e] = see ? s[n][b][e] : -INFINITY;
           }
-    } else {
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[n][b][e] = s[n][b][e] * ks4[b][e] * (BF ? rowc[n] : 1.f);
+      }
     }
-    float vmax = 0.f;
-    bool move = false;
+    float mx = -INFINITY;
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) vmax = fmaxf(vmax, vs4[b][e]);
-    move |= vmax > vref * (float)(1 << kLazy);
-    float mx[NT];
+      for (int e = 0; e < 4; ++e)
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      mx[n] = -INFINITY;
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) mx[n] = fmaxf(mx[n], s[n][b][e]);
-      move |= mx[n] > m[n] + (float)kLazy;
-    }
-    if (__any(move)) {
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) vmax = fmaxf(vmax, __shfl_xor(vmax, o, 64));
-      const float vnew = fmaxf(vref, vmax), vr_ = vref / vnew;
-      vref = vnew;
+        for (int n = 0; n < NT; ++n) mx = fmaxf(mx, s[n][b][e]);
+    if (pending || __any(mx > kLazy)) {
+      bool left = false;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        float x = fmaxf(mx[n], __shfl_xor(mx[n], 16, 64));
+        float x = -INFINITY;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x = fmaxf(x, s[n][b][e]);
+        x = fmaxf(x, __shfl_xor(x, 16, 64));
         x = fmaxf(x, __shfl_xor(x, 32, 64));
-        const float mn = fmaxf(m[n], x), alpha = exp2_raw(m[n] - mn);
-        m[n] = mn;
+        const float up = unset[n] ? (x == -INFINITY ? 0.f : x) : fmaxf(x, 0.f);
+        const float alpha = unset[n] ? 1.f : exp2_raw(-up);
+        unset[n] = unset[n] && x == -INFINITY;
+        left |= unset[n];
+        m[n] += up;
         l[n] *= alpha;
+        wsum[n] *= alpha;
 #pragma unroll
-        for (int i = 0; i < VB; ++i) acc[n][i] *= alpha * vr_;
+        for (int i = 0; i < VB; ++i) acc[n][i] *= alpha;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[n][b][e] -= up;
       }
+      pending = __any(left);
     }
-    // weights of V: probability x scale / vref, 0 for what a row does not see whatever the scale is
-    const float vinv = 1.f / vref;
-#pragma unroll
-    for (int b = 0; b < 2; ++b) vs4[b] *= vinv * exp2_raw(kPScale);
-    u32x4 pf[TERMS][NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -510,9 +512,9 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) attn_kv8_kernel(Kv8AttnA
         float w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float p = exp2_raw(s[n][b][e] - m[n]);
+          const float p = exp2_raw(s[n][b][e]);
           l[n] += p;
-          w[e] = s[n][b][e] == -INFINITY ? 0.f : p * vs4[b][e];
+          w[e] = p * vs4[b][e];
         }
 #pragma unroll
         for (int t = 0; t < TERMS; ++t)
@@ -524,82 +526,376 @@ __global__ void __launch_bounds__(256, NT == 1 ? 2 : 1) attn_kv8_kernel(Kv8AttnA
             w[e + 1] -= (float)hi.y;
           }
       }
+    const u32x4 ones = {0x00800080u, 0x00800080u, 0x00800080u, 0x00800080u};  // 128 x 2^-24
 #pragma unroll
-    for (int i = 0; i < VB; ++i) {
-      // dim VB c + i of the 8 positions: byte i & 3 of dword i / 4 of each row
-      const uint32_t sel = 0x0C000C00u | (uint32_t)((4 + (i & 3)) << 16) | (uint32_t)(i & 3);
-      const u32x4 vf = {bytes_f16(vr[1][i >> 2], vr[0][i >> 2], sel), bytes_f16(vr[3][i >> 2], vr[2][i >> 2], sel),
-                        bytes_f16(vr[5][i >> 2], vr[4][i >> 2], sel), bytes_f16(vr[7][i >> 2], vr[6][i >> 2], sel)};
+    for (int t = 0; t < TERMS; ++t)
 #pragma unroll
-      for (int t = 0; t < TERMS; ++t)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) acc[n][i] = mma16(vf, pf[t][n], acc[n][i]);
-    }
-    if (more) load_v(blk + 4);
+      for (int n = 0; n < NT; ++n) wsum[n] = mma16(ones, pf[t][n], wsum[n]);
   }
-  // merge of the waves, 16 rows at a time: every wave's maximum, sum and outputs (in V's own unit)
+  // output tile i += V's operand times the weights
+  __device__ void add(int i, u32x4 vf, const u32x4 (&pf)[TERMS][NT]) {
+#pragma unroll
+    for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) acc[n][i] = mma16(vf, pf[t][n], acc[n][i]);
+  }
+  __device__ void take_bias() {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < VB; ++i) acc[n][i] -= wsum[n];
+      wsum[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    }
+  }
+  __device__ float unit() const { return vref * exp2_raw(24.f - kPScale); }  // of acc
+  __device__ float top(int n) const { return unset[n] ? -FLT_MAX : m[n]; }
+  __device__ float sum(int n) const {  // over the lanes of a row
+    const float x = l[n] + __shfl_xor(l[n], 16, 64);
+    return x + __shfl_xor(x, 32, 64);
+  }
+};
+
+// N (4 or 8) gated outputs of a row, from dim d on
+template <bool BF, int N>
+__device__ __forceinline__ void kv8_out(const uint16_t* gate, uint16_t* out, const float (&o)[N], float inv) {
+  using E = E16<BF>;
+#pragma unroll
+  for (int i = 0; i < N; i += 4) {
+    const uint2 gw = *reinterpret_cast<const uint2*>(gate + i);
+    const uint16_t gv[4] = {(uint16_t)gw.x, (uint16_t)(gw.x >> 16), (uint16_t)gw.y, (uint16_t)(gw.y >> 16)};
+    uint32_t q[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) q[e] = E::mk(o[i + e] * inv * (1.f / (1.f + expf(-E::ld(gv[e])))));
+    *reinterpret_cast<uint2*>(out + i) = make_uint2(q[0] | (q[1] << 16), q[2] | (q[3] << 16));
+  }
+}
+
+// Few rows (16 a workgroup): the cache goes by once, and its bytes bound the kernel. Four waves take the
+// blocks in turn, each with a softmax of its own; K and V go from memory to registers in 16-byte pieces,
+// a block ahead, and are expanded there: no LDS and no barrier in the loop. The waves are merged at the end.
+template <bool BF, int HD>
+__global__ void __launch_bounds__(256, 2) attn_kv8_rows_kernel(Kv8AttnArgs a) {
+  constexpr int KS = HD / 32, KL = HD / 64, VB = HD / 16, RT = 16;  // VB: bytes of a lane's V piece
+  typedef uint32_t vpiece __attribute__((ext_vector_type(VB / 4)));
+  extern __shared__ __attribute__((aligned(16))) uint8_t kv8_lds[];
+  // queries, row factors and biases, scales of a wave's block; the merge of the waves takes the same memory
+  u32x4* const qs = reinterpret_cast<u32x4*>(kv8_lds);
+  float* const rowc_s = reinterpret_cast<float*>(kv8_lds + RT * HD * 2);
+  float* const bias_s = rowc_s + RT;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  float* const sc = bias_s + RT + wave * 64;
+  const int g = lane >> 4, c = lane & 15;
+  Kv8Task<RT> k(a);
+  if (row_invalid(k.posp, a.L, a.S, k.parents)) {
+    kv8_nan_rows<BF, HD>(a, k);
+    return;
+  }
+  if (!k.blocks(a)) return;  // the merge knows
+  const int64_t klast = k.pos + k.tlast;  // last position any row sees; later ones of a block repeat it
+  u32x4 kr[2][KL];
+  vpiece vr[8];
+  float scv = 0.f;  // lane l < 32: K scale of position l of the block; else V scale of l - 32
+  auto load_k = [&](int blk) {
+    const int64_t j0 = (int64_t)blk * 32;
+    const int left = (int)min(klast - j0, (int64_t)31);
+    const uint8_t* p = a.kc + (k.base + j0) * HD + 16 * g;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int s = 0; s < KL; ++s) kr[b][s] = *reinterpret_cast<const u32x4*>(p + min(16 * b + c, left) * HD + 64 * s);
+  };
+  auto load_v = [&](int blk) {
+    const int64_t j0 = (int64_t)blk * 32;
+    const int left = (int)min(klast - j0, (int64_t)31);
+    const uint8_t* p = a.vc + (k.base + j0) * HD + VB * c;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) vr[i] = *reinterpret_cast<const vpiece*>(p + min(16 * (i >> 2) + 4 * g + (i & 3), left) * HD);
+  };
+  auto load_s = [&](int blk) {
+    const int64_t j0 = (int64_t)blk * 32;
+    const int left = (int)min(klast - j0, (int64_t)31);
+    scv = (lane < 32 ? a.ks : a.vs)[k.base + j0 + min(lane & 31, left)];
+  };
+  int blk = k.blk0 + wave;
+  if (blk < k.blk1) {
+    load_k(blk);
+    load_v(blk);
+    load_s(blk);
+  }
+  kv8_stage_q<BF, HD>(a, k, qs, rowc_s, bias_s);
+  __syncthreads();
+  u32x4 qf[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) qf[s] = qs[s * 64 + lane];
+  Kv8Rows<BF, HD, 1> rows;
+  rows.init(rowc_s + c, bias_s + c);
+  const uint64_t paths = k.parents ? tree_path(k.parents, a.S) : 0;
+  for (int it = 1; blk < k.blk1; blk += 4, ++it) {
+    const bool more = blk + 4 < k.blk1;
+    // scales of the block's positions to the lanes that hold them (the wave's LDS operations are in order)
+    {
+      const float other = __shfl_xor(scv, 32, 64);
+      float x = lane < 32 ? scv : 0.f, y = lane < 32 ? other : scv;
+      rows.scales(x, y);
+      sc[lane] = lane < 32 ? x : y;
+    }
+    __builtin_amdgcn_wave_barrier();
+    f32x4 ks4[2], vs4[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      ks4[b] = *reinterpret_cast<const f32x4*>(sc + 16 * b + 4 * g);
+      vs4[b] = *reinterpret_cast<const f32x4*>(sc + 32 + 16 * b + 4 * g);
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (more) load_s(blk + 4);
+    f32x4 s[1][2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      s[0][b] = (f32x4){rows.bias[0], rows.bias[0], rows.bias[0], rows.bias[0]};
+#pragma unroll
+      for (int st = 0; st < KS; ++st)
+        s[0][b] = mma16(bytes8(kr[b][st >> 1][2 * (st & 1)], kr[b][st >> 1][2 * (st & 1) + 1]), qf[st], s[0][b]);
+    }
+    if (more) load_k(blk + 4);
+    const int64_t j0 = (int64_t)blk * 32;
+    u32x4 pf[Kv8Rows<BF, HD, 1>::TERMS][1];
+    rows.weights(a, k, k.r0, j0, k.parents ? j0 + 31 >= k.pos : j0 + 31 > k.pos + k.tfirst, paths, s, ks4, vs4, pf);
+#pragma unroll
+    for (int i = 0; i < VB; ++i)  // dim VB c + i of the 8 positions: byte i & 3 of dword i / 4 of each row
+      rows.add(i, (u32x4){byte_pair(vr[1][i >> 2], vr[0][i >> 2], i & 3), byte_pair(vr[3][i >> 2], vr[2][i >> 2], i & 3),
+                          byte_pair(vr[5][i >> 2], vr[4][i >> 2], i & 3), byte_pair(vr[7][i >> 2], vr[6][i >> 2], i & 3)}, pf);
+    if (more) load_v(blk + 4);
+    if (it % kBiasBlocks == 0 || !more) rows.take_bias();
+  }
+  // merge of the waves: every wave's maximum, sum and outputs (in V's own unit)
   constexpr int OS = HD + 4;
   float* const mo = reinterpret_cast<float*>(kv8_lds);             // [4][16][OS]
   float2* const ml = reinterpret_cast<float2*>(mo + 4 * 16 * OS);  // [4][16]
-  const float unit = vref * exp2_raw(-kPScale);
+  const float unit = rows.unit();
+  __syncthreads();  // queries and scales are no longer read
+  float* const mine = mo + (wave * 16 + c) * OS;
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    __syncthreads();  // queries, or the tile before, are no longer read
-    float* const mine = mo + (wave * 16 + c) * OS;
+  for (int e = 0; e < 4; ++e)
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+    for (int i = 0; i < VB; i += 4)
+      *reinterpret_cast<f32x4*>(mine + VB * (4 * g + e) + i) =
+          (f32x4){rows.acc[0][i][e], rows.acc[0][i + 1][e], rows.acc[0][i + 2][e], rows.acc[0][i + 3][e]} * unit;
+  const float ls = rows.sum(0);
+  if (g == 0) ml[wave * 16 + c] = make_float2(rows.top(0), ls);
+  __syncthreads();
+  for (int i = tid; i < 16 * HD / 4; i += 256) {
+    const int rr = i / (HD / 4), d = 4 * (i % (HD / 4)), r = k.r0 + rr;
+    if (r >= k.R) continue;
+    float mm = -FLT_MAX, ll = 0.f;
 #pragma unroll
-      for (int i = 0; i < VB; i += 4)
-        *reinterpret_cast<f32x4*>(mine + VB * (4 * g + e) + i) =
-            (f32x4){acc[n][i][e], acc[n][i + 1][e], acc[n][i + 2][e], acc[n][i + 3][e]} * unit;
-    float ls = l[n] + __shfl_xor(l[n], 16, 64);
-    ls += __shfl_xor(ls, 32, 64);
-    if (g == 0) ml[wave * 16 + c] = make_float2(m[n], ls);
-    __syncthreads();
-    for (int i = tid; i < 16 * HD / 4; i += 256) {
-      const int rr = i / (HD / 4), d = 4 * (i % (HD / 4)), r = r0 + 16 * n + rr;
-      if (r >= R) continue;
-      float mm = -FLT_MAX, ll = 0.f;
+    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, ml[w * 16 + rr].x);
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int w = 0; w < 4; ++w) mm = fmaxf(mm, ml[w * 16 + rr].x);
-      f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float2 x = ml[w * 16 + rr];
-        const float f = exp2_raw(x.x - mm);
-        ll += x.y * f;
-        o += *reinterpret_cast<const f32x4*>(mo + (w * 16 + rr) * OS + d) * f;
-      }
-      if (a.nsplit > 1) {
-        const int64_t rows = (int64_t)a.B * a.Hkv * R, at = (((int64_t)bb * a.Hkv + kvh) * R + r) * a.nsplit + z;
-        *reinterpret_cast<f32x4*>(a.part + at * HD + d) = o;
-        if (d == 0) *reinterpret_cast<float2*>(a.part + rows * a.nsplit * HD + 2 * at) = make_float2(mm, ll);
-      } else {
-        const uint16_t* gate = static_cast<const uint16_t*>(a.qg) + row_at(r, a.qg_stride, 2 * HD) + HD + d;
-        const uint2 gw = *reinterpret_cast<const uint2*>(gate);
-        const uint16_t gv[4] = {(uint16_t)gw.x, (uint16_t)(gw.x >> 16), (uint16_t)gw.y, (uint16_t)(gw.y >> 16)};
-        const float inv = 1.f / ll;
-        uint32_t q[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) q[e] = E::mk(o[e] * inv * (1.f / (1.f + expf(-E::ld(gv[e])))));
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + row_at(r, a.out_stride, HD) + d) =
-            make_uint2(q[0] | (q[1] << 16), q[2] | (q[3] << 16));
-      }
+    for (int w = 0; w < 4; ++w) {
+      const float2 x = ml[w * 16 + rr];
+      const float f = exp2_raw(x.x - mm);
+      ll += x.y * f;
+      o += *reinterpret_cast<const f32x4*>(mo + (w * 16 + rr) * OS + d) * f;
+    }
+    if (a.nsplit > 1) {
+      const int64_t all = (int64_t)a.B * a.Hkv * k.R, at = (((int64_t)k.bb * a.Hkv + k.kvh) * k.R + r) * a.nsplit + k.z;
+      *reinterpret_cast<f32x4*>(a.part + at * HD + d) = o;
+      if (d == 0) *reinterpret_cast<float2*>(a.part + all * a.nsplit * HD + 2 * at) = make_float2(mm, ll);
+    } else {
+      const float v[4] = {o[0], o[1], o[2], o[3]};
+      kv8_out<BF, 4>(static_cast<const uint16_t*>(a.qg) + k.row_at(a, r, a.qg_stride, 2 * HD) + HD + d,
+                     static_cast<uint16_t*>(a.out) + k.row_at(a, r, a.out_stride, HD) + d, v, 1.f / ll);
     }
   }
 }
 
-// Outputs of split positions: a wave per row weighs the splits that hold positions of the row's tile by
-// their maxima, normalizes and gates. Bound by reading the partial outputs once.
+// steps of a wave's queries that attn_kv8_tile_kernel reads from LDS
+constexpr int kv8_lds_steps(int hd, int nt) { return hd == 256 ? 1 : (hd == 128 && nt == 4 ? 2 : 0); }
+
+// Many rows: 16 NT a wave, four waves to a workgroup, over tiles of 64 positions whose bytes come to LDS by
+// DMA, a tile ahead (two buffers, one barrier a tile), and are read by every wave: 16 bytes of K or PW of V a
+// lane at a time, expanded in registers. Bound by the matrix cores and the vector instructions around
+// them (two waves a SIMD overlap them).
+//  * K's 16-byte pieces are XOR-swizzled by position, V's pieces (or rows) by bits 2 and 3 of it, so that the
+//    lanes of a read fall on different banks; the DMA's source address does it.
+template <bool BF, int HD, int NT>
+__global__ void __launch_bounds__(256, 2) attn_kv8_tile_kernel(Kv8AttnArgs a) {
+  constexpr int KS = HD / 32, VB = HD / 16, RT = 64 * NT, NC = HD / 16;  // NC: 16-byte pieces of a row
+  constexpr int PW = VB < 8 ? VB : 8, NP = VB / PW;                      // dims of a V piece, pieces of a lane
+  constexpr int SH = HD == 256 ? 0 : (HD == 128 ? 1 : 2);                // 2^SH rows to the 64 banks
+  constexpr int TB = 64 * HD;                                           // bytes of a tile of K or V
+  typedef uint32_t vpiece __attribute__((ext_vector_type(PW / 4)));
+  extern __shared__ __attribute__((aligned(16))) uint8_t kv8_lds[];
+  // two buffers of [K tile | V tile | K scales | V scales], then QL steps of the queries, for which there are
+  // not enough registers; all queries pass through before the first tile
+  constexpr int BUF = 2 * TB + 512, QL = kv8_lds_steps(HD, NT);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4, c = lane & 15;
+  Kv8Task<RT> k(a);
+  if (row_invalid(k.posp, a.L, a.S, k.parents)) {
+    kv8_nan_rows<BF, HD>(a, k);
+    return;
+  }
+  if (!k.blocks(a)) return;  // the merge knows
+  const int64_t klast = k.pos + k.tlast;
+  u32x4 qf[NT][KS];
+  u32x4* const ql = reinterpret_cast<u32x4*>(kv8_lds + 2 * BUF) + wave * NT * QL * 64 + lane;
+  Kv8Rows<BF, HD, NT> rows;
+  {
+    u32x4* const qs = reinterpret_cast<u32x4*>(kv8_lds);
+    float* const rowc_s = reinterpret_cast<float*>(kv8_lds + RT * HD * 2);
+    float* const bias_s = rowc_s + RT;
+    kv8_stage_q<BF, HD>(a, k, qs, rowc_s, bias_s);
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int s = 0; s < KS; ++s) qf[n][s] = qs[((wave * NT + n) * KS + s) * 64 + lane];
+    rows.init(rowc_s + 16 * NT * wave + c, bias_s + 16 * NT * wave + c);
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int s = 0; s < QL; ++s) ql[(n * QL + s) * 64] = qf[n][s];
+  }
+  // tile of blocks blk, blk + 1; positions past the last repeat it. Piece i of a wave: 64 / NC rows from
+  // 16 wave + i 64 / NC on, NC lanes a row.
+  auto issue = [&](int blk, uint8_t* buf) {
+    const int64_t j0 = (int64_t)blk * 32;
+    const int left = (int)min(klast - j0, (int64_t)63);
+    const uint8_t* const kp = a.kc + (k.base + j0) * HD;
+    const uint8_t* const vp = a.vc + (k.base + j0) * HD;
+    const int ln = anew(lane), first = 16 * wave + ln / NC;
+#pragma unroll
+    for (int i = 0; i < NC / 4; ++i) {
+      const int row = first + i * (64 / NC), o = (ln ^ (4 * i + (ln >> 4))) & (NC - 1);
+      // V: rows of 128 and 64 bytes change places, 16-byte pieces of longer ones
+      const int vrow = row ^ (HD == 128 ? (ln >> 5) & 1 : (HD == 64 ? ln >> 4 : 0)), vo = (ln ^ (HD == 256 ? 8 * (i & 1) : 0)) & (NC - 1);
+      uint8_t* const dst = buf + (wave * (NC / 4) + i) * 1024;
+      __builtin_amdgcn_global_load_lds(kp + (uint32_t)(min(row, left) * HD + 16 * o), (lds_ptr_t)dst, 16, 0, 0);
+      __builtin_amdgcn_global_load_lds(vp + (uint32_t)(min(vrow, left) * HD + 16 * vo), (lds_ptr_t)(dst + TB), 16, 0, 0);
+    }
+    if (wave < 2)
+      __builtin_amdgcn_global_load_lds((wave ? a.vs : a.ks) + k.base + j0 + (uint32_t)min(ln, left),
+                                       (lds_ptr_t)(buf + 2 * TB + wave * 256), 4, 0, 0);
+  };
+  const uint64_t paths = k.parents ? tree_path(k.parents, a.S) : 0;
+  const int r0 = k.r0 + 16 * NT * wave;
+  float* const sw = reinterpret_cast<float*>(kv8_lds + 2 * BUF + 4096 * NT * QL) + wave * 128;  // the wave's scales
+  const int64_t pfirst = k.pos + min(r0, k.R - 1) / k.rep, plast = k.pos + min(r0 + 16 * NT - 1, k.R - 1) / k.rep;
+  const bool on = r0 < k.R;
+  issue(k.blk0, kv8_lds);
+  int cur = 0;
+  for (int blk = k.blk0, it = 0; blk < k.blk1; blk += 2, ++it, cur ^= 1) {
+    // the tile has landed; every wave is done with the other buffer
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (blk + 2 < k.blk1) issue(blk + 2, kv8_lds + (cur ^ 1) * BUF);
+    const uint8_t* const kt = kv8_lds + cur * BUF;
+    if (on && (int64_t)blk * 32 <= plast) {
+      float x = reinterpret_cast<const float*>(kt + 2 * TB)[lane], y = reinterpret_cast<const float*>(kt + 2 * TB)[64 + lane];
+      rows.scales(x, y);
+      sw[lane] = x;
+      sw[64 + lane] = y;
+      __builtin_amdgcn_wave_barrier();
+    }
+#pragma unroll 1
+    for (int sb = 0; sb < 2; ++sb) {
+      const int64_t j0 = (int64_t)(blk + sb) * 32;
+      if (!on || blk + sb >= k.blk1 || j0 > plast) continue;
+      const int ln = anew(lane), g = ln >> 4, c = ln & 15;
+      const uint8_t* const kb = kt + (32 * sb + c) * HD;
+      const uint8_t* const vb = kt + TB;
+      const float* const sc = sw + 32 * sb + 4 * g;
+      f32x4 ks4[2], vs4[2], s[NT][2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        ks4[b] = *reinterpret_cast<const f32x4*>(sc + 16 * b);
+        vs4[b] = *reinterpret_cast<const f32x4*>(sc + 64 + 16 * b);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s[n][b] = (f32x4){rows.bias[n], rows.bias[n], rows.bias[n], rows.bias[n]};
+      }
+#pragma unroll
+      for (int st = 0; st < KS / 2; ++st) {
+        u32x4 w[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b)  // position 32 sb + 16 b + c: its swizzle does not depend on sb and b
+          w[b] = *reinterpret_cast<const u32x4*>(kb + 16 * b * HD + 16 * ((4 * st + g) ^ ((c >> SH) & (NC - 1))));
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const u32x4 kf = bytes8(w[b][2 * h], w[b][2 * h + 1]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+              s[n][b] = mma16(kf, 2 * st + h < QL ? ql[(n * QL + 2 * st + h) * 64] : qf[n][2 * st + h], s[n][b]);
+          }
+      }
+      u32x4 pf[Kv8Rows<BF, HD, NT>::TERMS][NT];
+      rows.weights(a, k, r0, j0, k.parents ? j0 + 31 >= k.pos : j0 + 31 > pfirst, paths, s, ks4, vs4, pf);
+#pragma unroll
+      for (int h = 0; h < NP; ++h) {
+        vpiece v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int key = 32 * sb + 16 * (i >> 2) + 4 * g + (i & 3);
+          const int row = HD == 256 ? key : key ^ (g & ((1 << SH) - 1));
+          const int at = HD == 256 ? ((128 * h + PW * c) ^ ((g & 1) << 7)) : PW * c;
+          v[i] = *reinterpret_cast<const vpiece*>(vb + row * HD + at);
+        }
+#pragma unroll
+        for (int i = 0; i < PW; ++i)  // dim (HD / NP) h + PW c + i of the 8 positions
+          rows.add(PW * h + i, (u32x4){byte_pair(v[1][i >> 2], v[0][i >> 2], i & 3), byte_pair(v[3][i >> 2], v[2][i >> 2], i & 3),
+                                       byte_pair(v[5][i >> 2], v[4][i >> 2], i & 3), byte_pair(v[7][i >> 2], v[6][i >> 2], i & 3)}, pf);
+      }
+    }
+    if (it % (kBiasBlocks / 2) == kBiasBlocks / 2 - 1 || blk + 2 >= k.blk1) rows.take_bias();
+  }
+  // a lane's outputs: row r0 + 16 n + c, dims (HD / NP) h + PW (4 g + e) + i
+  const float unit = rows.unit();
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int r = r0 + 16 * n + c;
+    const float ls = rows.sum(n);
+    if (r >= k.R) continue;
+    const int64_t all = (int64_t)a.B * a.Hkv * k.R, at = (((int64_t)k.bb * a.Hkv + k.kvh) * k.R + r) * a.nsplit + k.z;
+    if (a.nsplit > 1 && g == 0) *reinterpret_cast<float2*>(a.part + all * a.nsplit * HD + 2 * at) = make_float2(rows.top(n), ls);
+    const uint16_t* const gate = static_cast<const uint16_t*>(a.qg) + k.row_at(a, r, a.qg_stride, 2 * HD) + HD;
+    uint16_t* const out = static_cast<uint16_t*>(a.out) + k.row_at(a, r, a.out_stride, HD);
+#pragma unroll
+    for (int h = 0; h < NP; ++h)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = HD / NP * h + PW * (4 * g + e);
+        float o[PW];
+#pragma unroll
+        for (int i = 0; i < PW; ++i) o[i] = rows.acc[n][PW * h + i][e] * unit;
+        if (a.nsplit > 1) {
+#pragma unroll
+          for (int i = 0; i < PW; i += 4)
+            *reinterpret_cast<f32x4*>(a.part + at * HD + d + i) = (f32x4){o[i], o[i + 1], o[i + 2], o[i + 3]};
+        } else {
+          kv8_out<BF, PW>(gate + d, out + d, o, 1.f / ls);
+        }
+      }
+  }
+}
+
+// Outputs of split positions: a workgroup per row, a wave to every eight splits (up to 16 waves); each wave weighs
+// those of its splits that hold positions of the row's tile by their largest maximum, and the waves meet
+// in LDS. Bound by the latency of one read of the partial outputs, all in flight at once.
+constexpr int kMergeWaves = 16, kMergeSplits = 8;
+
 template <bool BF, int HD>
-__global__ void __launch_bounds__(256) attn_kv8_merge_kernel(Kv8AttnArgs a, int rt) {
+__global__ void __launch_bounds__(64 * kMergeWaves) attn_kv8_merge_kernel(Kv8AttnArgs a, int rt) {
   using E = E16<BF>;
   constexpr int V = HD / 64;
   typedef float vec_t __attribute__((ext_vector_type(V)));
-  const int rep = a.H / a.Hkv, R = a.S * rep;
-  const int64_t rows = (int64_t)a.B * a.Hkv * R, i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (i >= rows) return;
-  const int r = (int)(i % R), kvh = (int)(i / R % a.Hkv), d = V * (threadIdx.x & 63), t = r / rep;
+  extern __shared__ __attribute__((aligned(16))) float merge_lds[];  // [waves][HD], then (maximum, sum) of each
+  const int rep = a.H / a.Hkv, R = a.S * rep, nw = blockDim.x >> 6;
+  float2* const mls = reinterpret_cast<float2*>(merge_lds + nw * HD);
+  const int64_t rows = (int64_t)a.B * a.Hkv * R, i = blockIdx.x;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int r = (int)(i % R), kvh = (int)(i / R % a.Hkv), d = V * lane, t = r / rep;
   const int64_t bb = i / R / a.Hkv;
   const int64_t* const posp = a.pos + bb * a.pos_stride;
   const int32_t* const parents = a.parents ? a.parents + bb * a.parents_stride : nullptr;
@@ -607,7 +903,8 @@ __global__ void __launch_bounds__(256) attn_kv8_merge_kernel(Kv8AttnArgs a, int 
   uint16_t* const out = static_cast<uint16_t*>(a.out) + tok * a.out_stride + head * HD + d;
   const uint16_t* const gate = static_cast<const uint16_t*>(a.qg) + tok * a.qg_stride + head * 2 * HD + HD + d;
   if (row_invalid(posp, a.L, a.S, parents)) {
-    for (int j = 0; j < V; ++j) out[j] = E::mk(__builtin_nanf(""));
+    if (wave == 0)
+      for (int j = 0; j < V; ++j) out[j] = E::mk(__builtin_nanf(""));
     return;
   }
   const int nblk = kv8_blocks(posp[0], min(r / rt * rt + rt - 1, R - 1) / rep), per = (nblk + a.nsplit - 1) / a.nsplit;
@@ -616,11 +913,43 @@ __global__ void __launch_bounds__(256) attn_kv8_merge_kernel(Kv8AttnArgs a, int 
   const float* const po = a.part + i * a.nsplit * HD + d;
   float m = -FLT_MAX, l = 0.f;
   vec_t o = 0.f;
-  for (int z = 0; z < nz; ++z) m = fmaxf(m, ml[z].x);
-  for (int z = 0; z < nz; ++z) {
-    const float w = exp2_raw(ml[z].x - m);
-    l += ml[z].y * w;
-    o += *reinterpret_cast<const vec_t*>(po + (int64_t)z * HD) * w;
+  for (int z0 = wave * kMergeSplits; z0 < nz; z0 += nw * kMergeSplits) {
+    vec_t x[kMergeSplits];
+    float2 s[kMergeSplits];
+#pragma unroll
+    for (int u = 0; u < kMergeSplits; ++u) {
+      const int z = min(z0 + u, nz - 1);
+      x[u] = *reinterpret_cast<const vec_t*>(po + (int64_t)z * HD);
+      s[u] = ml[z];
+    }
+    float mn = m;
+#pragma unroll
+    for (int u = 0; u < kMergeSplits; ++u) mn = fmaxf(mn, s[u].x);
+    const float f = exp2_raw(m - mn);
+    l *= f;
+    o *= f;
+    m = mn;
+#pragma unroll
+    for (int u = 0; u < kMergeSplits; ++u) {
+      const float w = z0 + u < nz ? exp2_raw(s[u].x - m) : 0.f;
+      if (z0 + u < nz) {
+        l += s[u].y * w;
+        o += x[u] * w;
+      }
+    }
+  }
+  *reinterpret_cast<vec_t*>(merge_lds + wave * HD + d) = o;
+  if (lane == 0) mls[wave] = make_float2(m, l);
+  __syncthreads();
+  if (wave) return;
+  float mm = -FLT_MAX;
+  for (int w = 0; w < nw; ++w) mm = fmaxf(mm, mls[w].x);
+  o = 0.f;
+  l = 0.f;
+  for (int w = 0; w < nw; ++w) {
+    const float f = exp2_raw(mls[w].x - mm);
+    o += *reinterpret_cast<const vec_t*>(merge_lds + w * HD + d) * f;
+    l += mls[w].y * f;
   }
   const float inv = 1.f / l;
 #pragma unroll
@@ -658,26 +987,57 @@ hipError_t launch_kv8_read(int dt, const Kv8ReadArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 
-template <bool BF, int HD, int NT>
-static hipError_t launch_attn_kv8_t(const Kv8AttnArgs& a, hipStream_t s) {
-  constexpr int RT = 16 * NT;
-  constexpr int lds_q = RT * HD * 2 + RT * 4 + 4 * 64 * 4, lds_m = 4 * 16 * (HD + 4) * 4 + 4 * 16 * 8;
-  constexpr int lds = lds_q > lds_m ? lds_q : lds_m;
+// Workgroups of rt rows, and the merge of their splits; `launch` starts the kernel over a grid.
+template <bool BF, int HD, typename F>
+static hipError_t launch_attn_kv8_t(const Kv8AttnArgs& a, hipStream_t s, int rt, F launch) {
   const int64_t rows = (int64_t)a.S * (a.H / a.Hkv), all = rows * a.Hkv * a.B;
-  const int64_t wgs = (rows + RT - 1) / RT * a.Hkv * a.nsplit;
-  if (wgs >= (1ll << 31) || (a.nsplit > 1 && (all + 3) / 4 >= (1ll << 31))) return hipErrorInvalidValue;
-  static LdsLimit limit;
-  const hipError_t e = limit.raise((const void*)attn_kv8_kernel<BF, HD, NT>, lds);
+  const int64_t wgs = (rows + rt - 1) / rt * a.Hkv * a.nsplit;
+  if (wgs >= (1ll << 31) || (a.nsplit > 1 && all >= (1ll << 31))) return hipErrorInvalidValue;
+  const hipError_t e = launch(dim3((unsigned)wgs, (unsigned)a.B));
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((attn_kv8_kernel<BF, HD, NT>), dim3((unsigned)wgs, (unsigned)a.B), dim3(256), lds, s, a);
-  if (a.nsplit > 1)
-    hipLaunchKernelGGL((attn_kv8_merge_kernel<BF, HD>), dim3((unsigned)((all + 3) / 4)), dim3(256), 0, s, a, RT);
+  if (a.nsplit > 1) {
+    const int waves = std::min((a.nsplit + kMergeSplits - 1) / kMergeSplits, kMergeWaves);
+    hipLaunchKernelGGL((attn_kv8_merge_kernel<BF, HD>), dim3((unsigned)all), dim3(64 * waves), waves * (HD * 4 + 8), s, a, rt);
+  }
   return hipGetLastError();
 }
 
+template <bool BF, int HD>
+static hipError_t launch_attn_kv8_rows(const Kv8AttnArgs& a, hipStream_t s) {
+  constexpr int q = 16 * HD * 2 + 2 * 16 * 4 + 4 * 64 * 4, merge = 4 * 16 * (HD + 4) * 4 + 4 * 16 * 8;
+  constexpr int lds = q > merge ? q : merge;
+  return launch_attn_kv8_t<BF, HD>(a, s, 16, [&](dim3 grid) {
+    static LdsLimit limit;
+    const hipError_t e = limit.raise((const void*)attn_kv8_rows_kernel<BF, HD>, lds);
+    if (e == hipSuccess) hipLaunchKernelGGL((attn_kv8_rows_kernel<BF, HD>), grid, dim3(256), lds, s, a);
+    return e;
+  });
+}
+
+template <bool BF, int HD, int NT>
+static hipError_t launch_attn_kv8_tile(const Kv8AttnArgs& a, hipStream_t s) {
+  constexpr int q = 64 * NT * (HD * 2 + 8), tiles = 2 * (2 * 64 * HD + 512) + 4096 * NT * kv8_lds_steps(HD, NT) + 2048;
+  constexpr int lds = q > tiles ? q : tiles;
+  return launch_attn_kv8_t<BF, HD>(a, s, 64 * NT, [&](dim3 grid) {
+    static LdsLimit limit;
+    const hipError_t e = limit.raise((const void*)attn_kv8_tile_kernel<BF, HD, NT>, lds);
+    if (e == hipSuccess) hipLaunchKernelGGL((attn_kv8_tile_kernel<BF, HD, NT>), grid, dim3(256), lds, s, a);
+    return e;
+  });
+}
+
+constexpr int kv8_few_rows = 32;
+
 hipError_t launch_attn_kv8(bool bf16, const Kv8AttnArgs& a, hipStream_t s) {
+  const int64_t rows = (int64_t)a.S * (a.H / a.Hkv);
   auto tiles = [&](auto bf, auto hd) -> hipError_t {
-    return launch_attn_kv8_t<decltype(bf)::value, decltype(hd)::value, 1>(a, s);
+    constexpr bool BF = decltype(bf)::value;
+    constexpr int HD = decltype(hd)::value;
+    if (rows <= kv8_few_rows) return launch_attn_kv8_rows<BF, HD>(a, s);
+    if constexpr (HD < 256) {
+      if (rows > 128) return launch_attn_kv8_tile<BF, HD, 4>(a, s);
+    }
+    return launch_attn_kv8_tile<BF, HD, 2>(a, s);
   };
   auto dims = [&](auto bf) -> hipError_t {
     if (a.hd == 256) return tiles(bf, std::integral_constant<int, 256>{});

@@ -225,12 +225,16 @@ def _reference(t, H, G, hd):
             sc = torch.matmul(q[b, :, h], k.t().contiguous()) * hd ** -0.5
             p = torch.softmax(sc.masked_fill(~see, float("-inf")), -1)
             out[b, :, h] = torch.matmul(p, v)
-            size = torch.matmul(q[b, :, h].abs(), k.abs().t().contiguous()).mul(see).amax(-1, keepdim=True) * hd ** -0.5
+            # float32 sums run over bytes u = x / s + 128, not over x, and 128 times the factors' sum is taken off: a term
+            # is up to 255 s |factor| in size whatever x is
+            ks, vs = (255 * t[x][b, g, :n].double() for x in ("ks", "vs"))
+            size = (q[b, :, h].abs().sum(-1, keepdim=True) * ks * see).amax(-1, keepdim=True) * hd ** -0.5
             # a score: float32 sums of hd products in steps of 32 and a few more roundings, absolute; a weight: that in the
             # exponent (over and under the line), exp's and the scales' roundings, one fp16 rounding for bf16
             # outputs; sums over the positions
             weight = 2 * (hd / 32 + 8) * 2.0 ** -24 * size + 8 * 2.0 ** -24 + (2.0 ** -11 if bf else 2.0 ** -21)
-            tol[b, :, h] = (weight + (n / 32 + 16) * 2.0 ** -24) * torch.matmul(p, v.abs())
+            tol[b, :, h] = (weight * torch.matmul(p, v.abs())
+                            + (n / 32 + 16) * 2.0 ** -24 * torch.matmul(p, vs)[:, None])
     return out * gate, tol * gate
 
 
@@ -323,12 +327,13 @@ def test_attn_kv8_bf16_query_sizes():
 @pytest.mark.parametrize("splits", [1, 3])
 @pytest.mark.parametrize("tree", [None, "random"])
 def test_attn_kv8_not_finite(tree, splits):
-    """A NaN row of the cache, or a query or gate that is not finite, reaches the outputs that see it and
-    leaves every other as it was, bit for bit."""
+    """A NaN row of the cache, or a query or gate that is not finite, reaches the outputs that see it; every other
+    is what it is without it, within the rounding bound (the rows of a wave share when their references
+    move, so not bit for bit)."""
     B, S, pos, L, H, G, hd = 2, 40, [50, 61], 110, 4, 2, 64
     t = _attn_inputs(B, S, pos, L, H, G, hd, F16, tree)
-    clean = _attn(t, H, G, hd, splits=splits).view(B, S, H, hd)
-    assert torch.isfinite(clean).all()
+    clean, tol = _reference(t, H, G, hd)
+    _check(_attn(t, H, G, hd, splits=splits), clean, tol, F16)
 
     def sees(b, node):
         if tree is None:
@@ -337,7 +342,8 @@ def test_attn_kv8_not_finite(tree, splits):
 
     def check(changed, bad):
         got = _attn(dict(t, **changed), H, G, hd, splits=splits).view(B, S, H, hd)
-        assert torch.isnan(got[bad]).all() and torch.equal(got[~bad], clean[~bad])
+        assert torch.isnan(got[bad]).all()
+        _check(got[~bad], clean[~bad], tol[~bad], F16)
     for name in ("ks", "vs"):
         for node in (7, 33):
             x = t[name].clone()
