@@ -286,6 +286,10 @@ int gsq_kv8_read(const uint8_t* k_cache, const uint8_t* v_cache, const float* k_
                  void* v, int64_t heads, int64_t max_len, int64_t start, int64_t n, int64_t head_dim, int dtype,
                  void* stream);
 
+/* The splits with which gsq_attn_kv8 fills a device of `cus` CUs (1 for arguments that are none). */
+int64_t gsq_attn_kv8_splits(int64_t batch, int64_t seq, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                            int64_t max_len, int64_t cus);
+
 /* out = round(softmax(q K^T / sqrt(head_dim)) V * sigmoid(gate)) per head, gates in qg; token t attends to
  * positions 0 .. *pos + t, in a tree to 0 .. *pos - 1, its ancestors and itself. splits > 1: the
  * positions are shared out over that many workgroups for each tile of rows (at most 65535), whose sums

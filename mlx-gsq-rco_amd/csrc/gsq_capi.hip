@@ -38,6 +38,8 @@ hipError_t launch_attn_seq(bool bf16, const AttnSeqArgs& a, hipStream_t s);
 hipError_t launch_kv8_write(bool bf16, const Kv8WriteArgs& a, hipStream_t s);
 hipError_t launch_kv8_read(int dt, const Kv8ReadArgs& a, hipStream_t s);
 hipError_t launch_attn_kv8(bool bf16, const Kv8AttnArgs& a, hipStream_t s);
+int64_t attn_kv8_splits(int64_t batch, int64_t seq, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_len,
+                        int cus);
 hipError_t launch_attn_decode(int dt, const AttnArgs& a, hipStream_t s);
 int qmv_table_bytes(int qt);
 int build_qmv_table(int qt, const uint16_t* grid16, const uint8_t* ksigns, std::vector<uint8_t>& out);
@@ -885,6 +887,12 @@ int gsq_kv8_read(const uint8_t* k_cache, const uint8_t* v_cache, const float* k_
   hipError_t e = launch_kv8_read(dtype, a, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return fail(GSQ_E_HIP, "kv8_read launch: %s", hipGetErrorString(e));
   return GSQ_OK;
+}
+
+int64_t gsq_attn_kv8_splits(int64_t batch, int64_t seq, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                            int64_t max_len, int64_t cus) {
+  if (batch <= 0 || seq <= 0 || kv_heads <= 0 || heads < kv_heads || max_len <= 0 || cus <= 0) return 1;
+  return attn_kv8_splits(batch, seq, heads, kv_heads, head_dim, max_len, (int)std::min<int64_t>(cus, 1 << 20));
 }
 
 int gsq_attn_kv8(const void* q, int64_t q_stride, const void* qg, int64_t qg_stride, const uint8_t* k_cache,

@@ -42,6 +42,11 @@ struct E16 {
 // v_exp_f32: 2^x to one ulp (results below the normal range are 0)
 __device__ __forceinline__ float exp2_raw(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// 1 / (1 + e^-x) from the hardware's power of two and reciprocal, to a few ulps of float32
+__device__ __forceinline__ float sigmoid_raw(float x) {
+  return __builtin_amdgcn_rcpf(1.f + exp2_raw(x * -1.44269504088896340736f));
+}
+
 // True (uniformly) if row bb's new tokens do not all lie inside the cache, or its tree names a parent
 // that is not an earlier token: its outputs are then NaN and its cache rows are left alone.
 // Called by whole waves.
@@ -269,12 +274,12 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8ReadArgs a) {
 //    another output tile, and two rows give a pair of one tile's operand by one v_perm.
 //  * The reference of the exponent moves only when a score passes it by 2^kLazy, for all rows of the
 //    wave at once: mostly no rescaling and no exchange between lanes in the loop.
-//  * A weight (probability times V scale, 2^kPScale over the largest V scale met) is at most 2^(2 kLazy +
+//  * A weight (probability times V scale, 2^kPScale over the largest V scale met) is at most 2^(kLazy + 3 +
 //    kPScale) = 2^15 and held in fp16: for bf16 outputs in one value (11 bits, eight times finer than the
 //    output's own rounding), for fp16 outputs in two (22 bits, down to 2^-25 of the unit), as one would
 //    add an error as large as the output's rounding.
-constexpr float kLazy = 3.f;
-constexpr float kPScale = 9.f;
+constexpr float kLazy = 6.f;
+constexpr float kPScale = 6.f;
 constexpr int kBiasBlocks = 32;  // blocks between two subtractions of 128 times the weights
 
 __device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c) {
@@ -288,14 +293,26 @@ __device__ __forceinline__ int anew(int v) {
   return v;
 }
 
+// A selector of v_perm in a scalar register: the compiler would keep a vector register for each.
+__device__ __forceinline__ uint32_t scalar(uint32_t v) {
+  asm("" : "+s"(v));
+  return v;
+}
+
+// a value that is the same in every lane, in a scalar register
+__device__ __forceinline__ float uniform(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
+}
+
 // eight bytes as an operand of u 2^-24
 __device__ __forceinline__ u32x4 bytes8(uint32_t w0, uint32_t w1) {
-  return (u32x4){__builtin_amdgcn_perm(0, w0, 0x0C010C00), __builtin_amdgcn_perm(0, w0, 0x0C030C02),
-                 __builtin_amdgcn_perm(0, w1, 0x0C010C00), __builtin_amdgcn_perm(0, w1, 0x0C030C02)};
+  const uint32_t lo = scalar(0x0C010C00u), hi = scalar(0x0C030C02u);
+  return (u32x4){__builtin_amdgcn_perm(0, w0, lo), __builtin_amdgcn_perm(0, w0, hi), __builtin_amdgcn_perm(0, w1, lo),
+                 __builtin_amdgcn_perm(0, w1, hi)};
 }
 // byte i of two dwords as a pair
 __device__ __forceinline__ uint32_t byte_pair(uint32_t second, uint32_t first, int i) {
-  return __builtin_amdgcn_perm(second, first, 0x0C000C00u | (uint32_t)((4 + i) << 16) | (uint32_t)i);
+  return __builtin_amdgcn_perm(second, first, scalar(0x0C000C00u | (uint32_t)((4 + i) << 16) | (uint32_t)i));
 }
 
 // blocks of 32 positions that rows up to token t see
@@ -393,20 +410,19 @@ __device__ __forceinline__ void kv8_stage_q(const Kv8AttnArgs& a, const Kv8Task<
 template <bool BF, int HD, int NT>
 struct Kv8Rows {
   static constexpr int VB = HD / 16, TERMS = BF ? 1 : 2;  // output tiles; fp16 values that hold a weight
-  float rowc[NT], bias[NT], m[NT], l[NT];
+  float rowc[NT], m[NT], l[NT];
   bool unset[NT];  // the row has seen no position yet: m is 0
   bool pending;    // some row of the wave is unset
   float vref, vunit;  // largest V scale met (the weights' unit), and 2^kPScale over it
   f32x4 acc[NT][VB], wsum[NT];  // wsum: 128 times the weights, in acc's unit
 
-  __device__ void init(const float* rowc_s, const float* bias_s) {
+  __device__ void init(const float* rowc_s) {
     pending = true;
     vref = 0x1p-100f;
-    vunit = exp2_raw(kPScale + 100.f);
+    vunit = 0x1p106f;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       rowc[n] = rowc_s[16 * n];
-      bias[n] = bias_s[16 * n];
       m[n] = l[n] = 0.f;
       unset[n] = true;
       wsum[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -429,8 +445,8 @@ struct Kv8Rows {
 #pragma unroll
       for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o, 64));
       const float f = vref / x;
-      vref = x;
-      vunit = exp2_raw(kPScale) / x;
+      vref = uniform(x);
+      vunit = uniform(exp2_raw(kPScale) / x);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         wsum[n] *= f;
@@ -444,7 +460,7 @@ struct Kv8Rows {
   // scores s of a block from position j0 on to weights pf; ks4, vs4: scales() of this lane's positions; rows
   // r0 + lane % 16 + 16 n; masked: some position may lie behind a row's token, or off its path
   template <int RT>
-  __device__ void weights(const Kv8AttnArgs& a, const Kv8Task<RT>& k, int r0, int64_t j0, bool masked, uint64_t paths,
+  __device__ void weights(const Kv8AttnArgs& a, const Kv8Task<RT>& k, int r0, int64_t j0, bool masked, const uint64_t* paths,
                           f32x4 (&s)[NT][2], const f32x4 (&ks4)[2], const f32x4 (&vs4)[2], u32x4 (&pf)[TERMS][NT]) {
     const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
 #pragma unroll
@@ -460,7 +476,7 @@ struct Kv8Rows {
       for (int n = 0; n < NT; ++n) {
         const int tok = min(r0 + 16 * n + c, k.R - 1) / k.rep;
         uint64_t path = 0;
-        if (k.parents) path = __shfl((uint32_t)paths, tok, 64) | ((uint64_t)__shfl((uint32_t)(paths >> 32), tok, 64) << 32);
+        if (k.parents) path = paths[tok];
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -565,7 +581,7 @@ __device__ __forceinline__ void kv8_out(const uint16_t* gate, uint16_t* out, con
     const uint16_t gv[4] = {(uint16_t)gw.x, (uint16_t)(gw.x >> 16), (uint16_t)gw.y, (uint16_t)(gw.y >> 16)};
     uint32_t q[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) q[e] = E::mk(o[i + e] * inv * (1.f / (1.f + expf(-E::ld(gv[e])))));
+    for (int e = 0; e < 4; ++e) q[e] = E::mk(o[i + e] * inv * sigmoid_raw(E::ld(gv[e])));
     *reinterpret_cast<uint2*>(out + i) = make_uint2(q[0] | (q[1] << 16), q[2] | (q[3] << 16));
   }
 }
@@ -622,14 +638,16 @@ __global__ void __launch_bounds__(256, 2) attn_kv8_rows_kernel(Kv8AttnArgs a) {
     load_v(blk);
     load_s(blk);
   }
+  __shared__ uint64_t paths[64];
+  if (k.parents && wave == 0) paths[lane] = tree_path(k.parents, a.S);
   kv8_stage_q<BF, HD>(a, k, qs, rowc_s, bias_s);
   __syncthreads();
   u32x4 qf[KS];
 #pragma unroll
   for (int s = 0; s < KS; ++s) qf[s] = qs[s * 64 + lane];
   Kv8Rows<BF, HD, 1> rows;
-  rows.init(rowc_s + c, bias_s + c);
-  const uint64_t paths = k.parents ? tree_path(k.parents, a.S) : 0;
+  rows.init(rowc_s + c);
+  const float bias = bias_s[c];
   for (int it = 1; blk < k.blk1; blk += 4, ++it) {
     const bool more = blk + 4 < k.blk1;
     // scales of the block's positions to the lanes that hold them (the wave's LDS operations are in order)
@@ -651,7 +669,7 @@ __global__ void __launch_bounds__(256, 2) attn_kv8_rows_kernel(Kv8AttnArgs a) {
     f32x4 s[1][2];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      s[0][b] = (f32x4){rows.bias[0], rows.bias[0], rows.bias[0], rows.bias[0]};
+      s[0][b] = (f32x4){bias, bias, bias, bias};
 #pragma unroll
       for (int st = 0; st < KS; ++st)
         s[0][b] = mma16(bytes8(kr[b][st >> 1][2 * (st & 1)], kr[b][st >> 1][2 * (st & 1) + 1]), qf[st], s[0][b]);
@@ -710,7 +728,7 @@ __global__ void __launch_bounds__(256, 2) attn_kv8_rows_kernel(Kv8AttnArgs a) {
 }
 
 // steps of a wave's queries that attn_kv8_tile_kernel reads from LDS
-constexpr int kv8_lds_steps(int hd, int nt) { return hd == 256 ? 1 : (hd == 128 && nt == 4 ? 2 : 0); }
+constexpr int kv8_lds_steps(int hd) { return hd == 256 ? 1 : 0; }
 
 // Many rows: 16 NT a wave, four waves to a workgroup, over tiles of 64 positions whose bytes come to LDS by
 // DMA, a tile ahead (two buffers, one barrier a tile), and are read by every wave: 16 bytes of K or PW of V a
@@ -728,7 +746,7 @@ __global__ void __launch_bounds__(256, 2) attn_kv8_tile_kernel(Kv8AttnArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t kv8_lds[];
   // two buffers of [K tile | V tile | K scales | V scales], then QL steps of the queries, for which there are
   // not enough registers; all queries pass through before the first tile
-  constexpr int BUF = 2 * TB + 512, QL = kv8_lds_steps(HD, NT);
+  constexpr int BUF = 2 * TB + 512, QL = kv8_lds_steps(HD);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, c = lane & 15;
   Kv8Task<RT> k(a);
@@ -740,6 +758,10 @@ __global__ void __launch_bounds__(256, 2) attn_kv8_tile_kernel(Kv8AttnArgs a) {
   const int64_t klast = k.pos + k.tlast;
   u32x4 qf[NT][KS];
   u32x4* const ql = reinterpret_cast<u32x4*>(kv8_lds + 2 * BUF) + wave * NT * QL * 64 + lane;
+  float* const sw = reinterpret_cast<float*>(kv8_lds + 2 * BUF + 4096 * NT * QL) + wave * 128;  // the wave's scales
+  // the rows' biases as the first accumulator of their scores
+  f32x4* const bl = reinterpret_cast<f32x4*>(kv8_lds + 2 * BUF + 4096 * NT * QL + 2048) + wave * NT * 16;
+  uint64_t* const paths = reinterpret_cast<uint64_t*>(kv8_lds + 2 * BUF + 4096 * NT * QL + 2048 + 1024 * NT);  // of a tree
   Kv8Rows<BF, HD, NT> rows;
   {
     u32x4* const qs = reinterpret_cast<u32x4*>(kv8_lds);
@@ -751,8 +773,15 @@ __global__ void __launch_bounds__(256, 2) attn_kv8_tile_kernel(Kv8AttnArgs a) {
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int s = 0; s < KS; ++s) qf[n][s] = qs[((wave * NT + n) * KS + s) * 64 + lane];
-    rows.init(rowc_s + 16 * NT * wave + c, bias_s + 16 * NT * wave + c);
-    __syncthreads();
+    rows.init(rowc_s + 16 * NT * wave + c);
+    float bias[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) bias[n] = bias_s[16 * (NT * wave + n) + c];
+    __syncthreads();  // the buffers, and what lies behind them, may be written
+    if (k.parents && wave == 0) paths[lane] = tree_path(k.parents, a.S);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+      if (g == 0) bl[16 * n + c] = (f32x4){bias[n], bias[n], bias[n], bias[n]};
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -779,9 +808,7 @@ __global__ void __launch_bounds__(256, 2) attn_kv8_tile_kernel(Kv8AttnArgs a) {
       __builtin_amdgcn_global_load_lds((wave ? a.vs : a.ks) + k.base + j0 + (uint32_t)min(ln, left),
                                        (lds_ptr_t)(buf + 2 * TB + wave * 256), 4, 0, 0);
   };
-  const uint64_t paths = k.parents ? tree_path(k.parents, a.S) : 0;
   const int r0 = k.r0 + 16 * NT * wave;
-  float* const sw = reinterpret_cast<float*>(kv8_lds + 2 * BUF + 4096 * NT * QL) + wave * 128;  // the wave's scales
   const int64_t pfirst = k.pos + min(r0, k.R - 1) / k.rep, plast = k.pos + min(r0 + 16 * NT - 1, k.R - 1) / k.rep;
   const bool on = r0 < k.R;
   issue(k.blk0, kv8_lds);
@@ -806,14 +833,11 @@ __global__ void __launch_bounds__(256, 2) attn_kv8_tile_kernel(Kv8AttnArgs a) {
       const uint8_t* const kb = kt + (32 * sb + c) * HD;
       const uint8_t* const vb = kt + TB;
       const float* const sc = sw + 32 * sb + 4 * g;
-      f32x4 ks4[2], vs4[2], s[NT][2];
+      f32x4 s[NT][2];
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        ks4[b] = *reinterpret_cast<const f32x4*>(sc + 16 * b);
-        vs4[b] = *reinterpret_cast<const f32x4*>(sc + 64 + 16 * b);
+      for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) s[n][b] = (f32x4){rows.bias[n], rows.bias[n], rows.bias[n], rows.bias[n]};
-      }
+        for (int n = 0; n < NT; ++n) s[n][b] = bl[16 * n + c];
 #pragma unroll
       for (int st = 0; st < KS / 2; ++st) {
         u32x4 w[2];
@@ -829,6 +853,13 @@ __global__ void __launch_bounds__(256, 2) attn_kv8_tile_kernel(Kv8AttnArgs a) {
             for (int n = 0; n < NT; ++n)
               s[n][b] = mma16(kf, 2 * st + h < QL ? ql[(n * QL + 2 * st + h) * 64] : qf[n][2 * st + h], s[n][b]);
           }
+      }
+      if constexpr (HD == 256) __builtin_amdgcn_sched_barrier(0);  // what follows needs the registers of K's pieces
+      f32x4 ks4[2], vs4[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        ks4[b] = *reinterpret_cast<const f32x4*>(sc + 16 * b);
+        vs4[b] = *reinterpret_cast<const f32x4*>(sc + 64 + 16 * b);
       }
       u32x4 pf[Kv8Rows<BF, HD, NT>::TERMS][NT];
       rows.weights(a, k, r0, j0, k.parents ? j0 + 31 >= k.pos : j0 + 31 > pfirst, paths, s, ks4, vs4, pf);
@@ -953,7 +984,7 @@ __global__ void __launch_bounds__(64 * kMergeWaves) attn_kv8_merge_kernel(Kv8Att
   }
   const float inv = 1.f / l;
 #pragma unroll
-  for (int j = 0; j < V; ++j) out[j] = E::mk(o[j] * inv * (1.f / (1.f + expf(-E::ld(gate[j])))));
+  for (int j = 0; j < V; ++j) out[j] = E::mk(o[j] * inv * sigmoid_raw(E::ld(gate[j])));
 }
 
 // ---- launches ------------------------------------------------------------------------------------
@@ -1016,7 +1047,7 @@ static hipError_t launch_attn_kv8_rows(const Kv8AttnArgs& a, hipStream_t s) {
 
 template <bool BF, int HD, int NT>
 static hipError_t launch_attn_kv8_tile(const Kv8AttnArgs& a, hipStream_t s) {
-  constexpr int q = 64 * NT * (HD * 2 + 8), tiles = 2 * (2 * 64 * HD + 512) + 4096 * NT * kv8_lds_steps(HD, NT) + 2048;
+  constexpr int q = 64 * NT * (HD * 2 + 8), tiles = 2 * (2 * 64 * HD + 512) + 4096 * NT * kv8_lds_steps(HD) + 2560 + 1024 * NT;
   constexpr int lds = q > tiles ? q : tiles;
   return launch_attn_kv8_t<BF, HD>(a, s, 64 * NT, [&](dim3 grid) {
     static LdsLimit limit;
@@ -1026,16 +1057,37 @@ static hipError_t launch_attn_kv8_tile(const Kv8AttnArgs& a, hipStream_t s) {
   });
 }
 
-constexpr int kv8_few_rows = 32;
+// Rows of a workgroup. attn_kv8_rows_kernel (16) has the shorter chain, attn_kv8_tile_kernel takes a third less
+// time for each product: measured per tile of 16 rows and block of 32 positions, all CUs busy, head dim
+// 256, 0.56 against 0.37 us a SIMD; but 13 drafted tokens over 2000 positions 14 us against 33, and a prompt
+// of 333 19 against 46. So the tiles are for work of kTileBlocks and more. Head dim 64 takes 256 rows instead
+// of 128 where that makes two workgroups a CU (4096 tokens of 2 x 32 heads: 326 against 352 us); at 128 the
+// registers do not hold them (521 against 481).
+constexpr int64_t kTileBlocks = 32768;
+
+int attn_kv8_plan(int64_t batch, int64_t seq, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_len) {
+  const int64_t rows = seq * (heads / kv_heads), groups = batch * kv_heads;
+  if (rows <= 32 || (rows + 15) / 16 * groups * ((max_len + 31) / 32) < kTileBlocks) return 16;
+  return head_dim == 64 && (rows + 255) / 256 * groups >= 512 ? 256 : 128;
+}
+
+// Splits that give each of `cus` CUs two workgroups, of at least 256 positions each: below that a split's
+// share of the merge costs more than it saves.
+int64_t attn_kv8_splits(int64_t batch, int64_t seq, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_len,
+                        int cus) {
+  const int rt = attn_kv8_plan(batch, seq, heads, kv_heads, head_dim, max_len);
+  const int64_t wgs = (seq * (heads / kv_heads) + rt - 1) / rt * kv_heads * batch;
+  return std::max<int64_t>(1, std::min<int64_t>({2 * cus / std::max<int64_t>(wgs, 1), max_len / 256, 65535}));
+}
 
 hipError_t launch_attn_kv8(bool bf16, const Kv8AttnArgs& a, hipStream_t s) {
-  const int64_t rows = (int64_t)a.S * (a.H / a.Hkv);
+  const int rt = attn_kv8_plan(a.B, a.S, a.H, a.Hkv, a.hd, a.L);
   auto tiles = [&](auto bf, auto hd) -> hipError_t {
     constexpr bool BF = decltype(bf)::value;
     constexpr int HD = decltype(hd)::value;
-    if (rows <= kv8_few_rows) return launch_attn_kv8_rows<BF, HD>(a, s);
-    if constexpr (HD < 256) {
-      if (rows > 128) return launch_attn_kv8_tile<BF, HD, 4>(a, s);
+    if (rt == 16) return launch_attn_kv8_rows<BF, HD>(a, s);
+    if constexpr (HD == 64) {
+      if (rt == 256) return launch_attn_kv8_tile<BF, HD, 4>(a, s);
     }
     return launch_attn_kv8_tile<BF, HD, 2>(a, s);
   };

@@ -53,6 +53,7 @@ EXPORTS = {
     "gsq_kv8_write": (_I32, [_VP, _I64, _VP, _I64, _VP, _I64, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _I64, _VP, _I64,
                              _VP, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _F32, _I32, _VP]),
     "gsq_kv8_read": (_I32, [_VP, _VP, _VP, _VP, _VP, _VP, _I64, _I64, _I64, _I64, _I64, _I32, _VP]),
+    "gsq_attn_kv8_splits": (_I64, [_I64, _I64, _I64, _I64, _I64, _I64, _I64]),
     "gsq_attn_kv8": (_I32, [_VP, _I64, _VP, _I64, _VP, _VP, _VP, _VP, _VP, _I64, _VP, _I64, _VP, _I64, _VP, _I64, _I64,
                             _I64, _I64, _I64, _I64, _I64, _I32, _VP]),
     "gsq_last_error": (ctypes.c_char_p, []),

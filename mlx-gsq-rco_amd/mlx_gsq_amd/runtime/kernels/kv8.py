@@ -120,23 +120,12 @@ def _device_cus(dev) -> int:
     return n
 
 
-def attn_kv8_tile_rows(rows: int, head_dim: int) -> int:
-    """Rows (tokens x query heads of a KV head) that one workgroup takes: the launch rule of gsq_attn_kv8."""
-    return 16 if rows <= 32 else (128 if head_dim == 256 or rows <= 128 else 256)
-
-
-def attn_kv8_splits(workgroups: int, max_len: int, cus: int) -> int:
-    """Workgroups that share the positions of one tile of rows: as many as give every CU two, of at least
-    256 positions each."""
-    return max(1, min(2 * cus // max(1, workgroups), max_len // 256))
-
-
 def attn_kv8(q, qg, k_cache, v_cache, k_scale, v_scale, pos, *, heads: int, kv_heads: int, head_dim: int, parents=None,
              splits=None):
     """Gated grouped-query attention of the S tokens that ``kv8_write`` has written: q its queries (B, S,
     heads * head_dim), qg the [q | gate] rows it read. Token t attends to positions 0 .. pos + t; in a
     tree to those before ``pos``, its ancestors and itself. ``splits``: workgroups that share the positions
-    of one tile of rows (default: ``attn_kv8_splits``). Returns (B, S, heads * head_dim)."""
+    of one tile of rows (default: as many as fill the device). Returns (B, S, heads * head_dim)."""
     dev = _on_gpu(q, qg, k_cache, v_cache, k_scale, v_scale, pos, *(() if parents is None else (parents,)))
     _caches(k_cache, v_cache, k_scale, v_scale)
     B, S = q.shape[:2]
@@ -148,8 +137,7 @@ def attn_kv8(q, qg, k_cache, v_cache, k_scale, v_scale, pos, *, heads: int, kv_h
         raise ValueError("attention tensor shapes do not match the head configuration")
     out = torch.empty(B, S, heads * head_dim, dtype=q.dtype, device=dev)
     if splits is None:
-        rows = S * (heads // max(1, kv_heads))
-        splits = attn_kv8_splits(B * kv_heads * -(-rows // attn_kv8_tile_rows(rows, head_dim)), L, _device_cus(dev))
+        splits = _lib.lib().gsq_attn_kv8_splits(B, S, heads, kv_heads, head_dim, L, _device_cus(dev))
     work = None
     if splits > 1:
         work = torch.empty(B * heads * S * splits * (head_dim + 2), dtype=torch.float32, device=dev)

@@ -106,9 +106,15 @@ def test_tensor_checks():
 
 
 def test_splits_rule():
-    from mlx_gsq_amd.runtime.kernels.kv8 import attn_kv8_splits
-    assert attn_kv8_splits(4, 100, 256) == 1 and attn_kv8_splits(10 ** 6, 10 ** 6, 256) == 1
-    for wg in (1, 4, 100, 511):
-        for L in (1, 511, 512, 4096, 131072, 10 ** 6):
-            n = attn_kv8_splits(wg, L, 256)
-            assert 1 <= n <= 65535 and (n == 1 or (n * wg <= 512 and n * 256 <= L))
+    splits = _lib().lib().gsq_attn_kv8_splits
+    assert splits(1, 1, 24, 4, 256, 300, 256) == 1 and splits(1, 4096, 24, 4, 256, 4096, 256) == 1
+    assert splits(1, 1, 24, 4, 256, 131072, 256) == 128
+    for B, S, H, G, hd in ((1, 1, 24, 4, 256), (3, 64, 24, 4, 256), (1, 700, 32, 8, 128), (200, 1, 8, 8, 64), (1, 1, 1, 1, 64)):
+        for L in (S, S + 511, 4096, 131072, 10 ** 6):
+            n = splits(B, S, H, G, hd, L, 256)
+            assert 1 <= n <= 65535 and (n == 1 or n * 256 <= L)
+            rows = -(-S * (H // G) // 256) * G * B  # workgroups, at the least
+            assert n == 1 or n * rows <= 512
+    for bad in ((0, 1, 4, 1, 64, 8, 256), (1, 0, 4, 1, 64, 8, 256), (1, 1, 4, 0, 64, 8, 256), (1, 1, 4, 1, 64, 0, 256),
+                (1, 1, 4, 1, 64, 8, 0)):
+        assert splits(*bad) == 1
