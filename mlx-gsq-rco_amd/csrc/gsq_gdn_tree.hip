@@ -24,32 +24,76 @@ namespace gsq {
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kTreeConv = 8;  // largest convolution kernel
+constexpr int kTreeRows = 4;  // q or k rows of a wave whose inputs are in flight together
 
 __device__ __forceinline__ f32x4 mma4(float a, float b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
+__device__ __forceinline__ f32x4 mma16(f16x8 a, f16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// the value of lane 16 Q + lane % 16
+template <int Q>
+__device__ __forceinline__ float from_row(float v) {
+  const uint32_t x = __builtin_bit_cast(uint32_t, v);
+  const auto h = __builtin_amdgcn_permlane32_swap(x, x, false, false);  // rows 0 1 0 1, and 2 3 2 3
+  const uint32_t y = h[Q >> 1];
+  const auto r = __builtin_amdgcn_permlane16_swap(y, y, false, false);  // the even one four times, and the odd one
+  return __builtin_bit_cast(float, (uint32_t)r[Q & 1]);
+}
+
+// sum over the wave, in every lane: without LDS (the shuffles' round trips are what a row's norm waits for)
+__device__ __forceinline__ float lanes_sum(float v) {
+  auto dpp = [](float x, auto ctrl) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value,
+                                                                 0xF, 0xF, false));
+  };
+  v += dpp(v, std::integral_constant<int, 0xB1>{});   // quad_perm [1,0,3,2]
+  v += dpp(v, std::integral_constant<int, 0x4E>{});   // quad_perm [2,3,0,1]
+  v += dpp(v, std::integral_constant<int, 0x141>{});  // row_half_mirror
+  v += dpp(v, std::integral_constant<int, 0x140>{});  // row_mirror
+  uint32_t x = __builtin_bit_cast(uint32_t, v);
+  const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  v = __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+  x = __builtin_bit_cast(uint32_t, v);
+  const auto h = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return __builtin_bit_cast(float, (uint32_t)h[0]) + __builtin_bit_cast(float, (uint32_t)h[1]);
+}
+
+// x / (1 + e^-x) and 1 / sqrt(x) from the hardware's power of two, reciprocal and square root: a few ulps of float32
+__device__ __forceinline__ float silu_raw(float x) {
+  return x * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -1.44269504088896340736f));
+}
+__device__ __forceinline__ float rsqrt_raw(float x) { return __builtin_amdgcn_rsqf(x); }
+
 }  // namespace
 
 // One workgroup per (value head, batch row), a wave per 16 state columns, tokens in NI tiles of 16 rows.
-// All products are float32 MFMAs (16 x 16 x 4): for A a lane gives row lane % 16, for B and the result
-// column lane % 16; a product's step e takes dims 4 (lane / 16) + e, so operands are 16-byte pieces,
-// and a result (rows 4 (lane / 16) + e on its registers) is the B operand of the next product as it is.
+// Products that sum over the key dims take their float32 factors as two fp16 numbers each (hi + lo, 22 bits;
+// q and k before their constant factor, state columns over a power of two, so that both are of size 1 and
+// lo x lo, 2^-24 of the product, can go): three MFMAs of 32 dims in 48 cycles where float32 ones take 256. What
+// sums over tokens stays in float32 MFMAs (16 x 16 x 4): for A a lane gives row lane % 16, for B and the
+// result column lane % 16; step e takes rows 4 (lane / 16) + e, so that operands are 16-byte pieces and a
+// result is the B operand of the next product as it is.
 //  * q and k (convolution, SiLU, norm) go to LDS, a wave per row; v is formed where the system needs it;
 //  * tiles of k k^T and q k^T are shared out over the waves, weighted and masked into LDS;
 //  * each wave solves for its columns tile by tile: earlier tiles by MFMA, the 16 rows of a tile in turn;
 //  * outputs meet in LDS for the gated norm over the head.
-// A token whose u is not finite is taken out of the sums and its column's paths through it set to NaN:
+// A token whose u is not finite is taken out of the products and its column's paths through it set to NaN:
 // 0 x NaN would reach tokens that do not follow it.
-template <int DT, int DKP, int NI>
-__global__ void __launch_bounds__(1024) gdn_tree_kernel(GdnTreeArgs a) {
+template <int DT, int DKP, int NI, int TH>
+__global__ void __launch_bounds__(TH) gdn_tree_kernel(GdnTreeArgs a, bool pair) {
   using E = Elem<DT>;
   using T = typename E::T;
-  constexpr int QS = DKP + 4, MS = 16 * NI + 4, R = 16 * NI;  // LDS row strides, padded against bank conflicts
+  constexpr int QS = DKP + 8, MS = 16 * NI + 4, R = 16 * NI;  // LDS row strides, padded against bank conflicts
   extern __shared__ __attribute__((aligned(16))) float tree_lds[];
-  float* const kq = tree_lds;               // k rows, then q rows: [2][R][QS]; outputs [R][dv + 4] afterwards
+  // k rows, then q rows, hi then lo: [2][2 R][QS] of fp16; outputs [R][dv + 4] afterwards
+  _Float16* const kq = reinterpret_cast<_Float16*>(tree_lds);
   const int dv = a.dv, out_s = dv + 4;
   const int kq_size = 2 * R * QS > R * out_s ? 2 * R * QS : R * out_s;
   float* const mk = tree_lds + kq_size;     // weights of u_j in u_i, [j][i] (transposed)
@@ -59,6 +103,7 @@ __global__ void __launch_bounds__(1024) gdn_tree_kernel(GdnTreeArgs a) {
   float* const betas = grown + R;
   double* const logs = reinterpret_cast<double*>(betas + R);      // log G_i
   uint64_t* const paths = reinterpret_cast<uint64_t*>(logs + R);  // token i and its ancestors
+  const T** const where = reinterpret_cast<const T**>(paths + R);  // input i of token t's window: [kTreeConv][R], newest first
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), nw = blockDim.x >> 6;
   const int g = lane >> 4, c = lane & 15;
   const int h = blockIdx.x, bb = blockIdx.y, Hk = a.Hk, Hv = a.Hv, dk = a.dk, K = a.K, S = a.S, kh = h % Hk;
@@ -73,30 +118,130 @@ __global__ void __launch_bounds__(1024) gdn_tree_kernel(GdnTreeArgs a) {
   const T* const qkv = static_cast<const T*>(a.qkv) + (int64_t)bb * S * a.qkv_stride;
   const T* const cst = static_cast<const T*>(a.conv) + (int64_t)bb * (K - 1) * conv_dim;
 
-  // this wave's columns of the state: dims 16 s + 4 g + e of column 16 wave + c
-  float st[DKP / 4];
+  // this wave's columns of the state: dims 32 s + 8 g + j of column 16 wave + c
+  float sf[DKP / 32][8];
   {
     const float* Sp = a.rec + ((int64_t)bb * Hv + h) * dk * dv + 16 * wave + c;
 #pragma unroll
-    for (int s = 0; s < DKP / 16; ++s)
+    for (int s = 0; s < DKP / 32; ++s)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int d = 16 * s + 4 * g + e;
-        st[4 * s + e] = d < dk ? Sp[(int64_t)d * dv] : 0.f;
+      for (int j = 0; j < 8; ++j) {
+        const int d = 32 * s + 8 * g + j;
+        sf[s][j] = d < dk ? Sp[(int64_t)d * dv] : 0.f;
       }
   }
-  // paths, decays and beta of the tokens: lane i of the first wave
+  // a and b of the tokens: lane i of the first wave
+  float av = 0.f, bv = 0.f;
+  if (wave == 0 && lane < S) {
+    const T* abr = static_cast<const T*>(a.ab) + ((int64_t)bb * S + lane) * a.ab_stride;
+    av = E::ld(abr + h) + a.dt_bias[h];
+    bv = E::ld(abr + Hv + h);
+  }
+  // windows: lane t finds the rows that hold the inputs of token t, newest first (tokens past the last: the last's);
+  // negative: the state's rows, -1 its last
+  const T* in_at[kTreeConv];
+  {
+    int p = min(lane, S - 1);
+#pragma unroll
+    for (int i = 0; i < kTreeConv; ++i) {
+      in_at[i] = p >= 0 ? qkv + (int64_t)p * a.qkv_stride : cst + (int64_t)max(K - 1 + p, 0) * conv_dim;
+      if (i % nw == wave && lane < R) where[i * R + lane] = in_at[i];
+      const int up = __shfl(par, max(p, 0), 64);
+      p = p >= 0 ? up : p - 1;
+    }
+  }
+  auto row_of = [&](const T* p, int t) {  // lane t's
+    const uint64_t x = reinterpret_cast<uint64_t>(p);
+    return reinterpret_cast<const T*>((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)x, t) |
+                                      ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), t) << 32));
+  };
+  __syncthreads();  // the windows
+  // v of rows 16 i + 4 g + e, this lane's column; the first tile's inputs come while q and k are formed
+  const int vch = 2 * key_dim + h * dv + 16 * wave + c;
+  float vw[kTreeConv];
+  T vin[4][kTreeConv];
+  auto load_v = [&](int i) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int j = 0; j < kTreeConv; ++j)
+        if (j < K) vin[e][j] = where[j * R + 16 * i + 4 * g + e][vch];
+  };
+#pragma unroll
+  for (int i = 0; i < kTreeConv; ++i) vw[i] = i < K ? E::ld(static_cast<const T*>(a.conv_w) + (int64_t)vch * K + K - 1 - i) : 0.f;
+  load_v(0);
+  // q and k rows: half of the waves each, two channels a lane, kTreeRows rows' inputs in flight
+  {
+    const bool isq = wave >= nw / 2;
+    const int w0 = isq ? wave - nw / 2 : wave, ws = isq ? nw - nw / 2 : nw / 2, c0 = 2 * lane;
+    const bool on = c0 < dk;
+    const int ch = (isq ? 0 : key_dim) + kh * dk + min(c0, dk - 2);
+    const T* const cw = static_cast<const T*>(a.conv_w) + (int64_t)ch * K;
+    float wa[kTreeConv], wb[kTreeConv];
+#pragma unroll
+    for (int i = 0; i < kTreeConv; ++i) {
+      wa[i] = i < K ? E::ld(cw + K - 1 - i) : 0.f;
+      wb[i] = i < K ? E::ld(cw + 2 * K - 1 - i) : 0.f;
+    }
+    const float dki = 1.f / (float)dk;
+    _Float16* const dst = kq + (isq ? R * QS : 0);
+    for (int t0 = w0; t0 < R; t0 += kTreeRows * ws) {
+      struct alignas(2 * sizeof(T)) P { T e[2]; } in[kTreeRows][kTreeConv];
+#pragma unroll
+      for (int u = 0; u < kTreeRows; ++u)
+#pragma unroll
+        for (int i = 0; i < kTreeConv; ++i)
+          if (i < K) {
+            const T* const p = row_of(in_at[i], min(t0 + u * ws, S - 1)) + ch;
+            if (pair) {
+              in[u][i] = *reinterpret_cast<const P*>(p);
+            } else {
+              in[u][i].e[0] = p[0];
+              in[u][i].e[1] = p[1];
+            }
+          }
+#pragma unroll
+      for (int u = 0; u < kTreeRows; ++u) {
+        const int t = t0 + u * ws;
+        float x = 0.f, y = 0.f;
+#pragma unroll
+        for (int i = kTreeConv - 1; i >= 0; --i)
+          if (i < K) {
+            x += E::ld(&in[u][i].e[0]) * wa[i];
+            y += E::ld(&in[u][i].e[1]) * wb[i];
+          }
+        x = silu_raw(x);
+        y = silu_raw(y);
+        const float rn = rsqrt_raw(lanes_sum(on ? x * x + y * y : 0.f) * dki + 1e-6f);
+        x = on && t < S ? x * rn : 0.f;
+        y = on && t < S ? y * rn : 0.f;
+        if (c0 < DKP && t < R) {
+          const struct alignas(4) H { _Float16 e[2]; } hi = {{(_Float16)x, (_Float16)y}},
+              lo = {{(_Float16)(x - (float)hi.e[0]), (_Float16)(y - (float)hi.e[1])}};
+          *reinterpret_cast<H*>(dst + t * QS + c0) = hi;
+          *reinterpret_cast<H*>(dst + (2 * R + t) * QS + c0) = lo;
+        }
+      }
+    }
+  }
+  f32x4 u[NI];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    if (i) load_v(i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float x = 0.f;
+#pragma unroll
+      for (int j = kTreeConv - 1; j >= 0; --j)
+        if (j < K) x += E::ld(&vin[e][j]) * vw[j];
+      u[i][e] = 16 * i + 4 * g + e < S ? silu_raw(x) : 0.f;
+    }
+  }
+  // paths, decays and beta of the tokens
   if (wave == 0) {
     uint32_t lo = lane < 32 ? 1u << lane : 0u, hi = lane < 32 ? 0u : 1u << (lane - 32);
-    double lg = 0.0;
-    float beta = 0.f;
-    if (lane < S) {
-      const T* abr = static_cast<const T*>(a.ab) + ((int64_t)bb * S + lane) * a.ab_stride;
-      const float av = E::ld(abr + h) + a.dt_bias[h];
-      const float sp = av > 20.f ? av : log1pf(expf(av));  // softplus (torch's threshold 20)
-      lg = (double)(a.ssm_a[h] * sp);
-      beta = 1.f / (1.f + expf(-E::ld(abr + Hv + h)));
-    }
+    const float sp = av > 20.f ? av : log1pf(expf(av));  // softplus (torch's threshold 20)
+    double lg = lane < S ? (double)(a.ssm_a[h] * sp) : 0.0;
     int p = par;
 #pragma unroll
     for (int i = 0; i < 6; ++i) {  // pointer doubling: what p's path so far holds joins
@@ -112,100 +257,28 @@ __global__ void __launch_bounds__(1024) gdn_tree_kernel(GdnTreeArgs a) {
       paths[lane] = lane < S ? lo | ((uint64_t)hi << 32) : 0;
       logs[lane] = lg;
       grown[lane] = (float)exp(lg);
-      betas[lane] = beta;
+      betas[lane] = lane < S ? 1.f / (1.f + expf(-bv)) : 0.f;
     }
-  }
-  // window of token t (uniform): rows of the inputs, negative ones from the state; newest last
-  auto window = [&](int t, int (&at)[kTreeConv]) {
-    int p = t;
-#pragma unroll
-    for (int i = kTreeConv - 1; i >= 0; --i) {
-      at[i] = p;
-      p = p >= 0 ? parents[p] : p - 1;
-    }
-  };
-  auto input = [&](int p, int ch) {  // input p of a channel
-    return p >= 0 ? E::ld(qkv + (int64_t)p * a.qkv_stride + ch) : E::ld(cst + (int64_t)max(K - 1 + p, 0) * conv_dim + ch);
-  };
-  // q and k rows: half of the waves each, two channels a lane
-  {
-    const bool isq = wave >= nw / 2;
-    const int w0 = isq ? wave - nw / 2 : wave, ws = isq ? nw - nw / 2 : nw / 2, c0 = 2 * lane;
-    const bool on = c0 < dk;
-    const int ch = (isq ? 0 : key_dim) + kh * dk + min(c0, dk - 2);
-    const T* const cw = static_cast<const T*>(a.conv_w) + (int64_t)ch * K;
-    float wa[kTreeConv], wb[kTreeConv];
-#pragma unroll
-    for (int i = 0; i < kTreeConv; ++i) {
-      const int j = i - (kTreeConv - K);
-      wa[i] = j >= 0 ? E::ld(cw + j) : 0.f;
-      wb[i] = j >= 0 ? E::ld(cw + K + j) : 0.f;
-    }
-    const float sc = isq ? 1.f / (float)dk : 1.f / sqrtf((float)dk);
-    float* const dst = kq + (isq ? R * QS : 0);
-    for (int t = w0; t < R; t += ws) {
-      float x = 0.f, y = 0.f;
-      if (t < S) {
-        int at[kTreeConv];
-        window(t, at);
-#pragma unroll
-        for (int i = 0; i < kTreeConv; ++i)
-          if (i >= kTreeConv - K) {
-            x += input(at[i], ch) * wa[i];
-            y += input(at[i], ch + 1) * wb[i];
-          }
-        x = silu_f(x);
-        y = silu_f(y);
-        const float rn = 1.f / sqrtf(wave_sum(on ? x * x + y * y : 0.f) / (float)dk + 1e-6f) * sc;
-        x *= rn;
-        y *= rn;
-      }
-      if (c0 < DKP) *reinterpret_cast<float2*>(dst + t * QS + c0) = on && t < S ? make_float2(x, y) : make_float2(0.f, 0.f);
-    }
-  }
-  // v of rows 16 i + 4 g + e, this lane's column
-  f32x4 u[NI];
-  {
-    const int ch = 2 * key_dim + h * dv + 16 * wave + c;
-    const T* const cw = static_cast<const T*>(a.conv_w) + (int64_t)ch * K;
-    float w[kTreeConv];
-#pragma unroll
-    for (int i = 0; i < kTreeConv; ++i) {
-      const int j = i - (kTreeConv - K);
-      w[i] = j >= 0 ? E::ld(cw + j) : 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < NI; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int t = 16 * i + 4 * g + e;
-        float x = 0.f;
-        if (t < S) {
-          int at[kTreeConv];
-          window(t, at);
-#pragma unroll
-          for (int j = 0; j < kTreeConv; ++j)
-            if (j >= kTreeConv - K) x += input(at[j], ch) * w[j];
-          x = silu_f(x);
-        }
-        u[i][e] = x;
-      }
   }
   __syncthreads();
+  const float qscale = 1.f / (float)dk, kscale = 1.f / sqrtf((float)dk);
   // tiles (i, j <= i) of k k^T and q k^T
   for (int n = wave; n < NI * (NI + 1); n += nw) {
     const bool isq = n & 1;
     int i = 0, j = n >> 1;
     while (j > i) j -= ++i;
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
-    const float* const ra = kq + (isq ? R * QS : 0) + (16 * i + c) * QS + 4 * g;
-    const float* const rb = kq + (16 * j + c) * QS + 4 * g;
+    const _Float16* const ra = kq + ((isq ? R : 0) + 16 * i + c) * QS + 8 * g;
+    const _Float16* const rb = kq + (16 * j + c) * QS + 8 * g;
 #pragma unroll
-    for (int d = 0; d < DKP; d += 16) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(ra + d), y = *reinterpret_cast<const f32x4*>(rb + d);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s = mma4(x[e], y[e], s);
+    for (int d = 0; d < DKP; d += 32) {
+      const f16x8 xh = *reinterpret_cast<const f16x8*>(ra + d), xl = *reinterpret_cast<const f16x8*>(ra + 2 * R * QS + d);
+      const f16x8 yh = *reinterpret_cast<const f16x8*>(rb + d), yl = *reinterpret_cast<const f16x8*>(rb + 2 * R * QS + d);
+      s = mma16(xh, yh, s);
+      s = mma16(xh, yl, s);
+      s = mma16(xl, yh, s);
     }
+    s *= isq ? qscale * kscale : kscale * kscale;
     const int tj = 16 * j + c;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {  // row 16 i + 4 g + e, column tj
@@ -222,20 +295,40 @@ __global__ void __launch_bounds__(1024) gdn_tree_kernel(GdnTreeArgs a) {
     }
   }
   // products with the state
+  f16x8 sh[DKP / 32], sl[DKP / 32];
+  float mx = 0.f;
+#pragma unroll
+  for (int s = 0; s < DKP / 32; ++s)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) mx = fmaxf(mx, fabsf(sf[s][j]));
+  mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+  mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+  const int ex = mx > 0.f && mx <= FLT_MAX ? -ilogbf(mx) : 0;  // the column's largest: 1 .. 2
+#pragma unroll
+  for (int s = 0; s < DKP / 32; ++s)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float x = ldexpf(sf[s][j], ex);
+      sh[s][j] = (_Float16)x;
+      sl[s][j] = (_Float16)(x - (float)sh[s][j]);
+    }
+  const float ks_ = ldexpf(kscale, -ex), qs_ = ldexpf(qscale, -ex);
   f32x4 o[NI];
-  auto with_state = [&](const float* rows) {
+  auto with_state = [&](const _Float16* rows) {
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int d = 0; d < DKP / 16; ++d) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(rows + c * QS + 4 * g + 16 * d);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s = mma4(x[e], st[4 * d + e], s);
+    for (int d = 0; d < DKP / 32; ++d) {
+      const f16x8 xh = *reinterpret_cast<const f16x8*>(rows + c * QS + 8 * g + 32 * d);
+      const f16x8 xl = *reinterpret_cast<const f16x8*>(rows + (2 * R + c) * QS + 8 * g + 32 * d);
+      s = mma16(xh, sh[d], s);
+      s = mma16(xh, sl[d], s);
+      s = mma16(xl, sh[d], s);
     }
     return s;
   };
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
-    const f32x4 ks = with_state(kq + 16 * i * QS), qs = with_state(kq + (R + 16 * i) * QS);
+    const f32x4 ks = with_state(kq + 16 * i * QS) * ks_, qs = with_state(kq + (R + 16 * i) * QS) * qs_;
     const f32x4 gr = *reinterpret_cast<const f32x4*>(grown + 16 * i + 4 * g);
     const f32x4 be = *reinterpret_cast<const f32x4*>(betas + 16 * i + 4 * g);
     u[i] = be * (u[i] - gr * ks);
@@ -251,31 +344,43 @@ __global__ void __launch_bounds__(1024) gdn_tree_kernel(GdnTreeArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) u[i] = mma4(-w[e], u[j][e], u[i]);
     }
-    // the tile's rows in turn: row r is final, its share leaves the rows after it
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int t = 16 * i + r;
-      float x = __shfl(u[i][r & 3], 16 * (r >> 2) + c, 64);
-      const bool off = !(fabsf(x) <= FLT_MAX) || (paths[t] & bad);
-      if (off) {
-        bad |= 1ull << t;
-        x = 0.f;
-      }
-      if (g == (r >> 2)) u[i][r & 3] = x;
-      const f32x4 w = *reinterpret_cast<const f32x4*>(mk + t * MS + 16 * i + 4 * g);
+    if (i && __any(bad != 0))
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (4 * g + e > r) u[i][e] -= x == 0.f ? 0.f : w[e] * x;
+        if (paths[16 * i + 4 * g + e] & bad) u[i][e] = __builtin_nanf("");
+    // the tile's rows in turn: row r is final, its share leaves the rows that follow it (the others' weight is 0)
+    f32x4 w[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) w[r] = *reinterpret_cast<const f32x4*>(mk + (16 * i + r) * MS + 16 * i + 4 * g);
+#pragma unroll
+    for (int r = 0; r < 15; ++r) {
+      const float ur = u[i][r & 3];
+      const float x = r < 4 ? from_row<0>(ur) : (r < 8 ? from_row<1>(ur) : (r < 12 ? from_row<2>(ur) : from_row<3>(ur)));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) u[i][e] = w[r][e] == 0.f ? u[i][e] : __builtin_fmaf(-w[r][e], x, u[i][e]);
+    }
+    // what is not finite stays out of the products, and marks the tokens that follow it
+    uint32_t off = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (!(fabsf(u[i][e]) <= FLT_MAX)) {
+        off |= 1u << (4 * g + e);
+        u[i][e] = 0.f;
+      }
+    if (__any(off != 0)) {
+      off |= __shfl_xor(off, 16, 64);
+      off |= __shfl_xor(off, 32, 64);
+      bad |= (uint64_t)off << (16 * i);
     }
 #pragma unroll
     for (int j = 0; j <= i; ++j) {
-      const f32x4 w = *reinterpret_cast<const f32x4*>(mq + (16 * i + c) * MS + 16 * j + 4 * g);
+      const f32x4 wq = *reinterpret_cast<const f32x4*>(mq + (16 * i + c) * MS + 16 * j + 4 * g);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[i] = mma4(w[e], u[j][e], o[i]);
+      for (int e = 0; e < 4; ++e) o[i] = mma4(wq[e], u[j][e], o[i]);
     }
   }
   // outputs to LDS (q and k are no longer read), then a wave per row: gated norm over the head
-  float* const os = kq;
+  float* const os = tree_lds;
 #pragma unroll
   for (int i = 0; i < NI; ++i)
 #pragma unroll
@@ -284,45 +389,62 @@ __global__ void __launch_bounds__(1024) gdn_tree_kernel(GdnTreeArgs a) {
       os[t * out_s + 16 * wave + c] = paths[t] & bad ? __builtin_nanf("") : o[i][e];
     }
   __syncthreads();
-  const T* const nw_ = static_cast<const T*>(a.norm_w);
-  for (int t = wave; t < S; t += nw) {
-    const T* z = static_cast<const T*>(a.z) + ((int64_t)bb * S + t) * a.z_stride + (int64_t)h * dv;
-    float x[4], ss = 0.f;
+  const float dvi = 1.f / (float)dv;
+  float nm[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      x[j] = 64 * j < dv ? os[t * out_s + 64 * j + lane] : 0.f;
-      ss += x[j] * x[j];
-    }
-    const float rn = 1.f / sqrtf(wave_sum(ss) / (float)dv + a.eps);
+  for (int j = 0; j < 4; ++j) nm[j] = 64 * j < dv ? E::ld(static_cast<const T*>(a.norm_w) + 64 * j + lane) : 0.f;
+  for (int t0 = wave; t0 < S; t0 += kTreeRows * nw) {
+    T z[kTreeRows][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (64 * j < dv) {
-        const int d = 64 * j + lane;
-        out[(int64_t)t * a.out_stride + d] = E::mk(x[j] * rn * E::ld(nw_ + d) * silu_f(E::ld(z + d)));
+    for (int v = 0; v < kTreeRows; ++v)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (64 * j < dv)
+          z[v][j] = static_cast<const T*>(a.z)[((int64_t)bb * S + min(t0 + v * nw, S - 1)) * a.z_stride + (int64_t)h * dv + 64 * j + lane];
+#pragma unroll
+    for (int v = 0; v < kTreeRows; ++v) {
+      const int t = t0 + v * nw;
+      if (t >= S) break;
+      float x[4], ss = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[j] = 64 * j < dv ? os[t * out_s + 64 * j + lane] : 0.f;
+        ss += x[j] * x[j];
       }
+      const float rn = rsqrt_raw(lanes_sum(ss) * dvi + a.eps);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (64 * j < dv) out[(int64_t)t * a.out_stride + 64 * j + lane] = E::mk(x[j] * rn * nm[j] * silu_raw(E::ld(&z[v][j])));
+    }
   }
 }
 
-template <int DT, int DKP, int NI>
+template <int DT, int DKP, int NI, int TH>
 static hipError_t launch_gdn_tree_t(const GdnTreeArgs& a, hipStream_t s) {
+  using T = typename Elem<DT>::T;
   constexpr int R = 16 * NI;
-  const int kq = std::max(2 * R * (DKP + 4), R * (a.dv + 4));
-  const int lds = 4 * (kq + 3 * R * (R + 4) + 2 * R) + 16 * R;
-  static LdsLimit limit;  // the largest any call of this instance asks for: dv = 256
-  constexpr int most = 4 * (2 * R * (DKP + 4) > R * 260 ? 2 * R * (DKP + 4) : R * 260) + 4 * (3 * R * (R + 4) + 2 * R) + 16 * R;
-  static_assert(most <= 160 * 1024);
-  const hipError_t e = limit.raise((const void*)gdn_tree_kernel<DT, DKP, NI>, most);
+  constexpr auto bytes = [](int dv) { return 4 * (std::max(2 * R * (DKP + 8), R * (dv + 4)) + 3 * R * (R + 4) + 2 * R) + (16 + 8 * kTreeConv) * R; };
+  static_assert(bytes(256) <= 160 * 1024);
+  static LdsLimit limit;
+  const hipError_t e = limit.raise((const void*)gdn_tree_kernel<DT, DKP, NI, TH>, bytes(TH / 4));
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((gdn_tree_kernel<DT, DKP, NI>), dim3((unsigned)a.Hv, (unsigned)a.B), dim3((unsigned)(4 * a.dv)), lds, s, a);
+  // pairs of channels in one load: every row of inputs and states starts at a multiple of them
+  const bool pair = ((a.qkv_stride & 1) | ((reinterpret_cast<uintptr_t>(a.qkv) | reinterpret_cast<uintptr_t>(a.conv)) & (2 * sizeof(T) - 1))) == 0;
+  hipLaunchKernelGGL((gdn_tree_kernel<DT, DKP, NI, TH>), dim3((unsigned)a.Hv, (unsigned)a.B), dim3((unsigned)(4 * a.dv)),
+                     bytes(a.dv), s, a, pair);
   return hipGetLastError();
 }
 
 hipError_t launch_gdn_tree(int dt, const GdnTreeArgs& a, hipStream_t s) {
   auto rows = [&](auto t, auto d) -> hipError_t {
     constexpr int DT = decltype(t)::value, DKP = decltype(d)::value;
-    if (a.S <= 16) return launch_gdn_tree_t<DT, DKP, 1>(a, s);
-    if (a.S <= 32) return launch_gdn_tree_t<DT, DKP, 2>(a, s);
-    return launch_gdn_tree_t<DT, DKP, 4>(a, s);
+    auto threads = [&](auto n) -> hipError_t {
+      constexpr int NI = decltype(n)::value;
+      return a.dv <= 128 ? launch_gdn_tree_t<DT, DKP, NI, 512>(a, s) : launch_gdn_tree_t<DT, DKP, NI, 1024>(a, s);
+    };
+    if (a.S <= 16) return threads(std::integral_constant<int, 1>{});
+    if (a.S <= 32) return threads(std::integral_constant<int, 2>{});
+    return threads(std::integral_constant<int, 4>{});
   };
   auto dims = [&](auto t) -> hipError_t {
     return a.dk <= 64 ? rows(t, std::integral_constant<int, 64>{}) : rows(t, std::integral_constant<int, 128>{});
