@@ -37,6 +37,11 @@ one token of one sequence the norms and the SwiGLU go further, into the prologue
 projection that consumes them (``forward_pre``, libgsq ``gsq_qmv_pre``). The torch
 formulation below computes the same values and is what CPU tensors run (the structure test
 runs the model on the CPU with dense stand-ins for the packed layers).
+
+``new_cache(kv_bits=8)`` keeps K and V in 8 bits with a scale for each row (runtime/kernels/kv8.py). On
+such a cache ``Qwen35Model.verify`` runs a tree of drafted tokens in one pass without advancing the
+cache, and ``accept`` keeps one path of it: the GatedDeltaNet layers run along every path from the cached
+state (``gdn_tree``) and the kept tokens' inputs advance it afterwards.
 """
 from __future__ import annotations
 
@@ -111,14 +116,18 @@ class Qwen35Cache:
     """Per-layer decode state in fixed device buffers, and the position of the next token.
 
     ``pos`` is a one-element int64 device tensor (read by the captured graph); ``length`` is the
-    host's count of cached tokens, which guards ``max_len``.
+    host's count of cached tokens, which guards ``max_len``. ``kv_bits=8``: ``k`` and ``v`` hold bytes and
+    ``k_scale`` and ``v_scale`` a float32 for each row of them.
     """
 
-    def __init__(self, args: Qwen35Args, batch: int, max_len: int, device, dtype):
-        self.max_len = max_len
+    def __init__(self, args: Qwen35Args, batch: int, max_len: int, device, dtype, kv_bits: int = 16):
+        if kv_bits not in (8, 16):
+            raise ValueError(f"kv_bits must be 16 or 8, not {kv_bits}")
+        self.batch, self.max_len, self.kv_bits = batch, max_len, kv_bits
         self.length = 0
+        self.drafted = None  # parents of the tree that verify ran last, and the GatedDeltaNet layers' inputs
         self.pos = torch.zeros(1, dtype=torch.int64, device=device)
-        self.conv, self.rec, self.k, self.v = {}, {}, {}, {}
+        self.conv, self.rec, self.k, self.v, self.k_scale, self.v_scale = {}, {}, {}, {}, {}, {}
         for i in range(args.num_hidden_layers):
             if args.is_linear(i):
                 self.conv[i] = torch.zeros(batch, args.linear_conv_kernel_dim - 1, args.conv_dim, device=device,
@@ -127,11 +136,17 @@ class Qwen35Cache:
                                           args.linear_value_head_dim, device=device, dtype=torch.float32)
             else:
                 shape = (batch, args.num_key_value_heads, max_len, args.head_dim)
-                self.k[i] = torch.zeros(shape, device=device, dtype=dtype)
-                self.v[i] = torch.zeros(shape, device=device, dtype=dtype)
+                if kv_bits == 8:
+                    for t, scale in ((self.k, self.k_scale), (self.v, self.v_scale)):
+                        t[i] = torch.full(shape, 128, device=device, dtype=torch.uint8)
+                        scale[i] = torch.zeros(shape[:3], device=device)
+                else:
+                    self.k[i] = torch.zeros(shape, device=device, dtype=dtype)
+                    self.v[i] = torch.zeros(shape, device=device, dtype=dtype)
 
     def reset(self):
         self.length = 0
+        self.drafted = None
         self.pos.zero_()
         for t in (*self.conv.values(), *self.rec.values()):
             t.zero_()
@@ -166,34 +181,63 @@ class GatedDeltaNet(torch.nn.Module):
                                              **kw)
         return qkvz, work
 
-    def forward(self, x, cache: Qwen35Cache, first=None):
+    def forward(self, x, cache: Qwen35Cache, first=None, parents=None):
         """``first``: ``in_proj_qkvz(x)`` when the caller has computed it already, or
-        ``first_pre``'s (qkvz, convolution outputs)."""
+        ``first_pre``'s (qkvz, convolution outputs). ``parents``: the tokens are a drafted tree; the cache is
+        left alone, and the layer's inputs are kept for ``advance``."""
         a_ = self.args
-        B, S, _ = x.shape
-        hk, hv = a_.linear_num_key_heads, a_.linear_num_value_heads
-        dk, dv = a_.linear_key_head_dim, a_.linear_value_head_dim
-        kw = a_.linear_conv_kernel_dim
+        S = x.shape[1]
         conv_out = None
         if isinstance(first, tuple):
             first, conv_out = first
         qkvz = self.in_proj_qkvz(x) if first is None else first
         qkv, z = qkvz[..., :a_.conv_dim], qkvz[..., a_.conv_dim:]   # (B, S, conv_dim), (B, S, Hv * dv)
+        if parents is not None:
+            ab = F.linear(x, self.w_ab)
+            cache.drafted[1][self.layer] = (qkv, z, ab)
+            if x.is_cuda:
+                from ..runtime.kernels import model_ops
+                out = model_ops.gdn_tree(qkv, z, ab, cache.conv[self.layer], self.conv_w, self.ssm_a, self.dt_bias,
+                                         cache.rec[self.layer], self.norm_w, parents, **self._heads)
+            else:
+                out = self._mix_tree(qkv, z, ab, cache, parents).to(x.dtype)
+            return self.out_proj(out)
         if x.is_cuda:
             from ..runtime.kernels import model_ops
             if S == 1:  # the a / b projections happen inside the fused step
                 out = model_ops.gdn_step(qkv[:, 0], z[:, 0], x[:, 0], self.w_ab, cache.conv[self.layer], self.conv_w,
                                          self.ssm_a, self.dt_bias, cache.rec[self.layer], self.norm_w,
-                                         key_heads=hk, value_heads=hv, head_k_dim=dk, head_v_dim=dv,
-                                         eps=a_.rms_norm_eps, conv_out=conv_out)[:, None]
+                                         **self._heads, conv_out=conv_out)[:, None]
             else:  # a sequence: a / b of all tokens in one product, then one recurrence launch
                 out = model_ops.gdn_seq(qkv, z, F.linear(x, self.w_ab), cache.conv[self.layer], self.conv_w,
-                                        self.ssm_a, self.dt_bias, cache.rec[self.layer], self.norm_w,
-                                        key_heads=hk, value_heads=hv, head_k_dim=dk, head_v_dim=dv,
-                                        eps=a_.rms_norm_eps)
+                                        self.ssm_a, self.dt_bias, cache.rec[self.layer], self.norm_w, **self._heads)
             return self.out_proj(out)
-        z = z.view(B, S, hv, dv)
-        a, b = F.linear(x, self.w_ab).float().split(hv, dim=-1)  # (B, S, Hv) each
+        return self.out_proj(self._mix(qkv, z, F.linear(x, self.w_ab), cache).to(x.dtype))
+
+    @property
+    def _heads(self):
+        a_ = self.args
+        return dict(key_heads=a_.linear_num_key_heads, value_heads=a_.linear_num_value_heads,
+                    head_k_dim=a_.linear_key_head_dim, head_v_dim=a_.linear_value_head_dim, eps=a_.rms_norm_eps)
+
+    def advance(self, qkv, z, ab, cache: Qwen35Cache):
+        """The cache after tokens with these inputs (rows of a drafted tree that are kept)."""
+        if qkv.is_cuda:
+            from ..runtime.kernels import model_ops
+            model_ops.gdn_seq(qkv, z, ab, cache.conv[self.layer], self.conv_w, self.ssm_a, self.dt_bias,
+                              cache.rec[self.layer], self.norm_w, **self._heads)
+        else:
+            self._mix(qkv, z, ab, cache)
+
+    def _mix(self, qkv, z, ab, cache: Qwen35Cache):
+        """The torch formulation over S tokens, advancing the cache: (B, S, Hv * dv) in float32."""
+        a_ = self.args
+        B, S, _ = qkv.shape
+        hk, hv = a_.linear_num_key_heads, a_.linear_num_value_heads
+        dk, dv = a_.linear_key_head_dim, a_.linear_value_head_dim
+        kw = a_.linear_conv_kernel_dim
+        z = z.reshape(B, S, hv, dv)
+        a, b = ab.float().split(hv, dim=-1)  # (B, S, Hv) each
         # depthwise causal convolution over [3 cached inputs, S new ones]
         conv_in = torch.cat([cache.conv[self.layer], qkv.to(cache.conv[self.layer].dtype)], dim=1)
         cache.conv[self.layer].copy_(conv_in[:, S:])
@@ -223,7 +267,41 @@ class GatedDeltaNet(torch.nn.Module):
         cache.rec[self.layer].copy_(st)
         out = torch.stack(outs, dim=1)                                  # (B, S, Hv, dv), fp32
         out = rms_norm(out, self.norm_w, a_.rms_norm_eps) * F.silu(z.float())
-        return self.out_proj(out.to(x.dtype).reshape(B, S, hv * dv))
+        return out.reshape(B, S, hv * dv)
+
+    def _mix_tree(self, qkv, z, ab, cache: Qwen35Cache, parents):
+        """``_mix`` along every path of a tree, the cache left alone: each token's path as a sequence."""
+        i = self.layer
+        conv, rec = cache.conv[i], cache.rec[i]
+        out = torch.empty(*z.shape[:2], self.args.value_dim)
+        try:
+            for b, row in enumerate(parents.expand(z.shape[0], -1).tolist()):
+                for t in range(len(row)):
+                    cache.conv[i], cache.rec[i] = conv[b:b + 1].clone(), rec[b:b + 1].clone()
+                    path = _path(row, t)
+                    out[b, t] = self._mix(qkv[b:b + 1, path], z[b:b + 1, path], ab[b:b + 1, path], cache)[0, -1]
+        finally:
+            cache.conv[i], cache.rec[i] = conv, rec
+        return out
+
+
+def _path(parents, t):
+    """Tokens from the cache to token t of a tree."""
+    path = [t]
+    while parents[path[0]] != -1:
+        if not 0 <= parents[path[0]] < path[0]:
+            raise ValueError("a drafted token follows an earlier one, or -1")
+        path.insert(0, parents[path[0]])
+    return path
+
+
+def _quantise_rows(x):
+    """Rows of x as an 8-bit cache holds them: (bytes, scales), as gsq_kv8_write forms them."""
+    x = x.double()
+    scale = (x.abs().amax(-1) / 127).float()
+    fine = torch.isfinite(scale)
+    u = torch.where(scale[..., None] > 0, x / scale[..., None].double(), 0.0).round().clamp(-127, 127) + 128
+    return torch.where(fine[..., None], u, 128.0).to(torch.uint8), torch.where(fine, scale, float("nan"))
 
 
 def _has_derivative(t) -> bool:
@@ -250,12 +328,12 @@ class FullAttention(torch.nn.Module):
         self.register_buffer("inv_freq", 1.0 / (args.rope_theta ** (steps / rd)))
 
     def _rope(self, x, pos):
-        """x (B, S, H, hd); pos (S,) int64 positions."""
+        """x (B, S, H, hd); pos (S,) or (B, S) int64 positions."""
         rd = self.args.rotary_dim
-        ang = pos.to(torch.float64)[:, None] * self.inv_freq[None, :]   # (S, rd/2)
+        ang = pos.to(torch.float64)[..., None] * self.inv_freq   # (S, rd/2) or (B, S, rd/2)
         ang = torch.cat([ang, ang], dim=-1)
-        cos = ang.cos().float()[None, :, None, :]
-        sin = ang.sin().float()[None, :, None, :]
+        cos = ang.cos().float()[..., None, :]
+        sin = ang.sin().float()[..., None, :]
         xr = x[..., :rd].float()
         xr = xr * cos + _rotate_half(xr) * sin
         return torch.cat([xr.to(x.dtype), x[..., rd:]], dim=-1)
@@ -283,13 +361,62 @@ class FullAttention(torch.nn.Module):
                 and qk.shape[0] <= 65535 and qk.shape[1] <= rows[2].shape[2]
                 and not any(_has_derivative(t) for t in (*rows, *norms)))
 
-    def forward(self, x, cache: Qwen35Cache, first=None):
-        """``first``: ``qk_proj(x)`` when the caller has computed it already."""
+    def _kv8(self, qk, v, cache, parents):
+        """Attention over an 8-bit cache: (B, S, heads * head_dim)."""
+        a_, i = self.args, self.layer
+        B, S, _ = qk.shape
+        H, Hkv, hd = a_.num_attention_heads, a_.num_key_value_heads, a_.head_dim
+        norms, caches = (self.q_norm_w, self.k_norm_w), (cache.k[i], cache.v[i], cache.k_scale[i], cache.v_scale[i])
+        if any(_has_derivative(t) for t in (qk, v, *norms)):
+            raise ValueError("an 8-bit cache carries no derivative")
+        qg, k = qk[..., :H * 2 * hd], qk[..., H * 2 * hd:]
+        if qk.is_cuda:
+            from ..runtime.kernels import kv8
+            if (qk.dtype in (torch.float16, torch.bfloat16) and hd in kv8.HEAD_DIMS and self.inv_freq.dtype == torch.float64
+                    and all(t.dtype == qk.dtype and t.is_contiguous() for t in (qk, v, *norms))
+                    and qk.data_ptr() % 8 == 0 and qk.stride(1) % 4 == 0):
+                heads = dict(heads=H, kv_heads=Hkv, head_dim=hd, parents=parents)
+                q = kv8.kv8_write(qg, k, v, *norms, self.inv_freq, *caches, cache.pos, rotary_dim=a_.rotary_dim,
+                                  eps=a_.rms_norm_eps, **heads)
+                return kv8.attn_kv8(q, qg, *caches, cache.pos, **heads)
+        at = torch.arange(S, device=qk.device)
+        if parents is None:
+            depth, seen = at.expand(B, S), (at <= at[:, None]).expand(B, S, S)
+        else:
+            seen = torch.zeros(B, S, S, dtype=torch.bool)
+            for b, row in enumerate(parents.expand(B, -1).tolist()):
+                for t in range(S):
+                    seen[b, t, _path(row, t)] = True
+            seen = seen.to(qk.device)
+            depth = seen.sum(-1) - 1
+        qg = qg.reshape(B, S, H, 2 * hd)
+        q = self._rope(rms_norm(qg[..., :hd].float(), norms[0], a_.rms_norm_eps), cache.pos + depth).to(qk.dtype)
+        k = self._rope(rms_norm(k.reshape(B, S, Hkv, hd).float(), norms[1], a_.rms_norm_eps), cache.pos + depth)
+        for x, c, scale in ((k, caches[0], caches[2]), (v.reshape(B, S, Hkv, hd), caches[1], caches[3])):
+            u, s = _quantise_rows(x)
+            c.index_copy_(2, cache.pos + at, u.transpose(1, 2))
+            scale.index_copy_(2, cache.pos + at, s.transpose(1, 2))
+        L, rep = caches[0].shape[2], H // Hkv
+        new = torch.arange(L, device=qk.device) - cache.pos              # (L,): drafted or new token of a position
+        mask = torch.where(((new >= 0) & (new < S))[None, None], seen[:, :, new.clamp(0, S - 1)], new < 0)  # (B, S, L)
+        kf, vf = ((c.float() - 128) * s[..., None] for c, s in ((caches[0], caches[2]), (caches[1], caches[3])))
+        vf = torch.where((new < S)[:, None], vf, 0.0)                    # behind the new tokens lies anything
+        qf = q.float().transpose(1, 2).reshape(B, Hkv, rep * S, hd)
+        scores = torch.matmul(qf, kf.transpose(2, 3).contiguous()) * (hd ** -0.5)
+        scores = scores.masked_fill(~mask.repeat(1, rep, 1)[:, None], float("-inf"))
+        att = torch.matmul(torch.softmax(scores, dim=-1), vf).reshape(B, H, S, hd).transpose(1, 2)
+        return (att * torch.sigmoid(qg[..., hd:].float())).reshape(B, S, H * hd).to(qk.dtype)
+
+    def forward(self, x, cache: Qwen35Cache, first=None, parents=None):
+        """``first``: ``qk_proj(x)`` when the caller has computed it already. ``parents``: the tokens are a
+        drafted tree (8-bit caches)."""
         a_ = self.args
         B, S, _ = x.shape
         H, Hkv, hd = a_.num_attention_heads, a_.num_key_value_heads, a_.head_dim
         qk = self.qk_proj(x) if first is None else first
         v = self.v_proj(x)
+        if cache.kv_bits == 8:
+            return self.o_proj(self._kv8(qk, v, cache, parents))
         if x.is_cuda and S == 1:
             from ..runtime.kernels import model_ops
             out = model_ops.attn_decode(qk[:, 0, :H * 2 * hd], qk[:, 0, H * 2 * hd:], v[:, 0], self.q_norm_w,
@@ -353,9 +480,10 @@ class Qwen35Layer(torch.nn.Module):
         self.register_buffer("post_norm_w", post_norm_w)
         self.gate_up, self.down = gate_up, down  # gate_up: [gate | up] of the MLP in one product
 
-    def forward(self, x, delta, cache):
+    def forward(self, x, delta, cache, parents=None):
         eps = self.args.rms_norm_eps
-        if _fused_row(x, self.mixer.first_proj, self.gate_up, self.down):
+        # a drafted token leaves the convolution's state alone, which the fused projection would advance
+        if parents is None and _fused_row(x, self.mixer.first_proj, self.gate_up, self.down):
             h = torch.empty_like(x)                 # the normalized layer input
             x1 = x if delta is None else torch.empty_like(x)
             first = self.mixer.first_pre(x, cache, pre_a=delta, pre_w=self.input_norm_w, eps=eps,
@@ -364,7 +492,8 @@ class Qwen35Layer(torch.nn.Module):
             x2 = torch.empty_like(x)
             gu = self.gate_up.forward_pre(x1, "add_rms_norm", pre_a=m, pre_w=self.post_norm_w, eps=eps, res_out=x2)
             return x2, self.down.forward_pre(gu, "swiglu")
-        m = self.mixer(add_rms_norm(x, delta, self.input_norm_w, eps), cache)
+        h = add_rms_norm(x, delta, self.input_norm_w, eps)
+        m = self.mixer(h, cache) if parents is None else self.mixer(h, cache, parents=parents)
         gu = self.gate_up(add_rms_norm(x, m, self.post_norm_w, eps))
         if gu.is_cuda:
             from ..runtime.kernels import model_ops
@@ -384,26 +513,80 @@ class Qwen35Model(torch.nn.Module):
         self.layers = torch.nn.ModuleList(layers)
         self.register_buffer("norm_w", norm_w)
 
-    def new_cache(self, batch: int = 1, max_len: int = 4096, device=None) -> Qwen35Cache:
+    def new_cache(self, batch: int = 1, max_len: int = 4096, device=None, kv_bits: int = 16) -> Qwen35Cache:
         device = device if device is not None else self.norm_w.device
-        return Qwen35Cache(self.args, batch, max_len, device, self.dtype)
+        return Qwen35Cache(self.args, batch, max_len, device, self.dtype, kv_bits)
 
     def forward(self, ids, cache: Qwen35Cache):
+        S = ids.shape[1]
+        logits = self._run(ids, cache)
+        cache.drafted = None
+        cache.pos.add_(S)
+        cache.length += S
+        return logits
+
+    def _run(self, ids, cache: Qwen35Cache, parents=None):
         B, S = ids.shape
         if cache.length + S > cache.max_len:
             raise ValueError(f"cache holds {cache.max_len} positions; {cache.length} used, {S} more asked")
         x = self.embed(ids).to(self.dtype).reshape(B, S, -1).contiguous()
         delta = None
         for layer in self.layers:
-            x, delta = layer(x, delta, cache)
+            x, delta = layer(x, delta, cache) if parents is None else layer(x, delta, cache, parents)
         eps = self.args.rms_norm_eps
         if _fused_row(x, self.lm_head):
-            logits = self.lm_head.forward_pre(x, "add_rms_norm", pre_a=delta, pre_w=self.norm_w, eps=eps)
-        else:
-            logits = self.lm_head(add_rms_norm(x, delta, self.norm_w, eps))
-        cache.pos.add_(S)
-        cache.length += S
-        return logits
+            return self.lm_head.forward_pre(x, "add_rms_norm", pre_a=delta, pre_w=self.norm_w, eps=eps)
+        return self.lm_head(add_rms_norm(x, delta, self.norm_w, eps))
+
+    def verify(self, ids, cache: Qwen35Cache, parents):
+        """Logits (B, T, vocab) behind every token of a tree of T <= 64 drafted tokens (ids (B, T)), each run on
+        the cached tokens and its own ancestors: ``parents`` (T,) or (B, T) names for each token the drafted
+        one it follows (an earlier one) or -1. The cache (of 8 bits) is not advanced; ``accept`` keeps a path."""
+        B, T = ids.shape
+        if cache.kv_bits != 8:
+            raise ValueError("trees of drafted tokens need an 8-bit cache (new_cache(kv_bits=8))")
+        if not 1 <= T <= 64:
+            raise ValueError(f"a tree holds 1 to 64 tokens, not {T}")
+        parents = torch.as_tensor(parents)
+        if tuple(parents.shape) not in ((T,), (B, T)):
+            raise ValueError("parents must be (T,) or (B, T)")
+        if parents.device.type == "cpu" and bool(((parents < -1) | (parents >= torch.arange(T))).any()):
+            raise ValueError("a drafted token follows an earlier one, or -1")
+        parents = parents.to(device=cache.pos.device, dtype=torch.int32).contiguous()
+        cache.drafted = (parents, {})
+        return self._run(ids, cache, parents)
+
+    def accept(self, cache: Qwen35Cache, path):
+        """Keeps the drafted tokens ``path`` ((n,), or (B, n) for rows that keep other ones) of the tree that
+        ``verify`` ran last: a path from the cache on (its first token follows -1, each other the one before
+        it), possibly empty. The cache is advanced by them and the other drafted tokens are forgotten."""
+        if cache.drafted is None:
+            raise ValueError("no drafted tokens: verify comes first")
+        parents, inputs = cache.drafted
+        B, T = cache.batch, parents.shape[-1]
+        path = torch.as_tensor(path, dtype=torch.int64).cpu()
+        if path.dim() == 0 or path.dim() > 2 or (path.dim() == 2 and path.shape[0] != B):
+            raise ValueError("path must be (n,) or (B, n)")
+        path = path.expand(B, -1)
+        n = path.shape[1]
+        if n:
+            if bool(((path < 0) | (path >= T)).any()):
+                raise ValueError("path names tokens that were not drafted")
+            before = torch.cat([torch.full((B, 1), -1), path[:, :-1]], dim=1)
+            if not torch.equal(torch.gather(parents.cpu().long().expand(B, T), 1, path), before):
+                raise ValueError("path must lead from the cached tokens on, each token following the one before")
+            path = path.to(cache.pos.device)
+            row = torch.arange(B, device=path.device)[:, None]
+            to = cache.length + torch.arange(n, device=path.device)
+            for i in cache.k:
+                for t in (cache.k[i], cache.v[i], cache.k_scale[i], cache.v_scale[i]):
+                    t[row, :, to] = t[row, :, cache.length + path]  # the right side is a copy
+            for layer in self.layers:
+                if layer.mixer.layer in inputs:
+                    layer.mixer.advance(*(t[row, path] for t in inputs[layer.mixer.layer]), cache)
+        cache.drafted = None
+        cache.pos.add_(n)
+        cache.length += n
 
 
 class _SideBySide(torch.nn.Module):

@@ -1,0 +1,202 @@
+"""The Qwen3.5-hybrid decoder on an 8-bit K/V cache, and trees of drafted tokens through it (``verify``,
+``accept``): against HF's logits, and against the same tokens decoded one at a time.
+
+CPU: the torch formulation in float32 on dense stand-ins. GPU: the kernels (kv8_write, attn_kv8, gdn_tree,
+gdn_seq) between packed projections, fp16."""
+import pytest
+import torch
+
+from mlx_gsq_amd import tables
+from mlx_gsq_amd.models import GraphDecoder, build_qwen35
+from mlx_gsq_amd.models.qwen35 import Qwen35Cache
+from qwen35_fixture import ARGS, TABLES, TinyStore, dense_factories, hf_logits, hf_model, rel_l2
+
+IDS = [17, 301, 5, 77, 402, 9, 256, 130]
+# a tree behind the first 5 tokens: two continuations, one of which branches again
+DRAFT = [9, 44, 256, 130, 81, 300, 12]
+PARENTS = [-1, -1, 0, 2, 2, 1, 3]
+PATHS = [[0], [1], [0, 2], [0, 2, 3], [0, 2, 4], [1, 5], [0, 2, 3, 6]]
+
+
+@pytest.fixture(scope="module")
+def store():
+    return TinyStore("cpu", seed=1)
+
+
+def _cpu_model(store):
+    linear, fused, embedding = dense_factories(store)
+    return build_qwen35(store, dtype=torch.float32, args=ARGS, linear=linear, fused=fused, embedding=embedding)
+
+
+def _gpu_model():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    tables.set_tables(TABLES)
+    return build_qwen35(TinyStore(torch.device("cuda:0"), seed=1), dtype=torch.float16, args=ARGS)
+
+
+def _ids(model, tokens):
+    return torch.tensor([tokens], device=model.norm_w.device)
+
+
+def _one_at_a_time(model, tokens, batch=1):
+    cache = model.new_cache(batch=batch, max_len=32, kv_bits=8)
+    return torch.cat([model(_ids(model, [t]).expand(batch, 1), cache) for t in tokens], dim=1)
+
+
+def _check_tree(model, tol):
+    """Every node's logits are those of its path decoded one token at a time; each accepted path goes on as
+    that sequence does."""
+    with torch.no_grad():
+        cache = model.new_cache(max_len=32, kv_bits=8)
+        model(_ids(model, IDS[:5]), cache)
+        before = [t.clone() for t in (*cache.rec.values(), *cache.conv.values())]
+        logits = model.verify(_ids(model, DRAFT), cache, PARENTS)
+        assert cache.length == 5 and int(cache.pos) == 5
+        assert all(torch.equal(a, b) for a, b in zip(before, (*cache.rec.values(), *cache.conv.values())))
+        for t, path in enumerate(PATHS):
+            want = _one_at_a_time(model, IDS[:5] + [DRAFT[i] for i in path])[:, -1]
+            assert rel_l2(logits[:, t].float().cpu().numpy(), want.float().cpu().numpy()) <= tol, t
+        for path in ([0, 2, 3, 6], [1], [0, 2, 4], []):
+            cache = model.new_cache(max_len=32, kv_bits=8)
+            model(_ids(model, IDS[:5]), cache)
+            model.verify(_ids(model, DRAFT), cache, torch.tensor(PARENTS))
+            model.accept(cache, path)
+            assert cache.length == int(cache.pos) == 5 + len(path)
+            got = model(_ids(model, [77]), cache)[:, -1]
+            want = _one_at_a_time(model, IDS[:5] + [DRAFT[i] for i in path] + [77])[:, -1]
+            assert rel_l2(got.float().cpu().numpy(), want.float().cpu().numpy()) <= tol, path
+
+
+def test_cpu_8_bit_cache_matches_hf(store):
+    """K and V rows are off by half a step of their largest value over 127 at most: a root mean square error of
+    0.3 / 127 of about three standard deviations, 0.7 per cent of a row, in one layer of four."""
+    ref = hf_logits(hf_model(store), IDS)
+    model = _cpu_model(store)
+    with torch.no_grad():
+        pre = model(_ids(model, IDS), model.new_cache(max_len=16, kv_bits=8))
+        dec = _one_at_a_time(model, IDS)
+    assert 1e-6 < rel_l2(pre.numpy(), ref.numpy()) <= 7e-3
+    assert rel_l2(dec.numpy(), pre.numpy()) <= 1e-4
+
+
+def test_cpu_tree(store):
+    _check_tree(_cpu_model(store), 1e-4)
+
+
+def test_cpu_trees_of_a_batch(store):
+    """Rows with trees of their own, that keep different paths of one length."""
+    model = _cpu_model(store)
+    parents = torch.tensor([[-1, 0, 0, 2], [-1, -1, 1, 0]])
+    draft = torch.tensor([[9, 44, 256, 130], [81, 300, 12, 5]])
+    paths = [[0, 2, 3], [1, 2, 2]]
+    with torch.no_grad():
+        cache = model.new_cache(batch=2, max_len=16, kv_bits=8)
+        model(torch.tensor([IDS[:4], IDS[4:]]), cache)
+        logits = model.verify(draft, cache, parents)
+        with pytest.raises(ValueError, match="path"):
+            model.accept(cache, paths)  # token 2 does not follow itself
+        paths = [[0, 2], [1, 2]]
+        model.accept(cache, paths)
+        nxt = model(torch.tensor([[3], [3]]), cache)[:, -1]
+        for b, ids in enumerate((IDS[:4], IDS[4:])):
+            seq = _one_at_a_time(model, ids + [int(draft[b, i]) for i in paths[b]] + [3])
+            assert rel_l2(nxt[b].numpy(), seq[0, -1].numpy()) <= 1e-4
+            assert rel_l2(logits[b, paths[b][-1]].numpy(), seq[0, -2].numpy()) <= 1e-4
+
+
+def test_cpu_refusals(store):
+    model = _cpu_model(store)
+    with torch.no_grad():
+        with pytest.raises(ValueError, match="kv_bits"):
+            model.new_cache(kv_bits=4)
+        with pytest.raises(ValueError, match="8-bit"):
+            model.verify(_ids(model, DRAFT), model.new_cache(max_len=16), PARENTS)
+        cache = model.new_cache(max_len=8, kv_bits=8)
+        with pytest.raises(ValueError, match="verify"):
+            model.accept(cache, [0])
+        for bad in ([-1, 1, 0], [-1, 0, -2], [0, 0, 0], [-1, 0]):
+            with pytest.raises(ValueError):
+                model.verify(_ids(model, [1, 2, 3]), cache, bad)
+        with pytest.raises(ValueError, match="64"):
+            model.verify(_ids(model, [1] * 65), cache, [-1] * 65)
+        with pytest.raises(ValueError, match="positions"):
+            model.verify(_ids(model, [1] * 9), cache, [-1] * 9)
+        model.verify(_ids(model, [1, 2, 3]), cache, [-1, 0, 0])
+        for bad in ([1], [0, 1, 2], [3], [-1], [[0], [0]], [0, 0]):
+            with pytest.raises(ValueError):
+                model.accept(cache, bad)
+        model(_ids(model, [4]), cache)  # a plain step forgets the drafted tokens
+        with pytest.raises(ValueError, match="verify"):
+            model.accept(cache, [0])
+        cache.reset()
+        assert cache.length == 0 and cache.drafted is None
+    # no derivative goes through the cache
+    layer = model.layers[3].mixer
+    x = torch.randn(1, 2, ARGS.hidden_size, requires_grad=True)
+    with pytest.raises(ValueError, match="derivative"):
+        layer(x, Qwen35Cache(ARGS, 1, 8, "cpu", torch.float32, kv_bits=8))
+
+
+@pytest.mark.gpu
+def test_gpu_8_bit_cache_and_tree():
+    """Against the CPU's float32 model within the bound of the fp16 decoder (2e-2), and among themselves: trees
+    against single tokens, prompts against single tokens, graph replays against eager steps."""
+    model = _gpu_model()
+    cpu = _cpu_model(TinyStore("cpu", seed=1))
+    with torch.no_grad():
+        want = cpu(_ids(cpu, IDS), cpu.new_cache(max_len=16, kv_bits=8))
+        pre = model(_ids(model, IDS), model.new_cache(max_len=32, kv_bits=8))
+        dec = _one_at_a_time(model, IDS)
+        assert rel_l2(pre.float().cpu().numpy(), want.numpy()) <= 2e-2
+        assert rel_l2(dec.float().cpu().numpy(), want.numpy()) <= 2e-2
+        _check_tree(model, 2e-2)
+        cache = model.new_cache(max_len=32, kv_bits=8)
+        graph = GraphDecoder(model, cache)
+        for i, t in enumerate(IDS):
+            assert torch.equal(graph.step(_ids(model, [t]))[:, 0], dec[:, i]), i
+        # a tree behind replayed steps
+        logits = model.verify(_ids(model, DRAFT), cache, PARENTS)
+        model.accept(cache, [0, 2])
+        step = graph.step(_ids(model, [77]))[:, 0].clone()
+        seq = _one_at_a_time(model, IDS + [DRAFT[0], DRAFT[2], 77])
+        assert rel_l2(logits[:, 2].float().cpu().numpy(), seq[:, -2].float().cpu().numpy()) <= 2e-2
+        assert rel_l2(step.float().cpu().numpy(), seq[:, -1].float().cpu().numpy()) <= 2e-2
+        # single drafted token: the cache stays as it was
+        cache2 = model.new_cache(max_len=32, kv_bits=8)
+        model(_ids(model, IDS), cache2)
+        kept = [t.clone() for t in (*cache2.rec.values(), *cache2.conv.values())]
+        one = model.verify(_ids(model, [9]), cache2, [-1])
+        assert all(torch.equal(a, b) for a, b in zip(kept, (*cache2.rec.values(), *cache2.conv.values())))
+        assert rel_l2(one[:, 0].float().cpu().numpy(), _one_at_a_time(model, IDS + [9])[:, -1].float().cpu().numpy()) <= 2e-2
+        # parents on the device that are none: NaN, not a fault
+        bad = model.verify(_ids(model, DRAFT), cache2, torch.tensor([-1, 1, 0, 2, 2, 1, 3], device="cuda"))
+        assert torch.isnan(bad).all()
+
+
+@pytest.mark.gpu
+def test_gpu_float32_activations_take_the_torch_formulation():
+    """The kernels serve 16-bit activations; others run the same definition in torch ops on the GPU."""
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    from mlx_gsq_amd.models.qwen35 import FullAttention
+    g = torch.Generator().manual_seed(3)
+    a = ARGS
+    H, G, hd = a.num_attention_heads, a.num_key_value_heads, a.head_dim
+    rows = torch.randn(1, 6, H * 2 * hd + G * hd, generator=g), torch.randn(1, 6, G * hd, generator=g)
+
+    class Given(torch.nn.Module):
+        def __init__(self, v):
+            super().__init__()
+            self.v = v
+
+        def forward(self, x):
+            return self.v
+    outs = []
+    for dev in ("cpu", "cuda"):
+        qk, v = (t.to(dev) for t in rows)
+        m = FullAttention(a, 3, Given(qk), Given(v), torch.nn.Identity(), torch.ones(hd, device=dev), torch.ones(hd, device=dev))
+        cache = Qwen35Cache(a, 1, 16, dev, torch.float32, kv_bits=8)
+        parents = torch.tensor([-1, 0, 0, 1, 1, -1], dtype=torch.int32, device=dev)
+        outs.append(m(torch.zeros(1, 6, 8, device=dev), cache, parents=parents).cpu())
+    assert rel_l2(outs[1].numpy(), outs[0].numpy()) <= 1e-5
