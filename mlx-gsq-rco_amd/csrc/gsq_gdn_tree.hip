@@ -47,24 +47,6 @@ __device__ __forceinline__ float from_row(float v) {
   return __builtin_bit_cast(float, (uint32_t)r[Q & 1]);
 }
 
-// sum over the wave, in every lane: without LDS (the shuffles' round trips are what a row's norm waits for)
-__device__ __forceinline__ float lanes_sum(float v) {
-  auto dpp = [](float x, auto ctrl) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value,
-                                                                 0xF, 0xF, false));
-  };
-  v += dpp(v, std::integral_constant<int, 0xB1>{});   // quad_perm [1,0,3,2]
-  v += dpp(v, std::integral_constant<int, 0x4E>{});   // quad_perm [2,3,0,1]
-  v += dpp(v, std::integral_constant<int, 0x141>{});  // row_half_mirror
-  v += dpp(v, std::integral_constant<int, 0x140>{});  // row_mirror
-  uint32_t x = __builtin_bit_cast(uint32_t, v);
-  const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-  v = __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
-  x = __builtin_bit_cast(uint32_t, v);
-  const auto h = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-  return __builtin_bit_cast(float, (uint32_t)h[0]) + __builtin_bit_cast(float, (uint32_t)h[1]);
-}
-
 // x / (1 + e^-x) and 1 / sqrt(x) from the hardware's power of two, reciprocal and square root: a few ulps of float32
 __device__ __forceinline__ float silu_raw(float x) {
   return x * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -1.44269504088896340736f));

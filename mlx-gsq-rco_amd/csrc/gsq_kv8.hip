@@ -15,6 +15,7 @@
 #include <type_traits>
 
 #include "gsq_common.h"
+#include "gsq_elem.h"
 
 namespace gsq {
 
@@ -79,18 +80,20 @@ __device__ __forceinline__ uint64_t tree_path(const int32_t* parents, int S) {
 // ---- writing -----------------------------------------------------------------------------------
 // One workgroup per (token, share of the heads): a wave per head row, kWriteRows rows loaded before
 // the first is used. The rotary factors of the token's position are formed once per workgroup, angles
-// in double. k and v rows are handled in double: rounding to 8 bits jumps at values next to a border,
-// and so the bytes are those of the definition. Bound by memory latency (each row read and written
-// once).
-constexpr int kWriteRows = 4;
+// in double. Rounding to 8 bits jumps at values next to a border, so k is formed in double and a row that has
+// a quotient within 1e-4 of a border (five times what float32 can be off) divides in double too:
+// the bytes are those of the definition. Bound by the arithmetic of a row (2047 tokens of 24 + 2 x 4 heads
+// of 256: 60 MB in 23 us; one token of 8 rows 5.1 us).
+constexpr int kWriteRows = 2;
 
 template <bool BF, int HD>
-__global__ void __launch_bounds__(256) kv8_write_kernel(Kv8WriteArgs a) {
+__global__ void __launch_bounds__(256) kv8_write_kernel(Kv8WriteArgs a, bool wide) {
   using E = E16<BF>;
   constexpr int V = HD / 64;  // consecutive values per lane
   typedef uint16_t vec_t __attribute__((ext_vector_type(V)));
   typedef uint8_t bytes_t __attribute__((ext_vector_type(V)));
   __shared__ double row[4][HD], cs[HD / 2], sn[HD / 2];
+  __shared__ float csf[HD / 2], snf[HD / 2];
   __shared__ int depth;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, d0 = V * lane;
   const int t = blockIdx.x, bb = blockIdx.y, hr = a.rd / 2, nh = a.H + 2 * a.Hkv, step = 4 * gridDim.z;
@@ -98,28 +101,31 @@ __global__ void __launch_bounds__(256) kv8_write_kernel(Kv8WriteArgs a) {
   const int32_t* const parents = a.parents ? a.parents + (int64_t)bb * a.parents_stride : nullptr;
   const int64_t r = (int64_t)bb * a.S + t;
   uint16_t* const qo = static_cast<uint16_t*>(a.q) + r * a.H * HD + d0;
-  const bool invalid = row_invalid(pos, a.L, a.S, parents);
-  if (invalid) {
-    for (int h = blockIdx.z * 4 + wave; h < a.H; h += step)
-      for (int j = 0; j < V; ++j) qo[(int64_t)h * HD + j] = E::mk(__builtin_nanf(""));
-    return;
-  }
   const uint16_t* const qg = static_cast<const uint16_t*>(a.qg) + r * a.qg_stride + d0;
   const uint16_t* const kn = static_cast<const uint16_t*>(a.k) + r * a.k_stride + d0;
   const uint16_t* const vn = static_cast<const uint16_t*>(a.v) + r * a.v_stride + d0;
-  uint16_t x[kWriteRows][V];
+  vec_t x[kWriteRows];
   auto load = [&](int h0) {
 #pragma unroll
     for (int u = 0; u < kWriteRows; ++u) {
       const int h = min(h0 + u * step, nh - 1);
       const uint16_t* src = h < a.H ? qg + (int64_t)h * 2 * HD
                                     : (h < a.H + a.Hkv ? kn + (int64_t)(h - a.H) * HD : vn + (int64_t)(h - a.H - a.Hkv) * HD);
+      if (wide) {
+        x[u] = *reinterpret_cast<const vec_t*>(src);
+      } else {
 #pragma unroll
-      for (int j = 0; j < V; ++j) x[u][j] = src[j];
+        for (int j = 0; j < V; ++j) x[u][j] = src[j];
+      }
     }
   };
   int h0 = blockIdx.z * 4 + wave;
   load(h0);
+  if (row_invalid(pos, a.L, a.S, parents)) {
+    for (int h = blockIdx.z * 4 + wave; h < a.H; h += step)
+      for (int j = 0; j < V; ++j) qo[(int64_t)h * HD + j] = E::mk(__builtin_nanf(""));
+    return;
+  }
   if (parents) {  // rotary position: the token's depth in the tree behind the cache
     if (wave == 0) {
       const uint64_t path = tree_path(parents, a.S);
@@ -129,9 +135,10 @@ __global__ void __launch_bounds__(256) kv8_write_kernel(Kv8WriteArgs a) {
   }
   const int64_t rp = pos[0] + (parents ? depth : t), slot = pos[0] + t;
   if (tid < hr) {
-    const double ang = (double)rp * a.inv_freq[tid];
-    cs[tid] = cos(ang);
-    sn[tid] = sin(ang);
+    double si, co;
+    sincos((double)rp * a.inv_freq[tid], &si, &co);
+    csf[tid] = (float)(cs[tid] = co);
+    snf[tid] = (float)(sn[tid] = si);
   }
   float wq[V], wk[V];
 #pragma unroll
@@ -142,7 +149,7 @@ __global__ void __launch_bounds__(256) kv8_write_kernel(Kv8WriteArgs a) {
   __syncthreads();
   // x / rms(x) * w, rotated on its first rd dims, in T; through the wave's own row area, whose LDS
   // operations complete in order
-  auto norm_rope = [&](auto zero, const uint16_t (&in)[V], const float (&w)[V], auto (&f)[V]) {
+  auto norm_rope = [&](auto zero, const vec_t& in, const float (&w)[V], auto* cs, auto* sn, auto (&f)[V]) {
     using T = decltype(zero);
     T* const rw = reinterpret_cast<T*>(row[wave]);
     T ss = 0;
@@ -151,9 +158,10 @@ __global__ void __launch_bounds__(256) kv8_write_kernel(Kv8WriteArgs a) {
       f[j] = E::ld(in[j]);
       ss += f[j] * f[j];
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
-    const T rn = (T)1 / sqrt(ss / (T)HD + (T)a.eps);
+    ss = lanes_sum(ss) * (T)(1.0 / HD) + (T)a.eps;
+    T rn;
+    if constexpr (sizeof(T) == 4) rn = __builtin_amdgcn_rsqf(ss);
+    else rn = rsqrt(ss);
 #pragma unroll
     for (int j = 0; j < V; ++j) rw[d0 + j] = f[j] = f[j] * rn * (T)w[j];
     __builtin_amdgcn_wave_barrier();
@@ -163,17 +171,15 @@ __global__ void __launch_bounds__(256) kv8_write_kernel(Kv8WriteArgs a) {
       if (d < a.rd) {
         const int i = d < hr ? d : d - hr;
         const T other = d < hr ? -rw[d + hr] : rw[i];
-        f[j] = f[j] * (T)cs[i] + other * (T)sn[i];
+        f[j] = f[j] * cs[i] + other * sn[i];
       }
     }
     __builtin_amdgcn_wave_barrier();
   };
   for (; h0 < nh; h0 += step * kWriteRows) {
-    uint16_t cur[kWriteRows][V];
+    vec_t cur[kWriteRows];
 #pragma unroll
-    for (int u = 0; u < kWriteRows; ++u)
-#pragma unroll
-      for (int j = 0; j < V; ++j) cur[u][j] = x[u][j];
+    for (int u = 0; u < kWriteRows; ++u) cur[u] = x[u];
     if (h0 + step * kWriteRows < nh) load(h0 + step * kWriteRows);
 #pragma unroll
     for (int u = 0; u < kWriteRows; ++u) {
@@ -181,7 +187,7 @@ __global__ void __launch_bounds__(256) kv8_write_kernel(Kv8WriteArgs a) {
       if (h >= nh) break;
       if (h < a.H) {
         float f[V];
-        norm_rope(0.f, cur[u], wq, f);
+        norm_rope(0.f, cur[u], wq, csf, snf, f);
         vec_t o;
 #pragma unroll
         for (int j = 0; j < V; ++j) o[j] = E::mk(f[j]);
@@ -189,27 +195,52 @@ __global__ void __launch_bounds__(256) kv8_write_kernel(Kv8WriteArgs a) {
         continue;
       }
       const bool isk = h < a.H + a.Hkv;
-      double f[V], mx = 0;
-      if (isk) {
-        norm_rope(0.0, cur[u], wk, f);
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) f[j] = E::ld(cur[u][j]);
-      }
+      double f[V];
+      float x32[V];
+      float s;
       bool bad = false;
+      if (isk) {
+        norm_rope(0.0, cur[u], wk, cs, sn, f);
+        double mx = 0;
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        bad |= !(fabs(f[j]) <= DBL_MAX);
-        mx = fmax(mx, fabs(f[j]));
+        for (int j = 0; j < V; ++j) {
+          bad |= !(fabs(f[j]) <= DBL_MAX);
+          mx = fmax(mx, fabs(f[j]));
+          x32[j] = (float)f[j];
+        }
+        s = (float)(lanes_reduce(mx, [](double x, double y) { return fmax(x, y); }) / 127.0);
+      } else {
+        float mx = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          f[j] = x32[j] = E::ld(cur[u][j]);
+          bad |= !(fabsf(x32[j]) <= FLT_MAX);
+          mx = fmaxf(mx, fabsf(x32[j]));
+        }
+        s = (float)((double)lanes_reduce(mx, [](float x, float y) { return fmaxf(x, y); }) / 127.0);
       }
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) mx = fmax(mx, __shfl_xor(mx, o, 64));
-      float s = (float)(mx / 127.0);
       if (__any(bad) || !(s <= FLT_MAX)) s = __builtin_nanf("");
       bytes_t o;
+      if (s > 0.f) {
+        const float inv = 1.f / s;  // infinite for the smallest scales: their quotients are not finite, and divided in double
+        float n[V];
+        bool close = false;
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        o[j] = (uint8_t)(s > 0.f ? 128 + (int)fmin(fmax(rint(f[j] / (double)s), -127.0), 127.0) : 128);
+        for (int j = 0; j < V; ++j) {
+          const float t = x32[j] * inv;
+          n[j] = rintf(t);
+          close |= !(fabsf(t - n[j]) < 0.4999f);
+        }
+        if (__any(close)) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) n[j] = (float)fmin(fmax(rint(f[j] / (double)s), -127.0), 127.0);
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = (uint8_t)(128 + (int)n[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = 128;
+      }
       const int64_t at = ((int64_t)bb * a.Hkv + (isk ? h - a.H : h - a.H - a.Hkv)) * a.L + slot;
       *reinterpret_cast<bytes_t*>((isk ? a.kc : a.vc) + at * HD + d0) = o;
       if (lane == 0) (isk ? a.ks : a.vs)[at] = s;
@@ -996,7 +1027,11 @@ static hipError_t launch_kv8_write_t(const Kv8WriteArgs& a, hipStream_t s) {
   const int rows = a.H + 2 * a.Hkv, most = (rows + 4 * kWriteRows - 1) / (4 * kWriteRows);
   const dim3 grid((unsigned)a.S, (unsigned)a.B, (unsigned)(tokens >= 1024 ? 1 : most));
   auto launch = [&](auto hd) {
-    hipLaunchKernelGGL((kv8_write_kernel<BF, decltype(hd)::value>), grid, dim3(256), 0, s, a);
+    constexpr int HD = decltype(hd)::value;
+    // a lane's values in one load: every head row starts at a multiple of them
+    const bool wide = ((reinterpret_cast<uintptr_t>(a.qg) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v)) % (HD / 32) |
+                       (uintptr_t)((a.qg_stride | a.k_stride | a.v_stride) % (HD / 64))) == 0;
+    hipLaunchKernelGGL((kv8_write_kernel<BF, HD>), grid, dim3(256), 0, s, a, wide);
     return hipGetLastError();
   };
   if (a.hd == 256) return launch(std::integral_constant<int, 256>{});

@@ -151,37 +151,41 @@ def gdn_tree(qkv, z, ab, conv_state, conv_w, ssm_a, dt_bias, rec_state, norm_w, 
     cached ones (-1); parents int32 (S,) or (B, S) on the device. The states are only read: the tokens
     that are kept go through ``gdn_seq`` afterwards. Returns (B, S, Hv*dv), NaN in batch rows whose parents are
     not such."""
-    dev = _on_gpu(qkv, z, ab, conv_state, conv_w, ssm_a, dt_bias, rec_state, norm_w, parents)
-    B, S = qkv.shape[0], qkv.shape[1]
+    index = qkv.get_device()
+    if index < 0 or any(t.get_device() != index for t in (z, ab, conv_state, conv_w, ssm_a, dt_bias, rec_state, norm_w, parents)):
+        raise ValueError("tensors must be on one GPU device")
+    dtype = qkv.dtype
+    B, S = qkv.shape[:2]
+    conv_dim = 2 * key_heads * head_k_dim + value_heads * head_v_dim
     rows = []
-    for t in (qkv, z, ab):
-        if (t.dim() != 3 or tuple(t.shape[:2]) != (B, S) or t.stride(2) != 1 or t.dtype != qkv.dtype
-                or (S > 1 and B > 1 and t.stride(0) != S * t.stride(1))):
+    for t, n in ((qkv, conv_dim), (z, value_heads * head_v_dim), (ab, 2 * value_heads)):
+        if tuple(t.shape) != (B, S, n):
+            raise ValueError("GatedDeltaNet tensor shapes do not match the head configuration")
+        row, token, inner = t.stride()
+        if t.dtype is not dtype or inner != 1 or (S > 1 and B > 1 and row != S * token):
             raise ValueError("qkv, z and ab must be (B, S, n) of one dtype, unit inner stride, rows at one stride")
-        rows.append(t.stride(0) if S == 1 else t.stride(1))
+        rows.append(row if S == 1 else token)
     for t in (conv_state, conv_w, norm_w):
-        if t.dtype != qkv.dtype or not t.is_contiguous():
+        if t.dtype is not dtype or not t.is_contiguous():
             raise ValueError("conv_state, conv_w and norm_w must be contiguous in the activation dtype")
     for t in (ssm_a, dt_bias, rec_state):
-        if t.dtype != torch.float32 or not t.is_contiguous():
+        if t.dtype is not torch.float32 or not t.is_contiguous():
             raise ValueError("ssm_a, dt_bias and rec_state must be contiguous float32")
-    if parents.dtype != torch.int32 or tuple(parents.shape) not in ((S,), (B, S)) or not parents.is_contiguous():
+    if parents.dtype is not torch.int32 or tuple(parents.shape) not in ((S,), (B, S)) or not parents.is_contiguous():
         raise ValueError("parents must be contiguous int32 (S,) or (B, S)")
     if S > MAX_TREE:
         raise ValueError(f"a tree holds at most {MAX_TREE} tokens, not {S}")
-    conv_dim = 2 * key_heads * head_k_dim + value_heads * head_v_dim
     K = conv_w.shape[-1]
-    if (qkv.shape[2] != conv_dim or z.shape[2] != value_heads * head_v_dim or ab.shape[2] != 2 * value_heads
-            or tuple(conv_state.shape) != (B, K - 1, conv_dim) or conv_w.numel() != conv_dim * K
+    if (tuple(conv_state.shape) != (B, K - 1, conv_dim) or conv_w.numel() != conv_dim * K
             or tuple(rec_state.shape) != (B, value_heads, head_k_dim, head_v_dim) or norm_w.numel() != head_v_dim
             or ssm_a.numel() != value_heads or dt_bias.numel() != value_heads):
         raise ValueError("GatedDeltaNet tensor shapes do not match the head configuration")
-    out = torch.empty(B, S, value_heads * head_v_dim, dtype=qkv.dtype, device=dev)
-    _lib.launch("gsq_gdn_tree", dev, (
+    out = qkv.new_empty((B, S, value_heads * head_v_dim))
+    _lib.launch("gsq_gdn_tree", qkv.device, (
         qkv.data_ptr(), rows[0], z.data_ptr(), rows[1], ab.data_ptr(), rows[2], conv_state.data_ptr(), conv_w.data_ptr(),
         ssm_a.data_ptr(), dt_bias.data_ptr(), rec_state.data_ptr(), norm_w.data_ptr(), parents.data_ptr(),
         parents.shape[0] if parents.dim() == 2 else 1, out.data_ptr(), value_heads * head_v_dim, B, S, key_heads,
-        value_heads, head_k_dim, head_v_dim, K, float(eps), _dt(qkv)), "gdn_tree")
+        value_heads, head_k_dim, head_v_dim, K, eps, _dt(qkv)), "gdn_tree")
     return out
 
 

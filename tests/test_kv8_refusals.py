@@ -95,14 +95,14 @@ def test_tensor_checks():
                 (torch.zeros(2, 2, dtype=torch.int64)[:, 0], None, 2, 5)):
         with pytest.raises(ValueError):
             kv8._where(*bad)
-    x = torch.zeros(2, 5, 64).half()
-    assert kv8._rows("x", 2, 5, x, x[..., :16]) == [64, 64]
-    assert kv8._rows("x", 2, 1, x[:, :1]) == [320] and kv8._rows("x", 1, 5, x[1:]) == [64]
-    for bad in (x[..., ::2], x.transpose(0, 1), x[:, :4]):
+    x, half = torch.zeros(2, 5, 64).half(), torch.float16
+    assert kv8._row_stride(x, 2, 5, 64, half) == 64 and kv8._row_stride(x[..., :16], 2, 5, 16, half) == 64
+    assert kv8._row_stride(x[:, :1], 2, 1, 64, half) == 320 and kv8._row_stride(x[1:], 1, 5, 64, half) == 64
+    for bad, n in ((x[..., ::2], 32), (x.transpose(0, 1), 64), (x[:, :4], 64), (x, 32), (x[0], 64), (x.float(), 64)):
         with pytest.raises(ValueError):
-            kv8._rows("x", *bad.shape[:2], bad)
+            kv8._row_stride(bad, *bad.shape[:2], n, half)
     with pytest.raises(TypeError):
-        kv8._rows("x", 2, 5, x.float())
+        kv8._dtype_code(x.float())
 
 
 def test_splits_rule():
