@@ -876,7 +876,8 @@ int gsq_kv8_read(const uint8_t* k_cache, const uint8_t* v_cache, const float* k_
     return fail(GSQ_E_VALUE, "rows %lld .. + %lld of a cache of %lld", (long long)start, (long long)n, (long long)max_len);
   if (head_dim <= 0 || head_dim % 16 || head_dim > 65536) return fail(GSQ_E_VALUE, "head dim must be a multiple of 16");
   if (heads == 0 || n == 0) return GSQ_OK;
-  if (heads >= (1ll << 31) || max_len >= (1ll << 31)) return fail(GSQ_E_VALUE, "invalid cache shape");
+  if (heads >= (1ll << 31) || max_len >= (1ll << 31) || heads * max_len >= (1ll << 40))
+    return fail(GSQ_E_VALUE, "invalid cache shape");
   if (!k_cache || !v_cache || !k_scale || !v_scale || !k || !v) return fail(GSQ_E_VALUE, "NULL pointer");
   if ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache) | reinterpret_cast<uintptr_t>(k) |
        reinterpret_cast<uintptr_t>(v)) & 15)

@@ -348,6 +348,11 @@ __device__ __forceinline__ uint32_t byte_pair(uint32_t second, uint32_t first, i
 
 // blocks of 32 positions that rows up to token t see
 __device__ __forceinline__ int kv8_blocks(int64_t pos, int t) { return (int)((pos + t) / 32) + 1; }
+// blocks of a split, for workgroups of rt rows: whole tiles of two where those are what the kernel takes
+__device__ __forceinline__ int kv8_per_split(int nblk, int nsplit, int rt) {
+  const int per = (nblk + nsplit - 1) / nsplit;
+  return rt > 16 ? (per + 1) & ~1 : per;
+}
 
 // What a workgroup is asked to do: 16 NT rows of one (batch row, KV head), positions of one split.
 template <int RT>
@@ -374,7 +379,7 @@ struct Kv8Task {
   // the blocks of this split; false if there are none
   __device__ bool blocks(const Kv8AttnArgs& a) {
     pos = posp[0];
-    const int nblk = kv8_blocks(pos, tlast), per = (nblk + a.nsplit - 1) / a.nsplit;
+    const int nblk = kv8_blocks(pos, tlast), per = kv8_per_split(nblk, a.nsplit, RT);
     blk0 = z * per;
     blk1 = min(nblk, blk0 + per);
     return blk0 < blk1;
@@ -490,14 +495,14 @@ struct Kv8Rows {
 
   // scores s of a block from position j0 on to weights pf; ks4, vs4: scales() of this lane's positions; rows
   // r0 + lane % 16 + 16 n; masked: some position may lie behind a row's token, or off its path
-  template <int RT>
+  template <int RT, int NB>  // NB: groups of 16 positions
   __device__ void weights(const Kv8AttnArgs& a, const Kv8Task<RT>& k, int r0, int64_t j0, bool masked, const uint64_t* paths,
-                          f32x4 (&s)[NT][2], const f32x4 (&ks4)[2], const f32x4 (&vs4)[2], u32x4 (&pf)[TERMS][NT]) {
+                          f32x4 (&s)[NT][NB], const f32x4 (&ks4)[NB], const f32x4 (&vs4)[NB], u32x4 (&pf)[NB / 2][TERMS][NT]) {
     const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
+      for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           s[n][b][e] = __builtin_fmaf(BF ? s[n][b][e] * rowc[n] : s[n][b][e], ks4[b][e], -m[n]);
@@ -509,7 +514,7 @@ struct Kv8Rows {
         uint64_t path = 0;
         if (k.parents) path = paths[tok];
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int node = node0 + 16 * b + e;
@@ -520,7 +525,7 @@ struct Kv8Rows {
     }
     float mx = -INFINITY;
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
 #pragma unroll
@@ -531,7 +536,7 @@ struct Kv8Rows {
       for (int n = 0; n < NT; ++n) {
         float x = -INFINITY;
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
           for (int e = 0; e < 4; ++e) x = fmaxf(x, s[n][b][e]);
         x = fmaxf(x, __shfl_xor(x, 16, 64));
@@ -546,7 +551,7 @@ struct Kv8Rows {
 #pragma unroll
         for (int i = 0; i < VB; ++i) acc[n][i] *= alpha;
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[n][b][e] -= up;
       }
@@ -555,7 +560,7 @@ struct Kv8Rows {
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
+      for (int b = 0; b < NB; ++b) {
         float w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -568,16 +573,18 @@ struct Kv8Rows {
 #pragma unroll
           for (int e = 0; e < 4; e += 2) {
             const f16x2 hi = __builtin_convertvector((f32x2){w[e], w[e + 1]}, f16x2);
-            pf[t][n][2 * b + e / 2] = __builtin_bit_cast(uint32_t, hi);
+            pf[b / 2][t][n][2 * (b & 1) + e / 2] = __builtin_bit_cast(uint32_t, hi);
             w[e] -= (float)hi.x;  // what the term leaves, for the next one
             w[e + 1] -= (float)hi.y;
           }
       }
     const u32x4 ones = {0x00800080u, 0x00800080u, 0x00800080u, 0x00800080u};  // 128 x 2^-24
 #pragma unroll
-    for (int t = 0; t < TERMS; ++t)
+    for (int b = 0; b < NB / 2; ++b)
 #pragma unroll
-      for (int n = 0; n < NT; ++n) wsum[n] = mma16(ones, pf[t][n], wsum[n]);
+      for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) wsum[n] = mma16(ones, pf[b][t][n], wsum[n]);
   }
   // output tile i += V's operand times the weights
   __device__ void add(int i, u32x4 vf, const u32x4 (&pf)[TERMS][NT]) {
@@ -707,12 +714,12 @@ __global__ void __launch_bounds__(256, 2) attn_kv8_rows_kernel(Kv8AttnArgs a) {
     }
     if (more) load_k(blk + 4);
     const int64_t j0 = (int64_t)blk * 32;
-    u32x4 pf[Kv8Rows<BF, HD, 1>::TERMS][1];
+    u32x4 pf[1][Kv8Rows<BF, HD, 1>::TERMS][1];
     rows.weights(a, k, k.r0, j0, k.parents ? j0 + 31 >= k.pos : j0 + 31 > k.pos + k.tfirst, paths, s, ks4, vs4, pf);
 #pragma unroll
     for (int i = 0; i < VB; ++i)  // dim VB c + i of the 8 positions: byte i & 3 of dword i / 4 of each row
       rows.add(i, (u32x4){byte_pair(vr[1][i >> 2], vr[0][i >> 2], i & 3), byte_pair(vr[3][i >> 2], vr[2][i >> 2], i & 3),
-                          byte_pair(vr[5][i >> 2], vr[4][i >> 2], i & 3), byte_pair(vr[7][i >> 2], vr[6][i >> 2], i & 3)}, pf);
+                          byte_pair(vr[5][i >> 2], vr[4][i >> 2], i & 3), byte_pair(vr[7][i >> 2], vr[6][i >> 2], i & 3)}, pf[0]);
     if (more) load_v(blk + 4);
     if (it % kBiasBlocks == 0 || !more) rows.take_bias();
   }
@@ -772,6 +779,7 @@ __global__ void __launch_bounds__(256, 2) attn_kv8_tile_kernel(Kv8AttnArgs a) {
   constexpr int KS = HD / 32, VB = HD / 16, RT = 64 * NT, NC = HD / 16;  // NC: 16-byte pieces of a row
   constexpr int PW = VB < 8 ? VB : 8, NP = VB / PW;                      // dims of a V piece, pieces of a lane
   constexpr int SH = HD == 256 ? 0 : (HD == 128 ? 1 : 2);                // 2^SH rows to the 64 banks
+  constexpr int KB = HD == 256 || NT == 4 ? 1 : 2;  // blocks of 32 positions in one step, as the registers allow
   constexpr int TB = 64 * HD;                                           // bytes of a tile of K or V
   typedef uint32_t vpiece __attribute__((ext_vector_type(PW / 4)));
   extern __shared__ __attribute__((aligned(16))) uint8_t kv8_lds[];
@@ -857,28 +865,30 @@ __global__ void __launch_bounds__(256, 2) attn_kv8_tile_kernel(Kv8AttnArgs a) {
       __builtin_amdgcn_wave_barrier();
     }
 #pragma unroll 1
-    for (int sb = 0; sb < 2; ++sb) {
+    for (int sb = 0; sb < 2; sb += KB) {
       const int64_t j0 = (int64_t)(blk + sb) * 32;
       if (!on || blk + sb >= k.blk1 || j0 > plast) continue;
       const int ln = anew(lane), g = ln >> 4, c = ln & 15;
       const uint8_t* const kb = kt + (32 * sb + c) * HD;
       const uint8_t* const vb = kt + TB;
       const float* const sc = sw + 32 * sb + 4 * g;
-      f32x4 s[NT][2];
+      f32x4 s[NT][2 * KB];
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
+      for (int n = 0; n < NT; ++n) {
+        s[n][0] = bl[16 * n + c];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) s[n][b] = bl[16 * n + c];
+        for (int b = 1; b < 2 * KB; ++b) s[n][b] = s[n][0];
+      }
 #pragma unroll
       for (int st = 0; st < KS / 2; ++st) {
-        u32x4 w[2];
+        u32x4 w[2 * KB];
 #pragma unroll
-        for (int b = 0; b < 2; ++b)  // position 32 sb + 16 b + c: its swizzle does not depend on sb and b
+        for (int b = 0; b < 2 * KB; ++b)  // position 32 sb + 16 b + c: its swizzle does not depend on sb and b
           w[b] = *reinterpret_cast<const u32x4*>(kb + 16 * b * HD + 16 * ((4 * st + g) ^ ((c >> SH) & (NC - 1))));
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
+          for (int b = 0; b < 2 * KB; ++b) {
             const u32x4 kf = bytes8(w[b][2 * h], w[b][2 * h + 1]);
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -886,29 +896,34 @@ __global__ void __launch_bounds__(256, 2) attn_kv8_tile_kernel(Kv8AttnArgs a) {
           }
       }
       if constexpr (HD == 256) __builtin_amdgcn_sched_barrier(0);  // what follows needs the registers of K's pieces
-      f32x4 ks4[2], vs4[2];
+      f32x4 ks4[2 * KB], vs4[2 * KB];
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
+      for (int b = 0; b < 2 * KB; ++b) {
         ks4[b] = *reinterpret_cast<const f32x4*>(sc + 16 * b);
         vs4[b] = *reinterpret_cast<const f32x4*>(sc + 64 + 16 * b);
       }
-      u32x4 pf[Kv8Rows<BF, HD, NT>::TERMS][NT];
-      rows.weights(a, k, r0, j0, k.parents ? j0 + 31 >= k.pos : j0 + 31 > pfirst, paths, s, ks4, vs4, pf);
+      u32x4 pf[KB][Kv8Rows<BF, HD, NT>::TERMS][NT];
+      const int64_t end = j0 + 32 * KB - 1;
+      rows.weights(a, k, r0, j0, k.parents ? end >= k.pos : end > pfirst, paths, s, ks4, vs4, pf);
 #pragma unroll
-      for (int h = 0; h < NP; ++h) {
-        vpiece v[8];
+      for (int q = 0; q < KB; ++q)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int key = 32 * sb + 16 * (i >> 2) + 4 * g + (i & 3);
-          const int row = HD == 256 ? key : key ^ (g & ((1 << SH) - 1));
-          const int at = HD == 256 ? ((128 * h + PW * c) ^ ((g & 1) << 7)) : PW * c;
-          v[i] = *reinterpret_cast<const vpiece*>(vb + row * HD + at);
+        for (int h = 0; h < NP; ++h) {
+          vpiece v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int key = 32 * (sb + q) + 16 * (i >> 2) + 4 * g + (i & 3);
+            const int row = HD == 256 ? key : key ^ (g & ((1 << SH) - 1));
+            const int at = HD == 256 ? ((128 * h + PW * c) ^ ((g & 1) << 7)) : PW * c;
+            v[i] = *reinterpret_cast<const vpiece*>(vb + row * HD + at);
+          }
+#pragma unroll
+          for (int i = 0; i < PW; ++i)  // dim (HD / NP) h + PW c + i of the 8 positions
+            rows.add(PW * h + i,
+                     (u32x4){byte_pair(v[1][i >> 2], v[0][i >> 2], i & 3), byte_pair(v[3][i >> 2], v[2][i >> 2], i & 3),
+                             byte_pair(v[5][i >> 2], v[4][i >> 2], i & 3), byte_pair(v[7][i >> 2], v[6][i >> 2], i & 3)},
+                     pf[q]);
         }
-#pragma unroll
-        for (int i = 0; i < PW; ++i)  // dim (HD / NP) h + PW c + i of the 8 positions
-          rows.add(PW * h + i, (u32x4){byte_pair(v[1][i >> 2], v[0][i >> 2], i & 3), byte_pair(v[3][i >> 2], v[2][i >> 2], i & 3),
-                                       byte_pair(v[5][i >> 2], v[4][i >> 2], i & 3), byte_pair(v[7][i >> 2], v[6][i >> 2], i & 3)}, pf);
-      }
     }
     if (it % (kBiasBlocks / 2) == kBiasBlocks / 2 - 1 || blk + 2 >= k.blk1) rows.take_bias();
   }
@@ -969,7 +984,7 @@ __global__ void __launch_bounds__(64 * kMergeWaves) attn_kv8_merge_kernel(Kv8Att
       for (int j = 0; j < V; ++j) out[j] = E::mk(__builtin_nanf(""));
     return;
   }
-  const int nblk = kv8_blocks(posp[0], min(r / rt * rt + rt - 1, R - 1) / rep), per = (nblk + a.nsplit - 1) / a.nsplit;
+  const int nblk = kv8_blocks(posp[0], min(r / rt * rt + rt - 1, R - 1) / rep), per = kv8_per_split(nblk, a.nsplit, rt);
   const int nz = (nblk + per - 1) / per;
   const float2* const ml = reinterpret_cast<const float2*>(a.part + rows * a.nsplit * HD) + i * a.nsplit;
   const float* const po = a.part + i * a.nsplit * HD + d;

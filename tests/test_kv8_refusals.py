@@ -36,7 +36,7 @@ LAYOUT = [dict(heads=3, kv_heads=2), dict(kv_heads=0), dict(head_dim=96), dict(h
                                      dict(q=X + 8), dict(q_stride=516), dict(qg=X + 4), dict(qg_stride=1026),
                                      dict(out_stride=514), dict(out=X + 2)]),
     ("gsq_kv8_read", READ, [dict(n=101), dict(start=101, n=0), dict(start=1), dict(start=-1), dict(n=-1), dict(head_dim=100),
-                            dict(k_cache=None), dict(v=X + 8), dict(heads=-1)]),
+                            dict(k_cache=None), dict(v=X + 8), dict(heads=-1), dict(heads=1 << 30, max_len=1 << 20)]),
     ("gsq_gdn_tree", TREE, [dict(seq=65), dict(seq=-1), dict(batch=65536), dict(key_heads=3), dict(key_heads=0),
                             dict(head_k_dim=130), dict(head_k_dim=66), dict(head_v_dim=96), dict(head_v_dim=320),
                             dict(conv_kernel=1), dict(conv_kernel=9), dict(n_trees=3), dict(parents=None), dict(rec_state=None),
