@@ -250,7 +250,8 @@ __global__ void __launch_bounds__(256) kv8_write_kernel(Kv8WriteArgs a, bool wid
 
 // ---- reading back --------------------------------------------------------------------------------
 // out[b, h, j, :] = round((u - 128) s), the product in float32, of rows start .. start + n - 1 of both caches: a thread per 16
-// values, K's rows first. Bound by memory: hd + 4 bytes read and hd values written per row.
+// values, K's rows first. Bound by memory: hd + 4 bytes read and hd values written per row (8 rows of 4 x 512
+// positions, 25 MB, 7.8 us).
 template <int DT>  // 0 float32, 1 fp16, 2 bf16
 __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8ReadArgs a) {
   const int per = a.hd >> 4;  // threads per row
@@ -627,6 +628,9 @@ __device__ __forceinline__ void kv8_out(const uint16_t* gate, uint16_t* out, con
 // Few rows (16 a workgroup): the cache goes by once, and its bytes bound the kernel. Four waves take the
 // blocks in turn, each with a softmax of its own; K and V go from memory to registers in 16-byte pieces,
 // a block ahead, and are expanded there: no LDS and no barrier in the loop. The waves are merged at the end.
+// One token of 24 heads over 131071 positions (4 KV heads of 256, 272 MB): 44 us, 6.2 TB/s with part of it in
+// the last-level cache; 32 rows of 4096 to 8191 positions (414 MB) 76 us. Over 300 positions 10.5 us, all of it
+// latency: position, queries and first blocks, two more blocks, gates.
 template <bool BF, int HD>
 __global__ void __launch_bounds__(256, 2) attn_kv8_rows_kernel(Kv8AttnArgs a) {
   constexpr int KS = HD / 32, KL = HD / 64, VB = HD / 16, RT = 16;  // VB: bytes of a lane's V piece
@@ -770,10 +774,18 @@ constexpr int kv8_lds_steps(int hd) { return hd == 256 ? 1 : 0; }
 
 // Many rows: 16 NT a wave, four waves to a workgroup, over tiles of 64 positions whose bytes come to LDS by
 // DMA, a tile ahead (two buffers, one barrier a tile), and are read by every wave: 16 bytes of K or PW of V a
-// lane at a time, expanded in registers. Bound by the matrix cores and the vector instructions around
-// them (two waves a SIMD overlap them).
+// lane at a time, expanded in registers.
 //  * K's 16-byte pieces are XOR-swizzled by position, V's pieces (or rows) by bits 2 and 3 of it, so that the
 //    lanes of a read fall on different banks; the DMA's source address does it.
+//  * What bounds it are vector instructions and matrix cores: at head dim 256 a wave's 32 rows and a block of 32
+//    positions take 100 MFMAs (fp16: 1600 cycles; bf16 68) and about 330 vector instructions (128 of them
+//    expand bytes), two waves a SIMD overlapping them in part. Matrix instructions go at raised priority
+//    (353 -> 346 us). The accumulators and queries of two waves a SIMD fill the 512 registers: what the loop
+//    does not need in them lies in LDS (a step of the queries, biases, scales, paths), as spills would wait for the
+//    DMA in flight (413 -> 370).
+//  * 4096 tokens of 24 heads of 256 in fp16 346 us (0.60 PFLOP/s without the second term of the weights; a large
+//    library product 1.31), of which a fifth is the triangle's tail; 700 bf16 tokens of 2 x 32 heads of 128 behind
+//    5000 positions 270 (352 workgroups on 256 CUs); a tree of 64 tokens of 4 rows behind 8000 to 16000 134 + 15.
 template <bool BF, int HD, int NT>
 __global__ void __launch_bounds__(256, 2) attn_kv8_tile_kernel(Kv8AttnArgs a) {
   constexpr int KS = HD / 32, VB = HD / 16, RT = 64 * NT, NC = HD / 16;  // NC: 16-byte pieces of a row
@@ -879,6 +891,7 @@ __global__ void __launch_bounds__(256, 2) attn_kv8_tile_kernel(Kv8AttnArgs a) {
 #pragma unroll
         for (int b = 1; b < 2 * KB; ++b) s[n][b] = s[n][0];
       }
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int st = 0; st < KS / 2; ++st) {
         u32x4 w[2 * KB];
@@ -895,6 +908,7 @@ __global__ void __launch_bounds__(256, 2) attn_kv8_tile_kernel(Kv8AttnArgs a) {
               s[n][b] = mma16(kf, 2 * st + h < QL ? ql[(n * QL + 2 * st + h) * 64] : qf[n][2 * st + h], s[n][b]);
           }
       }
+      __builtin_amdgcn_s_setprio(0);
       if constexpr (HD == 256) __builtin_amdgcn_sched_barrier(0);  // what follows needs the registers of K's pieces
       f32x4 ks4[2 * KB], vs4[2 * KB];
 #pragma unroll
@@ -905,6 +919,7 @@ __global__ void __launch_bounds__(256, 2) attn_kv8_tile_kernel(Kv8AttnArgs a) {
       u32x4 pf[KB][Kv8Rows<BF, HD, NT>::TERMS][NT];
       const int64_t end = j0 + 32 * KB - 1;
       rows.weights(a, k, r0, j0, k.parents ? end >= k.pos : end > pfirst, paths, s, ks4, vs4, pf);
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int q = 0; q < KB; ++q)
 #pragma unroll
@@ -925,6 +940,7 @@ __global__ void __launch_bounds__(256, 2) attn_kv8_tile_kernel(Kv8AttnArgs a) {
                      pf[q]);
         }
     }
+    __builtin_amdgcn_s_setprio(0);
     if (it % (kBiasBlocks / 2) == kBiasBlocks / 2 - 1 || blk + 2 >= k.blk1) rows.take_bias();
   }
   // a lane's outputs: row r0 + 16 n + c, dims (HD / NP) h + PW (4 g + e) + i
@@ -959,7 +975,8 @@ __global__ void __launch_bounds__(256, 2) attn_kv8_tile_kernel(Kv8AttnArgs a) {
 
 // Outputs of split positions: a workgroup per row, a wave to every eight splits (up to 16 waves); each wave weighs
 // those of its splits that hold positions of the row's tile by their largest maximum, and the waves meet
-// in LDS. Bound by the latency of one read of the partial outputs, all in flight at once.
+// in LDS. Bound by the latency of one read of the partial outputs, all in flight at once (128 splits of 24 rows
+// 7 us, with one wave a row 49).
 constexpr int kMergeWaves = 16, kMergeSplits = 8;
 
 template <bool BF, int HD>
