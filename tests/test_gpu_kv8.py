@@ -198,9 +198,20 @@ def _attn_inputs(B, S, pos, L, H, G, hd, dtype, tree=None):
             "pos": torch.tensor(pos), "parents": None if tree is None else _tree(B, S, g, tree)}
 
 
-def _attn(t, H, G, hd, **kw):
+def _attn(t, H, G, hd, long=False, **kw):
+    """``long``: in caches long enough that the tile kernel is chosen (32768 tiles of 16 rows x blocks of 32
+    positions, for more than 32 rows of a KV head), which hold anything behind the tokens."""
     from mlx_gsq_amd.runtime.kernels import kv8
     d = {n: None if x is None else x.cuda() for n, x in t.items()}
+    if long:
+        B, S = t["q"].shape[:2]
+        tiles = -(-S * (H // G) // 16) * B * G
+        assert S * (H // G) > 32
+        for n in ("k", "v", "ks", "vs"):
+            x = d[n]
+            d[n] = x.new_full((B, G, max(x.shape[2], 32 * -(-32768 // tiles)), *x.shape[3:]), 255 if x.dtype == torch.uint8 else
+                              float("inf" if n == "vs" else "nan"))
+            d[n][:, :, :x.shape[2]] = x
     return kv8.attn_kv8(d["q"], d["qg"], d["k"], d["v"], d["ks"], d["vs"], d["pos"], heads=H, kv_heads=G, head_dim=hd,
                         parents=d["parents"], **kw).cpu()
 
@@ -275,6 +286,37 @@ def test_attn_kv8_matches_float64(case):
         t["ks"][b, :, end:], t["vs"][b, :, end:] = float("nan"), float("inf")
     _check(_attn(t, H, G, hd, splits=1), want, tol, dtype)
     _check(_attn(t, H, G, hd), want, tol, dtype)
+    if S * (H // G) > 32:
+        _check(_attn(t, H, G, hd, long=True, splits=1), want, tol, dtype)
+
+
+# rows around the 32-row waves and 128-row tiles, positions around the 64-position tiles
+TILES = [(1, 33, [0], 33, 1, 1, 256, F16, None), (1, 64, [63], 127, 2, 1, 256, BF16, None), (2, 43, [64, 0], 107, 6, 2, 128, F16, None),
+         (1, 129, [1], 130, 1, 1, 64, BF16, None), (3, 21, [95, 200, 31], 221, 24, 4, 256, F16, "random"),
+         (1, 64, [0], 64, 16, 2, 128, BF16, "random"), (1, 9, [129], 138, 64, 4, 64, F16, "chain"),
+         (1, 300, [700], 1000, 6, 1, 256, F16, None), (2, 100, [0], 100, 40, 8, 256, BF16, None)]
+
+
+@pytest.mark.parametrize("splits", [1, 2, 5, 64])
+@pytest.mark.parametrize("case", TILES, ids=_name)
+def test_attn_kv8_tiles(case, splits):
+    """The kernel of many rows, whose splits are whole tiles of 64 positions."""
+    B, S, pos, L, H, G, hd, dtype, tree = case
+    t = _attn_inputs(B, S, pos, L, H, G, hd, dtype, tree)
+    want, tol = _reference(t, H, G, hd)
+    _check(_attn(t, H, G, hd, long=True, splits=splits), want, tol, dtype)
+
+
+@pytest.mark.parametrize("tree", [None, "random"])
+def test_attn_kv8_tiles_of_256_rows(tree):
+    """Head dim 64 with 512 workgroups of them."""
+    B, S, pos, L, H, G, hd = 32, 40, [650 - 20 * i for i in range(32)], 700, 16, 16, 64
+    t = _attn_inputs(B, S, pos, L, H, G, hd, F16, tree)
+    got = _attn(t, H, G, hd, long=True, splits=1)
+    for b in (0, 13, 31):
+        one = {n: None if x is None else x[b:b + 1] for n, x in t.items()}
+        want, tol = _reference(one, H, G, hd)
+        _check(got[b:b + 1], want, tol, F16)
 
 
 @pytest.mark.parametrize("splits", [2, 3, 7, 64])
@@ -308,6 +350,9 @@ def test_attn_kv8_scores_and_scales_that_move(order, dtype):
     want, tol = _reference(t, H, G, hd)
     for splits in (1, 4):
         _check(_attn(t, H, G, hd, splits=splits), want, tol, dtype)
+    many = dict(t, q=t["q"].repeat(1, 4, 1)[:, :9], qg=t["qg"].repeat(1, 4, 1)[:, :9], pos=torch.tensor([494]))
+    want, tol = _reference(many, H, G, hd)
+    _check(_attn(many, H, G, hd, long=True, splits=1), want, tol, dtype)
 
 
 def test_attn_kv8_bf16_query_sizes():
@@ -324,16 +369,17 @@ def test_attn_kv8_bf16_query_sizes():
     _check(_attn(t, H, G, hd, splits=1), want, tol, BF16)
 
 
+@pytest.mark.parametrize("long", [False, True])
 @pytest.mark.parametrize("splits", [1, 3])
 @pytest.mark.parametrize("tree", [None, "random"])
-def test_attn_kv8_not_finite(tree, splits):
+def test_attn_kv8_not_finite(tree, splits, long):
     """A NaN row of the cache, or a query or gate that is not finite, reaches the outputs that see it; every other
     is what it is without it, within the rounding bound (the rows of a wave share when their references
     move, so not bit for bit)."""
     B, S, pos, L, H, G, hd = 2, 40, [50, 61], 110, 4, 2, 64
     t = _attn_inputs(B, S, pos, L, H, G, hd, F16, tree)
     clean, tol = _reference(t, H, G, hd)
-    _check(_attn(t, H, G, hd, splits=splits), clean, tol, F16)
+    _check(_attn(t, H, G, hd, long=long, splits=splits), clean, tol, F16)
 
     def sees(b, node):
         if tree is None:
@@ -341,7 +387,7 @@ def test_attn_kv8_not_finite(tree, splits):
         return [node in _chain(t["parents"][b], i) for i in range(S)]
 
     def check(changed, bad):
-        got = _attn(dict(t, **changed), H, G, hd, splits=splits).view(B, S, H, hd)
+        got = _attn(dict(t, **changed), H, G, hd, long=long, splits=splits).view(B, S, H, hd)
         assert torch.isnan(got[bad]).all()
         _check(got[~bad], clean[~bad], tol[~bad], F16)
     for name in ("ks", "vs"):
@@ -367,6 +413,19 @@ def test_attn_kv8_not_finite(tree, splits):
     bad = torch.zeros(B, S, H, hd, dtype=torch.bool)
     bad[1, 39, 1, 5] = True
     check({"qg": x}, bad)
+
+
+@pytest.mark.parametrize("splits", [1, 4])
+def test_attn_kv8_tiles_outside_the_cache(splits):
+    t = _attn_inputs(2, 40, [0, 7], 60, 2, 1, 64, F16, "random")
+    clean = _attn(t, 2, 1, 64, long=True, splits=splits)
+    bad = dict(t, pos=torch.tensor([-1, 7]))
+    got = _attn(bad, 2, 1, 64, long=True, splits=splits)
+    assert torch.isnan(got[0]).all() and torch.equal(got[1], clean[1]) and torch.isfinite(clean).all()
+    bad = dict(t, parents=t["parents"].clone())
+    bad["parents"][1, 39] = 39
+    got = _attn(bad, 2, 1, 64, long=True, splits=splits)
+    assert torch.isnan(got[1]).all() and torch.equal(got[0], clean[0])
 
 
 @pytest.mark.parametrize("splits", [1, 4])
