@@ -305,13 +305,17 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8ReadArgs a) {
 //    16 bytes hold. V's are spread so that a lane's piece of a row is PW neighbouring dims, each of
 //    another output tile, and two rows give a pair of one tile's operand by one v_perm.
 //  * The reference of the exponent moves only when a score passes it by 2^kLazy, for all rows of the
-//    wave at once: mostly no rescaling and no exchange between lanes in the loop.
+//    wave at once: mostly no rescaling and no exchange between lanes in the loop. It is a row's largest score,
+//    or lower where that position's V row is small against the largest one met: then what the row's largest
+//    weight is decides, as V rows that it does not see, or hardly, are not to take its weights' bits.
 //  * A weight (probability times V scale, 2^kPScale over the largest V scale met) is at most 2^(kLazy + 3 +
 //    kPScale) = 2^15 and held in fp16: for bf16 outputs in one value (11 bits, eight times finer than the
 //    output's own rounding), for fp16 outputs in two (22 bits, down to 2^-25 of the unit), as one would
 //    add an error as large as the output's rounding.
 constexpr float kLazy = 6.f;
 constexpr float kPScale = 6.f;
+constexpr float kLeast = 2.f;  // a row's largest weight stays above 2^kLeast
+constexpr float kFar = 60.f;   // as long as its scores pass the reference by less than that
 constexpr int kBiasBlocks = 32;  // blocks between two subtractions of 128 times the weights
 
 __device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c) {
@@ -448,15 +452,16 @@ template <bool BF, int HD, int NT>
 struct Kv8Rows {
   static constexpr int VB = HD / 16, TERMS = BF ? 1 : 2;  // output tiles; fp16 values that hold a weight
   float rowc[NT], m[NT], l[NT];
+  float* tops;  // LDS, row 16 n + c: power of two of the row's largest weight, as of the last move of its reference
   bool unset[NT];  // the row has seen no position yet: m is 0
   bool pending;    // some row of the wave is unset
-  float vref, vunit;  // largest V scale met (the weights' unit), and 2^kPScale over it
+  float vref, vunit;  // power of two below the largest V scale met (the weights' unit), and 2^kPScale over it
   f32x4 acc[NT][VB], wsum[NT];  // wsum: 128 times the weights, in acc's unit
 
   __device__ void init(const float* rowc_s) {
     pending = true;
-    vref = 0x1p-100f;
-    vunit = 0x1p106f;
+    vref = 0x1p-120f;
+    vunit = 0x1p126f;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       rowc[n] = rowc_s[16 * n];
@@ -466,6 +471,11 @@ struct Kv8Rows {
 #pragma unroll
       for (int i = 0; i < VB; ++i) acc[n][i] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
+  }
+  __device__ void init_tops(float* p) {
+    tops = p;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) tops[16 * n + (threadIdx.x & 15)] = -INFINITY;
   }
   // factor of K's scales: fp16 queries need none of their own
   __device__ static float key_factor() { return 1.44269504088896340736f / sqrtf((float)HD) * (BF ? 1.f : 0x1p24f); }
@@ -481,11 +491,19 @@ struct Kv8Rows {
       float x = vs;
 #pragma unroll
       for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o, 64));
-      const float f = vref / x;
-      vref = uniform(x);
-      vunit = uniform(exp2_raw(kPScale) / x);
+      const int ex = ilogbf(uniform(x)), c = anew(threadIdx.x) & 15;
+      const float d = (float)(ex - ilogbf(vref));
+      vref = uniform(ldexpf(1.f, ex));
+      vunit = uniform(ldexpf(exp2_raw(kPScale), -ex));
+      // the new unit comes off a row's reference, its weights stay as they are; off the weights only where
+      // the row's sum would leave float32
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
+        const float down = unset[n] ? 0.f : fminf(fmaxf(floorf(kFar + 20.f - __builtin_amdgcn_logf(sum(n))), 0.f), d);
+        const float f = exp2_raw(down - d);
+        m[n] -= down;
+        l[n] *= exp2_raw(down);
+        tops[16 * n + c] = tops[16 * n + c] + (down - d);
         wsum[n] *= f;
 #pragma unroll
         for (int i = 0; i < VB; ++i) acc[n][i] *= f;
@@ -533,17 +551,35 @@ struct Kv8Rows {
         for (int n = 0; n < NT; ++n) mx = fmaxf(mx, s[n][b][e]);
     if (pending || __any(mx > kLazy)) {
       bool left = false;
+      const int row = anew(threadIdx.x) & 15;
+      float xs[NT], ys[NT];  // largest scores and weights of the rows
+#pragma unroll
+      for (int n = 0; n < NT; ++n) xs[n] = ys[n] = -INFINITY;
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float v = __builtin_amdgcn_logf(vs4[b][e]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            xs[n] = fmaxf(xs[n], s[n][b][e]);
+            ys[n] = fmaxf(ys[n], s[n][b][e] + v);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        float x = -INFINITY;
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x = fmaxf(x, s[n][b][e]);
+        float x = xs[n], y = ys[n];
         x = fmaxf(x, __shfl_xor(x, 16, 64));
         x = fmaxf(x, __shfl_xor(x, 32, 64));
-        const float up = unset[n] ? (x == -INFINITY ? 0.f : x) : fmaxf(x, 0.f);
+        y = fmaxf(y, __shfl_xor(y, 16, 64));
+        y = fmaxf(y, __shfl_xor(y, 32, 64));
+        y = fmaxf(y, tops[16 * n + row]);
+        // to the largest score, as far as weights of 2^kLeast remain (they are at most 2^(x + 3 + kPScale))
+        const float to = fmaxf(fminf(x, y - kLeast), x - kFar);
+        const float up = unset[n] ? (x == -INFINITY ? 0.f : to) : fmaxf(to, 0.f);
         const float alpha = unset[n] ? 1.f : exp2_raw(-up);
+        tops[16 * n + row] = y - up;
         unset[n] = unset[n] && x == -INFINITY;
         left |= unset[n];
         m[n] += up;
@@ -636,7 +672,7 @@ __global__ void __launch_bounds__(256, 2) attn_kv8_rows_kernel(Kv8AttnArgs a) {
   constexpr int KS = HD / 32, KL = HD / 64, VB = HD / 16, RT = 16;  // VB: bytes of a lane's V piece
   typedef uint32_t vpiece __attribute__((ext_vector_type(VB / 4)));
   extern __shared__ __attribute__((aligned(16))) uint8_t kv8_lds[];
-  // queries, row factors and biases, scales of a wave's block; the merge of the waves takes the same memory
+  // queries, row factors and biases, scales of a wave's block, largest weights; the merge of the waves takes the same memory
   u32x4* const qs = reinterpret_cast<u32x4*>(kv8_lds);
   float* const rowc_s = reinterpret_cast<float*>(kv8_lds + RT * HD * 2);
   float* const bias_s = rowc_s + RT;
@@ -689,6 +725,7 @@ __global__ void __launch_bounds__(256, 2) attn_kv8_rows_kernel(Kv8AttnArgs a) {
   for (int s = 0; s < KS; ++s) qf[s] = qs[s * 64 + lane];
   Kv8Rows<BF, HD, 1> rows;
   rows.init(rowc_s + c);
+  rows.init_tops(bias_s + RT + 256 + wave * 16);
   const float bias = bias_s[c];
   for (int it = 1; blk < k.blk1; blk += 4, ++it) {
     const bool more = blk + 4 < k.blk1;
@@ -781,11 +818,11 @@ constexpr int kv8_lds_steps(int hd) { return hd == 256 ? 1 : 0; }
 //    positions take 100 MFMAs (fp16: 1600 cycles; bf16 68) and about 330 vector instructions (128 of them
 //    expand bytes), two waves a SIMD overlapping them in part. Matrix instructions go at raised priority
 //    (353 -> 346 us). The accumulators and queries of two waves a SIMD fill the 512 registers: what the loop
-//    does not need in them lies in LDS (a step of the queries, biases, scales, paths), as spills would wait for the
+//    does not need in them lies in LDS (a step of the queries, biases, scales, paths, largest weights), as spills would wait for the
 //    DMA in flight (413 -> 370).
-//  * 4096 tokens of 24 heads of 256 in fp16 346 us (0.60 PFLOP/s without the second term of the weights; a large
+//  * 4096 tokens of 24 heads of 256 in fp16 350 us (0.59 PFLOP/s without the second term of the weights; a large
 //    library product 1.31), of which a fifth is the triangle's tail; 700 bf16 tokens of 2 x 32 heads of 128 behind
-//    5000 positions 270 (352 workgroups on 256 CUs); a tree of 64 tokens of 4 rows behind 8000 to 16000 134 + 15.
+//    5000 positions 270 (352 workgroups on 256 CUs); a tree of 64 tokens of 4 rows behind 8000 to 16000 140 + 15.
 template <bool BF, int HD, int NT>
 __global__ void __launch_bounds__(256, 2) attn_kv8_tile_kernel(Kv8AttnArgs a) {
   constexpr int KS = HD / 32, VB = HD / 16, RT = 64 * NT, NC = HD / 16;  // NC: 16-byte pieces of a row
@@ -829,6 +866,7 @@ __global__ void __launch_bounds__(256, 2) attn_kv8_tile_kernel(Kv8AttnArgs a) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) bias[n] = bias_s[16 * (NT * wave + n) + c];
     __syncthreads();  // the buffers, and what lies behind them, may be written
+    rows.init_tops(reinterpret_cast<float*>(paths + 64) + wave * 16 * NT);
     if (k.parents && wave == 0) paths[lane] = tree_path(k.parents, a.S);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -1102,7 +1140,7 @@ static hipError_t launch_attn_kv8_t(const Kv8AttnArgs& a, hipStream_t s, int rt,
 
 template <bool BF, int HD>
 static hipError_t launch_attn_kv8_rows(const Kv8AttnArgs& a, hipStream_t s) {
-  constexpr int q = 16 * HD * 2 + 2 * 16 * 4 + 4 * 64 * 4, merge = 4 * 16 * (HD + 4) * 4 + 4 * 16 * 8;
+  constexpr int q = 16 * HD * 2 + 2 * 16 * 4 + 4 * 64 * 4 + 4 * 16 * 4, merge = 4 * 16 * (HD + 4) * 4 + 4 * 16 * 8;
   constexpr int lds = q > merge ? q : merge;
   return launch_attn_kv8_t<BF, HD>(a, s, 16, [&](dim3 grid) {
     static LdsLimit limit;
@@ -1114,7 +1152,7 @@ static hipError_t launch_attn_kv8_rows(const Kv8AttnArgs& a, hipStream_t s) {
 
 template <bool BF, int HD, int NT>
 static hipError_t launch_attn_kv8_tile(const Kv8AttnArgs& a, hipStream_t s) {
-  constexpr int q = 64 * NT * (HD * 2 + 8), tiles = 2 * (2 * 64 * HD + 512) + 4096 * NT * kv8_lds_steps(HD) + 2560 + 1024 * NT;
+  constexpr int q = 64 * NT * (HD * 2 + 8), tiles = 2 * (2 * 64 * HD + 512) + 4096 * NT * kv8_lds_steps(HD) + 2560 + (1024 + 256) * NT;
   constexpr int lds = q > tiles ? q : tiles;
   return launch_attn_kv8_t<BF, HD>(a, s, 64 * NT, [&](dim3 grid) {
     static LdsLimit limit;
@@ -1124,12 +1162,12 @@ static hipError_t launch_attn_kv8_tile(const Kv8AttnArgs& a, hipStream_t s) {
   });
 }
 
-// Rows of a workgroup. attn_kv8_rows_kernel (16) has the shorter chain, attn_kv8_tile_kernel takes a third less
-// time for each product: measured per tile of 16 rows and block of 32 positions, all CUs busy, head dim
-// 256, 0.56 against 0.37 us a SIMD; but 13 drafted tokens over 2000 positions 14 us against 33, and a prompt
-// of 333 19 against 46. So the tiles are for work of kTileBlocks and more. Head dim 64 takes 256 rows instead
-// of 128 where that makes two workgroups a CU (4096 tokens of 2 x 32 heads: 326 against 352 us); at 128 the
-// registers do not hold them (521 against 481).
+// Rows of a workgroup. attn_kv8_rows_kernel (16) has the shorter chain, attn_kv8_tile_kernel reads the cache once
+// for 128 rows: measured, 4 trees of 64 tokens behind up to 16000 positions took 315 us by rows of 16 and
+// take 149 by tiles, but 13 tokens behind 2000 take 14 us against 33, and a prompt of 333 19 against 46. So
+// the tiles are for work of kTileBlocks and more. Head dim 64 takes 256 rows instead of 128 where that makes
+// two workgroups a CU (4096 tokens of 2 x 32 heads: 326 against 352 us); at 128 the registers do not hold
+// them (521 against 481).
 constexpr int64_t kTileBlocks = 32768;
 
 int attn_kv8_plan(int64_t batch, int64_t seq, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_len) {

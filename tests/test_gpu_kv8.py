@@ -355,6 +355,43 @@ def test_attn_kv8_scores_and_scales_that_move(order, dtype):
     _check(_attn(many, H, G, hd, long=True, splits=1), want, tol, dtype)
 
 
+@pytest.mark.parametrize("dtype,power", [(F16, 14), (BF16, 14), (BF16, 45)])
+@pytest.mark.parametrize("tree", [None, "random"])
+@pytest.mark.parametrize("splits", [1, 3])
+def test_attn_kv8_large_values_elsewhere(dtype, power, tree, splits):
+    """V rows 2^power times the others', which most rows do not see (later tokens, other branches) or see with a
+    probability of next to nothing (keys against the queries): the others are what they would be."""
+    B, S, pos, L, H, G, hd = 2, 40, [300, 60], 340, 4, 2, 64
+    t = _attn_inputs(B, S, pos, L, H, G, hd, dtype, tree)
+    q = t["q"].view(B, S, H, hd)
+    q[..., 0] = 32.0
+    k, v = _values(t["k"], t["ks"]), _values(t["v"], t["vs"])
+    if dtype == F16:
+        v = v / 16
+    for b in range(B):
+        k[b, :, 20:24, 0] = -50.0     # 32 x 50 / 8 = 200 below the others: e^-200
+        v[b, :, 20:24] *= 2.0 ** power
+        v[b, :, pos[b] + 7::5] *= 2.0 ** power
+    t["k"], t["ks"] = _quantise(k)
+    t["v"], t["vs"] = _quantise(v)
+    want, tol = _reference(t, H, G, hd)
+    _check(_attn(t, H, G, hd, splits=splits), want, tol, dtype)
+    _check(_attn(t, H, G, hd, long=True, splits=splits), want, tol, dtype)
+
+
+@pytest.mark.parametrize("power", [-110, -60, 60, 100])
+def test_attn_kv8_small_and_large_values(power):
+    """bf16 V rows of any size, zeros among them."""
+    B, S, pos, L, H, G, hd = 1, 24, [150], 174, 4, 2, 64
+    t = _attn_inputs(B, S, pos, L, H, G, hd, BF16)
+    t["vs"][:, :, :70] = 0.0
+    want, tol = _reference(t, H, G, hd)
+    t["vs"] *= 2.0 ** power
+    for long in (False, True):
+        got = _attn(t, H, G, hd, long=long, splits=1)
+        _check((got.double() * 2.0 ** -power), want, tol, BF16)
+
+
 def test_attn_kv8_bf16_query_sizes():
     """bf16 queries of any size: rows of 2^-60, of 2^40 (with keys to match), and zeros, side by side."""
     B, S, pos, L, H, G, hd = 1, 4, [77], 90, 3, 1, 64
