@@ -1163,16 +1163,18 @@ static hipError_t launch_attn_kv8_tile(const Kv8AttnArgs& a, hipStream_t s) {
 }
 
 // Rows of a workgroup. attn_kv8_rows_kernel (16) has the shorter chain, attn_kv8_tile_kernel reads the cache once
-// for 128 rows: measured, 4 trees of 64 tokens behind up to 16000 positions took 315 us by rows of 16 and
-// take 149 by tiles, but 13 tokens behind 2000 take 14 us against 33, and a prompt of 333 19 against 46. So
-// the tiles are for work of kTileBlocks and more. Head dim 64 takes 256 rows instead of 128 where that makes
-// two workgroups a CU (4096 tokens of 2 x 32 heads: 326 against 352 us); at 128 the registers do not hold
-// them (521 against 481).
-constexpr int64_t kTileBlocks = 32768;
+// for 128 rows. Measured by rows and by tiles (24 heads of 256, fp16): 13 drafted tokens over 2000, 52000 and
+// 104000 positions 22 / 39, 71 / 79 and 135 / 110 us, 64 over 10800 and 21700 60 / 73 and 101 / 97, prompts
+// of 333, 1100 and 4096 17 / 49, 67 / 86 and 568 / 356. So the tiles are for kTileBlocks tiles of 16 rows by
+// 32 positions and more, where the two meet. Head dim 64 takes 256 rows instead of 128 where that makes two
+// workgroups a CU (4096 tokens of 2 x 32 heads: 326 against 352 us); at 128 the registers do not hold them
+// (521 against 481).
+constexpr int64_t kTileBlocks = 49152;
 
 int attn_kv8_plan(int64_t batch, int64_t seq, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_len) {
   const int64_t rows = seq * (heads / kv_heads), groups = batch * kv_heads;
-  if (rows <= 32 || (rows + 15) / 16 * groups * ((max_len + 31) / 32) < kTileBlocks) return 16;
+  // a row sees all but half of the new tokens on average
+  if (rows <= 32 || (rows + 15) / 16 * groups * ((max_len - seq / 2 + 31) / 32) < kTileBlocks) return 16;
   return head_dim == 64 && (rows + 255) / 256 * groups >= 512 ? 256 : 128;
 }
 

@@ -199,7 +199,7 @@ def _attn_inputs(B, S, pos, L, H, G, hd, dtype, tree=None):
 
 
 def _attn(t, H, G, hd, long=False, **kw):
-    """``long``: in caches long enough that the tile kernel is chosen (32768 tiles of 16 rows x blocks of 32
+    """``long``: in caches long enough that the tile kernel is chosen (49152 tiles of 16 rows x blocks of 32
     positions, for more than 32 rows of a KV head), which hold anything behind the tokens."""
     from mlx_gsq_amd.runtime.kernels import kv8
     d = {n: None if x is None else x.cuda() for n, x in t.items()}
@@ -209,7 +209,7 @@ def _attn(t, H, G, hd, long=False, **kw):
         assert S * (H // G) > 32
         for n in ("k", "v", "ks", "vs"):
             x = d[n]
-            d[n] = x.new_full((B, G, max(x.shape[2], 32 * -(-32768 // tiles)), *x.shape[3:]), 255 if x.dtype == torch.uint8 else
+            d[n] = x.new_full((B, G, max(x.shape[2], 32 * -(-49152 // tiles) + S), *x.shape[3:]), 255 if x.dtype == torch.uint8 else
                               float("inf" if n == "vs" else "nan"))
             d[n][:, :, :x.shape[2]] = x
     return kv8.attn_kv8(d["q"], d["qg"], d["k"], d["v"], d["ks"], d["vs"], d["pos"], heads=H, kv_heads=G, head_dim=hd,
