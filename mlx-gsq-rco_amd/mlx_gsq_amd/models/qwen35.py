@@ -548,13 +548,19 @@ class Qwen35Model(torch.nn.Module):
         if not 1 <= T <= 64:
             raise ValueError(f"a tree holds 1 to 64 tokens, not {T}")
         parents = torch.as_tensor(parents)
+        if B != cache.batch:
+            raise ValueError(f"ids of {B} rows for a cache of {cache.batch}")
         if tuple(parents.shape) not in ((T,), (B, T)):
             raise ValueError("parents must be (T,) or (B, T)")
         if parents.device.type == "cpu" and bool(((parents < -1) | (parents >= torch.arange(T))).any()):
             raise ValueError("a drafted token follows an earlier one, or -1")
         parents = parents.to(device=cache.pos.device, dtype=torch.int32).contiguous()
         cache.drafted = (parents, {})
-        return self._run(ids, cache, parents)
+        try:
+            return self._run(ids, cache, parents)
+        except BaseException:
+            cache.drafted = None  # what part of the layers has seen is no tree to accept from
+            raise
 
     def accept(self, cache: Qwen35Cache, path):
         """Keeps the drafted tokens ``path`` ((n,), or (B, n) for rows that keep other ones) of the tree that
@@ -572,8 +578,11 @@ class Qwen35Model(torch.nn.Module):
         if n:
             if bool(((path < 0) | (path >= T)).any()):
                 raise ValueError("path names tokens that were not drafted")
+            tree = parents.cpu().long()
+            if bool(((tree < -1) | (tree >= torch.arange(T))).any()):
+                raise ValueError("the drafted tokens were no tree: they are not in the cache")
             before = torch.cat([torch.full((B, 1), -1), path[:, :-1]], dim=1)
-            if not torch.equal(torch.gather(parents.cpu().long().expand(B, T), 1, path), before):
+            if not torch.equal(torch.gather(tree.expand(B, T), 1, path), before):
                 raise ValueError("path must lead from the cached tokens on, each token following the one before")
             path = path.to(cache.pos.device)
             row = torch.arange(B, device=path.device)[:, None]
@@ -709,5 +718,6 @@ class GraphDecoder:
             raise ValueError("cache is full")
         self.ids.copy_(ids.reshape(self.ids.shape))
         self.graph.replay()
+        self.cache.drafted = None
         self.cache.length += 1
         return self.logits

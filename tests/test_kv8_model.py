@@ -131,6 +131,19 @@ def test_cpu_refusals(store):
             model.accept(cache, [0])
         cache.reset()
         assert cache.length == 0 and cache.drafted is None
+        # a call that fails leaves no tree behind, the one before it included
+        model.verify(_ids(model, [1, 2, 3]), cache, [-1, 0, 0])
+        for ids, parents, match in ((_ids(model, [1] * 9), [-1] * 9, "positions"), (torch.tensor([[1], [2]]), [-1], "rows")):
+            with pytest.raises(ValueError, match=match):
+                model.verify(ids, cache, parents)
+        with pytest.raises(ValueError, match="verify"):
+            model.accept(cache, [0])
+        # parents that the device was asked to check, and that are no tree: the cache does not hold the tokens
+        model.verify(_ids(model, [1, 2, 3]), cache, [-1, 0, 0])
+        cache.drafted = (torch.tensor([-1, 0, 2], dtype=torch.int32), cache.drafted[1])
+        with pytest.raises(ValueError, match="no tree"):
+            model.accept(cache, [0, 1])
+        assert cache.length == 0
     # no derivative goes through the cache
     layer = model.layers[3].mixer
     x = torch.randn(1, 2, ARGS.hidden_size, requires_grad=True)
@@ -162,6 +175,11 @@ def test_gpu_8_bit_cache_and_tree():
         seq = _one_at_a_time(model, IDS + [DRAFT[0], DRAFT[2], 77])
         assert rel_l2(logits[:, 2].float().cpu().numpy(), seq[:, -2].float().cpu().numpy()) <= 2e-2
         assert rel_l2(step.float().cpu().numpy(), seq[:, -1].float().cpu().numpy()) <= 2e-2
+        # a replayed step forgets the drafted tokens
+        model.verify(_ids(model, DRAFT), cache, PARENTS)
+        graph.step(_ids(model, [5]))
+        with pytest.raises(ValueError, match="verify"):
+            model.accept(cache, [0])
         # single drafted token: the cache stays as it was
         cache2 = model.new_cache(max_len=32, kv_bits=8)
         model(_ids(model, IDS), cache2)
