@@ -1095,6 +1095,7 @@ static hipError_t launch_kv8_write_t(const Kv8WriteArgs& a, hipStream_t s) {
   // few tokens: the heads of one are shared out over several workgroups
   const int64_t tokens = (int64_t)a.B * a.S;
   const int rows = a.H + 2 * a.Hkv, most = (rows + 4 * kWriteRows - 1) / (4 * kWriteRows);
+  if (a.S >= 1 << 24) return hipErrorInvalidValue;  // a launch counts its threads along x in 32 bits
   const dim3 grid((unsigned)a.S, (unsigned)a.B, (unsigned)(tokens >= 1024 ? 1 : most));
   auto launch = [&](auto hd) {
     constexpr int HD = decltype(hd)::value;
@@ -1128,11 +1129,12 @@ template <bool BF, int HD, typename F>
 static hipError_t launch_attn_kv8_t(const Kv8AttnArgs& a, hipStream_t s, int rt, F launch) {
   const int64_t rows = (int64_t)a.S * (a.H / a.Hkv), all = rows * a.Hkv * a.B;
   const int64_t wgs = (rows + rt - 1) / rt * a.Hkv * a.nsplit;
-  if (wgs >= (1ll << 31) || (a.nsplit > 1 && all >= (1ll << 31))) return hipErrorInvalidValue;
+  const int waves = std::min((a.nsplit + kMergeSplits - 1) / kMergeSplits, kMergeWaves);
+  // a launch counts its threads along x in 32 bits
+  if (wgs >= (1ll << 24) || (a.nsplit > 1 && all >= (1ll << 26) / waves)) return hipErrorInvalidValue;
   const hipError_t e = launch(dim3((unsigned)wgs, (unsigned)a.B));
   if (e != hipSuccess) return e;
   if (a.nsplit > 1) {
-    const int waves = std::min((a.nsplit + kMergeSplits - 1) / kMergeSplits, kMergeWaves);
     hipLaunchKernelGGL((attn_kv8_merge_kernel<BF, HD>), dim3((unsigned)all), dim3(64 * waves), waves * (HD * 4 + 8), s, a, rt);
   }
   return hipGetLastError();

@@ -46,4 +46,12 @@ for i, fn in enumerate((lambda: attn(2, 1, BF16, 64), lambda: attn(4000, 1, BF16
         knob("stub_device", device)
         assert fn() == 0, (i, lib.gsq_last_error())
     assert [stub.stub_attr_device(j) for j in range(stub.stub_attrs())] == [0, 1, 70, 70], i
+# more threads than a launch counts (32 bits along x): refused before anything runs
+stub.stub_clear()
+knob("stub_device", 0)
+before = stub.stub_launches()
+for call in (lambda: attn(400000, 4000, max_len=500000), lambda: attn(400000, 128, max_len=500000)):
+    assert call() != 0 and b"launch" in lib.gsq_last_error() and stub.stub_launches() == before
+assert lib.gsq_kv8_write(X, 128, X, 64, X, 64, X, X, X, X, X, X, X, X, 1, None, 0, Y, 1, 1 << 24, 1, 1, 64, 0, 1 << 25, 1e-6,
+                         F16, S) != 0 and stub.stub_launches() == before
 """)
