@@ -822,7 +822,7 @@ constexpr int kv8_lds_steps(int hd) { return hd == 256 ? 1 : 0; }
 //    DMA in flight (413 -> 370).
 //  * 4096 tokens of 24 heads of 256 in fp16 350 us (0.59 PFLOP/s without the second term of the weights; a large
 //    library product 1.31), of which a fifth is the triangle's tail; 700 bf16 tokens of 2 x 32 heads of 128 behind
-//    5000 positions 270 (352 workgroups on 256 CUs); a tree of 64 tokens of 4 rows behind 8000 to 16000 140 + 15.
+//    5000 positions 270 (352 workgroups on 256 CUs); a tree of 64 tokens of 4 rows behind 8000 to 16000 144 + 15.
 template <bool BF, int HD, int NT>
 __global__ void __launch_bounds__(256, 2) attn_kv8_tile_kernel(Kv8AttnArgs a) {
   constexpr int KS = HD / 32, VB = HD / 16, RT = 64 * NT, NC = HD / 16;  // NC: 16-byte pieces of a row
