@@ -294,10 +294,11 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8ReadArgs a) {
 //    and positions 16 b + 4 (lane / 16) + e of a block of 32 on its registers, which is the layout of the B
 //    operand of O^T = V^T P^T: probabilities never leave their lane.
 //  * A byte u with a zero byte above it is the fp16 (subnormal) number u 2^-24, which the matrix cores
-//    take as it is: one v_perm expands two bytes, and K and V cost no rounding. What the 128 in u adds
-//    is known: -128 sum(q) starts the score's accumulator, and a product with a constant row sums the
-//    weights of V, whose 128-fold leaves the outputs every kBiasBlocks blocks (so that float32 sums of
-//    a long context are not those of numbers a hundred times their size).
+//    take as it is: one v_perm expands two bytes, and K and V cost no rounding. What the 128 in u adds to a
+//    score is known: -128 sum(q) starts its accumulator. V's bytes lose their 128 as pairs, before the product: sums
+//    over u, with 128 times the weights' sum taken off, end 1.4 to 2.8 x 2^-24 of the rows' largest values low in all dims
+//    alike, as the matrix cores truncate (over u - 128: 0.3 to 0.7), which an average over 131072 positions shows (4.5e-5 of
+//    the output against 1.7e-5; cost: prompt of 4096 320 -> 329 us, none where the cache's bytes bound it).
 //  * The scale of a K row multiplies its scores, that of a V row its probabilities. bf16 queries are
 //    scaled to fp16 by a power of two for each row: their 8 bits fit, and what falls below 2^-38 of the
 //    row's largest cannot be seen in float32 sums.
@@ -316,7 +317,6 @@ constexpr float kLazy = 6.f;
 constexpr float kPScale = 6.f;
 constexpr float kLeast = 2.f;  // a row's largest weight stays above 2^kLeast
 constexpr float kFar = 60.f;   // as long as its scores pass the reference by less than that
-constexpr int kBiasBlocks = 32;  // blocks between two subtractions of 128 times the weights
 
 __device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -346,9 +346,10 @@ __device__ __forceinline__ u32x4 bytes8(uint32_t w0, uint32_t w1) {
   return (u32x4){__builtin_amdgcn_perm(0, w0, lo), __builtin_amdgcn_perm(0, w0, hi), __builtin_amdgcn_perm(0, w1, lo),
                  __builtin_amdgcn_perm(0, w1, hi)};
 }
-// byte i of two dwords as a pair
+// byte i of two dwords as a pair of (u - 128) 2^-24 (fp16 sums of subnormal numbers are exact)
 __device__ __forceinline__ uint32_t byte_pair(uint32_t second, uint32_t first, int i) {
-  return __builtin_amdgcn_perm(second, first, scalar(0x0C000C00u | (uint32_t)((4 + i) << 16) | (uint32_t)i));
+  const uint32_t u = __builtin_amdgcn_perm(second, first, scalar(0x0C000C00u | (uint32_t)((4 + i) << 16) | (uint32_t)i));
+  return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, u) + (f16x2){(_Float16)-0x1p-17f, (_Float16)-0x1p-17f});
 }
 
 // blocks of 32 positions that rows up to token t see
@@ -456,7 +457,7 @@ struct Kv8Rows {
   bool unset[NT];  // the row has seen no position yet: m is 0
   bool pending;    // some row of the wave is unset
   float vref, vunit;  // power of two below the largest V scale met (the weights' unit), and 2^kPScale over it
-  f32x4 acc[NT][VB], wsum[NT];  // wsum: 128 times the weights, in acc's unit
+  f32x4 acc[NT][VB];
 
   __device__ void init(const float* rowc_s) {
     pending = true;
@@ -467,7 +468,6 @@ struct Kv8Rows {
       rowc[n] = rowc_s[16 * n];
       m[n] = l[n] = 0.f;
       unset[n] = true;
-      wsum[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < VB; ++i) acc[n][i] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
@@ -504,7 +504,6 @@ struct Kv8Rows {
         m[n] -= down;
         l[n] *= exp2_raw(down);
         tops[16 * n + c] = tops[16 * n + c] + (down - d);
-        wsum[n] *= f;
 #pragma unroll
         for (int i = 0; i < VB; ++i) acc[n][i] *= f;
       }
@@ -584,7 +583,6 @@ struct Kv8Rows {
         left |= unset[n];
         m[n] += up;
         l[n] *= alpha;
-        wsum[n] *= alpha;
 #pragma unroll
         for (int i = 0; i < VB; ++i) acc[n][i] *= alpha;
 #pragma unroll
@@ -615,13 +613,6 @@ struct Kv8Rows {
             w[e + 1] -= (float)hi.y;
           }
       }
-    const u32x4 ones = {0x00800080u, 0x00800080u, 0x00800080u, 0x00800080u};  // 128 x 2^-24
-#pragma unroll
-    for (int b = 0; b < NB / 2; ++b)
-#pragma unroll
-      for (int t = 0; t < TERMS; ++t)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) wsum[n] = mma16(ones, pf[b][t][n], wsum[n]);
   }
   // output tile i += V's operand times the weights
   __device__ void add(int i, u32x4 vf, const u32x4 (&pf)[TERMS][NT]) {
@@ -629,14 +620,6 @@ struct Kv8Rows {
     for (int t = 0; t < TERMS; ++t)
 #pragma unroll
       for (int n = 0; n < NT; ++n) acc[n][i] = mma16(vf, pf[t][n], acc[n][i]);
-  }
-  __device__ void take_bias() {
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-      for (int i = 0; i < VB; ++i) acc[n][i] -= wsum[n];
-      wsum[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    }
   }
   __device__ float unit() const { return vref * exp2_raw(24.f - kPScale); }  // of acc
   __device__ float top(int n) const { return unset[n] ? -FLT_MAX : m[n]; }
@@ -727,7 +710,7 @@ __global__ void __launch_bounds__(256, 2) attn_kv8_rows_kernel(Kv8AttnArgs a) {
   rows.init(rowc_s + c);
   rows.init_tops(bias_s + RT + 256 + wave * 16);
   const float bias = bias_s[c];
-  for (int it = 1; blk < k.blk1; blk += 4, ++it) {
+  for (; blk < k.blk1; blk += 4) {
     const bool more = blk + 4 < k.blk1;
     // scales of the block's positions to the lanes that hold them (the wave's LDS operations are in order)
     {
@@ -762,7 +745,6 @@ __global__ void __launch_bounds__(256, 2) attn_kv8_rows_kernel(Kv8AttnArgs a) {
       rows.add(i, (u32x4){byte_pair(vr[1][i >> 2], vr[0][i >> 2], i & 3), byte_pair(vr[3][i >> 2], vr[2][i >> 2], i & 3),
                           byte_pair(vr[5][i >> 2], vr[4][i >> 2], i & 3), byte_pair(vr[7][i >> 2], vr[6][i >> 2], i & 3)}, pf[0]);
     if (more) load_v(blk + 4);
-    if (it % kBiasBlocks == 0 || !more) rows.take_bias();
   }
   // merge of the waves: every wave's maximum, sum and outputs (in V's own unit)
   constexpr int OS = HD + 4;
@@ -815,7 +797,7 @@ constexpr int kv8_lds_steps(int hd) { return hd == 256 ? 1 : 0; }
 //  * K's 16-byte pieces are XOR-swizzled by position, V's pieces (or rows) by bits 2 and 3 of it, so that the
 //    lanes of a read fall on different banks; the DMA's source address does it.
 //  * What bounds it are vector instructions and matrix cores: at head dim 256 a wave's 32 rows and a block of 32
-//    positions take 100 MFMAs (fp16: 1600 cycles; bf16 68) and about 330 vector instructions (128 of them
+//    positions take 96 MFMAs (fp16: 1536 cycles; bf16 64) and about 390 vector instructions (192 of them
 //    expand bytes), two waves a SIMD overlapping them in part. Matrix instructions go at raised priority
 //    (353 -> 346 us). The accumulators and queries of two waves a SIMD fill the 512 registers: what the loop
 //    does not need in them lies in LDS (a step of the queries, biases, scales, paths, largest weights), as spills would wait for the
@@ -902,7 +884,7 @@ __global__ void __launch_bounds__(256, 2) attn_kv8_tile_kernel(Kv8AttnArgs a) {
   const bool on = r0 < k.R;
   issue(k.blk0, kv8_lds);
   int cur = 0;
-  for (int blk = k.blk0, it = 0; blk < k.blk1; blk += 2, ++it, cur ^= 1) {
+  for (int blk = k.blk0; blk < k.blk1; blk += 2, cur ^= 1) {
     // the tile has landed; every wave is done with the other buffer
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     if (blk + 2 < k.blk1) issue(blk + 2, kv8_lds + (cur ^ 1) * BUF);
@@ -979,7 +961,6 @@ __global__ void __launch_bounds__(256, 2) attn_kv8_tile_kernel(Kv8AttnArgs a) {
         }
     }
     __builtin_amdgcn_s_setprio(0);
-    if (it % (kBiasBlocks / 2) == kBiasBlocks / 2 - 1 || blk + 2 >= k.blk1) rows.take_bias();
   }
   // a lane's outputs: row r0 + 16 n + c, dims (HD / NP) h + PW (4 g + e) + i
   const float unit = rows.unit();

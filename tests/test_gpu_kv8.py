@@ -584,3 +584,26 @@ def test_kv8_empty_calls():
         out = kv8.attn_kv8(d["q"][:B, :S], d["qg"][:B, :S], d["k"][:B], d["v"][:B], d["ks"][:B], d["vs"][:B], d["pos"], heads=4,
                            kv_heads=2, head_dim=64)
         assert out.shape == (B, S, 256)
+
+
+@pytest.mark.parametrize("long", [False, True])
+def test_attn_kv8_outputs_are_not_shifted(long):
+    """Averages over thousands of positions, far smaller than the values, whose sizes vary: what the float32 sums
+    leave in all dims alike is within one float32 rounding of the rows' largest values (2^-24 times their
+    weighted mean)."""
+    B, S, pos, L, H, G, hd = 1, 24, [8000], 8024, 64, 8, 256
+    t = _attn_inputs(B, S, pos, L, H, G, hd, F16)
+    t["qg"].view(B, S, H, 2 * hd)[..., hd:] = 60.0  # gates of 1
+    got = _attn(t, H, G, hd, long=long).double().view(B, S, H, hd)
+    want, _ = _reference(t, H, G, hd)
+    largest = torch.empty(B, S, H, 1, dtype=torch.float64)
+    see = torch.arange(L)[None, :] <= pos[0] + torch.arange(S)[:, None]
+    for h in range(H):
+        k, q = _values(t["k"][0, h // 8], t["ks"][0, h // 8]), t["q"][0].double().view(S, H, hd)[:, h]
+        p = torch.softmax((torch.matmul(q, k.t().contiguous()) * hd ** -0.5).masked_fill(~see, float("-inf")), -1)
+        largest[0, :, h, 0] = 127 * torch.matmul(p, t["vs"][0, h // 8].double())
+    # the rounding to fp16 has no direction: of B S H hd outputs, each off by 2^-11 / sqrt(3) of itself at most (root
+    # mean square), it leaves this in the mean (4 sigma)
+    noise = 4 * float((want / largest).square().mean().sqrt()) * 2.0 ** -11 / math.sqrt(3 * want.numel())
+    assert noise < 2.0 ** -25
+    assert abs(float(((got - want) / largest).mean())) <= 2.0 ** -24 + noise
