@@ -310,9 +310,10 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8ReadArgs a) {
 //    or lower where that position's V row is small against the largest one met: then what the row's largest
 //    weight is decides, as V rows that it does not see, or hardly, are not to take its weights' bits.
 //  * A weight (probability times V scale, 2^kPScale over the largest V scale met) is at most 2^(kLazy + 3 +
-//    kPScale) = 2^15 and held in fp16: for bf16 outputs in one value (11 bits, eight times finer than the
-//    output's own rounding), for fp16 outputs in two (22 bits, down to 2^-25 of the unit), as one would
-//    add an error as large as the output's rounding.
+//    kPScale) = 2^15 and held in two fp16 values (22 bits, down to 2^-25 of the unit). With one (11 bits) fp16
+//    outputs would be off by 1.4 times their rounding and 3 to 9 of 100 bf16 outputs would take the other neighbour
+//    (0.01 of 100 with two); it would save a third of the matrix instructions (700 bf16 tokens behind 5000: 267
+//    against 310 us, a tree of 64 tokens of 4 rows 152 against 175; few rows the same).
 constexpr float kLazy = 6.f;
 constexpr float kPScale = 6.f;
 constexpr float kLeast = 2.f;  // a row's largest weight stays above 2^kLeast
@@ -451,7 +452,7 @@ __device__ __forceinline__ void kv8_stage_q(const Kv8AttnArgs& a, const Kv8Task<
 // The softmax and the sums of a wave's 16 NT rows over the blocks it has seen.
 template <bool BF, int HD, int NT>
 struct Kv8Rows {
-  static constexpr int VB = HD / 16, TERMS = BF ? 1 : 2;  // output tiles; fp16 values that hold a weight
+  static constexpr int VB = HD / 16, TERMS = 2;  // output tiles; fp16 values that hold a weight
   float rowc[NT], m[NT], l[NT];
   float* tops;  // LDS, row 16 n + c: power of two of the row's largest weight, as of the last move of its reference
   bool unset[NT];  // the row has seen no position yet: m is 0
@@ -797,7 +798,7 @@ constexpr int kv8_lds_steps(int hd) { return hd == 256 ? 1 : 0; }
 //  * K's 16-byte pieces are XOR-swizzled by position, V's pieces (or rows) by bits 2 and 3 of it, so that the
 //    lanes of a read fall on different banks; the DMA's source address does it.
 //  * What bounds it are vector instructions and matrix cores: at head dim 256 a wave's 32 rows and a block of 32
-//    positions take 96 MFMAs (fp16: 1536 cycles; bf16 64) and about 390 vector instructions (192 of them
+//    positions take 96 MFMAs (1536 cycles) and about 390 vector instructions (192 of them
 //    expand bytes), two waves a SIMD overlapping them in part. Matrix instructions go at raised priority
 //    (353 -> 346 us). The accumulators and queries of two waves a SIMD fill the 512 registers: what the loop
 //    does not need in them lies in LDS (a step of the queries, biases, scales, paths, largest weights), as spills would wait for the

@@ -607,3 +607,26 @@ def test_attn_kv8_outputs_are_not_shifted(long):
     noise = 4 * float((want / largest).square().mean().sqrt()) * 2.0 ** -11 / math.sqrt(3 * want.numel())
     assert noise < 2.0 ** -25
     assert abs(float(((got - want) / largest).mean())) <= 2.0 ** -24 + noise
+
+
+@pytest.mark.parametrize("long", [False, True])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_attn_kv8_outputs_are_rounded_once(dtype, long):
+    """Scores, weights and sums as float32 has them: an output differs from the rounded float64 value only where that
+    lies within eight float32 roundings of the rows' largest values (2^-24 times their weighted mean) of a border."""
+    B, S, pos, L, H, G, hd = 2, 12, [300, 211], 312, 24, 4, 128
+    t = _attn_inputs(B, S, pos, L, H, G, hd, dtype)
+    t["qg"].view(B, S, H, 2 * hd)[..., hd:] = 60.0  # gates of 1
+    got = _attn(t, H, G, hd, long=long).view(B, S, H, hd)
+    want, _ = _reference(t, H, G, hd)
+    off = torch.empty(B, S, H, 1, dtype=torch.float64)
+    for b in range(B):
+        n = pos[b] + S
+        see = torch.arange(n)[None, :] <= pos[b] + torch.arange(S)[:, None]
+        for h in range(H):
+            k, q = _values(t["k"][b, h // 6, :n], t["ks"][b, h // 6, :n]), t["q"][b].double().view(S, H, hd)[:, h]
+            p = torch.softmax((torch.matmul(q, k.t().contiguous()) * hd ** -0.5).masked_fill(~see, float("-inf")), -1)
+            off[b, :, h, 0] = 8 * 2.0 ** -24 * 127 * torch.matmul(p, t["vs"][b, h // 6, :n].double())
+    step = torch.finfo(dtype).eps * 2.0 ** want.abs().clamp(min=2.0 ** -14).log2().floor()
+    near = (2 * off / step).clamp(max=1.0).sum()  # borders lie a step apart
+    assert int((got != want.to(dtype)).sum()) <= float(near)
