@@ -520,7 +520,6 @@ class Qwen35Model(torch.nn.Module):
     def forward(self, ids, cache: Qwen35Cache):
         S = ids.shape[1]
         logits = self._run(ids, cache)
-        cache.drafted = None
         cache.pos.add_(S)
         cache.length += S
         return logits
@@ -530,6 +529,8 @@ class Qwen35Model(torch.nn.Module):
         if cache.length + S > cache.max_len:
             raise ValueError(f"cache holds {cache.max_len} positions; {cache.length} used, {S} more asked")
         x = self.embed(ids).to(self.dtype).reshape(B, S, -1).contiguous()
+        if parents is None:
+            cache.drafted = None  # before the first layer: a step that fails has overwritten drafted tokens all the same
         delta = None
         for layer in self.layers:
             x, delta = layer(x, delta, cache) if parents is None else layer(x, delta, cache, parents)
@@ -717,7 +718,7 @@ class GraphDecoder:
         if self.cache.length + 1 > self.cache.max_len:
             raise ValueError("cache is full")
         self.ids.copy_(ids.reshape(self.ids.shape))
-        self.graph.replay()
         self.cache.drafted = None
+        self.graph.replay()
         self.cache.length += 1
         return self.logits

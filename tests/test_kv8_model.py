@@ -151,6 +151,40 @@ def test_cpu_refusals(store):
         layer(x, Qwen35Cache(ARGS, 1, 8, "cpu", torch.float32, kv_bits=8))
 
 
+class _Fails(torch.nn.Module):
+    def forward(self, *args, **kw):
+        raise RuntimeError("out of memory")
+
+    replay = forward
+
+
+@pytest.mark.parametrize("where", ["last layer", "head", "replay"])
+def test_cpu_failed_step_leaves_nothing_to_accept(store, where):
+    """A plain step that fails has overwritten drafted tokens and advanced layers; one that is refused has not."""
+    model = _cpu_model(store)
+    with torch.no_grad():
+        cache = model.new_cache(max_len=16, kv_bits=8)
+        model(_ids(model, IDS[:5]), cache)
+        model.verify(_ids(model, DRAFT), cache, PARENTS)
+        with pytest.raises(ValueError, match="positions"):
+            model(_ids(model, [1] * 12), cache)
+        assert cache.drafted is not None
+        if where == "replay":
+            graph = object.__new__(GraphDecoder)
+            graph.cache, graph.ids, graph.graph = cache, _ids(model, [0]), _Fails()
+            step = graph.step
+        else:
+            step = lambda ids: model(ids, cache)  # noqa: E731
+            if where == "head":
+                model.lm_head = _Fails()
+            else:
+                model.layers[-1].down = _Fails()
+        with pytest.raises(RuntimeError, match="memory"):
+            step(_ids(model, [4]))
+        with pytest.raises(ValueError, match="verify"):
+            model.accept(cache, [1, 5])
+
+
 @pytest.mark.gpu
 def test_gpu_8_bit_cache_and_tree():
     """Against the CPU's float32 model within the bound of the fp16 decoder (2e-2), and among themselves: trees
