@@ -566,7 +566,8 @@ class Qwen35Model(torch.nn.Module):
     def accept(self, cache: Qwen35Cache, path):
         """Keeps the drafted tokens ``path`` ((n,), or (B, n) for rows that keep other ones) of the tree that
         ``verify`` ran last: a path from the cache on (its first token follows -1, each other the one before
-        it), possibly empty. The cache is advanced by them and the other drafted tokens are forgotten."""
+        it), possibly empty. The cache is advanced by them and the other drafted tokens are forgotten. A call that
+        fails after its checks leaves a cache to ``reset``."""
         if cache.drafted is None:
             raise ValueError("no drafted tokens: verify comes first")
         parents, inputs = cache.drafted
@@ -585,6 +586,7 @@ class Qwen35Model(torch.nn.Module):
             before = torch.cat([torch.full((B, 1), -1), path[:, :-1]], dim=1)
             if not torch.equal(torch.gather(tree.expand(B, T), 1, path), before):
                 raise ValueError("path must lead from the cached tokens on, each token following the one before")
+            cache.drafted = None  # before the first write: a call that fails part way cannot be repeated
             path = path.to(cache.pos.device)
             row = torch.arange(B, device=path.device)[:, None]
             to = cache.length + torch.arange(n, device=path.device)

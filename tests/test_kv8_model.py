@@ -185,6 +185,25 @@ def test_cpu_failed_step_leaves_nothing_to_accept(store, where):
             model.accept(cache, [1, 5])
 
 
+def test_cpu_failed_accept_is_not_repeated(store, monkeypatch):
+    """A layer's state that cannot be advanced: earlier layers have been, and K and V rows moved. A path that is
+    refused changes nothing and may be followed by another."""
+    model = _cpu_model(store)
+    with torch.no_grad():
+        cache = model.new_cache(max_len=16, kv_bits=8)
+        model(_ids(model, IDS[:5]), cache)
+        model.verify(_ids(model, DRAFT), cache, PARENTS)
+        with pytest.raises(ValueError, match="path"):
+            model.accept(cache, [5])
+        assert cache.drafted is not None
+        monkeypatch.setattr(model.layers[1].mixer, "advance", _Fails().forward)
+        with pytest.raises(RuntimeError, match="memory"):
+            model.accept(cache, [1, 5])
+        monkeypatch.undo()
+        with pytest.raises(ValueError, match="verify"):
+            model.accept(cache, [1, 5])
+
+
 @pytest.mark.gpu
 def test_gpu_8_bit_cache_and_tree():
     """Against the CPU's float32 model within the bound of the fp16 decoder (2e-2), and among themselves: trees
