@@ -400,7 +400,11 @@ class FullAttention(torch.nn.Module):
         new = torch.arange(L, device=qk.device) - cache.pos              # (L,): drafted or new token of a position
         mask = torch.where(((new >= 0) & (new < S))[None, None], seen[:, :, new.clamp(0, S - 1)], new < 0)  # (B, S, L)
         kf, vf = ((c.float() - 128) * s[..., None] for c, s in ((caches[0], caches[2]), (caches[1], caches[3])))
-        vf = torch.where((new < S)[:, None], vf, 0.0)                    # behind the new tokens lies anything
+        # behind the new tokens lies anything; a V row that is not finite makes its position's scores NaN instead, so that it
+        # does not reach the tokens that do not see it (0 x NaN would)
+        fine = torch.isfinite(caches[3])
+        vf = torch.where((fine & (new < S))[..., None], vf, 0.0)
+        kf = torch.where(fine[..., None], kf, float("nan"))
         qf = q.float().transpose(1, 2).reshape(B, Hkv, rep * S, hd)
         scores = torch.matmul(qf, kf.transpose(2, 3).contiguous()) * (hd ** -0.5)
         scores = scores.masked_fill(~mask.repeat(1, rep, 1)[:, None], float("-inf"))

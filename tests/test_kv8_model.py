@@ -204,6 +204,52 @@ def test_cpu_failed_accept_is_not_repeated(store, monkeypatch):
             model.accept(cache, [1, 5])
 
 
+class _Returns(torch.nn.Module):
+    def __init__(self, out):
+        super().__init__()
+        self.out = out
+
+    def forward(self, x):
+        return self.out
+
+
+@pytest.mark.parametrize("name", ["k", "v"])
+@pytest.mark.parametrize("parents", [None, [-1, 0, 0, 1, 1, -1]])
+def test_cpu_rows_that_are_not_finite(parents, name):
+    """A new token's K or V row with a NaN or an infinity reaches the tokens that see it, in its KV head's query heads,
+    and no other."""
+    from mlx_gsq_amd.models.qwen35 import FullAttention
+    g = torch.Generator().manual_seed(7)
+    a, B, S = ARGS, 2, 6
+    H, G, hd = a.num_attention_heads, a.num_key_value_heads, a.head_dim
+    rows = {"qk": torch.randn(B, S, H * 2 * hd + G * hd, generator=g), "v": torch.randn(B, S, G * hd, generator=g)}
+    tree = None if parents is None else torch.tensor(parents, dtype=torch.int32)
+
+    def run(qk, v):
+        m = FullAttention(a, 3, _Returns(qk), _Returns(v), torch.nn.Identity(), torch.ones(hd), torch.ones(hd))
+        with torch.no_grad():
+            return m(torch.zeros(B, S, 8), Qwen35Cache(a, B, 16, "cpu", torch.float32, kv_bits=8), parents=tree).view(B, S, H, hd)
+    clean = run(**rows)
+    assert torch.isfinite(clean).all()
+    for node, value in ((5, float("nan")), (1, float("inf"))):
+        bad = {n: t.clone() for n, t in rows.items()}
+        if name == "k":
+            bad["qk"][1, node, H * 2 * hd + (G - 1) * hd + 3] = value
+        else:
+            bad["v"][1, node, (G - 1) * hd + 3] = value
+        got = run(**bad)
+        sees = [node <= t if parents is None else _on_path(parents, node, t) for t in range(S)]
+        hit = torch.zeros(B, S, H, hd, dtype=torch.bool)
+        hit[1, sees, H - H // G:] = True
+        assert torch.isnan(got[hit]).all() and torch.equal(got[~hit], clean[~hit])
+
+
+def _on_path(parents, node, t):
+    while t > node:
+        t = parents[t]
+    return t == node
+
+
 @pytest.mark.gpu
 def test_gpu_8_bit_cache_and_tree():
     """Against the CPU's float32 model within the bound of the fp16 decoder (2e-2), and among themselves: trees
