@@ -9,7 +9,8 @@ first new token. ``parents`` (int32 on the device, (S,) or (B, S), S <= 64) make
 drafted ones: token t follows token ``parents[t] < t``, or the cached tokens (-1), sits at cache
 position ``pos + t`` and is rotated at ``pos`` + its depth. Rows whose tokens do not all lie inside the
 cache, or whose parents are not such, get NaN outputs and keep their cache. Tensors on one GPU, fp16 or
-bf16 activations, head_dim 64, 128 or 256; calls run on the current stream and may be captured.
+bf16 activations, head_dim 64, 128 or 256; calls run on the current stream and may be captured. They carry
+no derivative, and refuse tensors that autograd follows.
 """
 from __future__ import annotations
 
@@ -18,7 +19,7 @@ from functools import lru_cache
 import torch
 
 from ... import _lib
-from .model_ops import MAX_TREE
+from .model_ops import MAX_TREE, no_derivative
 
 HEAD_DIMS = (64, 128, 256)
 
@@ -96,6 +97,7 @@ def kv8_write(qg, k, v, q_norm_w, k_norm_w, inv_freq, k_cache, v_cache, k_scale,
     RMS-normalized per head (``q_norm_w``, ``k_norm_w``, eps) and rotated on their first rotary_dim dims
     (rotate-half, inv_freq (rotary_dim / 2,) float64); k and v go into the caches, quantised from their
     unrounded values. Returns the queries (B, S, heads * head_dim) for ``attn_kv8``."""
+    no_derivative(qg, k, v, q_norm_w, k_norm_w, inv_freq, k_scale, v_scale)
     dev = _one_gpu(qg, k, v, q_norm_w, k_norm_w, inv_freq, k_cache, v_cache, k_scale, v_scale, pos, parents)
     dtype, code = qg.dtype, _dtype_code(qg)
     B, S = qg.shape[:2]
@@ -121,6 +123,7 @@ def kv8_write(qg, k, v, q_norm_w, k_norm_w, inv_freq, k_cache, v_cache, k_scale,
 def kv8_read(k_cache, v_cache, k_scale, v_scale, *, dtype, start: int = 0, length=None):
     """The values that positions ``start .. start + length - 1`` (default: to the end) of both caches stand
     for, rounded to ``dtype`` (float32, float16 or bfloat16): (k, v), each (B, kv_heads, length, head_dim)."""
+    no_derivative(k_scale, v_scale)
     dev = _one_gpu(k_cache, v_cache, k_scale, v_scale)
     B, G, L, hd = _caches(k_cache, v_cache, k_scale, v_scale)
     if dtype not in _lib.DTYPE_CODES:
@@ -157,6 +160,7 @@ def attn_kv8(q, qg, k_cache, v_cache, k_scale, v_scale, pos, *, heads: int, kv_h
     heads * head_dim), qg the [q | gate] rows it read. Token t attends to positions 0 .. pos + t; in a
     tree to those before ``pos``, its ancestors and itself. ``splits``: workgroups that share the positions
     of one tile of rows (default: as many as fill the device). Returns (B, S, heads * head_dim)."""
+    no_derivative(q, qg, k_scale, v_scale)
     dev = _one_gpu(q, qg, k_cache, v_cache, k_scale, v_scale, pos, parents)
     dtype, code = q.dtype, _dtype_code(q)
     B, S = q.shape[:2]

@@ -9,6 +9,7 @@ GPU (there is no CPU path here) and share one dtype: float32, float16 or bfloat1
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from ... import _lib
 
@@ -145,12 +146,24 @@ def gdn_seq(qkv, z, ab, conv_state, conv_w, ssm_a, dt_bias, rec_state, norm_w, *
 MAX_TREE = 64  # tokens of a drafted tree
 
 
+def no_derivative(*ts):
+    """Refuses tensors that autograd follows, in reverse or forward mode: the kernels' outputs would drop it."""
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t.requires_grad:
+                raise ValueError("the kernel carries no derivative: call it under no_grad, or detach its inputs")
+    # a look at each tensor only while a level of forward mode is open (or torch does not say)
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise ValueError("the kernel carries no derivative: give it the primal tensors")
+
+
 def gdn_tree(qkv, z, ab, conv_state, conv_w, ssm_a, dt_bias, rec_state, norm_w, parents, *, key_heads: int,
              value_heads: int, head_k_dim: int, head_v_dim: int, eps: float):
     """``gdn_seq`` over a tree of S <= 64 drafted tokens: token t follows token ``parents[t] < t``, or the
     cached ones (-1); parents int32 (S,) or (B, S) on the device. The states are only read: the tokens
     that are kept go through ``gdn_seq`` afterwards. Returns (B, S, Hv*dv), NaN in batch rows whose parents are
-    not such."""
+    not such. Tensors that autograd follows are refused."""
+    no_derivative(qkv, z, ab, conv_state, conv_w, ssm_a, dt_bias, rec_state, norm_w)
     index = qkv.get_device()
     if index < 0 or any(t.get_device() != index for t in (z, ab, conv_state, conv_w, ssm_a, dt_bias, rec_state, norm_w, parents)):
         raise ValueError("tensors must be on one GPU device")

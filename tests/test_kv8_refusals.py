@@ -118,3 +118,34 @@ def test_splits_rule():
     for bad in ((0, 1, 4, 1, 64, 8, 256), (1, 0, 4, 1, 64, 8, 256), (1, 1, 4, 0, 64, 8, 256), (1, 1, 4, 1, 64, 0, 256),
                 (1, 1, 4, 1, 64, 8, 0)):
         assert splits(*bad) == 1
+
+
+@pytest.mark.parametrize("mode", ["reverse", "forward"])
+def test_python_refuses_derivatives(mode):
+    """Tensors that autograd follows, one at a time, before anything else is looked at; without a mode that records
+    they are as good as others."""
+    from contextlib import nullcontext
+
+    from torch.autograd import forward_ad
+
+    from mlx_gsq_amd.runtime.kernels import kv8, model_ops
+    p, w, u = torch.zeros(1, dtype=torch.int64), torch.zeros(64).half(), torch.zeros(1, 1, 8, 64, dtype=torch.uint8)
+    q, h, s, f = torch.zeros(1, 2, 64).half(), torch.zeros(1, 2, 128).half(), torch.zeros(1, 1, 8), torch.zeros(1).double()
+    kw = dict(heads=1, kv_heads=1, head_dim=64)
+    calls = [(lambda *t: kv8.kv8_write(*t[:6], u, u, *t[6:], p, rotary_dim=2, eps=1e-6, **kw), [h, q, q, w, w, f, s, s]),
+             (lambda *t: kv8.kv8_read(u, u, *t, dtype=torch.float16), [s, s]),
+             (lambda *t: kv8.attn_kv8(*t[:2], u, u, *t[2:], p, **kw), [q, h, s, s]),
+             (lambda *t: model_ops.gdn_tree(*t, p.int(), key_heads=1, value_heads=1, head_k_dim=32, head_v_dim=64, eps=1e-6),
+              [h, q, q, q, q, s, s, s, w])]
+    with forward_ad.dual_level() if mode == "forward" else nullcontext():
+        for call, args in calls:
+            with pytest.raises(ValueError, match="GPU"):
+                call(*args)
+            for i, t in enumerate(args):
+                t = forward_ad.make_dual(t, torch.ones_like(t)) if mode == "forward" else t.clone().requires_grad_()
+                changed = args[:i] + [t] + args[i + 1:]
+                with pytest.raises(ValueError, match="derivative"):
+                    call(*changed)
+                if mode == "reverse":
+                    with torch.no_grad(), pytest.raises(ValueError, match="GPU"):
+                        call(*changed)
