@@ -414,6 +414,8 @@ class FullAttention(torch.nn.Module):
     def forward(self, x, cache: Qwen35Cache, first=None, parents=None):
         """``first``: ``qk_proj(x)`` when the caller has computed it already. ``parents``: the tokens are a
         drafted tree (8-bit caches)."""
+        if parents is not None and cache.kv_bits != 8:
+            raise ValueError("trees of drafted tokens need an 8-bit cache (new_cache(kv_bits=8))")
         a_ = self.args
         B, S, _ = x.shape
         H, Hkv, hd = a_.num_attention_heads, a_.num_key_value_heads, a_.head_dim

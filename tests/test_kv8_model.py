@@ -204,6 +204,18 @@ def test_cpu_failed_accept_is_not_repeated(store, monkeypatch):
             model.accept(cache, [1, 5])
 
 
+def test_cpu_attention_layer_refuses_a_tree_on_a_16_bit_cache(store):
+    """It would run as a sequence there."""
+    layer, x = _cpu_model(store).layers[3].mixer, torch.randn(1, 3, ARGS.hidden_size)
+    tree = torch.tensor([-1, 0, 0], dtype=torch.int32)
+    with torch.no_grad():
+        cache = Qwen35Cache(ARGS, 1, 8, "cpu", torch.float32)
+        with pytest.raises(ValueError, match="8-bit"):
+            layer(x, cache, parents=tree)
+        assert not cache.k[3].any()
+        layer(x, Qwen35Cache(ARGS, 1, 8, "cpu", torch.float32, kv_bits=8), parents=tree)
+
+
 class _Returns(torch.nn.Module):
     def __init__(self, out):
         super().__init__()
