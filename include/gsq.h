@@ -292,7 +292,7 @@ int64_t gsq_attn_kv8_splits(int64_t batch, int64_t seq, int64_t heads, int64_t k
 
 /* out = round(softmax(q K^T / sqrt(head_dim)) V * sigmoid(gate)) per head, gates in qg; token t attends to
  * positions 0 .. *pos + t, in a tree to 0 .. *pos - 1, its ancestors and itself. splits > 1: the
- * positions are shared out over that many workgroups for each tile of rows (at most 65535), whose sums
+ * positions are shared out over that many workgroups for each tile of rows (at most 65535), whose averages
  * meet in work (batch * heads * seq * splits * (head_dim + 2) floats) and are combined by a second
  * kernel; work is not used with splits = 1. Caches, work and rows of q 16-byte aligned, rows of qg and
  * out 8-byte aligned. */

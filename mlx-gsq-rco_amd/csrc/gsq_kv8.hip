@@ -622,7 +622,9 @@ struct Kv8Rows {
 #pragma unroll
       for (int n = 0; n < NT; ++n) acc[n][i] = mma16(vf, pf[t][n], acc[n][i]);
   }
-  __device__ float unit() const { return vref * exp2_raw(24.f - kPScale); }  // of acc
+  // what leaves the kernel are averages of V rows, which float32 holds whatever the rows' size; sums of rows near its
+  // largest number it would not: acc over a row's sum l (0: no position), then vref
+  __device__ static float over(float l) { return l == 0.f ? 0.f : exp2_raw(24.f - kPScale) / l; }
   __device__ float top(int n) const { return unset[n] ? -FLT_MAX : m[n]; }
   __device__ float sum(int n) const {  // over the lanes of a row
     const float x = l[n] + __shfl_xor(l[n], 16, 64);
@@ -632,7 +634,7 @@ struct Kv8Rows {
 
 // N (4 or 8) gated outputs of a row, from dim d on
 template <bool BF, int N>
-__device__ __forceinline__ void kv8_out(const uint16_t* gate, uint16_t* out, const float (&o)[N], float inv) {
+__device__ __forceinline__ void kv8_out(const uint16_t* gate, uint16_t* out, const float (&o)[N]) {
   using E = E16<BF>;
 #pragma unroll
   for (int i = 0; i < N; i += 4) {
@@ -640,7 +642,7 @@ __device__ __forceinline__ void kv8_out(const uint16_t* gate, uint16_t* out, con
     const uint16_t gv[4] = {(uint16_t)gw.x, (uint16_t)(gw.x >> 16), (uint16_t)gw.y, (uint16_t)(gw.y >> 16)};
     uint32_t q[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) q[e] = E::mk(o[i + e] * inv * sigmoid_raw(E::ld(gv[e])));
+    for (int e = 0; e < 4; ++e) q[e] = E::mk(o[i + e] * sigmoid_raw(E::ld(gv[e])));
     *reinterpret_cast<uint2*>(out + i) = make_uint2(q[0] | (q[1] << 16), q[2] | (q[3] << 16));
   }
 }
@@ -747,11 +749,11 @@ __global__ void __launch_bounds__(256, 2) attn_kv8_rows_kernel(Kv8AttnArgs a) {
                           byte_pair(vr[5][i >> 2], vr[4][i >> 2], i & 3), byte_pair(vr[7][i >> 2], vr[6][i >> 2], i & 3)}, pf[0]);
     if (more) load_v(blk + 4);
   }
-  // merge of the waves: every wave's maximum, sum and outputs (in V's own unit)
+  // merge of the waves: every wave's maximum, sum and outputs over its own sum
   constexpr int OS = HD + 4;
   float* const mo = reinterpret_cast<float*>(kv8_lds);             // [4][16][OS]
   float2* const ml = reinterpret_cast<float2*>(mo + 4 * 16 * OS);  // [4][16]
-  const float unit = rows.unit();
+  const float ls = rows.sum(0), over = rows.over(ls), vref = rows.vref;
   __syncthreads();  // queries and scales are no longer read
   float* const mine = mo + (wave * 16 + c) * OS;
 #pragma unroll
@@ -759,24 +761,25 @@ __global__ void __launch_bounds__(256, 2) attn_kv8_rows_kernel(Kv8AttnArgs a) {
 #pragma unroll
     for (int i = 0; i < VB; i += 4)
       *reinterpret_cast<f32x4*>(mine + VB * (4 * g + e) + i) =
-          (f32x4){rows.acc[0][i][e], rows.acc[0][i + 1][e], rows.acc[0][i + 2][e], rows.acc[0][i + 3][e]} * unit;
-  const float ls = rows.sum(0);
+          (f32x4){rows.acc[0][i][e], rows.acc[0][i + 1][e], rows.acc[0][i + 2][e], rows.acc[0][i + 3][e]} * over * vref;
   if (g == 0) ml[wave * 16 + c] = make_float2(rows.top(0), ls);
   __syncthreads();
   for (int i = tid; i < 16 * HD / 4; i += 256) {
     const int rr = i / (HD / 4), d = 4 * (i % (HD / 4)), r = k.r0 + rr;
     if (r >= k.R) continue;
-    float mm = -FLT_MAX, ll = 0.f;
+    float mm = -FLT_MAX, ll = 0.f, f[4];
 #pragma unroll
     for (int w = 0; w < 4; ++w) mm = fmaxf(mm, ml[w * 16 + rr].x);
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       const float2 x = ml[w * 16 + rr];
-      const float f = exp2_raw(x.x - mm);
-      ll += x.y * f;
-      o += *reinterpret_cast<const f32x4*>(mo + (w * 16 + rr) * OS + d) * f;
+      f[w] = x.y * exp2_raw(x.x - mm);
+      ll += f[w];
     }
+    const float inv = ll == 0.f ? 0.f : 1.f / ll;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) o += *reinterpret_cast<const f32x4*>(mo + (w * 16 + rr) * OS + d) * (f[w] * inv);
     if (a.nsplit > 1) {
       const int64_t all = (int64_t)a.B * a.Hkv * k.R, at = (((int64_t)k.bb * a.Hkv + k.kvh) * k.R + r) * a.nsplit + k.z;
       *reinterpret_cast<f32x4*>(a.part + at * HD + d) = o;
@@ -784,7 +787,7 @@ __global__ void __launch_bounds__(256, 2) attn_kv8_rows_kernel(Kv8AttnArgs a) {
     } else {
       const float v[4] = {o[0], o[1], o[2], o[3]};
       kv8_out<BF, 4>(static_cast<const uint16_t*>(a.qg) + k.row_at(a, r, a.qg_stride, 2 * HD) + HD + d,
-                     static_cast<uint16_t*>(a.out) + k.row_at(a, r, a.out_stride, HD) + d, v, 1.f / ll);
+                     static_cast<uint16_t*>(a.out) + k.row_at(a, r, a.out_stride, HD) + d, v);
     }
   }
 }
@@ -964,11 +967,10 @@ __global__ void __launch_bounds__(256, 2) attn_kv8_tile_kernel(Kv8AttnArgs a) {
     __builtin_amdgcn_s_setprio(0);
   }
   // a lane's outputs: row r0 + 16 n + c, dims (HD / NP) h + PW (4 g + e) + i
-  const float unit = rows.unit();
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int r = r0 + 16 * n + c;
-    const float ls = rows.sum(n);
+    const float ls = rows.sum(n), over = rows.over(ls), vref = rows.vref;
     if (r >= k.R) continue;
     const int64_t all = (int64_t)a.B * a.Hkv * k.R, at = (((int64_t)k.bb * a.Hkv + k.kvh) * k.R + r) * a.nsplit + k.z;
     if (a.nsplit > 1 && g == 0) *reinterpret_cast<float2*>(a.part + all * a.nsplit * HD + 2 * at) = make_float2(rows.top(n), ls);
@@ -981,20 +983,20 @@ __global__ void __launch_bounds__(256, 2) attn_kv8_tile_kernel(Kv8AttnArgs a) {
         const int d = HD / NP * h + PW * (4 * g + e);
         float o[PW];
 #pragma unroll
-        for (int i = 0; i < PW; ++i) o[i] = rows.acc[n][PW * h + i][e] * unit;
+        for (int i = 0; i < PW; ++i) o[i] = rows.acc[n][PW * h + i][e] * over * vref;
         if (a.nsplit > 1) {
 #pragma unroll
           for (int i = 0; i < PW; i += 4)
             *reinterpret_cast<f32x4*>(a.part + at * HD + d + i) = (f32x4){o[i], o[i + 1], o[i + 2], o[i + 3]};
         } else {
-          kv8_out<BF, PW>(gate + d, out + d, o, 1.f / ls);
+          kv8_out<BF, PW>(gate + d, out + d, o);
         }
       }
   }
 }
 
 // Outputs of split positions: a workgroup per row, a wave to every eight splits (up to 16 waves); each wave weighs
-// those of its splits that hold positions of the row's tile by their largest maximum, and the waves meet
+// those of its splits that hold positions of the row's tile by their share of its sum, and the waves meet
 // in LDS. Bound by the latency of one read of the partial outputs, all in flight at once (128 splits of 24 rows
 // 7 us, with one wave a row 49).
 constexpr int kMergeWaves = 16, kMergeSplits = 8;
@@ -1039,18 +1041,20 @@ __global__ void __launch_bounds__(64 * kMergeWaves) attn_kv8_merge_kernel(Kv8Att
     float mn = m;
 #pragma unroll
     for (int u = 0; u < kMergeSplits; ++u) mn = fmaxf(mn, s[u].x);
-    const float f = exp2_raw(m - mn);
-    l *= f;
-    o *= f;
-    m = mn;
+    float w[kMergeSplits];
+    const float before = l * exp2_raw(m - mn);
+    l = before;
 #pragma unroll
     for (int u = 0; u < kMergeSplits; ++u) {
-      const float w = z0 + u < nz ? exp2_raw(s[u].x - m) : 0.f;
-      if (z0 + u < nz) {
-        l += s[u].y * w;
-        o += x[u] * w;
-      }
+      w[u] = z0 + u < nz ? s[u].y * exp2_raw(s[u].x - mn) : 0.f;
+      l += w[u];
     }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    o *= before * inv;
+    m = mn;
+#pragma unroll
+    for (int u = 0; u < kMergeSplits; ++u)
+      if (z0 + u < nz) o += x[u] * (w[u] * inv);
   }
   *reinterpret_cast<vec_t*>(merge_lds + wave * HD + d) = o;
   if (lane == 0) mls[wave] = make_float2(m, l);
@@ -1058,16 +1062,14 @@ __global__ void __launch_bounds__(64 * kMergeWaves) attn_kv8_merge_kernel(Kv8Att
   if (wave) return;
   float mm = -FLT_MAX;
   for (int w = 0; w < nw; ++w) mm = fmaxf(mm, mls[w].x);
-  o = 0.f;
   l = 0.f;
-  for (int w = 0; w < nw; ++w) {
-    const float f = exp2_raw(mls[w].x - mm);
-    o += *reinterpret_cast<const vec_t*>(merge_lds + w * HD + d) * f;
-    l += mls[w].y * f;
-  }
-  const float inv = 1.f / l;
+  for (int w = 0; w < nw; ++w) l += mls[w].y * exp2_raw(mls[w].x - mm);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  o = 0.f;
+  for (int w = 0; w < nw; ++w)
+    o += *reinterpret_cast<const vec_t*>(merge_lds + w * HD + d) * (mls[w].y * exp2_raw(mls[w].x - mm) * inv);
 #pragma unroll
-  for (int j = 0; j < V; ++j) out[j] = E::mk(o[j] * inv * sigmoid_raw(E::ld(gate[j])));
+  for (int j = 0; j < V; ++j) out[j] = E::mk(o[j] * sigmoid_raw(E::ld(gate[j])));
 }
 
 // ---- launches ------------------------------------------------------------------------------------

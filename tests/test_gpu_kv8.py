@@ -630,3 +630,17 @@ def test_attn_kv8_outputs_are_rounded_once(dtype, long):
     step = torch.finfo(dtype).eps * 2.0 ** want.abs().clamp(min=2.0 ** -14).log2().floor()
     near = (2 * off / step).clamp(max=1.0).sum()  # borders lie a step apart
     assert int((got != want.to(dtype)).sum()) <= float(near)
+
+
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("long", [False, True])
+def test_attn_kv8_values_next_to_the_largest(long, splits):
+    """bf16 V rows of up to 127 x 2^121, next to float32's largest number, which any sum of two of them passes:
+    their averages are finite."""
+    B, S, pos, L, H, G, hd = 1, 24, [350], 374, 4, 2, 64
+    t = _attn_inputs(B, S, pos, L, H, G, hd, BF16)
+    t["vs"] = 0.25 + 0.75 * t["vs"] / t["vs"].amax()
+    want, tol = _reference(t, H, G, hd)
+    t["vs"] = t["vs"] * 2.0 ** 121
+    got = _attn(t, H, G, hd, long=long, splits=splits)
+    _check(got.double() * 2.0 ** -121, want, tol, BF16)
