@@ -210,7 +210,8 @@ int gsq_gdn_seq(const void* qkv, int64_t qkv_stride, const void* z, int64_t z_st
  * n_trees = 1 or batch rows of seq. Outputs as gsq_gdn_seq over each token's path gives them (float32
  * sums in another order); the states are only read: the tokens that are kept go through gsq_gdn_seq
  * afterwards. A batch row whose parents are not such gets NaN outputs; a value that is not finite makes the
- * outputs of its token's path and of those that follow it NaN, in the heads it belongs to. */
+ * outputs of its token's path and of those that follow it NaN, in the heads it belongs to (an infinite a is a decay of
+ * 0 or 1, as for gsq_gdn_seq). */
 int gsq_gdn_tree(const void* qkv, int64_t qkv_stride, const void* z, int64_t z_stride, const void* ab, int64_t ab_stride,
                  const void* conv_state, const void* conv_w, const float* ssm_a, const float* dt_bias,
                  const float* rec_state, const void* norm_w, const int32_t* parents, int64_t n_trees, void* out,

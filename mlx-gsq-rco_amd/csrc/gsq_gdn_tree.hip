@@ -227,6 +227,8 @@ __global__ void __launch_bounds__(TH) gdn_tree_kernel(GdnTreeArgs a, bool pair) 
     uint32_t lo = lane < 32 ? 1u << lane : 0u, hi = lane < 32 ? 0u : 1u << (lane - 32);
     const float sp = av > 20.f ? av : log1pf(expf(av));  // softplus (torch's threshold 20)
     double lg = lane < S ? (double)(a.ssm_a[h] * sp) : 0.0;
+    // a decay below e^-1000 is 0 for any use of it; its logarithm would take the others' bits from the sums along the path
+    lg = lg < -1000.0 ? -1000.0 : lg;
     int p = par;
 #pragma unroll
     for (int i = 0; i < 6; ++i) {  // pointer doubling: what p's path so far holds joins

@@ -199,3 +199,19 @@ def test_gdn_tree_graph_replays():
         d["rows"].mul_(0.9)
         d["rec"].mul_(1.1)
         d["parents"][:, 1:].clamp_(max=i)
+
+
+@pytest.mark.parametrize("a", [3e4, 1e18, float("inf")])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_gdn_tree_decays_of_nothing(dtype, a):
+    """Tokens that forget everything before them (decays of e^-3e4 and less): the decays of those that follow keep
+    their bits."""
+    case = (1, 40, 2, 4, 64, 64, 4, 0, dtype, "random")
+    t = _inputs(case, 13)
+    t["ab"][:, 3::9, :4] = a
+    want = _reference(case, t)
+    assert torch.isfinite(want).all()
+    assert _rel(_run(case, t), want) <= _bound(dtype)
+    chain = dict(t, parents=(torch.arange(40, dtype=torch.int32) - 1)[None].contiguous())
+    want = _reference(case, chain)
+    assert _rel(_run(case, chain), want) <= _bound(dtype) and _rel(_run(case, chain, "gdn_seq"), want) <= _bound(dtype)
