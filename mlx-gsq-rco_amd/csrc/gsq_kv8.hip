@@ -776,7 +776,7 @@ __global__ void __launch_bounds__(256, 2) attn_kv8_rows_kernel(Kv8AttnArgs a) {
       f[w] = x.y * exp2_raw(x.x - mm);
       ll += f[w];
     }
-    const float inv = ll == 0.f ? 0.f : 1.f / ll;
+    const float inv = ll == 0.f && a.nsplit > 1 ? 0.f : 1.f / ll;  // no weight at all: NaN, unless another split has one
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < 4; ++w) o += *reinterpret_cast<const f32x4*>(mo + (w * 16 + rr) * OS + d) * (f[w] * inv);
@@ -970,7 +970,8 @@ __global__ void __launch_bounds__(256, 2) attn_kv8_tile_kernel(Kv8AttnArgs a) {
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int r = r0 + 16 * n + c;
-    const float ls = rows.sum(n), over = rows.over(ls), vref = rows.vref;
+    const float ls = rows.sum(n), vref = rows.vref;
+    const float over = ls == 0.f && a.nsplit == 1 ? __builtin_nanf("") : rows.over(ls);
     if (r >= k.R) continue;
     const int64_t all = (int64_t)a.B * a.Hkv * k.R, at = (((int64_t)k.bb * a.Hkv + k.kvh) * k.R + r) * a.nsplit + k.z;
     if (a.nsplit > 1 && g == 0) *reinterpret_cast<float2*>(a.part + all * a.nsplit * HD + 2 * at) = make_float2(rows.top(n), ls);
@@ -1064,7 +1065,7 @@ __global__ void __launch_bounds__(64 * kMergeWaves) attn_kv8_merge_kernel(Kv8Att
   for (int w = 0; w < nw; ++w) mm = fmaxf(mm, mls[w].x);
   l = 0.f;
   for (int w = 0; w < nw; ++w) l += mls[w].y * exp2_raw(mls[w].x - mm);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = 1.f / l;
   o = 0.f;
   for (int w = 0; w < nw; ++w)
     o += *reinterpret_cast<const vec_t*>(merge_lds + w * HD + d) * (mls[w].y * exp2_raw(mls[w].x - mm) * inv);

@@ -644,3 +644,21 @@ def test_attn_kv8_values_next_to_the_largest(long, splits):
     t["vs"] = t["vs"] * 2.0 ** 121
     got = _attn(t, H, G, hd, long=long, splits=splits)
     _check(got.double() * 2.0 ** -121, want, tol, BF16)
+
+
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("long", [False, True])
+def test_attn_kv8_scores_below_the_range(long, splits):
+    """A row whose scores all pass float32's range downwards has no weights: NaN, as their softmax gives; the
+    other rows are what they are without it."""
+    B, S, pos, L, H, G, hd = 1, 40, [300], 340, 4, 2, 64
+    t = _attn_inputs(B, S, pos, L, H, G, hd, BF16)
+    t["k"], t["ks"] = _quantise(_values(t["k"], t["ks"]).abs() + 1)
+    clean, tol = _reference(t, H, G, hd)
+    q = t["q"].view(B, S, H, hd)
+    q[0, 12, 1] = -3e38
+    got = _attn(t, H, G, hd, long=long, splits=splits).view(B, S, H, hd)
+    assert torch.isnan(got[0, 12, 1]).all()
+    keep = torch.ones(B, S, H, dtype=torch.bool)
+    keep[0, 12, 1] = False
+    _check(got[keep], clean[keep], tol[keep], BF16)
