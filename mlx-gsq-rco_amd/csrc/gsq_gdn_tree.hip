@@ -28,6 +28,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kTreeConv = 8;  // largest convolution kernel
 constexpr int kTreeRows = 4;  // q or k rows of a wave whose inputs are in flight together
+constexpr float kTreeUnit = 4096.f;  // q and k rows in fp16 numbers: normalized they are at most sqrt(128) in size
 
 __device__ __forceinline__ f32x4 mma4(float a, float b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
@@ -57,8 +58,8 @@ __device__ __forceinline__ float rsqrt_raw(float x) { return __builtin_amdgcn_rs
 
 // One workgroup per (value head, batch row), a wave per 16 state columns, tokens in NI tiles of 16 rows.
 // Products that sum over the key dims take their float32 factors as two fp16 numbers each (hi + lo, 22 bits;
-// q and k before their constant factor, state columns over a power of two, so that both are of size 1 and
-// lo x lo, 2^-24 of the product, can go): three MFMAs of 32 dims in 48 cycles where float32 ones take 256. What
+// q and k before their constant factor, state columns over a power of two, so that both are of one size and
+// lo x lo, 2^-24 of the product, can go; q and k times 2^12, so that rows far below the norm's epsilon keep their bits too): three MFMAs of 32 dims in 48 cycles where float32 ones take 256. What
 // sums over tokens stays in float32 MFMAs (16 x 16 x 4): for A a lane gives row lane % 16, for B and the
 // result column lane % 16; step e takes rows 4 (lane / 16) + e, so that operands are 16-byte pieces and a
 // result is the B operand of the next product as it is.
@@ -197,7 +198,7 @@ __global__ void __launch_bounds__(TH) gdn_tree_kernel(GdnTreeArgs a, bool pair) 
           }
         x = silu_raw(x);
         y = silu_raw(y);
-        const float rn = rsqrt_raw(lanes_sum(on ? x * x + y * y : 0.f) * dki + 1e-6f);
+        const float rn = rsqrt_raw(lanes_sum(on ? x * x + y * y : 0.f) * dki + 1e-6f) * kTreeUnit;
         x = on && t < S ? x * rn : 0.f;
         y = on && t < S ? y * rn : 0.f;
         if (c0 < DKP && t < R) {
@@ -248,7 +249,7 @@ __global__ void __launch_bounds__(TH) gdn_tree_kernel(GdnTreeArgs a, bool pair) 
     }
   }
   __syncthreads();
-  const float qscale = 1.f / (float)dk, kscale = 1.f / sqrtf((float)dk);
+  const float qscale = 1.f / (kTreeUnit * (float)dk), kscale = 1.f / (kTreeUnit * sqrtf((float)dk));
   // tiles (i, j <= i) of k k^T and q k^T
   for (int n = wave; n < NI * (NI + 1); n += nw) {
     const bool isq = n & 1;

@@ -215,3 +215,15 @@ def test_gdn_tree_decays_of_nothing(dtype, a):
     chain = dict(t, parents=(torch.arange(40, dtype=torch.int32) - 1)[None].contiguous())
     want = _reference(case, chain)
     assert _rel(_run(case, chain), want) <= _bound(dtype) and _rel(_run(case, chain, "gdn_seq"), want) <= _bound(dtype)
+
+
+@pytest.mark.parametrize("size", [1e-5, 1e-7])
+def test_gdn_tree_small_queries_and_keys(size):
+    """q and k inputs far below the norm's epsilon (their rows are 1000 times the inputs, not of size 1): float32's bits
+    all the same."""
+    case = (1, 20, 2, 4, 128, 64, 4, 0, F32, "random")
+    t = _inputs(case, 17)
+    n = 2 * 2 * 128
+    t["rows"][..., :n] *= size
+    t["conv"][..., :n] *= size
+    assert _rel(_run(case, t), _reference(case, t)) <= _bound(F32)
