@@ -83,7 +83,7 @@ __device__ __forceinline__ uint64_t tree_path(const int32_t* parents, int S) {
 // in double. Rounding to 8 bits jumps at values next to a border, so k is formed in double and a row that has
 // a quotient within 1e-4 of a border (five times what float32 can be off) divides in double too:
 // the bytes are those of the definition. Bound by the arithmetic of a row (2047 tokens of 24 + 2 x 4 heads
-// of 256: 60 MB in 23 us; one token of 8 rows 5.1 us).
+// of 256: 60 MB in 22 us; one token of 8 rows 5.1 us).
 constexpr int kWriteRows = 2;
 
 template <bool BF, int HD>
@@ -651,7 +651,7 @@ __device__ __forceinline__ void kv8_out(const uint16_t* gate, uint16_t* out, con
 // blocks in turn, each with a softmax of its own; K and V go from memory to registers in 16-byte pieces,
 // a block ahead, and are expanded there: no LDS and no barrier in the loop. The waves are merged at the end.
 // One token of 24 heads over 131071 positions (4 KV heads of 256, 272 MB): 44 us, 6.2 TB/s with part of it in
-// the last-level cache; 32 rows of 4096 to 8191 positions (414 MB) 76 us. Over 300 positions 10.5 us, all of it
+// the last-level cache; 32 rows of 4096 to 8191 positions (414 MB) 76 us. Over 300 positions 11 us, all of it
 // latency: position, queries and first blocks, two more blocks, gates.
 template <bool BF, int HD>
 __global__ void __launch_bounds__(256, 2) attn_kv8_rows_kernel(Kv8AttnArgs a) {
@@ -808,7 +808,7 @@ constexpr int kv8_lds_steps(int hd) { return hd == 256 ? 1 : 0; }
 //    DMA in flight (413 -> 370).
 //  * 4096 tokens of 24 heads of 256 in fp16 350 us (0.59 PFLOP/s without the second term of the weights; a large
 //    library product 1.31), of which a fifth is the triangle's tail; 700 bf16 tokens of 2 x 32 heads of 128 behind
-//    5000 positions 270 (352 workgroups on 256 CUs); a tree of 64 tokens of 4 rows behind 8000 to 16000 144 + 15.
+//    5000 positions 322 (352 workgroups on 256 CUs); a tree of 64 tokens of 4 rows behind 8000 to 16000 162 + 16.
 template <bool BF, int HD, int NT>
 __global__ void __launch_bounds__(256, 2) attn_kv8_tile_kernel(Kv8AttnArgs a) {
   constexpr int KS = HD / 32, VB = HD / 16, RT = 64 * NT, NC = HD / 16;  // NC: 16-byte pieces of a row
@@ -1077,7 +1077,8 @@ __global__ void __launch_bounds__(64 * kMergeWaves) attn_kv8_merge_kernel(Kv8Att
 
 template <bool BF>
 static hipError_t launch_kv8_write_t(const Kv8WriteArgs& a, hipStream_t s) {
-  // few tokens: the heads of one are shared out over several workgroups
+  // few tokens: the heads of one are shared out over several workgroups (24 + 2 x 4 heads of 256, shared or not: one token
+  // 3.8 / 7.6 us, 512 tokens 8.1 / 9.5, 768 11.0 / 10.6, 1024 13.9 / 12.1, 2047 24.7 / 20.6)
   const int64_t tokens = (int64_t)a.B * a.S;
   const int rows = a.H + 2 * a.Hkv, most = (rows + 4 * kWriteRows - 1) / (4 * kWriteRows);
   if (a.S >= 1 << 24) return hipErrorInvalidValue;  // a launch counts its threads along x in 32 bits
@@ -1150,12 +1151,24 @@ static hipError_t launch_attn_kv8_tile(const Kv8AttnArgs& a, hipStream_t s) {
 }
 
 // Rows of a workgroup. attn_kv8_rows_kernel (16) has the shorter chain, attn_kv8_tile_kernel reads the cache once
-// for 128 rows. Measured by rows and by tiles (24 heads of 256, fp16): 13 drafted tokens over 2000, 52000 and
-// 104000 positions 22 / 39, 71 / 79 and 135 / 110 us, 64 over 10800 and 21700 60 / 73 and 101 / 97, prompts
-// of 333, 1100 and 4096 17 / 49, 67 / 86 and 568 / 356. So the tiles are for kTileBlocks tiles of 16 rows by
-// 32 positions and more, where the two meet. Head dim 64 takes 256 rows instead of 128 where that makes two
-// workgroups a CU (4096 tokens of 2 x 32 heads: 326 against 352 us); at 128 the registers do not hold them
-// (521 against 481).
+// for 128 rows. The tiles are for kTileBlocks tiles of 16 rows by 32 positions and more, where the two meet: by rows
+// and by tiles, in us, in caches as long as their content,
+//                                      at half of it   at it         twice         four times
+//   24 heads of 256   13 drafted         57 /  64      102 /  89     199 / 149     399 / 250
+//   (4 KV heads)      64 drafted         48 /  66       79 /  82     139 / 114     261 / 180
+//                     400 tokens         54 /  66       97 /  82     182 / 115     342 / 184
+//   32 heads of 128   13 drafted         32 /  44       51 /  61      88 /  98     183 / 173
+//   (8)               64 drafted         33 /  44       50 /  52      84 /  73     151 / 112
+//                     400 tokens         33 /  48       54 /  59      97 /  81     184 / 127
+//   64 heads of 64    13 drafted         25 /  34       38 /  38      62 /  55     111 /  87
+//   (8)               64 drafted         26 /  33       38 /  40      62 /  55     110 /  79
+//                     400 tokens         22 /  44       32 /  53      52 /  71      91 / 106
+// in fp16; in bf16 both are up to 8 per cent slower and meet at the same places. Prompts of 333, 1100 and 1600 without a
+// cache: 16 / 44, 68 / 83, 112 / 127 at head dim 256; 13 / 27, 45 / 55, 78 / 78 at 128; 14 / 20, 49 / 44, 87 / 73 at 64.
+// What the host knows is the capacity (max_len), not the positions in use: in a cache with room left fewer
+// tokens take the tiles (333 behind none in 4096 positions: 51 us).
+// Head dim 64 takes 256 rows instead of 128 where that makes two workgroups a CU (4096 tokens of 2 x 32 heads: over 4 KV
+// heads 302 against 325 us, over 32 336 against 340); at 128 the registers do not hold them (with sums over u, 521 against 481).
 constexpr int64_t kTileBlocks = 49152;
 
 int attn_kv8_plan(int64_t batch, int64_t seq, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_len) {
