@@ -295,11 +295,12 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8ReadArgs a) {
 //    operand of O^T = V^T P^T: probabilities never leave their lane.
 //  * A byte u with a zero byte above it is the fp16 (subnormal) number u 2^-24, which the matrix cores
 //    take as it is: one v_perm expands two bytes, and K and V cost no rounding. What the 128 in u adds to a
-//    score is known: -128 sum(q) starts its accumulator (queries of one sign, 4 to 16 times their spread, leave fp16
-//    outputs 0.4 per cent more error than their rounding; without the offset none, for 5 per cent of the time). V's bytes lose their 128 as pairs, before the product: sums
-//    over u, with 128 times the weights' sum taken off, end 1.4 to 2.8 x 2^-24 of the rows' largest values low in all dims
-//    alike, as the matrix cores truncate (over u - 128: 0.3 to 0.7), which an average over 131072 positions shows (4.5e-5 of
-//    the output against 1.7e-5; cost: prompt of 4096 320 -> 329 us, none where the cache's bytes bound it).
+//    score is known: -128 sum(q) starts its accumulator (queries of one sign, 4 to 16 times their spread,
+//    leave fp16 outputs 0.4 per cent more error than their rounding; without the offset none, for 5 per cent of
+//    the time). V's bytes lose their 128 as pairs, before the product: sums over u, with 128 times the weights'
+//    sum taken off, end 1.4 to 2.8 x 2^-24 of the rows' largest values low in all dims alike, as the matrix
+//    cores truncate (over u - 128: 0.3 to 0.7), which an average over 131072 positions shows (4.5e-5 of the
+//    output against 1.7e-5; cost: prompt of 4096 320 -> 329 us, none where the cache's bytes bound it).
 //  * The scale of a K row multiplies its scores, that of a V row its probabilities. bf16 queries are
 //    scaled to fp16 by a power of two for each row: their 8 bits fit, and what falls below 2^-38 of the
 //    row's largest cannot be seen in float32 sums.
