@@ -303,6 +303,77 @@ int gsq_attn_kv8(const void* q, int64_t q_stride, const void* qg, int64_t qg_str
                  int64_t batch, int64_t seq, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_len, int dtype,
                  void* stream);
 
+/* ---- steps that serve many requests, over paged caches ----
+ * A step packs the new tokens of `sequences` (at most 1024) requests behind one another, `tokens` rows in all: those of
+ * sequence b are rows cu[b] .. cu[b + 1] - 1. rows[b] is its request (0 .. n_requests - 1; -1: it is not served) and
+ * lens[b] its length, the new tokens among it: token i of sequence b sits at position lens[b] - (cu[b + 1] - cu[b]) + i. K
+ * and V lie in pages [n_pages, kv_heads, page_size, head_dim] (page_size 16, 32, 64, 128 or 256): position p of request r is
+ * row p % page_size of page table[r * max_pages + p / page_size]. All of these are int32 on the device (positions and
+ * slots int64), read when the work runs: a captured call follows them. Rows of a sequence that is not served, or whose
+ * numbers do not fit the shapes or the pages, get NaN outputs and leave caches and states alone; rows behind the
+ * last sequence get zeros. */
+
+/* The layout of a step: requests[b] brings new_tokens[b] tokens behind its lengths[r] cached ones. Pages for them that
+ * the request does not hold yet (held[r], the first entries of its table row) are taken from the end of free_pages (its first
+ * *n_free are free): sequence by sequence, need_b = max(0, ceil((lengths[r] + new_tokens[b]) / page_size) - held[r]). A
+ * sequence is served unless its request is out of range or named by an earlier sequence, it does not fit its table row or
+ * the `tokens` rows, or it needs pages and the running sum of the needs passes *n_free. table, held and n_free are
+ * updated; lengths are not (gsq_page_advance), so that the same call again gives the same step. Out: cu (sequences + 1), rows and
+ * lens (-1 and 0 if not served), pos and slots (page * page_size + row) of each of the `tokens` rows, -1 where there is none. */
+int gsq_page_plan(const int32_t* requests, const int32_t* new_tokens, const int32_t* lengths, int32_t* held, int32_t* table,
+                  const int32_t* free_pages, int32_t* n_free, int64_t sequences, int64_t n_requests, int64_t max_pages,
+                  int64_t n_pages, int64_t tokens, int64_t page_size, int32_t* cu, int32_t* rows, int32_t* lens, int64_t* pos,
+                  int64_t* slots, void* stream);
+
+/* lengths[rows[b]] = lens[b] of the sequences served: the step's tokens are cached. */
+int gsq_page_advance(const int32_t* rows, const int32_t* lens, int32_t* lengths, int64_t sequences, int64_t n_requests,
+                     void* stream);
+
+/* The pages of these requests back to free_pages, in the opposite order of gsq_page_plan's taking; their lengths, pages
+ * held and table entries are cleared. Requests out of range, or named before, are passed over. */
+int gsq_page_release(const int32_t* requests, int32_t* lengths, int32_t* held, int32_t* table, int32_t* free_pages,
+                     int32_t* n_free, int64_t sequences, int64_t n_requests, int64_t max_pages, int64_t n_pages, void* stream);
+
+/* q (heads) and k (kv_heads) of each token RMS-normalized per head (weights, eps) and rotated on their first
+ * rotary_dim dims (rotate-half, angle pos * inv_freq[i]) in float32, rounded once: q into q_out [tokens, heads, head_dim],
+ * k and v into row slots[t] of the pages; tokens without a slot get zeros and write nothing. Slots of one call must differ.
+ * Token and head strides of q, k, v in elements. fp16 or bf16; head_dim 64, 128 or 256; pages and q_out 16-byte aligned. */
+int gsq_paged_write(const void* q, int64_t q_stride, int64_t q_head_stride, const void* k, int64_t k_stride,
+                    int64_t k_head_stride, const void* v, int64_t v_stride, int64_t v_head_stride, const void* q_norm_w,
+                    const void* k_norm_w, const double* inv_freq, void* k_pages, void* v_pages, const int64_t* pos,
+                    const int64_t* slots, void* q_out, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                    int64_t rotary_dim, int64_t n_pages, int64_t page_size, float eps, int dtype, void* stream);
+
+/* Floats of work that gsq_attn_paged needs on a device of `cus` CUs (-1 for sizes that it refuses). */
+int64_t gsq_attn_paged_work(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                            int64_t max_pages, int64_t page_size, int64_t max_new, int64_t cus);
+
+/* out = round(softmax(q K^T / sqrt(head_dim)) V [* sigmoid(gate)]) of every packed token and head (kv head h / (heads /
+ * kv_heads)) over positions 0 .. its own. q and out [tokens, heads, head_dim], 16-byte aligned as the pages and work; gate
+ * NULL, or with strides in elements between tokens and heads. max_new: most new tokens that a sequence is expected to
+ * bring; it chooses kernels, longer ones are served too. */
+int gsq_attn_paged(const void* q, const void* gate, int64_t gate_stride, int64_t gate_head_stride, const void* k_pages,
+                   const void* v_pages, const int32_t* table, const int32_t* cu, const int32_t* rows, const int32_t* lens,
+                   void* out, float* work, int64_t tokens, int64_t sequences, int64_t n_requests, int64_t max_pages,
+                   int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t n_pages, int64_t page_size, int64_t max_new,
+                   int64_t cus, int dtype, void* stream);
+
+/* Floats of work that gsq_gdn_packed needs (-1 for sizes that it refuses). */
+int64_t gsq_gdn_packed_work(int64_t tokens, int64_t sequences, int64_t key_heads, int64_t value_heads, int64_t head_k_dim,
+                            int64_t head_v_dim, int64_t conv_kernel, int64_t max_new);
+
+/* gsq_gdn_seq over the packed sequences of a step (rows of qkv, z, ab and out are packed tokens), request r with the states
+ * conv_state [n_requests, conv_kernel - 1, conv_dim] and rec_state [n_requests, value_heads, head_k_dim, head_v_dim] of its
+ * own; a sequence that begins its request (lens = its new tokens) begins from zeros, whatever they hold. Two sequences of a step
+ * must not name one request. fp16 or bf16; head_k_dim 32, 64 or 128, head_v_dim 64, 128 or 256, conv_kernel 2..8; rec_state
+ * and work (gsq_gdn_packed_work floats) 16-byte aligned. max_new as for gsq_attn_paged. */
+int gsq_gdn_packed(const void* qkv, int64_t qkv_stride, const void* z, int64_t z_stride, const void* ab, int64_t ab_stride,
+                   void* conv_state, const void* conv_w, const float* ssm_a, const float* dt_bias, float* rec_state,
+                   const void* norm_w, const int32_t* cu, const int32_t* rows, const int32_t* lens, void* out,
+                   int64_t out_stride, float* work, int64_t tokens, int64_t sequences, int64_t n_requests, int64_t key_heads,
+                   int64_t value_heads, int64_t head_k_dim, int64_t head_v_dim, int64_t conv_kernel, float eps,
+                   int64_t max_new, int dtype, void* stream);
+
 /* Message of the last failed call on this thread ("" if none). */
 const char* gsq_last_error(void);
 

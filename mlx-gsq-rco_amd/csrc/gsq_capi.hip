@@ -41,6 +41,14 @@ hipError_t launch_attn_kv8(bool bf16, const Kv8AttnArgs& a, hipStream_t s);
 int64_t attn_kv8_splits(int64_t batch, int64_t seq, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_len,
                         int cus);
 hipError_t launch_attn_decode(int dt, const AttnArgs& a, hipStream_t s);
+hipError_t launch_page_plan(const PagePlanArgs& a, hipStream_t s);
+hipError_t launch_page_advance(const int32_t* rows, const int32_t* lens, int32_t* lengths, int B, int R, hipStream_t s);
+hipError_t launch_page_release(const PageReleaseArgs& a, hipStream_t s);
+hipError_t launch_paged_write(bool bf16, const PagedWriteArgs& a, hipStream_t s);
+int64_t attn_paged_work(const AttnPagedArgs& a);
+hipError_t launch_attn_paged(bool bf16, const AttnPagedArgs& a, hipStream_t s);
+int64_t gdn_packed_work(const GdnPackedArgs& a);
+hipError_t launch_gdn_packed(bool bf16, const GdnPackedArgs& a, hipStream_t s);
 int qmv_table_bytes(int qt);
 int build_qmv_table(int qt, const uint16_t* grid16, const uint8_t* ksigns, std::vector<uint8_t>& out);
 int qmm_table_bytes(int qt);
@@ -919,6 +927,202 @@ int gsq_attn_kv8(const void* q, int64_t q_stride, const void* qg, int64_t qg_str
   a.B = (int)batch; a.S = (int)seq; a.H = (int)heads; a.Hkv = (int)kv_heads; a.hd = (int)head_dim; a.nsplit = (int)splits;
   hipError_t e = launch_attn_kv8(dtype == GSQ_BF16, a, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return fail(GSQ_E_HIP, "attn_kv8 launch: %s", hipGetErrorString(e));
+  return GSQ_OK;
+}
+
+// What the calls on paged caches share: sequences of a step, requests and the block table's columns.
+static int check_sequences(int64_t sequences, int64_t n_requests, int64_t tokens) {
+  if (sequences < 0 || sequences > 1024) return fail(GSQ_E_VALUE, "a step holds at most 1024 sequences");
+  if (n_requests <= 0 || n_requests >= (1ll << 31)) return fail(GSQ_E_VALUE, "invalid number of requests");
+  if (tokens < 0 || tokens >= (1ll << 31) - 1024) return fail(GSQ_E_VALUE, "invalid number of tokens");
+  return GSQ_OK;
+}
+
+static int check_pages(int64_t max_pages, int64_t n_pages, int64_t page_size) {
+  if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)))
+    return fail(GSQ_E_VALUE, "a page holds 16, 32, 64, 128 or 256 positions");
+  if (n_pages <= 0 || n_pages >= (1ll << 31)) return fail(GSQ_E_VALUE, "invalid number of pages");
+  if (max_pages <= 0 || max_pages * page_size >= (1ll << 31) - 1024) return fail(GSQ_E_VALUE, "invalid block table width");
+  return GSQ_OK;
+}
+
+int gsq_page_plan(const int32_t* requests, const int32_t* new_tokens, const int32_t* lengths, int32_t* held, int32_t* table,
+                  const int32_t* free_pages, int32_t* n_free, int64_t sequences, int64_t n_requests, int64_t max_pages,
+                  int64_t n_pages, int64_t tokens, int64_t page_size, int32_t* cu, int32_t* rows, int32_t* lens, int64_t* pos,
+                  int64_t* slots, void* stream) {
+  if (int rc = check_sequences(sequences, n_requests, tokens)) return rc;
+  if (int rc = check_pages(max_pages, n_pages, page_size)) return rc;
+  if (!lengths || !held || !table || !free_pages || !n_free || !cu || (sequences && (!requests || !new_tokens || !rows || !lens)) ||
+      (tokens && (!pos || !slots)))
+    return fail(GSQ_E_VALUE, "NULL pointer");
+  PagePlanArgs a;
+  a.requests = requests; a.fresh = new_tokens; a.lengths = lengths; a.held = held; a.table = table; a.free = free_pages;
+  a.n_free = n_free; a.cu = cu; a.rows = rows; a.lens = lens; a.pos = pos; a.slots = slots; a.W = max_pages; a.N = tokens;
+  a.B = (int)sequences; a.R = (int)n_requests; a.n_pages = (int)n_pages; a.P = (int)page_size;
+  hipError_t e = launch_page_plan(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(GSQ_E_HIP, "page_plan launch: %s", hipGetErrorString(e));
+  return GSQ_OK;
+}
+
+int gsq_page_advance(const int32_t* rows, const int32_t* lens, int32_t* lengths, int64_t sequences, int64_t n_requests,
+                     void* stream) {
+  if (int rc = check_sequences(sequences, n_requests, 0)) return rc;
+  if (sequences == 0) return GSQ_OK;
+  if (!rows || !lens || !lengths) return fail(GSQ_E_VALUE, "NULL pointer");
+  hipError_t e = launch_page_advance(rows, lens, lengths, (int)sequences, (int)n_requests, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(GSQ_E_HIP, "page_advance launch: %s", hipGetErrorString(e));
+  return GSQ_OK;
+}
+
+int gsq_page_release(const int32_t* requests, int32_t* lengths, int32_t* held, int32_t* table, int32_t* free_pages,
+                     int32_t* n_free, int64_t sequences, int64_t n_requests, int64_t max_pages, int64_t n_pages, void* stream) {
+  if (int rc = check_sequences(sequences, n_requests, 0)) return rc;
+  if (int rc = check_pages(max_pages, n_pages, 16)) return rc;
+  if (sequences == 0) return GSQ_OK;
+  if (!requests || !lengths || !held || !table || !free_pages || !n_free) return fail(GSQ_E_VALUE, "NULL pointer");
+  PageReleaseArgs a;
+  a.requests = requests; a.lengths = lengths; a.held = held; a.table = table; a.free = free_pages; a.n_free = n_free;
+  a.W = max_pages; a.B = (int)sequences; a.R = (int)n_requests; a.n_pages = (int)n_pages;
+  hipError_t e = launch_page_release(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(GSQ_E_HIP, "page_release launch: %s", hipGetErrorString(e));
+  return GSQ_OK;
+}
+
+static int check_heads(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim) {
+  if (kv_heads <= 0 || heads <= 0 || heads % kv_heads || heads > 65535)
+    return fail(GSQ_E_VALUE, "heads must be a positive multiple of kv heads (at most 65535)");
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256) return fail(GSQ_E_VALUE, "head dim must be 64, 128 or 256");
+  if (tokens * heads >= (1ll << 31)) return fail(GSQ_E_VALUE, "too many query rows");
+  return GSQ_OK;
+}
+
+int gsq_paged_write(const void* q, int64_t q_stride, int64_t q_head_stride, const void* k, int64_t k_stride,
+                    int64_t k_head_stride, const void* v, int64_t v_stride, int64_t v_head_stride, const void* q_norm_w,
+                    const void* k_norm_w, const double* inv_freq, void* k_pages, void* v_pages, const int64_t* pos,
+                    const int64_t* slots, void* q_out, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                    int64_t rotary_dim, int64_t n_pages, int64_t page_size, float eps, int dtype, void* stream) {
+  if (dtype != GSQ_F16 && dtype != GSQ_BF16) return fail(GSQ_E_TYPE, "unsupported dtype code %d", dtype);
+  // a launch counts its threads along x in 32 bits
+  if (tokens < 0 || tokens >= (1ll << 24)) return fail(GSQ_E_VALUE, "tokens must be 0..2^24 - 1");
+  if (int rc = check_heads(tokens, heads, kv_heads, head_dim)) return rc;
+  if (int rc = check_pages(1, n_pages, page_size)) return rc;
+  if (rotary_dim < 0 || rotary_dim > head_dim || rotary_dim % 2) return fail(GSQ_E_VALUE, "invalid rotary dim");
+  if (!(eps >= 0.f)) return fail(GSQ_E_VALUE, "eps must be >= 0");
+  if (tokens == 0) return GSQ_OK;
+  if (!q || !k || !v || !q_norm_w || !k_norm_w || (!inv_freq && rotary_dim) || !k_pages || !v_pages || !pos || !slots || !q_out)
+    return fail(GSQ_E_VALUE, "NULL pointer");
+  if ((reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages) | reinterpret_cast<uintptr_t>(q_out)) & 15)
+    return fail(GSQ_E_VALUE, "k_pages, v_pages and q_out must be 16-byte aligned");
+  PagedWriteArgs a;
+  a.q = q; a.k = k; a.v = v; a.q_norm_w = q_norm_w; a.k_norm_w = k_norm_w; a.inv_freq = inv_freq; a.kp = k_pages;
+  a.vp = v_pages; a.pos = pos; a.slots = slots; a.out = q_out; a.q_stride = q_stride; a.q_head = q_head_stride;
+  a.k_stride = k_stride; a.k_head = k_head_stride; a.v_stride = v_stride; a.v_head = v_head_stride;
+  a.n_slots = n_pages * page_size; a.N = (int)tokens; a.H = (int)heads; a.Hkv = (int)kv_heads; a.hd = (int)head_dim;
+  a.rd = (int)rotary_dim; a.P = (int)page_size; a.eps = eps;
+  hipError_t e = launch_paged_write(dtype == GSQ_BF16, a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(GSQ_E_HIP, "paged_write launch: %s", hipGetErrorString(e));
+  return GSQ_OK;
+}
+
+static AttnPagedArgs attn_paged_sizes(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                      int64_t max_pages, int64_t page_size, int64_t max_new, int64_t cus) {
+  AttnPagedArgs a = {};
+  a.N = (int)tokens; a.B = (int)sequences; a.H = (int)heads; a.Hkv = (int)kv_heads; a.hd = (int)head_dim; a.W = max_pages;
+  a.P = (int)page_size; a.max_new = (int)std::min(max_new, tokens); a.cus = (int)cus;
+  return a;
+}
+
+static int check_attn_paged(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                            int64_t max_pages, int64_t page_size, int64_t max_new, int64_t cus) {
+  if (int rc = check_sequences(sequences, 1, tokens)) return rc;
+  if (int rc = check_heads(tokens, heads, kv_heads, head_dim)) return rc;
+  if (int rc = check_pages(max_pages, 1, page_size)) return rc;
+  if (max_new < 0) return fail(GSQ_E_VALUE, "max_new must not be negative");
+  if (cus <= 0 || cus > 65535) return fail(GSQ_E_VALUE, "invalid number of CUs");
+  return GSQ_OK;
+}
+
+int64_t gsq_attn_paged_work(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                            int64_t max_pages, int64_t page_size, int64_t max_new, int64_t cus) {
+  if (check_attn_paged(tokens, sequences, heads, kv_heads, head_dim, max_pages, page_size, max_new, cus)) return -1;
+  return attn_paged_work(attn_paged_sizes(tokens, sequences, heads, kv_heads, head_dim, max_pages, page_size, max_new, cus));
+}
+
+int gsq_attn_paged(const void* q, const void* gate, int64_t gate_stride, int64_t gate_head_stride, const void* k_pages,
+                   const void* v_pages, const int32_t* table, const int32_t* cu, const int32_t* rows, const int32_t* lens,
+                   void* out, float* work, int64_t tokens, int64_t sequences, int64_t n_requests, int64_t max_pages,
+                   int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t n_pages, int64_t page_size, int64_t max_new,
+                   int64_t cus, int dtype, void* stream) {
+  if (dtype != GSQ_F16 && dtype != GSQ_BF16) return fail(GSQ_E_TYPE, "unsupported dtype code %d", dtype);
+  if (int rc = check_attn_paged(tokens, sequences, heads, kv_heads, head_dim, max_pages, page_size, max_new, cus)) return rc;
+  if (int rc = check_sequences(sequences, n_requests, tokens)) return rc;
+  if (int rc = check_pages(max_pages, n_pages, page_size)) return rc;
+  if (tokens == 0) return GSQ_OK;
+  if (!q || !k_pages || !v_pages || !table || !cu || (sequences && (!rows || !lens)) || !out)
+    return fail(GSQ_E_VALUE, "NULL pointer");
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages) |
+       reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(work)) & 15)
+    return fail(GSQ_E_VALUE, "q, k_pages, v_pages, out and work must be 16-byte aligned");
+  AttnPagedArgs a = attn_paged_sizes(tokens, sequences, heads, kv_heads, head_dim, max_pages, page_size, max_new, cus);
+  if (!work && attn_paged_work(a)) return fail(GSQ_E_VALUE, "work must not be NULL");
+  a.q = q; a.gate = gate; a.kp = k_pages; a.vp = v_pages; a.table = table; a.cu = cu; a.rows = rows; a.lens = lens;
+  a.out = out; a.part = work; a.gate_stride = gate_stride; a.gate_head = gate_head_stride; a.R = (int)n_requests;
+  a.n_pages = (int)n_pages;
+  hipError_t e = launch_attn_paged(dtype == GSQ_BF16, a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(GSQ_E_HIP, "attn_paged launch: %s", hipGetErrorString(e));
+  return GSQ_OK;
+}
+
+static int check_gdn_packed(int64_t tokens, int64_t sequences, int64_t key_heads, int64_t value_heads, int64_t head_k_dim,
+                            int64_t head_v_dim, int64_t conv_kernel, int64_t max_new) {
+  if (int rc = check_sequences(sequences, 1, tokens)) return rc;
+  if (key_heads <= 0 || value_heads <= 0 || value_heads % key_heads || value_heads > 4096)
+    return fail(GSQ_E_VALUE, "value heads must be a positive multiple of key heads (at most 4096)");
+  if (head_k_dim != 32 && head_k_dim != 64 && head_k_dim != 128) return fail(GSQ_E_VALUE, "key head dim must be 32, 64 or 128");
+  if (head_v_dim != 64 && head_v_dim != 128 && head_v_dim != 256) return fail(GSQ_E_VALUE, "value head dim must be 64, 128 or 256");
+  if (conv_kernel < 2 || conv_kernel > 8) return fail(GSQ_E_VALUE, "convolution kernel must be 2..8");
+  if (tokens > 65535 * 8) return fail(GSQ_E_VALUE, "at most 524280 tokens");
+  if (max_new < 0) return fail(GSQ_E_VALUE, "max_new must not be negative");
+  return GSQ_OK;
+}
+
+static GdnPackedArgs gdn_packed_sizes(int64_t tokens, int64_t sequences, int64_t key_heads, int64_t value_heads,
+                                      int64_t head_k_dim, int64_t head_v_dim, int64_t conv_kernel, int64_t max_new) {
+  GdnPackedArgs a = {};
+  a.N = (int)tokens; a.B = (int)sequences; a.Hk = (int)key_heads; a.Hv = (int)value_heads; a.dk = (int)head_k_dim;
+  a.dv = (int)head_v_dim; a.K = (int)conv_kernel; a.max_new = (int)std::min(max_new, tokens);
+  return a;
+}
+
+int64_t gsq_gdn_packed_work(int64_t tokens, int64_t sequences, int64_t key_heads, int64_t value_heads, int64_t head_k_dim,
+                            int64_t head_v_dim, int64_t conv_kernel, int64_t max_new) {
+  if (check_gdn_packed(tokens, sequences, key_heads, value_heads, head_k_dim, head_v_dim, conv_kernel, max_new)) return -1;
+  return gdn_packed_work(gdn_packed_sizes(tokens, sequences, key_heads, value_heads, head_k_dim, head_v_dim, conv_kernel, max_new));
+}
+
+int gsq_gdn_packed(const void* qkv, int64_t qkv_stride, const void* z, int64_t z_stride, const void* ab, int64_t ab_stride,
+                   void* conv_state, const void* conv_w, const float* ssm_a, const float* dt_bias, float* rec_state,
+                   const void* norm_w, const int32_t* cu, const int32_t* rows, const int32_t* lens, void* out,
+                   int64_t out_stride, float* work, int64_t tokens, int64_t sequences, int64_t n_requests, int64_t key_heads,
+                   int64_t value_heads, int64_t head_k_dim, int64_t head_v_dim, int64_t conv_kernel, float eps,
+                   int64_t max_new, int dtype, void* stream) {
+  if (dtype != GSQ_F16 && dtype != GSQ_BF16) return fail(GSQ_E_TYPE, "unsupported dtype code %d", dtype);
+  if (int rc = check_gdn_packed(tokens, sequences, key_heads, value_heads, head_k_dim, head_v_dim, conv_kernel, max_new)) return rc;
+  if (int rc = check_sequences(sequences, n_requests, tokens)) return rc;
+  if (!(eps >= 0.f)) return fail(GSQ_E_VALUE, "eps must be >= 0");
+  if (tokens == 0) return GSQ_OK;
+  if (!qkv || !z || !ab || !conv_state || !conv_w || !ssm_a || !dt_bias || !rec_state || !norm_w || !cu ||
+      (sequences && (!rows || !lens)) || !out || !work)
+    return fail(GSQ_E_VALUE, "NULL pointer");
+  if ((reinterpret_cast<uintptr_t>(rec_state) | reinterpret_cast<uintptr_t>(work)) & 15)
+    return fail(GSQ_E_VALUE, "rec_state and work must be 16-byte aligned");
+  GdnPackedArgs a = gdn_packed_sizes(tokens, sequences, key_heads, value_heads, head_k_dim, head_v_dim, conv_kernel, max_new);
+  a.qkv = qkv; a.z = z; a.ab = ab; a.conv = conv_state; a.conv_w = conv_w; a.ssm_a = ssm_a; a.dt_bias = dt_bias;
+  a.rec = rec_state; a.norm_w = norm_w; a.cu = cu; a.rows = rows; a.lens = lens; a.out = out; a.work = work;
+  a.qkv_stride = qkv_stride; a.z_stride = z_stride; a.ab_stride = ab_stride; a.out_stride = out_stride;
+  a.R = (int)n_requests; a.eps = eps;
+  hipError_t e = launch_gdn_packed(dtype == GSQ_BF16, a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(GSQ_E_HIP, "gdn_packed launch: %s", hipGetErrorString(e));
   return GSQ_OK;
 }
 

@@ -255,6 +255,90 @@ struct Kv8AttnArgs {
   int B, S, H, Hkv, hd, nsplit;
 };
 
+// Arguments of the operators on paged caches (kernels in gsq_paged.hip, gsq_gdn_packed.hip). A step packs the new
+// tokens of B sequences behind one another: sequence b's are tokens cu[b] .. cu[b + 1] - 1 of N, it belongs to request
+// rows[b] (none: not served) of R, and has lens[b] positions, the new ones among them. Position p of request r lies
+// in page table[r * W + p / P] at row p % P.
+struct PagePlanArgs {
+  const int32_t* requests;
+  const int32_t* fresh;    // new tokens of each sequence
+  const int32_t* lengths;  // [R]
+  int32_t* held;           // [R] pages of each request
+  int32_t* table;          // [R, W]
+  const int32_t* free;     // [n_pages], the first *n_free of them free ones
+  int32_t* n_free;
+  int32_t* cu;    // [B + 1]
+  int32_t* rows;  // [B]
+  int32_t* lens;  // [B]
+  int64_t* pos;   // [N]
+  int64_t* slots;  // [N]
+  int64_t W, N;
+  int B, R, n_pages, P;
+};
+
+struct PageReleaseArgs {
+  const int32_t* requests;
+  int32_t* lengths;
+  int32_t* held;
+  int32_t* table;
+  int32_t* free;
+  int32_t* n_free;
+  int64_t W;
+  int B, R, n_pages;
+};
+
+struct PagedWriteArgs {
+  const void* q;  // [N, H] rows of hd values, strides in elements
+  const void* k;  // [N, Hkv]
+  const void* v;
+  const void* q_norm_w;  // [hd]
+  const void* k_norm_w;
+  const double* inv_freq;  // [rd / 2]
+  void* kp;  // [n_pages, Hkv, P, hd]
+  void* vp;
+  const int64_t* pos;    // [N]
+  const int64_t* slots;  // [N]
+  void* out;             // [N, H, hd]: normalized, rotated queries
+  int64_t q_stride, q_head, k_stride, k_head, v_stride, v_head, n_slots;
+  int N, H, Hkv, hd, rd, P;
+  float eps;
+};
+
+struct AttnPagedArgs {
+  const void* q;     // [N, H, hd]
+  const void* gate;  // [N, H] rows of hd, or null
+  const void* kp;    // [n_pages, Hkv, P, hd]
+  const void* vp;
+  const int32_t* table;  // [R, W]
+  const int32_t* cu;
+  const int32_t* rows;
+  const int32_t* lens;
+  void* out;    // [N, H, hd]
+  float* part;  // partial outputs of split positions
+  int64_t gate_stride, gate_head, W;
+  int N, B, R, H, Hkv, hd, n_pages, P, max_new, cus;
+};
+
+struct GdnPackedArgs {
+  const void* qkv;  // rows of conv_dim values
+  const void* z;    // rows of Hv * dv
+  const void* ab;   // 2 Hv values per row: a, then b
+  void* conv;       // [R, K-1, conv_dim]
+  const void* conv_w;  // [conv_dim, K]
+  const float* ssm_a;
+  const float* dt_bias;
+  float* rec;  // [R, Hv, dk, dv]
+  const void* norm_w;
+  const int32_t* cu;
+  const int32_t* rows;
+  const int32_t* lens;
+  void* out;
+  float* work;
+  int64_t qkv_stride, z_stride, ab_stride, out_stride;
+  int N, B, R, Hk, Hv, dk, dv, K, max_new;
+  float eps;
+};
+
 // A kernel's raised dynamic LDS limit (one static object per kernel): a function attribute belongs to
 // one device, so it is set on each device's first launch, and again after a failure. Devices past
 // the first 64 are not remembered.

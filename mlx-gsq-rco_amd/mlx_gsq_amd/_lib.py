@@ -56,6 +56,14 @@ EXPORTS = {
     "gsq_attn_kv8_splits": (_I64, [_I64, _I64, _I64, _I64, _I64, _I64, _I64]),
     "gsq_attn_kv8": (_I32, [_VP, _I64, _VP, _I64, _VP, _VP, _VP, _VP, _VP, _I64, _VP, _I64, _VP, _I64, _VP, _I64, _I64,
                             _I64, _I64, _I64, _I64, _I64, _I32, _VP]),
+    "gsq_page_plan": (_I32, [_VP] * 7 + [_I64] * 6 + [_VP] * 6),
+    "gsq_page_advance": (_I32, [_VP] * 3 + [_I64] * 2 + [_VP]),
+    "gsq_page_release": (_I32, [_VP] * 6 + [_I64] * 4 + [_VP]),
+    "gsq_paged_write": (_I32, [_VP, _I64, _I64] * 3 + [_VP] * 8 + [_I64] * 7 + [_F32, _I32, _VP]),
+    "gsq_attn_paged_work": (_I64, [_I64] * 9),
+    "gsq_attn_paged": (_I32, [_VP, _VP, _I64, _I64] + [_VP] * 8 + [_I64] * 11 + [_I32, _VP]),
+    "gsq_gdn_packed_work": (_I64, [_I64] * 8),
+    "gsq_gdn_packed": (_I32, [_VP, _I64] * 3 + [_VP] * 10 + [_I64, _VP] + [_I64] * 8 + [_F32, _I64, _I32, _VP]),
     "gsq_last_error": (ctypes.c_char_p, []),
 }
 
