@@ -1,7 +1,20 @@
 // Attention of packed sequences over a paged K/V cache: single tokens, chunks of prompts and whole prompts in one call
 // (the reference runs mlx-lm's attention over one sequence, mlx_gsq/models/qwen35.py:114-152).
+//
+// The rows of a (sequence, KV head) are its rep = heads / kv_heads query heads of every new token, row t rep + r for
+// head r of token t. Two kernels share the arithmetic: attn_paged_rows_kernel for few rows, whose waves share a tile of
+// 16 rows and take its positions in turn, attn_paged_tile_kernel for many, whose waves share tiles of K and V in LDS.
+// Both products run on the 16-bit matrix cores, transposed: S^T = K Q^T puts a row on each lane column, lane % 16, and
+// positions 16 b + 4 (lane / 16) + e of a block of 32 on its registers, which is the layout of the B operand of
+// O^T = V^T P^T: weights never leave their lane.
+//
+// What a workgroup does follows from the lengths on the device (PagedTask): no host knows them, and a captured call
+// follows them. Positions are split over workgroups so that the step's work fills the device, in pieces of one length
+// for all its sequences; what pieces of one row leave meets in attn_paged_merge_kernel.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+#include <cfloat>
 #include <cstdint>
 #include <type_traits>
 
@@ -11,80 +24,787 @@
 
 namespace gsq {
 
-// A wave per (token, head): one pass over the positions the token sees, the running maximum and sum of the softmax and
-// the output in registers.
-template <bool BF, int HD>
-__global__ void __launch_bounds__(256) attn_paged_wave_kernel(AttnPagedArgs a) {
-  using E = Half<BF>;
-  constexpr int V = HD / 64;
-  const int lane = threadIdx.x & 63, d = V * lane;
-  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (i >= (int64_t)a.N * a.H) return;
-  const int t = (int)(i / a.H), h = (int)(i % a.H), b = seq_of(a.cu, a.B, t), kvh = h / (a.H / a.Hkv);
-  uint16_t* const out = static_cast<uint16_t*>(a.out) + i * HD + d;
-  float o[V], q[V];
-#pragma unroll
-  for (int j = 0; j < V; ++j) o[j] = 0.f;
-  if (b >= a.B) {  // behind the last sequence
-#pragma unroll
-    for (int j = 0; j < V; ++j) out[j] = 0;
-    return;
+// Which sequences a launch serves: all, or those of few or of many rows.
+enum { kAll = 0, kFew = 1, kMany = 2 };
+
+struct PagedSched {
+  int rt;         // rows of a workgroup
+  int which;      // kAll, kFew or kMany
+  int target;     // workgroups that fill the device
+  int least;      // fewest blocks of 32 positions to a piece
+  int64_t parts;  // pieces whose partial outputs `part` holds
+};
+
+namespace {
+
+// Transposing LDS read: 16 lanes read 4 rows of 16 values (lane j: values 4 (j % 4) .. + 3 of row
+// j / 4, 8 bytes); lane j gets column j of the four rows.
+__device__ __forceinline__ s16x4 tr_read(const uint8_t* p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+}
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+constexpr int kRowsTile = 16;   // rows of a workgroup of attn_paged_rows_kernel
+constexpr int kTileRows = 128;  // of attn_paged_tile_kernel
+constexpr int kFewRows = 32;    // rows up to which a sequence takes the first
+
+// Lane's view of a sequence.
+struct SeqLane {
+  int n, tiles, blocks;
+  __device__ SeqLane(const AttnPagedArgs& a, const PagedSched& p, int b) {
+    n = tiles = blocks = 0;
+    if (b >= a.B) return;
+    const int t0 = min(max(a.cu[b], 0), a.N), t1 = min(max(a.cu[b + 1], t0), a.N), rep = a.H / a.Hkv;
+    const PackedSeq s(a.cu, a.rows, a.lens, b, a.N, a.R, a.W * a.P);
+    n = t1 - t0;
+    const bool few = (int64_t)n * rep <= kFewRows;
+    if (p.which != kAll && few != (p.which == kFew)) n = 0;
+    tiles = (n * rep + p.rt - 1) / p.rt;
+    blocks = s.fine ? (s.len + 31) / 32 : 1;  // one that is not served: its rows are NaN, in one piece
   }
-  const PackedSeq sq(a.cu, a.rows, a.lens, b, a.N, a.R, a.W * a.P);
-  bool bad = !sq.fine || t < sq.t0 || t - sq.t0 >= sq.n;
-  float m = -INFINITY, l = 0.f;
-  if (!bad) {
-    const int last = sq.len - sq.n + (t - sq.t0);
+  __device__ int splits(int chunk) const { return (blocks + chunk - 1) / chunk; }
+};
+
+template <typename T>
+__device__ __forceinline__ T wave_scan(T v) {  // inclusive
+  const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int j = 0; j < V; ++j) q[j] = E::ld(static_cast<const uint16_t*>(a.q)[i * HD + d + j]);
-    const float scale = 1.44269504088896340736f / sqrtf((float)HD);
-    for (int p = 0; p <= last; ++p) {
-      const int page = a.table[sq.row * a.W + p / a.P];
-      if (page < 0 || page >= a.n_pages) {
-        bad = true;
-        break;
+  for (int o = 1; o < 64; o <<= 1) {
+    const T u = __shfl_up(v, o, 64);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+
+// Blocks to a piece: the step's work (tiles of rows times blocks) over as many workgroups as fill the device.
+__device__ __forceinline__ int chunk_of(const AttnPagedArgs& a, const PagedSched& p) {
+  int64_t total = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const SeqLane s(a, p, b0 + (threadIdx.x & 63));
+    total += (int64_t)s.tiles * s.blocks;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
+  return max(p.least, (int)min((total * a.Hkv + p.target - 1) / p.target, (int64_t)(1 << 26)));
+}
+
+// What workgroup `item` of a launch is asked to do: rows r0 .. of sequence b and KV head kvh, positions of piece z of nz.
+// Called by whole waves.
+struct PagedTask {
+  int b = -1, kvh, z, nz, r0, rows, t0, len, pos, row;  // pos: position of the sequence's first new token
+  int64_t part;  // its piece among those that leave partial outputs
+  bool fine;
+  __device__ PagedTask(const AttnPagedArgs& a, const PagedSched& p, int item) {
+    const int chunk = chunk_of(a, p), lane = threadIdx.x & 63;
+    int64_t before = 0, split_before = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+      const SeqLane s(a, p, b0 + lane);
+      const int mine = s.tiles * a.Hkv * s.splits(chunk);
+      const int upto = wave_scan(mine), split = wave_scan(s.splits(chunk) > 1 ? mine : 0);
+      const int k = __popcll(__ballot(before + upto <= item));
+      if (k < 64 && b0 + k < a.B) {
+        b = b0 + k;
+        const int inside = item - (int)before - (k ? __shfl(upto, k - 1, 64) : 0);
+        nz = __shfl(s.splits(chunk), k, 64);
+        rows = __shfl(s.n, k, 64) * (a.H / a.Hkv);
+        part = split_before + (k ? __shfl(split, k - 1, 64) : 0) + inside;
+        const int tiles = __shfl(s.tiles, k, 64);
+        kvh = inside % a.Hkv;  // neighbours: other KV heads, then other pieces of the same rows
+        const int rest = inside / a.Hkv;
+        z = rest % nz;
+        r0 = (tiles - 1 - rest / nz) * p.rt;  // the last rows see most: first
+        const PackedSeq q(a.cu, a.rows, a.lens, b, a.N, a.R, a.W * a.P);
+        t0 = min(max(q.t0, 0), a.N);
+        len = q.len;
+        pos = q.len - q.n;
+        row = q.row;
+        fine = q.fine && (nz == 1 || part < p.parts);
+        return;
       }
-      const int64_t at = (((int64_t)page * a.Hkv + kvh) * a.P + p % a.P) * HD + d;
-      float s = 0.f, v[V];
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        s += q[j] * E::ld(static_cast<const uint16_t*>(a.kp)[at + j]);
-        v[j] = E::ld(static_cast<const uint16_t*>(a.vp)[at + j]);
-      }
-      s = wave_sum(s) * scale;
-      const float mn = fmaxf(m, s), keep = m == mn ? 1.f : exp2_raw(m - mn), w = exp2_raw(s - mn);
-      m = mn;
-      l = l * keep + w;
-#pragma unroll
-      for (int j = 0; j < V; ++j) o[j] = o[j] * keep + w * v[j];
+      before += __shfl(upto, 63, 64);
+      split_before += __shfl(split, 63, 64);
     }
   }
+  __device__ int rep(const AttnPagedArgs& a) const { return a.H / a.Hkv; }
+  // (token, head) of row r in q, gate and out, as one index
+  __device__ int64_t at(const AttnPagedArgs& a, int r) const {
+    const int rp = rep(a), t = r / rp;
+    return (int64_t)(t0 + t) * a.H + kvh * rp + (r - t * rp);
+  }
+  // blocks of the piece for a tile whose last token is tlast
+  __device__ void blocks(int tlast, int& blk0, int& blk1) const {
+    const int all = (pos + tlast) / 32 + 1, per = (all + nz - 1) / nz;
+    blk0 = min(z * per, all);
+    blk1 = min(blk0 + per, all);
+  }
+};
+
+// Output d .. d + M - 1 (M 4 or 8) of (token, head) i: rounded once, after the gate.
+template <bool BF, int M>
+__device__ __forceinline__ void put(const AttnPagedArgs& a, int64_t i, int d, const float* v) {
+  using E = Half<BF>;
+  float o[M];
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    float g = 1.f;
-    if (a.gate) g = sigmoid_raw(E::ld(static_cast<const uint16_t*>(a.gate)[(int64_t)t * a.gate_stride + h * a.gate_head + d + j]));
-    out[j] = E::mk(bad ? __builtin_nanf("") : o[j] / l * g);
+  for (int e = 0; e < M; ++e) o[e] = v[e];
+  if (a.gate) {
+    const int64_t t = i / a.H;
+    const uint16_t* const g = static_cast<const uint16_t*>(a.gate) + t * a.gate_stride + (i - t * a.H) * a.gate_head + d;
+#pragma unroll
+    for (int e = 0; e < M; ++e) o[e] *= sigmoid_raw(E::ld(g[e]));
+  }
+  uint32_t w[M / 2];
+#pragma unroll
+  for (int e = 0; e < M / 2; ++e) w[e] = E::pack((f32x2){o[2 * e], o[2 * e + 1]});
+  uint16_t* const out = static_cast<uint16_t*>(a.out);
+  if constexpr (M == 8) *reinterpret_cast<u32x4*>(out + i * a.hd + d) = (u32x4){w[0], w[1], w[2], w[3]};
+  else *reinterpret_cast<uint2*>(out + i * a.hd + d) = make_uint2(w[0], w[1]);
+}
+
+// Zeros in the rows behind the last sequence, shared out over the launch.
+__device__ __forceinline__ void clear_tail(const AttnPagedArgs& a) {
+  const int from = a.B ? max(a.cu[a.B], 0) : 0;
+  const int64_t n8 = (int64_t)(a.N - min(from, a.N)) * a.H * (a.hd / 8);
+  u32x4* const p = reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.out) + (int64_t)from * a.H * a.hd);
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n8; i += (int64_t)gridDim.x * blockDim.x) p[i] = (u32x4){0, 0, 0, 0};
+}
+
+// The softmax and the sums of a wave's 16 NT rows over the positions it has seen. Weights are powers of two over a
+// reference m that moves only when a score passes it by 2^kLazy, for all rows of the wave at once: mostly no rescaling
+// and no exchange between lanes in the loop. They are held in two 16-bit values, cut off and the rest: fp16 times
+// 2^kScale (22 bits; 2^15 at most), bf16 16 bits (2^-17 of a weight; with one value of 8 bits outputs would be off by 1.4
+// times their rounding), small enough that sums of V rows next to float32's largest number stay finite.
+constexpr float kLazy = 6.f;
+
+template <bool BF, int HD, int NT>
+struct PagedRows {
+  using E = Half<BF>;
+  static constexpr int VB = HD / 16;
+  static constexpr float kScale = BF ? -24.f : 9.f;  // log2
+  float m[NT], l[NT];  // l: this lane's share of the sum
+  f32x4 acc[NT][VB];
+
+  __device__ void init() {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      m[n] = -INFINITY;
+      l[n] = 0.f;
+#pragma unroll
+      for (int i = 0; i < VB; ++i) acc[n][i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    }
+  }
+  // scores s of 16 NB positions to weights pf (and, in s, as float32); last[n]: the last position that the lane's row
+  // n sees, as an offset from the first of these
+  template <int NB>
+  __device__ void weights(f32x4 (&s)[NT][NB], bool masked, const int (&last)[NT], u32x4 (&pf)[NB / 2][2][NT]) {
+    const int g = (threadIdx.x & 63) >> 4;
+    const float c = 1.44269504088896340736f / sqrtf((float)HD);
+    float mx[NT];
+    bool far = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      if (masked) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (16 * b + 4 * g + e > last[n]) s[n][b][e] = -INFINITY;
+      }
+      mx[n] = s[n][0][0];
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx[n] = fmaxf(mx[n], s[n][b][e]);
+      far |= (mx[n] - m[n]) * c > kLazy;  // not for -inf - -inf
+    }
+    if (__any(far)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float x = fmaxf(mx[n], __shfl_xor(mx[n], 16, 64));
+        x = fmaxf(x, __shfl_xor(x, 32, 64));
+        x = fmaxf(x, m[n]);
+        const float alpha = m[n] == x ? 1.f : exp2_raw((m[n] - x) * c);
+        m[n] = x;
+        l[n] *= alpha;
+#pragma unroll
+        for (int i = 0; i < VB; ++i) acc[n][i] *= alpha;
+      }
+    }
+    // a rest of 0 times a visible V of infinity would be NaN, where its weight is not 0 and the sum is infinite
+    const uint16_t one = masked ? 0 : E::kLeast;
+    const u16x2 least = {one, one};
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const float off = kScale - (m[n] == -INFINITY ? 0.f : m[n]) * c;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[n][b][e] = exp2_raw(__builtin_fmaf(s[n][b][e], c, off));
+          l[n] += s[n][b][e];
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const f32x2 p = j ? s[n][b].zw : s[n][b].xy;
+          const uint32_t hi = E::chop(p);
+          pf[b / 2][0][n][2 * (b & 1) + j] = hi;
+          pf[b / 2][1][n][2 * (b & 1) + j] =
+              __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, E::pack(p - E::unpack(hi))), least));
+        }
+      }
+    }
+  }
+  // output tile i += V's operand times the weights
+  __device__ void add(int i, u32x4 vf, const u32x4 (&pf)[2][NT]) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) acc[n][i] = E::mma(vf, pf[t][n], acc[n][i]);
+  }
+  __device__ float sum(int n) const {  // over the lanes of a row
+    const float x = l[n] + __shfl_xor(l[n], 16, 64);
+    return x + __shfl_xor(x, 32, 64);
+  }
+  // reference of a row in powers of two
+  __device__ float top(int n) const { return m[n] == -INFINITY ? -FLT_MAX : m[n] * (1.44269504088896340736f / sqrtf((float)HD)); }
+};
+
+// V rows that some of a tile's rows do not see would reach those as 0 x NaN if they are not finite. Blocks with such
+// positions are looked at: values that are not finite are taken out of the product, and put into the outputs that see them
+// when the sums are done (put_odd).
+template <bool BF>
+__device__ __forceinline__ bool odd_pair(uint32_t w) {  // whether a pair of values holds one that is not finite
+  const uint32_t e = BF ? 0x7F80u : 0x7C00u;
+  return (w & e) == e || ((w >> 16) & e) == e;
+}
+template <bool BF>
+__device__ __forceinline__ uint32_t clean_pair(uint32_t w) {
+  const uint32_t e = BF ? 0x7F80u : 0x7C00u;
+  if ((w & e) == e) w &= 0xFFFF0000u;
+  if (((w >> 16) & e) == e) w &= 0x0000FFFFu;
+  return w;
+}
+// output x of dim d and a row that sees positions up to last: with the values of V at positions j0 .. j1 that were taken out
+template <bool BF, int HD>
+__device__ __forceinline__ float put_odd(const AttnPagedArgs& a, const int32_t* table, int kvh, int d, int j0, int j1, int last, float x) {
+#pragma unroll 1
+  for (int j = j0; j <= min(j1, last); ++j) {
+    const int page = table[j / a.P];
+    if (page < 0 || page >= a.n_pages) continue;
+    const float v = Half<BF>::ld(static_cast<const uint16_t*>(a.vp)[(((int64_t)page * a.Hkv + kvh) * a.P + j % a.P) * HD + d]);
+    if (!(fabsf(v) <= FLT_MAX)) x += v;
+  }
+  return x;
+}
+
+// NaN in the task's rows (of rt), by the whole workgroup
+template <bool BF>
+__device__ __forceinline__ void nan_rows(const AttnPagedArgs& a, const PagedTask& k, int rt) {
+  const float v[8] = {NAN, NAN, NAN, NAN, NAN, NAN, NAN, NAN};
+  for (int i = threadIdx.x; i < rt * (a.hd / 8); i += blockDim.x)
+    if (k.r0 + i / (a.hd / 8) < k.rows) put<BF, 8>(a, k.at(a, k.r0 + i / (a.hd / 8)), 8 * (i % (a.hd / 8)), v);
+}
+
+}  // namespace
+
+// Few rows (16 a workgroup): the cache goes by once, and its bytes bound the kernel. Four waves take the
+// blocks in turn, each with a softmax of its own; K and V go from memory to registers in 16-byte pieces, a block
+// ahead: no LDS and no barrier in the loop. K's lanes read 8 dims of one position, V's PW neighbouring dims of eight
+// positions, each dim of another output tile, so that two rows give a pair of a tile's operand by one permute. The
+// waves are merged at the end.
+template <bool BF, int HD>
+__global__ void __launch_bounds__(256, 2) attn_paged_rows_kernel(AttnPagedArgs a, PagedSched p) {
+  using E = Half<BF>;
+  constexpr int KS = HD / 32, VB = HD / 16, PW = VB < 8 ? VB : 8, NP = VB / PW;
+  typedef uint32_t vpiece __attribute__((ext_vector_type(PW / 2)));
+  constexpr int OS = HD + 4;
+  __shared__ __attribute__((aligned(16))) float mo[4 * 16 * OS];
+  __shared__ float2 ml[4 * 16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), g = lane >> 4, c = lane & 15;
+  clear_tail(a);
+  const PagedTask k(a, p, blockIdx.x);
+  if (k.b < 0) return;
+  if (!k.fine) {
+    if (k.nz == 1) nan_rows<BF>(a, k, kRowsTile);
+    return;
+  }
+  const int rep = k.rep(a), tfirst = k.r0 / rep, tlast = min(k.r0 + 15, k.rows - 1) / rep;
+  int blk0, blk1;
+  k.blocks(tlast, blk0, blk1);
+  if (blk0 >= blk1) return;  // the merge knows
+  const int klast = k.pos + tlast;  // last position any row sees; later ones of a block repeat it
+  const int32_t* const table = a.table + (int64_t)k.row * a.W;
+  const int64_t page_size = (int64_t)a.Hkv * a.P * HD, head = (int64_t)k.kvh * a.P * HD;
+  bool bad = false;
+  // first value of positions 16 j .. + 15 of K or V: they lie in one page
+  auto group_at = [&](int j) {
+    const int first = min(16 * j, klast), page = uniform(table[first / a.P]);
+    const bool out = page < 0 || page >= a.n_pages;
+    bad |= out;
+    return (out ? 0 : (int64_t)page * page_size) + head + (int64_t)(first % a.P & ~15) * HD;
+  };
+  u32x4 kr[2][KS];
+  vpiece vr[8][NP];
+  int64_t at[2];
+  auto load_k = [&](int blk) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int left = max(klast - 32 * blk - 16 * b, 0);
+      const uint16_t* const src = static_cast<const uint16_t*>(a.kp) + at[b] + 8 * g;
+      const int r = left < 15 ? min(c, left & 15) : c;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) kr[b][s] = *reinterpret_cast<const u32x4*>(src + r * HD + 32 * s);
+    }
+  };
+  auto load_v = [&](int blk) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int left = max(klast - 32 * blk - 16 * (i >> 2), 0), r = min(4 * g + (i & 3), left);
+      const uint16_t* const src = static_cast<const uint16_t*>(a.vp) + at[i >> 2] + r * HD + PW * c;
+#pragma unroll
+      for (int h = 0; h < NP; ++h) vr[i][h] = *reinterpret_cast<const vpiece*>(src + (HD / NP) * h);
+    }
+  };
+  // a group that lies behind the last position repeats the group that holds it
+  auto locate = [&](int blk) {
+    at[0] = group_at(2 * blk);
+    at[1] = group_at(2 * blk + 1);
+  };
+  int blk = blk0 + wave;
+  if (blk < blk1) {
+    locate(blk);
+    load_k(blk);
+  }
+  u32x4 qf[KS];
+  {
+    const uint16_t* const q = static_cast<const uint16_t*>(a.q) + k.at(a, min(k.r0 + c, k.rows - 1)) * HD + 8 * g;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const u32x4*>(q + 32 * s);
+  }
+  if (blk < blk1) load_v(blk);
+  const int qpos = k.pos + min(k.r0 + c, k.rows - 1) / rep;
+  PagedRows<BF, HD, 1> rows;
+  rows.init();
+  bool any_odd = false;
+  for (; blk < blk1; blk += 4) {
+    const bool more = blk + 4 < blk1;
+    f32x4 s[1][2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      s[0][b] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int st = 0; st < KS; ++st) s[0][b] = E::mma(kr[b][st], qf[st], s[0][b]);
+    }
+    if (more) {
+      locate(blk + 4);
+      load_k(blk + 4);
+    }
+    const int last[1] = {qpos - 32 * blk};
+    const bool masked = 32 * blk + 31 > k.pos + tfirst;
+    u32x4 pf[1][2][1];
+    rows.weights(s, masked, last, pf);
+    bool odd = false;
+    if (masked && tfirst != tlast) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int h = 0; h < NP; ++h)
+#pragma unroll
+          for (int w = 0; w < PW / 2; ++w) odd |= odd_pair<BF>(vr[i][h][w]);
+    }
+    if (__any(odd)) {
+      any_odd = true;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int h = 0; h < NP; ++h)
+#pragma unroll
+          for (int w = 0; w < PW / 2; ++w) vr[i][h][w] = clean_pair<BF>(vr[i][h][w]);
+    }
+#pragma unroll
+    for (int h = 0; h < NP; ++h)
+#pragma unroll
+      for (int i = 0; i < PW; ++i) {  // dim (HD / NP) h + PW c + i of the 8 positions
+        u32x4 vf;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          vf[j] = __builtin_amdgcn_perm(vr[2 * j + 1][h][i >> 1], vr[2 * j][h][i >> 1], i & 1 ? 0x07060302u : 0x05040100u);
+        rows.add(PW * h + i, vf, pf[0]);
+      }
+    if (more) load_v(blk + 4);
+  }
+  // merge of the waves: every wave's reference, sum and outputs over its own sum
+  const float ls = bad ? NAN : rows.sum(0), over = ls == 0.f ? 0.f : 1.f / ls;
+  float* const mine = mo + (wave * 16 + c) * OS;
+#pragma unroll
+  for (int h = 0; h < NP; ++h)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int i = 0; i < PW; i += 4)
+        *reinterpret_cast<f32x4*>(mine + (HD / NP) * h + PW * (4 * g + e) + i) =
+            (f32x4){rows.acc[0][PW * h + i][e], rows.acc[0][PW * h + i + 1][e], rows.acc[0][PW * h + i + 2][e],
+                    rows.acc[0][PW * h + i + 3][e]} * over;
+  if (g == 0) ml[wave * 16 + c] = make_float2(rows.top(0), ls);
+  if (any_odd) {  // the wave's blocks that were looked at
+    for (int x = blk0 + wave; x < blk1; x += 4)
+      if (32 * x + 31 > k.pos + tfirst)
+        for (int d = g; d < HD; d += 4) mine[d] = put_odd<BF, HD>(a, table, k.kvh, d, 32 * x, min(32 * x + 31, klast), qpos, mine[d]);
+  }
+  __syncthreads();
+  for (int i = tid; i < 16 * HD / 8; i += 256) {
+    const int rr = i / (HD / 8), d = 8 * (i % (HD / 8)), r = k.r0 + rr;
+    if (r >= k.rows) continue;
+    float mm = -FLT_MAX, ll = 0.f, f[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, ml[w * 16 + rr].x);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float2 x = ml[w * 16 + rr];
+      f[w] = x.y == 0.f ? 0.f : x.y * exp2_raw(x.x - mm);
+      ll += f[w];
+    }
+    const float inv = ll == 0.f && k.nz > 1 ? 0.f : 1.f / ll;  // no weight at all: NaN, unless another piece has one
+    f32x4 o[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) o[j] += *reinterpret_cast<const f32x4*>(mo + (w * 16 + rr) * OS + d + 4 * j) * (f[w] * inv);
+    if (k.nz > 1) {
+      float* const to = a.part + (k.part * kRowsTile + rr) * (HD + 2);
+      // rows of HD + 2 floats: pairs are aligned
+#pragma unroll
+      for (int j = 0; j < 4; ++j) *reinterpret_cast<float2*>(to + d + 2 * j) = make_float2(o[j >> 1][2 * (j & 1)], o[j >> 1][2 * (j & 1) + 1]);
+      if (d == 0) *reinterpret_cast<float2*>(to + HD) = make_float2(mm, ll);
+    } else {
+      const float v[8] = {o[0][0], o[0][1], o[0][2], o[0][3], o[1][0], o[1][1], o[1][2], o[1][3]};
+      put<BF, 8>(a, k.at(a, r), d, v);
+    }
   }
 }
 
-template <bool BF>
-static hipError_t launch_attn_paged_t(const AttnPagedArgs& a, hipStream_t s) {
-  const dim3 grid((unsigned)(((int64_t)a.N * a.H + 3) / 4));
-  auto launch = [&](auto hd) {
-    constexpr int HD = decltype(hd)::value;
-    hipLaunchKernelGGL((attn_paged_wave_kernel<BF, HD>), grid, dim3(256), 0, s, a);
-    return hipGetLastError();
+// Many rows: 32 a wave, four waves to a workgroup, over tiles of KT positions that come to LDS by DMA, a tile ahead (two
+// buffers, one barrier a tile). K's operand is read as it lies, V's by transposing reads (four positions x 16
+// dims per 16 lanes); 16-byte pieces of a row are XOR-swizzled by position so that reads are free of bank conflicts.
+constexpr int tile_keys(int hd) { return hd == 256 ? 32 : 64; }
+constexpr int tile_lds(int hd) { return 2 * 2 * tile_keys(hd) * hd * 2; }
+
+template <bool BF, int HD>
+__global__ void __launch_bounds__(256, 2) attn_paged_tile_kernel(AttnPagedArgs a, PagedSched p) {
+  using E = Half<BF>;
+  constexpr int NT = 2, KS = HD / 32, VB = HD / 16, KT = tile_keys(HD), NB = 2, RB = 2 * HD, NO = HD / 8;  // RB: bytes of a row
+  constexpr int TB = KT * RB, NI = KT * NO / 256;  // bytes of a tile; DMA instructions of a wave for one
+  constexpr int SH = HD == 64 ? 1 : 0;             // 128-byte rows: two rows to the 64 banks
+  extern __shared__ __attribute__((aligned(16))) uint8_t paged_lds[];
+  __shared__ int bad_s[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), g = lane >> 4, c = lane & 15;
+  clear_tail(a);
+  const PagedTask k(a, p, blockIdx.x);
+  if (k.b < 0) return;
+  if (!k.fine) {
+    if (k.nz == 1) nan_rows<BF>(a, k, kTileRows);
+    return;
+  }
+  const int rep = k.rep(a), tlast = min(k.r0 + kTileRows - 1, k.rows - 1) / rep;
+  int blk0, blk1;
+  k.blocks(tlast, blk0, blk1);
+  if (blk0 >= blk1) return;  // the merge knows
+  const int klast = k.pos + tlast;
+  const int32_t* const table = a.table + (int64_t)k.row * a.W;
+  const int64_t page_size = (int64_t)a.Hkv * a.P * HD, head = (int64_t)k.kvh * a.P * HD;
+  auto ksw = [](int key) { return (key >> SH) & (NO < 16 ? NO - 1 : 15); };
+  auto vsw = [](int key) { return ((key >> SH) & (NO < 16 ? NO / 2 - 1 : 7)) << 1; };
+  constexpr int WR = KT / 4;  // positions that a wave brings: they lie in one page
+  int bad = 0;
+  auto page_of = [&](int j0) { return table[min(j0 + WR * wave, klast) / a.P]; };
+  auto issue = [&](int j0, int page, uint8_t* buf) {  // positions past the last repeat it
+    page = uniform(page);
+    const bool out = page < 0 || page >= a.n_pages;
+    bad |= out;
+    const int first = min(j0 + WR * wave, klast), left = klast - first, off = first % a.P;
+    const int64_t base = (out ? 0 : (int64_t)page * page_size) + head + (int64_t)off * HD;
+    const uint16_t* const kp = static_cast<const uint16_t*>(a.kp) + base;
+    const uint16_t* const vp = static_cast<const uint16_t*>(a.vp) + base;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int e = i * 64 + lane, r = e / NO, key = WR * wave + r, ko = (e % NO) ^ ksw(key), vo = (e % NO) ^ vsw(key);
+      uint8_t* const dst = buf + wave * WR * RB + i * 1024;
+      __builtin_amdgcn_global_load_lds(kp + min(r, left) * HD + 8 * ko, (lds_ptr_t)dst, 16, 0, 0);
+      __builtin_amdgcn_global_load_lds(vp + min(r, left) * HD + 8 * vo, (lds_ptr_t)(dst + TB), 16, 0, 0);
+    }
   };
-  if (a.hd == 256) return launch(std::integral_constant<int, 256>{});
-  if (a.hd == 128) return launch(std::integral_constant<int, 128>{});
-  if (a.hd == 64) return launch(std::integral_constant<int, 64>{});
-  return hipErrorInvalidValue;
+  const int j_end = 32 * blk1;
+  int j0 = 32 * blk0;
+  issue(j0, page_of(j0), paged_lds);
+  int next_page = page_of(j0 + KT);
+  const int rw = k.r0 + 32 * wave;
+  const bool on = rw < k.rows;
+  u32x4 qf[NT][KS];
+  int qpos[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int r = min(rw + 16 * n + c, k.rows - 1);
+    const uint16_t* const q = static_cast<const uint16_t*>(a.q) + k.at(a, r) * HD + 8 * g;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qf[n][s] = *reinterpret_cast<const u32x4*>(q + 32 * s);
+    qpos[n] = k.pos + r / rep;
+  }
+  const int pfirst = k.pos + min(rw, k.rows - 1) / rep, plast = k.pos + min(rw + 31, k.rows - 1) / rep;
+  PagedRows<BF, HD, NT> rows;
+  rows.init();
+  bool any_odd = false;
+  const int kx = ksw(c), vkey = 4 * g + (c >> 2), vx = vsw(vkey);
+  const int vlane = vkey * RB + (((c & 3) >> 1) << 4) + ((c & 1) << 3);
+  int cur = 0;
+  for (; j0 < j_end; j0 += KT, cur ^= 1) {
+    // the tile has landed; every wave is done with the other buffer
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (j0 + KT < j_end) {
+      issue(j0 + KT, next_page, paged_lds + (cur ^ 1) * 2 * TB);
+      next_page = page_of(j0 + 2 * KT);
+    }
+    const uint8_t* const kt = paged_lds + cur * 2 * TB;
+#pragma unroll 1
+    for (int sb = 0; sb < KT; sb += 32) {
+      const int js = j0 + sb;
+      if (!on || js > plast || js >= j_end) continue;
+      f32x4 s[NT][NB];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) s[n][b] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      const uint8_t* const kb = kt + (sb + c) * RB;
+#pragma unroll
+      for (int st = 0; st < KS; ++st)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          const u32x4 kf = *reinterpret_cast<const u32x4*>(kb + 16 * b * RB + (((4 * st + g) ^ kx) << 4));
+#pragma unroll
+          for (int n = 0; n < NT; ++n) s[n][b] = E::mma(kf, qf[n][st], s[n][b]);
+        }
+      int last[NT];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) last[n] = qpos[n] - js;
+      const bool masked = js + 31 > pfirst;
+      u32x4 pf[1][2][NT];
+      rows.weights(s, masked, last, pf);
+      const uint8_t* const vb = kt + TB + sb * RB;
+      bool odd = false;
+      if (masked) {
+        for (int i = lane; i < 32 * RB / 16; i += 64) {
+          const u32x4 w = *reinterpret_cast<const u32x4*>(vb + 16 * i);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) odd |= odd_pair<BF>(w[e]);
+        }
+      }
+      auto operand = [&](int i) {
+        const uint8_t* const va = vb + vlane + (((2 * i) ^ vx) << 4);
+        const s16x4 lo = tr_read(va), hi = tr_read(va + 16 * RB);
+        return __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+      };
+      if (__any(odd)) {
+        any_odd = true;
+#pragma unroll
+        for (int i = 0; i < VB; ++i) {
+          u32x4 vf = operand(i);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) vf[e] = clean_pair<BF>(vf[e]);
+          rows.add(i, vf, pf[0]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < VB; ++i) rows.add(i, operand(i), pf[0]);
+      }
+    }
+  }
+  if (lane == 0) bad_s[wave] = bad;
+  __syncthreads();
+  bad = bad_s[0] | bad_s[1] | bad_s[2] | bad_s[3];
+  // a lane's outputs: row rw + 16 n + c, dims 16 i + 4 g + e
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int r = rw + 16 * n + c;
+    const float ls = bad ? NAN : rows.sum(n), over = ls == 0.f && k.nz > 1 ? 0.f : 1.f / ls;
+    if (r >= k.rows) continue;
+    float* const to = a.part + (k.part * kTileRows + (r - k.r0)) * (HD + 2);
+    const int64_t i0 = k.at(a, r);
+    if (k.nz > 1 && g == 0) *reinterpret_cast<float2*>(to + HD) = make_float2(rows.top(n), ls);
+#pragma unroll
+    for (int i = 0; i < VB; ++i) {
+      float v[4] = {rows.acc[n][i][0] * over, rows.acc[n][i][1] * over, rows.acc[n][i][2] * over, rows.acc[n][i][3] * over};
+      if (any_odd) {  // the piece's positions in blocks that were looked at
+        const int from = max(32 * blk0, (pfirst + 1) / 32 * 32);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          v[e] = put_odd<BF, HD>(a, table, k.kvh, 16 * i + 4 * g + e, from, min(j_end - 1, plast), qpos[n], v[e]);
+      }
+      if (k.nz > 1) {
+        *reinterpret_cast<float2*>(to + 16 * i + 4 * g) = make_float2(v[0], v[1]);
+        *reinterpret_cast<float2*>(to + 16 * i + 4 * g + 2) = make_float2(v[2], v[3]);
+      } else {
+        put<BF, 4>(a, i0, 16 * i + 4 * g, v);
+      }
+    }
+  }
 }
 
-int64_t attn_paged_work(const AttnPagedArgs&) { return 0; }
+// Outputs of split positions: a workgroup per (token, head) of a split sequence; its waves take the pieces in turn and
+// weigh them by their share of the row's sum.
+template <bool BF, int HD>
+__global__ void __launch_bounds__(256) attn_paged_merge_kernel(AttnPagedArgs a, PagedSched p) {
+  constexpr int V = HD / 64;
+  typedef float vec_t __attribute__((ext_vector_type(V)));
+  __shared__ __attribute__((aligned(16))) float mo[4][HD];
+  __shared__ float2 ml[4];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), d = V * lane, rep = a.H / a.Hkv;
+  const int chunk = chunk_of(a, p);
+  int64_t before = 0, part0 = 0;
+  int64_t row = blockIdx.x;  // of the split sequences' rows, all heads
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const SeqLane s(a, p, b0 + lane);
+    const int nz_l = s.splits(chunk), mine = nz_l > 1 ? s.n * a.H : 0, pieces = nz_l > 1 ? s.tiles * a.Hkv * nz_l : 0;
+    const int upto = wave_scan(mine), part_upto = wave_scan(pieces);
+    const int all = __shfl(upto, 63, 64);
+    for (; row < before + all; row += gridDim.x) {
+      const int k = __popcll(__ballot(before + upto <= row));
+      const int inside = (int)(row - before) - (k ? __shfl(upto, k - 1, 64) : 0);
+      const int nz = __shfl(nz_l, k, 64), tiles = __shfl(s.tiles, k, 64), n = __shfl(s.n, k, 64);
+      const int64_t part = part0 + (k ? __shfl(part_upto, k - 1, 64) : 0);
+      const PackedSeq q(a.cu, a.rows, a.lens, b0 + k, a.N, a.R, a.W * a.P);
+      const int h = inside % a.H, t = inside / a.H, kvh = h / rep, r = t * rep + h - kvh * rep, tile = r / p.rt;
+      const int tlast = min(tile * p.rt + p.rt - 1, n * rep - 1) / rep;
+      const int blocks = (q.len - q.n + tlast) / 32 + 1, per = (blocks + nz - 1) / nz, live = (blocks + per - 1) / per;
+      // piece z of the tile's rows
+      auto piece = [&](int z) {
+        const int64_t i = part + (int64_t)((tiles - 1 - tile) * nz + z) * a.Hkv + kvh;
+        return a.part + (i * p.rt + r - tile * p.rt) * (HD + 2);
+      };
+      float m = -FLT_MAX, l = 0.f;
+      vec_t o = 0.f;
+      const bool fits = part + (int64_t)tiles * nz * a.Hkv <= p.parts;
+      if (fits) {
+        for (int z = wave; z < live; z += 4) {
+          const float* const x = piece(z);
+          const float2 s2 = *reinterpret_cast<const float2*>(x + HD);
+          vec_t v;
+#pragma unroll
+          for (int j = 0; j < V; ++j) v[j] = x[d + j];
+          const float mn = fmaxf(m, s2.x), f = s2.y == 0.f ? 0.f : s2.y * exp2_raw(s2.x - mn), keep = l * exp2_raw(m - mn);
+          l = keep + f;
+          m = mn;
+          const float inv = l == 0.f ? 0.f : 1.f / l;
+          o = o * (keep * inv);
+          if (f != 0.f) o += v * (f * inv);
+        }
+      } else {
+        l = NAN;
+      }
+      __syncthreads();
+      *reinterpret_cast<vec_t*>(&mo[wave][d]) = o;
+      if (lane == 0) ml[wave] = make_float2(m, l);
+      __syncthreads();
+      if (wave == 0) {
+        float mm = -FLT_MAX, ll = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) mm = fmaxf(mm, ml[w].x);
+        float f[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          f[w] = ml[w].y == 0.f ? 0.f : ml[w].y * exp2_raw(ml[w].x - mm);
+          ll += f[w];
+        }
+        o = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          if (f[w] != 0.f) o += *reinterpret_cast<const vec_t*>(&mo[w][d]) * (f[w] / ll);
+        if (ll == 0.f) o = NAN;  // no weight at all
+        const int64_t i = (int64_t)(q.t0 + t) * a.H + h;
+        const int64_t tok = q.t0 + t;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          float x = o[j];
+          if (a.gate) x *= sigmoid_raw(Half<BF>::ld(static_cast<const uint16_t*>(a.gate)[tok * a.gate_stride + h * a.gate_head + d + j]));
+          static_cast<uint16_t*>(a.out)[i * HD + d + j] = Half<BF>::mk(x);
+        }
+      }
+    }
+    before += all;
+    part0 += __shfl(part_upto, 63, 64);
+  }
+}
+
+// ---- launches ------------------------------------------------------------------------------------
+
+namespace {
+
+struct PagedPlan {
+  PagedSched rows, tile;
+  bool tiles;           // whether sequences of many rows may be there
+  bool split_r, split_t;  // whether positions can be split at all
+  int64_t floats_r, floats_t;
+};
+
+// Pieces and workspaces that a launch may need, from what the host knows. A piece holds more than `target`-th of the work or
+// `least` blocks, and every split tile at least two halves of one, so split pieces are fewer than 2 target.
+PagedPlan paged_plan(const AttnPagedArgs& a) {
+  PagedPlan r = {};
+  const int64_t rep = a.H / a.Hkv, blocks = (a.W * a.P + 31) / 32;
+  r.tiles = (int64_t)a.max_new * rep > kFewRows;
+  r.rows = {kRowsTile, r.tiles ? kFew : kAll, 4 * a.cus, 8, 0};
+  r.tile = {kTileRows, kMany, 2 * a.cus, 8, 0};
+  auto pieces = [&](const PagedSched& s, int64_t tiles) {
+    const int64_t most = (blocks + s.least - 1) / s.least;
+    return most > 1 ? std::min<int64_t>(2 * s.target + 2, tiles * a.Hkv * most) : 0;
+  };
+  r.rows.parts = pieces(r.rows, (int64_t)a.N * rep / kRowsTile + a.B);
+  r.floats_r = r.rows.parts * kRowsTile * (a.hd + 2);
+  if (r.tiles) {
+    r.tile.parts = pieces(r.tile, (int64_t)a.N * rep / kTileRows + a.B);
+    r.floats_t = r.tile.parts * kTileRows * (a.hd + 2);
+  }
+  return r;
+}
+
+template <bool BF, int HD>
+hipError_t launch_attn_paged_t(const AttnPagedArgs& a, hipStream_t s) {
+  const PagedPlan p = paged_plan(a);
+  const int64_t rep = a.H / a.Hkv;
+  auto grid = [&](const PagedSched& q) {
+    return std::min<int64_t>(((int64_t)a.N * rep / q.rt + a.B) * a.Hkv + q.target, (1ll << 24) - 1);
+  };
+  AttnPagedArgs at = a;
+  if (p.tiles) {
+    static LdsLimit limit;
+    const hipError_t e = limit.raise((const void*)attn_paged_tile_kernel<BF, HD>, tile_lds(HD));
+    if (e != hipSuccess) return e;
+    at.part = a.part ? a.part + p.floats_r : nullptr;
+    hipLaunchKernelGGL((attn_paged_tile_kernel<BF, HD>), dim3((unsigned)grid(p.tile)), dim3(256), tile_lds(HD), s, at, p.tile);
+  }
+  hipLaunchKernelGGL((attn_paged_rows_kernel<BF, HD>), dim3((unsigned)grid(p.rows)), dim3(256), 0, s, a, p.rows);
+  const unsigned most = (unsigned)std::min<int64_t>((int64_t)a.N * a.H, 8 * a.cus);
+  if (p.rows.parts) hipLaunchKernelGGL((attn_paged_merge_kernel<BF, HD>), dim3(most), dim3(256), 0, s, a, p.rows);
+  if (p.tiles && p.tile.parts) hipLaunchKernelGGL((attn_paged_merge_kernel<BF, HD>), dim3(most), dim3(256), 0, s, at, p.tile);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+int64_t attn_paged_work(const AttnPagedArgs& a) {
+  if (a.N == 0) return 0;
+  const PagedPlan p = paged_plan(a);
+  return p.floats_r + p.floats_t;
+}
 
 hipError_t launch_attn_paged(bool bf16, const AttnPagedArgs& a, hipStream_t s) {
-  return bf16 ? launch_attn_paged_t<true>(a, s) : launch_attn_paged_t<false>(a, s);
+  auto dims = [&](auto bf) -> hipError_t {
+    constexpr bool BF = decltype(bf)::value;
+    if (a.hd == 256) return launch_attn_paged_t<BF, 256>(a, s);
+    if (a.hd == 128) return launch_attn_paged_t<BF, 128>(a, s);
+    if (a.hd == 64) return launch_attn_paged_t<BF, 64>(a, s);
+    return hipErrorInvalidValue;
+  };
+  return bf16 ? dims(std::true_type{}) : dims(std::false_type{});
 }
 
 }  // namespace gsq

@@ -15,6 +15,7 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
@@ -27,6 +28,9 @@ struct Half<false> {
   __device__ static uint16_t mk(float v) { return __builtin_bit_cast(uint16_t, (_Float16)v); }
   __device__ static uint32_t pack(f32x2 v) { return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2)); }
   __device__ static f32x2 unpack(uint32_t w) { return __builtin_convertvector(__builtin_bit_cast(f16x2, w), f32x2); }
+  // towards zero, so that what is left of a positive value is not negative
+  __device__ static uint32_t chop(f32x2 v) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(v.x, v.y)); }
+  static constexpr uint16_t kLeast = 1;  // least positive value that the matrix instruction does not take for 0
   __device__ static f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
@@ -37,6 +41,11 @@ struct Half<true> {
   __device__ static uint16_t mk(float v) { return (uint16_t)f32_to_bf16_bits(v); }
   __device__ static uint32_t pack(f32x2 v) { return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2)); }
   __device__ static f32x2 unpack(uint32_t w) { return (f32x2){ld((uint16_t)w), ld((uint16_t)(w >> 16))}; }
+  __device__ static uint32_t chop(f32x2 v) {
+    const float x = v.x, y = v.y;  // a bit cast of a vector's element takes the first
+    return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, y), __builtin_bit_cast(uint32_t, x), 0x07060302u);
+  }
+  static constexpr uint16_t kLeast = 0x80;
   __device__ static f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
