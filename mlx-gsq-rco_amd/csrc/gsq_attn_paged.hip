@@ -45,6 +45,13 @@ __device__ __forceinline__ s16x4 tr_read(const uint8_t* p) {
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
+// v, as a value that nothing is known about: what is formed from it is formed there, not kept in a register
+// through the loop around it
+__device__ __forceinline__ int anew(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
 constexpr int kRowsTile = 16;   // rows of a workgroup of attn_paged_rows_kernel
 constexpr int kTileRows = 128;  // of attn_paged_tile_kernel
 constexpr int kFewRows = 32;    // rows up to which a sequence takes the first
@@ -104,22 +111,24 @@ struct PagedTask {
       const int upto = wave_scan(mine), split = wave_scan(s.splits(chunk) > 1 ? mine : 0);
       const int k = __popcll(__ballot(before + upto <= item));
       if (k < 64 && b0 + k < a.B) {
-        b = b0 + k;
-        const int inside = item - (int)before - (k ? __shfl(upto, k - 1, 64) : 0);
-        nz = __shfl(s.splits(chunk), k, 64);
-        rows = __shfl(s.n, k, 64) * (a.H / a.Hkv);
-        part = split_before + (k ? __shfl(split, k - 1, 64) : 0) + inside;
-        const int tiles = __shfl(s.tiles, k, 64);
+        // the same in every lane, as the compiler cannot see: scalar registers
+        const int at = uniform(k);
+        b = b0 + at;
+        const int inside = uniform(item - (int)before - (at ? __shfl(upto, at - 1, 64) : 0));
+        nz = uniform(__shfl(s.splits(chunk), at, 64));
+        rows = uniform(__shfl(s.n, at, 64)) * (a.H / a.Hkv);
+        part = uniform((int)split_before + (at ? __shfl(split, at - 1, 64) : 0)) + inside;
+        const int tiles = uniform(__shfl(s.tiles, at, 64));
         kvh = inside % a.Hkv;  // neighbours: other KV heads, then other pieces of the same rows
         const int rest = inside / a.Hkv;
         z = rest % nz;
         r0 = (tiles - 1 - rest / nz) * p.rt;  // the last rows see most: first
         const PackedSeq q(a.cu, a.rows, a.lens, b, a.N, a.R, a.W * a.P);
-        t0 = min(max(q.t0, 0), a.N);
-        len = q.len;
-        pos = q.len - q.n;
-        row = q.row;
-        fine = q.fine && (nz == 1 || part < p.parts);
+        t0 = uniform(min(max(q.t0, 0), a.N));
+        len = uniform(q.len);
+        pos = uniform(q.len - q.n);
+        row = uniform(q.row);
+        fine = uniform(q.fine) && (nz == 1 || part < p.parts);
         return;
       }
       before += __shfl(upto, 63, 64);
@@ -271,7 +280,7 @@ struct PagedRows {
 
 // V rows that some of a tile's rows do not see would reach those as 0 x NaN if they are not finite. Blocks with such
 // positions are looked at: values that are not finite are taken out of the product, and put into the outputs that see them
-// when the sums are done (put_odd).
+// when the sums are done (odd_sum).
 template <bool BF>
 __device__ __forceinline__ bool odd_pair(uint32_t w) {  // whether a pair of values holds one that is not finite
   const uint32_t e = BF ? 0x7F80u : 0x7C00u;
@@ -284,11 +293,12 @@ __device__ __forceinline__ uint32_t clean_pair(uint32_t w) {
   if (((w >> 16) & e) == e) w &= 0x0000FFFFu;
   return w;
 }
-// output x of dim d and a row that sees positions up to last: with the values of V at positions j0 .. j1 that were taken out
+// the sum of such values of V, dim d, at positions j0 .. j1 (0 if there is none)
 template <bool BF, int HD>
-__device__ __forceinline__ float put_odd(const AttnPagedArgs& a, const int32_t* table, int kvh, int d, int j0, int j1, int last, float x) {
+__device__ __forceinline__ float odd_sum(const AttnPagedArgs& a, const int32_t* table, int kvh, int d, int j0, int j1) {
+  float x = 0.f;
 #pragma unroll 1
-  for (int j = j0; j <= min(j1, last); ++j) {
+  for (int j = j0; j <= j1; ++j) {
     const int page = table[j / a.P];
     if (page < 0 || page >= a.n_pages) continue;
     const float v = Half<BF>::ld(static_cast<const uint16_t*>(a.vp)[(((int64_t)page * a.Hkv + kvh) * a.P + j % a.P) * HD + d]);
@@ -313,7 +323,7 @@ __device__ __forceinline__ void nan_rows(const AttnPagedArgs& a, const PagedTask
 // positions, each dim of another output tile, so that two rows give a pair of a tile's operand by one permute. The
 // waves are merged at the end.
 template <bool BF, int HD>
-__global__ void __launch_bounds__(256, 2) attn_paged_rows_kernel(AttnPagedArgs a, PagedSched p) {
+__global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) attn_paged_rows_kernel(AttnPagedArgs a, PagedSched p) {
   using E = Half<BF>;
   constexpr int KS = HD / 32, VB = HD / 16, PW = VB < 8 ? VB : 8, NP = VB / PW;
   typedef uint32_t vpiece __attribute__((ext_vector_type(PW / 2)));
@@ -449,7 +459,7 @@ __global__ void __launch_bounds__(256, 2) attn_paged_rows_kernel(AttnPagedArgs a
   if (any_odd) {  // the wave's blocks that were looked at
     for (int x = blk0 + wave; x < blk1; x += 4)
       if (32 * x + 31 > k.pos + tfirst)
-        for (int d = g; d < HD; d += 4) mine[d] = put_odd<BF, HD>(a, table, k.kvh, d, 32 * x, min(32 * x + 31, klast), qpos, mine[d]);
+        for (int d = g; d < HD; d += 4) mine[d] += odd_sum<BF, HD>(a, table, k.kvh, d, 32 * x, min(32 * x + 31, qpos));
   }
   __syncthreads();
   for (int i = tid; i < 16 * HD / 8; i += 256) {
@@ -487,7 +497,9 @@ __global__ void __launch_bounds__(256, 2) attn_paged_rows_kernel(AttnPagedArgs a
 // buffers, one barrier a tile). K's operand is read as it lies, V's by transposing reads (four positions x 16
 // dims per 16 lanes); 16-byte pieces of a row are XOR-swizzled by position so that reads are free of bank conflicts.
 constexpr int tile_keys(int hd) { return hd == 256 ? 32 : 64; }
-constexpr int tile_lds(int hd) { return 2 * 2 * tile_keys(hd) * hd * 2; }
+// steps of a wave's queries that it reads from LDS, as its registers do not hold them
+constexpr int tile_lds_steps(int hd) { return hd == 256 ? 1 : 0; }
+constexpr int tile_lds(int hd) { return 2 * 2 * tile_keys(hd) * hd * 2 + 8192 * tile_lds_steps(hd); }
 
 template <bool BF, int HD>
 __global__ void __launch_bounds__(256, 2) attn_paged_tile_kernel(AttnPagedArgs a, PagedSched p) {
@@ -495,8 +507,9 @@ __global__ void __launch_bounds__(256, 2) attn_paged_tile_kernel(AttnPagedArgs a
   constexpr int NT = 2, KS = HD / 32, VB = HD / 16, KT = tile_keys(HD), NB = 2, RB = 2 * HD, NO = HD / 8;  // RB: bytes of a row
   constexpr int TB = KT * RB, NI = KT * NO / 256;  // bytes of a tile; DMA instructions of a wave for one
   constexpr int SH = HD == 64 ? 1 : 0;             // 128-byte rows: two rows to the 64 banks
+  constexpr int QL = tile_lds_steps(HD);
+  __shared__ int bad_s[4], odd_s[2];
   extern __shared__ __attribute__((aligned(16))) uint8_t paged_lds[];
-  __shared__ int bad_s[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), g = lane >> 4, c = lane & 15;
   clear_tail(a);
   const PagedTask k(a, p, blockIdx.x);
@@ -525,12 +538,13 @@ __global__ void __launch_bounds__(256, 2) attn_paged_tile_kernel(AttnPagedArgs a
     const int64_t base = (out ? 0 : (int64_t)page * page_size) + head + (int64_t)off * HD;
     const uint16_t* const kp = static_cast<const uint16_t*>(a.kp) + base;
     const uint16_t* const vp = static_cast<const uint16_t*>(a.vp) + base;
+    const int ln = anew(lane);
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const int e = i * 64 + lane, r = e / NO, key = WR * wave + r, ko = (e % NO) ^ ksw(key), vo = (e % NO) ^ vsw(key);
+      const int e = i * 64 + ln, r = e / NO, key = WR * wave + r, ko = (e % NO) ^ ksw(key), vo = (e % NO) ^ vsw(key);
       uint8_t* const dst = buf + wave * WR * RB + i * 1024;
-      __builtin_amdgcn_global_load_lds(kp + min(r, left) * HD + 8 * ko, (lds_ptr_t)dst, 16, 0, 0);
-      __builtin_amdgcn_global_load_lds(vp + min(r, left) * HD + 8 * vo, (lds_ptr_t)(dst + TB), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds(kp + (uint32_t)(min(r, left) * HD + 8 * ko), (lds_ptr_t)dst, 16, 0, 0);
+      __builtin_amdgcn_global_load_lds(vp + (uint32_t)(min(r, left) * HD + 8 * vo), (lds_ptr_t)(dst + TB), 16, 0, 0);
     }
   };
   const int j_end = 32 * blk1;
@@ -539,22 +553,27 @@ __global__ void __launch_bounds__(256, 2) attn_paged_tile_kernel(AttnPagedArgs a
   int next_page = page_of(j0 + KT);
   const int rw = k.r0 + 32 * wave;
   const bool on = rw < k.rows;
-  u32x4 qf[NT][KS];
+  u32x4 qf[NT][KS - QL];
+  u32x4* const ql = reinterpret_cast<u32x4*>(paged_lds + 4 * TB) + wave * NT * QL * 64 + lane;
   int qpos[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int r = min(rw + 16 * n + c, k.rows - 1);
     const uint16_t* const q = static_cast<const uint16_t*>(a.q) + k.at(a, r) * HD + 8 * g;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) qf[n][s] = *reinterpret_cast<const u32x4*>(q + 32 * s);
+    for (int s = 0; s < KS; ++s) {
+      const u32x4 w = *reinterpret_cast<const u32x4*>(q + 32 * s);
+      if (s < QL) ql[(n * QL + s) * 64] = w;
+      else qf[n][s - QL] = w;
+    }
     qpos[n] = k.pos + r / rep;
   }
   const int pfirst = k.pos + min(rw, k.rows - 1) / rep, plast = k.pos + min(rw + 31, k.rows - 1) / rep;
   PagedRows<BF, HD, NT> rows;
   rows.init();
   bool any_odd = false;
-  const int kx = ksw(c), vkey = 4 * g + (c >> 2), vx = vsw(vkey);
-  const int vlane = vkey * RB + (((c & 3) >> 1) << 4) + ((c & 1) << 3);
+  const int wfirst = k.pos + k.r0 / rep;  // the workgroup's first token
+  if (tid == 0) odd_s[0] = 0;
   int cur = 0;
   for (; j0 < j_end; j0 += KT, cur ^= 1) {
     // the tile has landed; every wave is done with the other buffer
@@ -563,7 +582,28 @@ __global__ void __launch_bounds__(256, 2) attn_paged_tile_kernel(AttnPagedArgs a
       issue(j0 + KT, next_page, paged_lds + (cur ^ 1) * 2 * TB);
       next_page = page_of(j0 + 2 * KT);
     }
-    const uint8_t* const kt = paged_lds + cur * 2 * TB;
+    uint8_t* const kt = paged_lds + cur * 2 * TB;
+    if (tid == 0) odd_s[cur ^ 1] = 0;
+    if (j0 + KT - 1 > wfirst) {  // positions that some rows do not see
+      u32x4* const v = reinterpret_cast<u32x4*>(kt + TB);
+      bool odd = false;
+#pragma unroll 1
+      for (int i = tid; i < TB / 16; i += 256) {
+        const u32x4 w = v[i];
+        odd |= odd_pair<BF>(w[0]) || odd_pair<BF>(w[1]) || odd_pair<BF>(w[2]) || odd_pair<BF>(w[3]);
+      }
+      if (odd) odd_s[cur] = 1;
+      lds_sync();
+      if (odd_s[cur]) {
+        any_odd = true;
+#pragma unroll 1
+        for (int i = tid; i < TB / 16; i += 256) {
+          const u32x4 w = v[i];
+          v[i] = (u32x4){clean_pair<BF>(w[0]), clean_pair<BF>(w[1]), clean_pair<BF>(w[2]), clean_pair<BF>(w[3])};
+        }
+        lds_sync();
+      }
+    }
 #pragma unroll 1
     for (int sb = 0; sb < KT; sb += 32) {
       const int js = j0 + sb;
@@ -573,14 +613,16 @@ __global__ void __launch_bounds__(256, 2) attn_paged_tile_kernel(AttnPagedArgs a
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int b = 0; b < NB; ++b) s[n][b] = (f32x4){0.f, 0.f, 0.f, 0.f};
-      const uint8_t* const kb = kt + (sb + c) * RB;
+      const uint8_t* const ks = kt + sb * RB;
+      const int ln = anew(lane), g = ln >> 4, c = ln & 15;
 #pragma unroll
       for (int st = 0; st < KS; ++st)
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-          const u32x4 kf = *reinterpret_cast<const u32x4*>(kb + 16 * b * RB + (((4 * st + g) ^ kx) << 4));
+          // a swizzle changes 4 bits of a piece's number, the others are constants of the step
+          const u32x4 kf = *reinterpret_cast<const u32x4*>(ks + c * RB + (((4 * (st & 3) + g) ^ ksw(c)) << 4) + 16 * b * RB + st / 4 * 256);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) s[n][b] = E::mma(kf, qf[n][st], s[n][b]);
+          for (int n = 0; n < NT; ++n) s[n][b] = E::mma(kf, st < QL ? ql[(n * QL + st) * 64] : qf[n][st < QL ? 0 : st - QL], s[n][b]);
         }
       int last[NT];
 #pragma unroll
@@ -589,33 +631,14 @@ __global__ void __launch_bounds__(256, 2) attn_paged_tile_kernel(AttnPagedArgs a
       u32x4 pf[1][2][NT];
       rows.weights(s, masked, last, pf);
       const uint8_t* const vb = kt + TB + sb * RB;
-      bool odd = false;
-      if (masked) {
-        for (int i = lane; i < 32 * RB / 16; i += 64) {
-          const u32x4 w = *reinterpret_cast<const u32x4*>(vb + 16 * i);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) odd |= odd_pair<BF>(w[e]);
-        }
-      }
+      const int vkey = 4 * g + (c >> 2), vlane = vkey * RB + (((c & 3) >> 1) << 4) + ((c & 1) << 3);
       auto operand = [&](int i) {
-        const uint8_t* const va = vb + vlane + (((2 * i) ^ vx) << 4);
-        const s16x4 lo = tr_read(va), hi = tr_read(va + 16 * RB);
+        const uint8_t* const at = vb + vlane + (((2 * (i & 7)) ^ vsw(vkey)) << 4) + i / 8 * 256;
+        const s16x4 lo = tr_read(at), hi = tr_read(at + 16 * RB);
         return __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
       };
-      if (__any(odd)) {
-        any_odd = true;
 #pragma unroll
-        for (int i = 0; i < VB; ++i) {
-          u32x4 vf = operand(i);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) vf[e] = clean_pair<BF>(vf[e]);
-          rows.add(i, vf, pf[0]);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < VB; ++i) rows.add(i, operand(i), pf[0]);
-      }
+      for (int i = 0; i < VB; ++i) rows.add(i, operand(i), pf[0]);
     }
   }
   if (lane == 0) bad_s[wave] = bad;
@@ -632,19 +655,26 @@ __global__ void __launch_bounds__(256, 2) attn_paged_tile_kernel(AttnPagedArgs a
     if (k.nz > 1 && g == 0) *reinterpret_cast<float2*>(to + HD) = make_float2(rows.top(n), ls);
 #pragma unroll
     for (int i = 0; i < VB; ++i) {
-      float v[4] = {rows.acc[n][i][0] * over, rows.acc[n][i][1] * over, rows.acc[n][i][2] * over, rows.acc[n][i][3] * over};
-      if (any_odd) {  // the piece's positions in blocks that were looked at
-        const int from = max(32 * blk0, (pfirst + 1) / 32 * 32);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          v[e] = put_odd<BF, HD>(a, table, k.kvh, 16 * i + 4 * g + e, from, min(j_end - 1, plast), qpos[n], v[e]);
-      }
+      const float v[4] = {rows.acc[n][i][0] * over, rows.acc[n][i][1] * over, rows.acc[n][i][2] * over, rows.acc[n][i][3] * over};
       if (k.nz > 1) {
         *reinterpret_cast<float2*>(to + 16 * i + 4 * g) = make_float2(v[0], v[1]);
         *reinterpret_cast<float2*>(to + 16 * i + 4 * g + 2) = make_float2(v[2], v[3]);
       } else {
         put<BF, 4>(a, i0, 16 * i + 4 * g, v);
       }
+    }
+  }
+  if (any_odd) {  // over what was stored: the piece's positions in blocks that were looked at
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const int from = max(32 * blk0, wfirst + 1 - KT);
+#pragma unroll 1
+    for (int i = lane; i < 32 * HD; i += 64) {
+      const int r = rw + i / HD, d = i % HD;
+      if (r >= k.rows) break;
+      const float x = odd_sum<BF, HD>(a, table, k.kvh, d, from, min(j_end - 1, k.pos + r / rep));
+      if (x == 0.f) continue;
+      if (k.nz > 1) a.part[(k.part * kTileRows + (r - k.r0)) * (HD + 2) + d] = x;
+      else static_cast<uint16_t*>(a.out)[k.at(a, r) * HD + d] = E::mk(x);
     }
   }
 }
