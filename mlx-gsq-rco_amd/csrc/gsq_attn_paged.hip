@@ -28,11 +28,13 @@ namespace gsq {
 enum { kAll = 0, kFew = 1, kMany = 2 };
 
 struct PagedSched {
-  int rt;         // rows of a workgroup
+  int lrt;        // log2 of the rows of a workgroup
   int which;      // kAll, kFew or kMany
   int target;     // workgroups that fill the device
   int least;      // fewest blocks of 32 positions to a piece
-  int64_t parts;  // pieces whose partial outputs `part` holds
+  int64_t parts;    // pieces whose partial outputs `part` holds
+  int64_t part_at;  // the first of them, in floats
+  __device__ __host__ int rt() const { return 1 << lrt; }
 };
 
 namespace {
@@ -52,8 +54,8 @@ __device__ __forceinline__ int anew(int v) {
   return v;
 }
 
-constexpr int kRowsTile = 16;   // rows of a workgroup of attn_paged_rows_kernel
-constexpr int kTileRows = 128;  // of attn_paged_tile_kernel
+constexpr int kRowsTile = 16;   // rows of a workgroup of attn_paged_rows_kernel: 2^4
+constexpr int kTileRows = 128;  // of attn_paged_tile_kernel: 2^7
 constexpr int kFewRows = 32;    // rows up to which a sequence takes the first
 
 // Lane's view of a sequence.
@@ -62,15 +64,16 @@ struct SeqLane {
   __device__ SeqLane(const AttnPagedArgs& a, const PagedSched& p, int b) {
     n = tiles = blocks = 0;
     if (b >= a.B) return;
-    const int t0 = min(max(a.cu[b], 0), a.N), t1 = min(max(a.cu[b + 1], t0), a.N), rep = a.H / a.Hkv;
+    const int t0 = min(max(a.cu[b], 0), a.N), t1 = min(max(a.cu[b + 1], t0), a.N);
     const PackedSeq s(a.cu, a.rows, a.lens, b, a.N, a.R, a.W * a.P);
     n = t1 - t0;
-    const bool few = (int64_t)n * rep <= kFewRows;
+    const bool few = n * a.rep <= kFewRows;
     if (p.which != kAll && few != (p.which == kFew)) n = 0;
-    tiles = (n * rep + p.rt - 1) / p.rt;
+    tiles = (n * a.rep + p.rt() - 1) >> p.lrt;
     blocks = s.fine ? (s.len + 31) / 32 : 1;  // one that is not served: its rows are NaN, in one piece
   }
-  __device__ int splits(int chunk) const { return (blocks + chunk - 1) / chunk; }
+  // pieces of `per` blocks (1 / per given), or one more: what counts is that all workgroups get the same
+  __device__ int splits(float over) const { return max((int)ceilf((float)blocks * over), 1); }
 };
 
 template <typename T>
@@ -84,17 +87,41 @@ __device__ __forceinline__ T wave_scan(T v) {  // inclusive
   return v;
 }
 
-// Blocks to a piece: the step's work (tiles of rows times blocks) over as many workgroups as fill the device.
-__device__ __forceinline__ int chunk_of(const AttnPagedArgs& a, const PagedSched& p) {
-  int64_t total = 0;
+// One over the blocks of a piece. Few rows: the step's work (tiles of rows times blocks) over as many workgroups as
+// fill the device. Many rows: the longest sequence in 1 .. 64 pieces, whichever ends first when workgroups of one piece each
+// fill the device in turn (kPieceCost blocks for what a piece costs besides: its partial outputs, written and merged); with
+// enough tiles of rows, or many sequences of them, none is split.
+constexpr int kPieceCost = 10;
+
+__device__ __forceinline__ float over_chunk(const AttnPagedArgs& a, const PagedSched& p) {
+  const int lane = threadIdx.x & 63;
+  float total = 0.f;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const SeqLane s(a, p, b0 + (threadIdx.x & 63));
-    total += (int64_t)s.tiles * s.blocks;
+    const SeqLane s(a, p, b0 + lane);
+    total += (float)s.tiles * (float)(p.which == kMany ? 1 : s.blocks);
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
-  return max(p.least, (int)min((total * a.Hkv + p.target - 1) / p.target, (int64_t)(1 << 26)));
+  total = lanes_sum(total) * (float)a.Hkv;
+  if (p.which != kMany) return __builtin_amdgcn_rcpf(fmaxf(total / (float)p.target, (float)p.least));
+  if (total >= 8.f * (float)p.target || a.B > 64) return 0.f;
+  const SeqLane s(a, p, lane);
+  uint64_t many = __ballot(s.tiles > 0);
+  if (__popcll(many) > 16) return 0.f;
+  int longest = s.tiles > 0 ? s.blocks : 0;
+  longest = (int)lanes_reduce((float)longest, [](float x, float y) { return fmaxf(x, y); });
+  const float chunk = fmaxf((float)longest / (float)(lane + 1), (float)p.least), over = 0.99999f * __builtin_amdgcn_rcpf(chunk);  // not one piece more by its rounding
+  float items = 0.f;
+  for (; many; many &= many - 1) {
+    const int i = __builtin_ctzll(many);
+    items += (float)__builtin_amdgcn_readlane(s.tiles, i) * ceilf((float)__builtin_amdgcn_readlane(s.blocks, i) * over);
+  }
+  float cost = ceilf(items * (float)a.Hkv / (float)p.target) * (chunk + (float)(lane ? kPieceCost : 0));
+  const float best = lanes_reduce(cost, [](float x, float y) { return fminf(x, y); });
+  const int pick = __builtin_ctzll(__ballot(cost <= best) | (1ull << 63));
+  return pick ? __shfl(over, pick, 64) : 0.f;
 }
+
+// token of row r of a (sequence, KV head)
+__device__ __forceinline__ int token_of(const AttnPagedArgs& a, int r) { return (int)(__umulhi(2u * (uint32_t)r, a.rep_mul) >> a.rep_shift); }
 
 // What workgroup `item` of a launch is asked to do: rows r0 .. of sequence b and KV head kvh, positions of piece z of nz.
 // Called by whole waves.
@@ -103,26 +130,27 @@ struct PagedTask {
   int64_t part;  // its piece among those that leave partial outputs
   bool fine;
   __device__ PagedTask(const AttnPagedArgs& a, const PagedSched& p, int item) {
-    const int chunk = chunk_of(a, p), lane = threadIdx.x & 63;
+    const float over = over_chunk(a, p);
+    const int lane = threadIdx.x & 63;
     int64_t before = 0, split_before = 0;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
       const SeqLane s(a, p, b0 + lane);
-      const int mine = s.tiles * a.Hkv * s.splits(chunk);
-      const int upto = wave_scan(mine), split = wave_scan(s.splits(chunk) > 1 ? mine : 0);
+      const int pieces = s.splits(over), mine = s.tiles * a.Hkv * pieces;
+      const int upto = wave_scan(mine), split = wave_scan(pieces > 1 ? mine : 0);
       const int k = __popcll(__ballot(before + upto <= item));
       if (k < 64 && b0 + k < a.B) {
         // the same in every lane, as the compiler cannot see: scalar registers
         const int at = uniform(k);
         b = b0 + at;
         const int inside = uniform(item - (int)before - (at ? __shfl(upto, at - 1, 64) : 0));
-        nz = uniform(__shfl(s.splits(chunk), at, 64));
-        rows = uniform(__shfl(s.n, at, 64)) * (a.H / a.Hkv);
+        nz = uniform(__shfl(pieces, at, 64));
+        rows = uniform(__shfl(s.n, at, 64)) * a.rep;
         part = uniform((int)split_before + (at ? __shfl(split, at - 1, 64) : 0)) + inside;
         const int tiles = uniform(__shfl(s.tiles, at, 64));
         kvh = inside % a.Hkv;  // neighbours: other KV heads, then other pieces of the same rows
         const int rest = inside / a.Hkv;
         z = rest % nz;
-        r0 = (tiles - 1 - rest / nz) * p.rt;  // the last rows see most: first
+        r0 = (tiles - 1 - rest / nz) << p.lrt;  // the last rows see most: first
         const PackedSeq q(a.cu, a.rows, a.lens, b, a.N, a.R, a.W * a.P);
         t0 = uniform(min(max(q.t0, 0), a.N));
         len = uniform(q.len);
@@ -135,11 +163,15 @@ struct PagedTask {
       split_before += __shfl(split, 63, 64);
     }
   }
-  __device__ int rep(const AttnPagedArgs& a) const { return a.H / a.Hkv; }
   // (token, head) of row r in q, gate and out, as one index
   __device__ int64_t at(const AttnPagedArgs& a, int r) const {
-    const int rp = rep(a), t = r / rp;
-    return (int64_t)(t0 + t) * a.H + kvh * rp + (r - t * rp);
+    const int t = token_of(a, r);
+    return (int64_t)(t0 + t) * a.H + kvh * a.rep + (r - t * a.rep);
+  }
+  // its gates
+  __device__ int64_t gate_at(const AttnPagedArgs& a, int r) const {
+    const int t = token_of(a, r);
+    return (int64_t)(t0 + t) * a.gate_stride + (int64_t)(kvh * a.rep + (r - t * a.rep)) * a.gate_head;
   }
   // blocks of the piece for a tile whose last token is tlast
   __device__ void blocks(int tlast, int& blk0, int& blk1) const {
@@ -149,18 +181,27 @@ struct PagedTask {
   }
 };
 
-// Output d .. d + M - 1 (M 4 or 8) of (token, head) i: rounded once, after the gate.
+// Output d .. d + M - 1 (M 4 or 8) of (token, head) i, its gates at `gate`: rounded once, after the gate.
 template <bool BF, int M>
-__device__ __forceinline__ void put(const AttnPagedArgs& a, int64_t i, int d, const float* v) {
+__device__ __forceinline__ void put(const AttnPagedArgs& a, int64_t i, int64_t gate, int d, const float* v) {
   using E = Half<BF>;
   float o[M];
 #pragma unroll
   for (int e = 0; e < M; ++e) o[e] = v[e];
   if (a.gate) {
-    const int64_t t = i / a.H;
-    const uint16_t* const g = static_cast<const uint16_t*>(a.gate) + t * a.gate_stride + (i - t * a.H) * a.gate_head + d;
+    const uint16_t* const g = static_cast<const uint16_t*>(a.gate) + gate + d;
+    if (a.gate_wide) {
 #pragma unroll
-    for (int e = 0; e < M; ++e) o[e] *= sigmoid_raw(E::ld(g[e]));
+      for (int e = 0; e < M; e += 4) {
+        const uint2 w = *reinterpret_cast<const uint2*>(g + e);
+        const uint32_t x[2] = {w.x, w.y};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[e + j] *= sigmoid_raw(E::ld((uint16_t)(x[j >> 1] >> (16 * (j & 1)))));
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < M; ++e) o[e] *= sigmoid_raw(E::ld(g[e]));
+    }
   }
   uint32_t w[M / 2];
 #pragma unroll
@@ -258,7 +299,7 @@ struct PagedRows {
           const uint32_t hi = E::chop(p);
           pf[b / 2][0][n][2 * (b & 1) + j] = hi;
           pf[b / 2][1][n][2 * (b & 1) + j] =
-              __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, E::pack(p - E::unpack(hi))), least));
+              __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, E::rest(p, hi)), least));
         }
       }
     }
@@ -299,9 +340,9 @@ __device__ __forceinline__ float odd_sum(const AttnPagedArgs& a, const int32_t* 
   float x = 0.f;
 #pragma unroll 1
   for (int j = j0; j <= j1; ++j) {
-    const int page = table[j / a.P];
+    const int page = table[j >> a.lp];
     if (page < 0 || page >= a.n_pages) continue;
-    const float v = Half<BF>::ld(static_cast<const uint16_t*>(a.vp)[(((int64_t)page * a.Hkv + kvh) * a.P + j % a.P) * HD + d]);
+    const float v = Half<BF>::ld(static_cast<const uint16_t*>(a.vp)[(((int64_t)page * a.Hkv + kvh) * a.P + (j & (a.P - 1))) * HD + d]);
     if (!(fabsf(v) <= FLT_MAX)) x += v;
   }
   return x;
@@ -312,7 +353,7 @@ template <bool BF>
 __device__ __forceinline__ void nan_rows(const AttnPagedArgs& a, const PagedTask& k, int rt) {
   const float v[8] = {NAN, NAN, NAN, NAN, NAN, NAN, NAN, NAN};
   for (int i = threadIdx.x; i < rt * (a.hd / 8); i += blockDim.x)
-    if (k.r0 + i / (a.hd / 8) < k.rows) put<BF, 8>(a, k.at(a, k.r0 + i / (a.hd / 8)), 8 * (i % (a.hd / 8)), v);
+    if (k.r0 + i / (a.hd / 8) < k.rows) put<BF, 8>(a, k.at(a, k.r0 + i / (a.hd / 8)), k.gate_at(a, k.r0 + i / (a.hd / 8)), 8 * (i % (a.hd / 8)), v);
 }
 
 }  // namespace
@@ -323,22 +364,23 @@ __device__ __forceinline__ void nan_rows(const AttnPagedArgs& a, const PagedTask
 // positions, each dim of another output tile, so that two rows give a pair of a tile's operand by one permute. The
 // waves are merged at the end.
 template <bool BF, int HD>
-__global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) attn_paged_rows_kernel(AttnPagedArgs a, PagedSched p) {
+__device__ __forceinline__ void paged_rows(const AttnPagedArgs& a, const PagedSched& p, int item, uint8_t* lds) {
   using E = Half<BF>;
   constexpr int KS = HD / 32, VB = HD / 16, PW = VB < 8 ? VB : 8, NP = VB / PW;
   typedef uint32_t vpiece __attribute__((ext_vector_type(PW / 2)));
   constexpr int OS = HD + 4;
-  __shared__ __attribute__((aligned(16))) float mo[4 * 16 * OS];
-  __shared__ float2 ml[4 * 16];
+  // queries in operand order, which a wave reads a step at a time; the merge of the waves takes the same memory
+  u32x4* const qs = reinterpret_cast<u32x4*>(lds);
+  float* const mo = reinterpret_cast<float*>(lds);
+  float2* const ml = reinterpret_cast<float2*>(mo + 4 * 16 * OS);
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), g = lane >> 4, c = lane & 15;
-  clear_tail(a);
-  const PagedTask k(a, p, blockIdx.x);
+  const PagedTask k(a, p, item);
   if (k.b < 0) return;
   if (!k.fine) {
     if (k.nz == 1) nan_rows<BF>(a, k, kRowsTile);
     return;
   }
-  const int rep = k.rep(a), tfirst = k.r0 / rep, tlast = min(k.r0 + 15, k.rows - 1) / rep;
+  const int tfirst = uniform(token_of(a, k.r0)), tlast = uniform(token_of(a, min(k.r0 + 15, k.rows - 1)));
   int blk0, blk1;
   k.blocks(tlast, blk0, blk1);
   if (blk0 >= blk1) return;  // the merge knows
@@ -348,31 +390,36 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) attn_paged_rows_kernel
   bool bad = false;
   // first value of positions 16 j .. + 15 of K or V: they lie in one page
   auto group_at = [&](int j) {
-    const int first = min(16 * j, klast), page = uniform(table[first / a.P]);
+    const int first = min(16 * j, klast), page = scalar_at(table, first >> a.lp);
     const bool out = page < 0 || page >= a.n_pages;
     bad |= out;
-    return (out ? 0 : (int64_t)page * page_size) + head + (int64_t)(first % a.P & ~15) * HD;
+    return (out ? 0 : (int64_t)page * page_size) + head + (int64_t)(first & (a.P - 1) & ~15) * HD;
   };
   u32x4 kr[2][KS];
   vpiece vr[8][NP];
   int64_t at[2];
-  auto load_k = [&](int blk) {
+  auto load_k = [&](int blk, int b) {
+    const int ln = anew(lane), left = max(klast - 32 * blk - 16 * b, 0);  // rows of the group behind it repeat one
+    const uint16_t* const src = static_cast<const uint16_t*>(a.kp) + at[b];
+    const uint32_t off = (uint32_t)((left < 15 ? min(ln & 15, left) : ln & 15) * HD + 8 * (ln >> 4));
+#pragma unroll
+    for (int s = 0; s < KS; ++s) kr[b][s] = *reinterpret_cast<const u32x4*>(src + off + 32 * s);
+  };
+  auto load_v = [&](int blk, int h) {  // dims (HD / NP) h ..
+    const int ln = anew(lane);
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       const int left = max(klast - 32 * blk - 16 * b, 0);
-      const uint16_t* const src = static_cast<const uint16_t*>(a.kp) + at[b] + 8 * g;
-      const int r = left < 15 ? min(c, left & 15) : c;
+      const uint16_t* const src = static_cast<const uint16_t*>(a.vp) + at[b] + (HD / NP) * h;
+      if (left >= 15) {
+        const uint32_t off = (uint32_t)(4 * (ln >> 4) * HD + PW * (ln & 15));
 #pragma unroll
-      for (int s = 0; s < KS; ++s) kr[b][s] = *reinterpret_cast<const u32x4*>(src + r * HD + 32 * s);
-    }
-  };
-  auto load_v = [&](int blk) {
+        for (int i = 0; i < 4; ++i) vr[4 * b + i][h] = *reinterpret_cast<const vpiece*>(src + off + i * HD);
+      } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int left = max(klast - 32 * blk - 16 * (i >> 2), 0), r = min(4 * g + (i & 3), left);
-      const uint16_t* const src = static_cast<const uint16_t*>(a.vp) + at[i >> 2] + r * HD + PW * c;
-#pragma unroll
-      for (int h = 0; h < NP; ++h) vr[i][h] = *reinterpret_cast<const vpiece*>(src + (HD / NP) * h);
+        for (int i = 0; i < 4; ++i)
+          vr[4 * b + i][h] = *reinterpret_cast<const vpiece*>(src + (uint32_t)(min(4 * (ln >> 4) + i, left) * HD + PW * (ln & 15)));
+      }
     }
   };
   // a group that lies behind the last position repeats the group that holds it
@@ -383,56 +430,56 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) attn_paged_rows_kernel
   int blk = blk0 + wave;
   if (blk < blk1) {
     locate(blk);
-    load_k(blk);
+    load_k(blk, 0);
+    load_k(blk, 1);
   }
-  u32x4 qf[KS];
   {
     const uint16_t* const q = static_cast<const uint16_t*>(a.q) + k.at(a, min(k.r0 + c, k.rows - 1)) * HD + 8 * g;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const u32x4*>(q + 32 * s);
+    for (int s = wave; s < KS; s += 4) qs[s * 64 + lane] = *reinterpret_cast<const u32x4*>(q + 32 * s);
   }
-  if (blk < blk1) load_v(blk);
-  const int qpos = k.pos + min(k.r0 + c, k.rows - 1) / rep;
+  if (blk < blk1) load_v(blk, 0);
+  lds_sync();
+  const int qpos = k.pos + token_of(a, min(k.r0 + c, k.rows - 1));
   PagedRows<BF, HD, 1> rows;
   rows.init();
   bool any_odd = false;
   for (; blk < blk1; blk += 4) {
     const bool more = blk + 4 < blk1;
-    f32x4 s[1][2];
+    const u32x4* const ql = qs + anew(lane);
+    f32x4 s[1][2] = {{{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}};
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      s[0][b] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    for (int st = 0; st < KS; ++st) {
+      const u32x4 q = ql[st * 64];
 #pragma unroll
-      for (int st = 0; st < KS; ++st) s[0][b] = E::mma(kr[b][st], qf[st], s[0][b]);
+      for (int b = 0; b < 2; ++b) s[0][b] = E::mma(kr[b][st], q, s[0][b]);
     }
+    // where two halves of V are not held beside the next K's: the second half now, K's where the first was
+    if (NP == 2) load_v(blk, 1);
     if (more) {
       locate(blk + 4);
-      load_k(blk + 4);
+      load_k(blk + 4, 0);
+      if (NP == 1) load_k(blk + 4, 1);
     }
     const int last[1] = {qpos - 32 * blk};
     const bool masked = 32 * blk + 31 > k.pos + tfirst;
     u32x4 pf[1][2][1];
     rows.weights(s, masked, last, pf);
-    bool odd = false;
-    if (masked && tfirst != tlast) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+    for (int h = 0; h < NP; ++h) {
+      if (masked && tfirst != tlast) {
+        bool odd = false;
 #pragma unroll
-        for (int h = 0; h < NP; ++h)
+        for (int i = 0; i < 8; ++i)
 #pragma unroll
           for (int w = 0; w < PW / 2; ++w) odd |= odd_pair<BF>(vr[i][h][w]);
-    }
-    if (__any(odd)) {
-      any_odd = true;
+        if (__any(odd)) {
+          any_odd = true;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+          for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int h = 0; h < NP; ++h)
-#pragma unroll
-          for (int w = 0; w < PW / 2; ++w) vr[i][h][w] = clean_pair<BF>(vr[i][h][w]);
-    }
-#pragma unroll
-    for (int h = 0; h < NP; ++h)
+            for (int w = 0; w < PW / 2; ++w) vr[i][h][w] = clean_pair<BF>(vr[i][h][w]);
+        }
+      }
 #pragma unroll
       for (int i = 0; i < PW; ++i) {  // dim (HD / NP) h + PW c + i of the 8 positions
         u32x4 vf;
@@ -441,9 +488,12 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) attn_paged_rows_kernel
           vf[j] = __builtin_amdgcn_perm(vr[2 * j + 1][h][i >> 1], vr[2 * j][h][i >> 1], i & 1 ? 0x07060302u : 0x05040100u);
         rows.add(PW * h + i, vf, pf[0]);
       }
-    if (more) load_v(blk + 4);
+      if (NP == 2 && h == 0 && more) load_k(blk + 4, 1);
+    }
+    if (more) load_v(blk + 4, 0);
   }
   // merge of the waves: every wave's reference, sum and outputs over its own sum
+  lds_sync();  // queries are no longer read
   const float ls = bad ? NAN : rows.sum(0), over = ls == 0.f ? 0.f : 1.f / ls;
   float* const mine = mo + (wave * 16 + c) * OS;
 #pragma unroll
@@ -481,14 +531,14 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) attn_paged_rows_kernel
 #pragma unroll
       for (int j = 0; j < 2; ++j) o[j] += *reinterpret_cast<const f32x4*>(mo + (w * 16 + rr) * OS + d + 4 * j) * (f[w] * inv);
     if (k.nz > 1) {
-      float* const to = a.part + (k.part * kRowsTile + rr) * (HD + 2);
+      float* const to = a.part + p.part_at + (k.part * kRowsTile + rr) * (HD + 2);
       // rows of HD + 2 floats: pairs are aligned
 #pragma unroll
       for (int j = 0; j < 4; ++j) *reinterpret_cast<float2*>(to + d + 2 * j) = make_float2(o[j >> 1][2 * (j & 1)], o[j >> 1][2 * (j & 1) + 1]);
       if (d == 0) *reinterpret_cast<float2*>(to + HD) = make_float2(mm, ll);
     } else {
       const float v[8] = {o[0][0], o[0][1], o[0][2], o[0][3], o[1][0], o[1][1], o[1][2], o[1][3]};
-      put<BF, 8>(a, k.at(a, r), d, v);
+      put<BF, 8>(a, k.at(a, r), k.gate_at(a, r), d, v);
     }
   }
 }
@@ -502,23 +552,21 @@ constexpr int tile_lds_steps(int hd) { return hd == 256 ? 1 : 0; }
 constexpr int tile_lds(int hd) { return 2 * 2 * tile_keys(hd) * hd * 2 + 8192 * tile_lds_steps(hd); }
 
 template <bool BF, int HD>
-__global__ void __launch_bounds__(256, 2) attn_paged_tile_kernel(AttnPagedArgs a, PagedSched p) {
+__device__ __forceinline__ void paged_tile(const AttnPagedArgs& a, const PagedSched& p, int item, uint8_t* paged_lds) {
   using E = Half<BF>;
   constexpr int NT = 2, KS = HD / 32, VB = HD / 16, KT = tile_keys(HD), NB = 2, RB = 2 * HD, NO = HD / 8;  // RB: bytes of a row
   constexpr int TB = KT * RB, NI = KT * NO / 256;  // bytes of a tile; DMA instructions of a wave for one
   constexpr int SH = HD == 64 ? 1 : 0;             // 128-byte rows: two rows to the 64 banks
   constexpr int QL = tile_lds_steps(HD);
   __shared__ int bad_s[4], odd_s[2];
-  extern __shared__ __attribute__((aligned(16))) uint8_t paged_lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), g = lane >> 4, c = lane & 15;
-  clear_tail(a);
-  const PagedTask k(a, p, blockIdx.x);
+  const PagedTask k(a, p, item);
   if (k.b < 0) return;
   if (!k.fine) {
     if (k.nz == 1) nan_rows<BF>(a, k, kTileRows);
     return;
   }
-  const int rep = k.rep(a), tlast = min(k.r0 + kTileRows - 1, k.rows - 1) / rep;
+  const int tlast = uniform(token_of(a, min(k.r0 + kTileRows - 1, k.rows - 1)));
   int blk0, blk1;
   k.blocks(tlast, blk0, blk1);
   if (blk0 >= blk1) return;  // the merge knows
@@ -529,12 +577,11 @@ __global__ void __launch_bounds__(256, 2) attn_paged_tile_kernel(AttnPagedArgs a
   auto vsw = [](int key) { return ((key >> SH) & (NO < 16 ? NO / 2 - 1 : 7)) << 1; };
   constexpr int WR = KT / 4;  // positions that a wave brings: they lie in one page
   int bad = 0;
-  auto page_of = [&](int j0) { return table[min(j0 + WR * wave, klast) / a.P]; };
+  auto page_of = [&](int j0) { return scalar_at(table, min(j0 + WR * wave, klast) >> a.lp); };
   auto issue = [&](int j0, int page, uint8_t* buf) {  // positions past the last repeat it
-    page = uniform(page);
     const bool out = page < 0 || page >= a.n_pages;
     bad |= out;
-    const int first = min(j0 + WR * wave, klast), left = klast - first, off = first % a.P;
+    const int first = min(j0 + WR * wave, klast), left = klast - first, off = first & (a.P - 1);
     const int64_t base = (out ? 0 : (int64_t)page * page_size) + head + (int64_t)off * HD;
     const uint16_t* const kp = static_cast<const uint16_t*>(a.kp) + base;
     const uint16_t* const vp = static_cast<const uint16_t*>(a.vp) + base;
@@ -566,13 +613,13 @@ __global__ void __launch_bounds__(256, 2) attn_paged_tile_kernel(AttnPagedArgs a
       if (s < QL) ql[(n * QL + s) * 64] = w;
       else qf[n][s - QL] = w;
     }
-    qpos[n] = k.pos + r / rep;
+    qpos[n] = k.pos + token_of(a, r);
   }
-  const int pfirst = k.pos + min(rw, k.rows - 1) / rep, plast = k.pos + min(rw + 31, k.rows - 1) / rep;
+  const int pfirst = uniform(k.pos + token_of(a, min(rw, k.rows - 1))), plast = uniform(k.pos + token_of(a, min(rw + 31, k.rows - 1)));
   PagedRows<BF, HD, NT> rows;
   rows.init();
   bool any_odd = false;
-  const int wfirst = k.pos + k.r0 / rep;  // the workgroup's first token
+  const int wfirst = uniform(k.pos + token_of(a, k.r0));  // the workgroup's first token
   if (tid == 0) odd_s[0] = 0;
   int cur = 0;
   for (; j0 < j_end; j0 += KT, cur ^= 1) {
@@ -650,8 +697,8 @@ __global__ void __launch_bounds__(256, 2) attn_paged_tile_kernel(AttnPagedArgs a
     const int r = rw + 16 * n + c;
     const float ls = bad ? NAN : rows.sum(n), over = ls == 0.f && k.nz > 1 ? 0.f : 1.f / ls;
     if (r >= k.rows) continue;
-    float* const to = a.part + (k.part * kTileRows + (r - k.r0)) * (HD + 2);
-    const int64_t i0 = k.at(a, r);
+    float* const to = a.part + p.part_at + (k.part * kTileRows + (r - k.r0)) * (HD + 2);
+    const int64_t i0 = k.at(a, r), g0 = k.gate_at(a, r);
     if (k.nz > 1 && g == 0) *reinterpret_cast<float2*>(to + HD) = make_float2(rows.top(n), ls);
 #pragma unroll
     for (int i = 0; i < VB; ++i) {
@@ -660,7 +707,7 @@ __global__ void __launch_bounds__(256, 2) attn_paged_tile_kernel(AttnPagedArgs a
         *reinterpret_cast<float2*>(to + 16 * i + 4 * g) = make_float2(v[0], v[1]);
         *reinterpret_cast<float2*>(to + 16 * i + 4 * g + 2) = make_float2(v[2], v[3]);
       } else {
-        put<BF, 4>(a, i0, 16 * i + 4 * g, v);
+        put<BF, 4>(a, i0, g0, 16 * i + 4 * g, v);
       }
     }
   }
@@ -671,96 +718,141 @@ __global__ void __launch_bounds__(256, 2) attn_paged_tile_kernel(AttnPagedArgs a
     for (int i = lane; i < 32 * HD; i += 64) {
       const int r = rw + i / HD, d = i % HD;
       if (r >= k.rows) break;
-      const float x = odd_sum<BF, HD>(a, table, k.kvh, d, from, min(j_end - 1, k.pos + r / rep));
+      const float x = odd_sum<BF, HD>(a, table, k.kvh, d, from, min(j_end - 1, k.pos + token_of(a, r)));
       if (x == 0.f) continue;
-      if (k.nz > 1) a.part[(k.part * kTileRows + (r - k.r0)) * (HD + 2) + d] = x;
+      if (k.nz > 1) a.part[p.part_at + (k.part * kTileRows + (r - k.r0)) * (HD + 2) + d] = x;
       else static_cast<uint16_t*>(a.out)[k.at(a, r) * HD + d] = E::mk(x);
     }
   }
 }
 
-// Outputs of split positions: a workgroup per (token, head) of a split sequence; its waves take the pieces in turn and
-// weigh them by their share of the row's sum.
+// One launch for both: workgroups of few and of many rows in turn, so that those bound by the cache's bytes run beside
+// those bound by the matrix cores; kTurn of them at a time, one to each shader engine of each XCD, as workgroups go round
+// those in order (8 at a time, all of one kind met in half of the engines: 1.78 ms in place of 1.1).
+constexpr int kTurn = 32;
+
 template <bool BF, int HD>
-__global__ void __launch_bounds__(256) attn_paged_merge_kernel(AttnPagedArgs a, PagedSched p) {
+__global__ void __launch_bounds__(256, 2) attn_paged_kernel(AttnPagedArgs a, PagedSched few, PagedSched many, int few_wgs, int many_wgs) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t paged_lds[];
+  clear_tail(a);
+  const int group = blockIdx.x / kTurn, both = 2 * (min(few_wgs, many_wgs) / kTurn);
+  bool tile;
+  int item;
+  if (group < both) {
+    tile = group & 1;
+    item = kTurn * (group >> 1) + blockIdx.x % kTurn;
+  } else {
+    tile = few_wgs < many_wgs;
+    item = blockIdx.x - kTurn / 2 * both;
+  }
+  if (tile) paged_tile<BF, HD>(a, many, item, paged_lds);
+  else paged_rows<BF, HD>(a, few, item, paged_lds);
+}
+
+// Outputs of split positions, from their pieces' averages weighed by their share of the row's sum: a wave to a row of
+// (token, head), or, of more than kMergePieces pieces, the workgroup's waves in turn; loads of eight pieces are in
+// flight at once.
+constexpr int kMergeWaves = 8, kMergePieces = 16;
+
+template <bool BF, int HD>
+__global__ void __launch_bounds__(64 * kMergeWaves) attn_paged_merge_kernel(AttnPagedArgs a, PagedSched few, PagedSched many, int both) {
   constexpr int V = HD / 64;
   typedef float vec_t __attribute__((ext_vector_type(V)));
-  __shared__ __attribute__((aligned(16))) float mo[4][HD];
-  __shared__ float2 ml[4];
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), d = V * lane, rep = a.H / a.Hkv;
-  const int chunk = chunk_of(a, p);
-  int64_t before = 0, part0 = 0;
-  int64_t row = blockIdx.x;  // of the split sequences' rows, all heads
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const SeqLane s(a, p, b0 + lane);
-    const int nz_l = s.splits(chunk), mine = nz_l > 1 ? s.n * a.H : 0, pieces = nz_l > 1 ? s.tiles * a.Hkv * nz_l : 0;
-    const int upto = wave_scan(mine), part_upto = wave_scan(pieces);
-    const int all = __shfl(upto, 63, 64);
-    for (; row < before + all; row += gridDim.x) {
-      const int k = __popcll(__ballot(before + upto <= row));
-      const int inside = (int)(row - before) - (k ? __shfl(upto, k - 1, 64) : 0);
-      const int nz = __shfl(nz_l, k, 64), tiles = __shfl(s.tiles, k, 64), n = __shfl(s.n, k, 64);
-      const int64_t part = part0 + (k ? __shfl(part_upto, k - 1, 64) : 0);
-      const PackedSeq q(a.cu, a.rows, a.lens, b0 + k, a.N, a.R, a.W * a.P);
-      const int h = inside % a.H, t = inside / a.H, kvh = h / rep, r = t * rep + h - kvh * rep, tile = r / p.rt;
-      const int tlast = min(tile * p.rt + p.rt - 1, n * rep - 1) / rep;
-      const int blocks = (q.len - q.n + tlast) / 32 + 1, per = (blocks + nz - 1) / nz, live = (blocks + per - 1) / per;
-      // piece z of the tile's rows
-      auto piece = [&](int z) {
-        const int64_t i = part + (int64_t)((tiles - 1 - tile) * nz + z) * a.Hkv + kvh;
-        return a.part + (i * p.rt + r - tile * p.rt) * (HD + 2);
-      };
-      float m = -FLT_MAX, l = 0.f;
-      vec_t o = 0.f;
-      const bool fits = part + (int64_t)tiles * nz * a.Hkv <= p.parts;
-      if (fits) {
-        for (int z = wave; z < live; z += 4) {
-          const float* const x = piece(z);
-          const float2 s2 = *reinterpret_cast<const float2*>(x + HD);
-          vec_t v;
+  __shared__ __attribute__((aligned(16))) float mo[kMergeWaves][HD];
+  __shared__ float2 ml[kMergeWaves];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), d = V * lane;
+  int64_t group = blockIdx.x;  // of rows: one, or as many as there are waves
+  for (int pass = 0; pass < 1 + both; ++pass) {
+    const PagedSched& p = pass ? many : few;
+    const float over = over_chunk(a, p);
+    int64_t before = 0, part0 = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+      const SeqLane s(a, p, b0 + lane);
+      const int nz_l = s.splits(over), rows_l = nz_l > 1 ? s.n * a.H : 0, pieces = nz_l > 1 ? s.tiles * a.Hkv * nz_l : 0;
+      const int upto = wave_scan(nz_l > kMergePieces ? rows_l : (rows_l + kMergeWaves - 1) / kMergeWaves);
+      const int part_upto = wave_scan(pieces), all = __shfl(upto, 63, 64);
+      for (; group < before + all; group += gridDim.x) {
+        const int k = uniform(__popcll(__ballot(before + upto <= group)));
+        const int inside = uniform((int)(group - before) - (k ? __shfl(upto, k - 1, 64) : 0));
+        const int nz = uniform(__shfl(nz_l, k, 64)), tiles = uniform(__shfl(s.tiles, k, 64)), n = uniform(__shfl(s.n, k, 64));
+        const int64_t part = part0 + uniform(k ? __shfl(part_upto, k - 1, 64) : 0);
+        const PackedSeq q(a.cu, a.rows, a.lens, b0 + k, a.N, a.R, a.W * a.P);
+        const bool shared = nz > kMergePieces;
+        const int row = shared ? inside : inside * kMergeWaves + wave;
+        const bool on = row < n * a.H;
+        const int t = row / a.H, h = row - t * a.H, kvh = token_of(a, h), r = t * a.rep + h - kvh * a.rep, tile = r >> p.lrt;
+        const int tlast = token_of(a, min(((tile + 1) << p.lrt) - 1, n * a.rep - 1));
+        const int blocks = (q.len - q.n + tlast) / 32 + 1, per = (blocks + nz - 1) / nz, live = (blocks + per - 1) / per;
+        float m = -FLT_MAX, l = 0.f;
+        vec_t o = 0.f;
+        if (!q.fine || part + (int64_t)tiles * nz * a.Hkv > p.parts) {
+          l = NAN;
+        } else if (on) {
+          // pieces of the tile's rows, a.Hkv apart
+          const float* const first = a.part + p.part_at + ((part + (int64_t)(tiles - 1 - tile) * nz * a.Hkv + kvh) * p.rt() + (r - (tile << p.lrt))) * (HD + 2);
+          const int64_t next = (int64_t)a.Hkv * p.rt() * (HD + 2);
+          const int z0 = shared ? wave : 0, step = shared ? kMergeWaves : 1;
+          for (int z = z0; z < live; z += 8 * step) {
+            vec_t x[8];
+            float2 w[8];
 #pragma unroll
-          for (int j = 0; j < V; ++j) v[j] = x[d + j];
-          const float mn = fmaxf(m, s2.x), f = s2.y == 0.f ? 0.f : s2.y * exp2_raw(s2.x - mn), keep = l * exp2_raw(m - mn);
-          l = keep + f;
-          m = mn;
-          const float inv = l == 0.f ? 0.f : 1.f / l;
-          o = o * (keep * inv);
-          if (f != 0.f) o += v * (f * inv);
+            for (int u = 0; u < 8; ++u) {
+              const float* const at = first + min(z + u * step, live - 1) * next;
+              w[u] = *reinterpret_cast<const float2*>(at + HD);
+#pragma unroll
+              for (int j = 0; j < V; ++j) x[u][j] = at[d + j];
+            }
+            float mn = m;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) mn = fmaxf(mn, w[u].x);
+            const float keep = l * exp2_raw(m - mn);
+            float f[8];
+            l = keep;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+              f[u] = z + u * step < live && w[u].y != 0.f ? w[u].y * exp2_raw(w[u].x - mn) : 0.f;
+              l += f[u];
+            }
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            o *= keep * inv;
+            m = mn;
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+              if (f[u] != 0.f) o += x[u] * (f[u] * inv);
+          }
         }
-      } else {
-        l = NAN;
-      }
-      __syncthreads();
-      *reinterpret_cast<vec_t*>(&mo[wave][d]) = o;
-      if (lane == 0) ml[wave] = make_float2(m, l);
-      __syncthreads();
-      if (wave == 0) {
-        float mm = -FLT_MAX, ll = 0.f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) mm = fmaxf(mm, ml[w].x);
-        float f[4];
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          f[w] = ml[w].y == 0.f ? 0.f : ml[w].y * exp2_raw(ml[w].x - mm);
-          ll += f[w];
+        if (shared) {
+          __syncthreads();
+          *reinterpret_cast<vec_t*>(&mo[wave][d]) = o;
+          if (lane == 0) ml[wave] = make_float2(m, l);
+          __syncthreads();
+          if (wave) continue;
+          m = -FLT_MAX;
+          for (int w = 0; w < kMergeWaves; ++w) m = fmaxf(m, ml[w].x);
+          l = 0.f;
+          o = 0.f;
+          for (int w = 0; w < kMergeWaves; ++w) {
+            const float f = ml[w].y == 0.f ? 0.f : ml[w].y * exp2_raw(ml[w].x - m);
+            l += f;
+            if (f != 0.f) o += *reinterpret_cast<const vec_t*>(&mo[w][d]) * f;
+          }
+          o *= 1.f / l;
         }
-        o = 0.f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-          if (f[w] != 0.f) o += *reinterpret_cast<const vec_t*>(&mo[w][d]) * (f[w] / ll);
-        if (ll == 0.f) o = NAN;  // no weight at all
-        const int64_t i = (int64_t)(q.t0 + t) * a.H + h;
+        if (!on) continue;
+        if (l == 0.f || l != l) o = NAN;  // no weight at all
         const int64_t tok = q.t0 + t;
+        if (tok < 0 || tok >= a.N) continue;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           float x = o[j];
           if (a.gate) x *= sigmoid_raw(Half<BF>::ld(static_cast<const uint16_t*>(a.gate)[tok * a.gate_stride + h * a.gate_head + d + j]));
-          static_cast<uint16_t*>(a.out)[i * HD + d + j] = Half<BF>::mk(x);
+          static_cast<uint16_t*>(a.out)[(tok * a.H + h) * HD + d + j] = Half<BF>::mk(x);
         }
       }
+      before += all;
+      part0 += __shfl(part_upto, 63, 64);
     }
-    before += all;
-    part0 += __shfl(part_upto, 63, 64);
+    group -= before;
   }
 }
 
@@ -769,52 +861,53 @@ __global__ void __launch_bounds__(256) attn_paged_merge_kernel(AttnPagedArgs a, 
 namespace {
 
 struct PagedPlan {
-  PagedSched rows, tile;
-  bool tiles;           // whether sequences of many rows may be there
-  bool split_r, split_t;  // whether positions can be split at all
-  int64_t floats_r, floats_t;
+  PagedSched few, many;
+  bool tiles;  // whether sequences of many rows may be there
+  int64_t floats;
 };
 
-// Pieces and workspaces that a launch may need, from what the host knows. A piece holds more than `target`-th of the work or
-// `least` blocks, and every split tile at least two halves of one, so split pieces are fewer than 2 target.
+// Pieces and workspaces that a launch may need, from what the host knows. A piece of a split sequence holds more than half
+// of `target`-th of the work, so there are fewer than 2 target of them (many rows: as many as the search in over_chunk
+// may make of fewer than 8 target tiles, eight rounds of them at most).
 PagedPlan paged_plan(const AttnPagedArgs& a) {
   PagedPlan r = {};
-  const int64_t rep = a.H / a.Hkv, blocks = (a.W * a.P + 31) / 32;
-  r.tiles = (int64_t)a.max_new * rep > kFewRows;
-  r.rows = {kRowsTile, r.tiles ? kFew : kAll, 4 * a.cus, 8, 0};
-  r.tile = {kTileRows, kMany, 2 * a.cus, 8, 0};
-  auto pieces = [&](const PagedSched& s, int64_t tiles) {
-    const int64_t most = (blocks + s.least - 1) / s.least;
-    return most > 1 ? std::min<int64_t>(2 * s.target + 2, tiles * a.Hkv * most) : 0;
+  const int64_t blocks = (a.W * a.P + 31) / 32;
+  r.tiles = (int64_t)a.max_new * a.rep > kFewRows;
+  r.few = {4, r.tiles ? kFew : kAll, 4 * a.cus, 8, 0, 0};
+  r.many = {7, kMany, (a.hd == 64 ? 4 : 2) * a.cus, 8, 0, 0};
+  auto pieces = [&](const PagedSched& s, int64_t tiles, int64_t most) {
+    const int64_t each = (blocks + s.least - 1) / s.least;
+    return each > 1 ? std::min<int64_t>(most, tiles * a.Hkv * (each + 1)) : 0;
   };
-  r.rows.parts = pieces(r.rows, (int64_t)a.N * rep / kRowsTile + a.B);
-  r.floats_r = r.rows.parts * kRowsTile * (a.hd + 2);
+  r.few.parts = pieces(r.few, ((int64_t)a.N * a.rep >> 4) + a.B, 2 * r.few.target + 64);
+  r.floats = r.few.parts * kRowsTile * (a.hd + 2);
   if (r.tiles) {
-    r.tile.parts = pieces(r.tile, (int64_t)a.N * rep / kTileRows + a.B);
-    r.floats_t = r.tile.parts * kTileRows * (a.hd + 2);
+    r.many.parts = pieces(r.many, ((int64_t)a.N * a.rep >> 7) + a.B, 9 * r.many.target);
+    r.many.part_at = r.floats;
+    r.floats += r.many.parts * kTileRows * (a.hd + 2);
   }
   return r;
 }
 
 template <bool BF, int HD>
 hipError_t launch_attn_paged_t(const AttnPagedArgs& a, hipStream_t s) {
+  constexpr int rows_lds = 4 * 16 * (HD + 4) * 4 + 4 * 16 * 8, most_lds = std::max(rows_lds, tile_lds(HD));
   const PagedPlan p = paged_plan(a);
-  const int64_t rep = a.H / a.Hkv;
-  auto grid = [&](const PagedSched& q) {
-    return std::min<int64_t>(((int64_t)a.N * rep / q.rt + a.B) * a.Hkv + q.target, (1ll << 24) - 1);
+  auto grid = [&](const PagedSched& q) {  // whole turns
+    int64_t tiles = ((int64_t)a.N * a.rep >> q.lrt) + a.B;
+    if (q.which == kFew) tiles = std::min<int64_t>(tiles, (int64_t)a.B * (kFewRows >> q.lrt));
+    return (int)((std::min<int64_t>(tiles * a.Hkv + q.target + 64 + (q.which == kMany ? q.parts : 0), 1 << 23) + kTurn - 1) / kTurn * kTurn);
   };
-  AttnPagedArgs at = a;
-  if (p.tiles) {
-    static LdsLimit limit;
-    const hipError_t e = limit.raise((const void*)attn_paged_tile_kernel<BF, HD>, tile_lds(HD));
-    if (e != hipSuccess) return e;
-    at.part = a.part ? a.part + p.floats_r : nullptr;
-    hipLaunchKernelGGL((attn_paged_tile_kernel<BF, HD>), dim3((unsigned)grid(p.tile)), dim3(256), tile_lds(HD), s, at, p.tile);
+  const int few = grid(p.few), many = p.tiles ? grid(p.many) : 0;
+  static LdsLimit limit;
+  const hipError_t e = limit.raise((const void*)attn_paged_kernel<BF, HD>, most_lds);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((attn_paged_kernel<BF, HD>), dim3((unsigned)(few + many)), dim3(256), p.tiles ? most_lds : rows_lds, s, a,
+                     p.few, p.many, few, many);
+  if (p.few.parts || p.many.parts) {
+    const unsigned most = (unsigned)std::min<int64_t>((int64_t)a.N * a.H, 4 * a.cus);
+    hipLaunchKernelGGL((attn_paged_merge_kernel<BF, HD>), dim3(most), dim3(64 * kMergeWaves), 0, s, a, p.few, p.many, (int)p.tiles);
   }
-  hipLaunchKernelGGL((attn_paged_rows_kernel<BF, HD>), dim3((unsigned)grid(p.rows)), dim3(256), 0, s, a, p.rows);
-  const unsigned most = (unsigned)std::min<int64_t>((int64_t)a.N * a.H, 8 * a.cus);
-  if (p.rows.parts) hipLaunchKernelGGL((attn_paged_merge_kernel<BF, HD>), dim3(most), dim3(256), 0, s, a, p.rows);
-  if (p.tiles && p.tile.parts) hipLaunchKernelGGL((attn_paged_merge_kernel<BF, HD>), dim3(most), dim3(256), 0, s, at, p.tile);
   return hipGetLastError();
 }
 
@@ -822,8 +915,7 @@ hipError_t launch_attn_paged_t(const AttnPagedArgs& a, hipStream_t s) {
 
 int64_t attn_paged_work(const AttnPagedArgs& a) {
   if (a.N == 0) return 0;
-  const PagedPlan p = paged_plan(a);
-  return p.floats_r + p.floats_t;
+  return paged_plan(a).floats;
 }
 
 hipError_t launch_attn_paged(bool bf16, const AttnPagedArgs& a, hipStream_t s) {

@@ -1029,6 +1029,10 @@ static AttnPagedArgs attn_paged_sizes(int64_t tokens, int64_t sequences, int64_t
   AttnPagedArgs a = {};
   a.N = (int)tokens; a.B = (int)sequences; a.H = (int)heads; a.Hkv = (int)kv_heads; a.hd = (int)head_dim; a.W = max_pages;
   a.P = (int)page_size; a.max_new = (int)std::min(max_new, tokens); a.cus = (int)cus;
+  a.rep = (int)(heads / kv_heads);
+  while ((1ll << a.lp) < page_size) ++a.lp;
+  while ((1ll << a.rep_shift) < a.rep) ++a.rep_shift;
+  a.rep_mul = (uint32_t)(((1ull << (31 + a.rep_shift)) + a.rep - 1) / a.rep);
   return a;
 }
 
@@ -1067,6 +1071,7 @@ int gsq_attn_paged(const void* q, const void* gate, int64_t gate_stride, int64_t
   if (!work && attn_paged_work(a)) return fail(GSQ_E_VALUE, "work must not be NULL");
   a.q = q; a.gate = gate; a.kp = k_pages; a.vp = v_pages; a.table = table; a.cu = cu; a.rows = rows; a.lens = lens;
   a.out = out; a.part = work; a.gate_stride = gate_stride; a.gate_head = gate_head_stride; a.R = (int)n_requests;
+  a.gate_wide = ((reinterpret_cast<uintptr_t>(gate) & 7) | (uintptr_t)((gate_stride | gate_head_stride) & 3)) == 0;
   a.n_pages = (int)n_pages;
   hipError_t e = launch_attn_paged(dtype == GSQ_BF16, a, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return fail(GSQ_E_HIP, "attn_paged launch: %s", hipGetErrorString(e));

@@ -317,6 +317,9 @@ struct AttnPagedArgs {
   float* part;  // partial outputs of split positions
   int64_t gate_stride, gate_head, W;
   int N, B, R, H, Hkv, hd, n_pages, P, max_new, cus;
+  int rep, lp;  // H / Hkv, log2 P
+  uint32_t rep_mul, rep_shift;  // r / rep = umulhi(2 r, rep_mul) >> rep_shift for 0 <= r < 2^31
+  int gate_wide;                // gates in pieces of four
 };
 
 struct GdnPackedArgs {

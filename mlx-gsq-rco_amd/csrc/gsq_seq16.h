@@ -30,6 +30,11 @@ struct Half<false> {
   __device__ static f32x2 unpack(uint32_t w) { return __builtin_convertvector(__builtin_bit_cast(f16x2, w), f32x2); }
   // towards zero, so that what is left of a positive value is not negative
   __device__ static uint32_t chop(f32x2 v) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(v.x, v.y)); }
+  // a pair of values less what is cut off, rounded: one instruction each takes the 16-bit values off
+  __device__ static uint32_t rest(f32x2 v, uint32_t cut) {
+    const f16x2 h = __builtin_bit_cast(f16x2, cut);
+    return pack((f32x2){__builtin_fmaf((float)h.x, -1.f, v.x), __builtin_fmaf((float)h.y, -1.f, v.y)});
+  }
   static constexpr uint16_t kLeast = 1;  // least positive value that the matrix instruction does not take for 0
   __device__ static f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -45,6 +50,7 @@ struct Half<true> {
     const float x = v.x, y = v.y;  // a bit cast of a vector's element takes the first
     return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, y), __builtin_bit_cast(uint32_t, x), 0x07060302u);
   }
+  __device__ static uint32_t rest(f32x2 v, uint32_t cut) { return pack(v - unpack(cut)); }
   static constexpr uint16_t kLeast = 0x80;
   __device__ static f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -66,6 +72,11 @@ __device__ __forceinline__ int seq_of(const int32_t* cu, int B, int t) {
   for (int i = threadIdx.x & 63; i - (int)(threadIdx.x & 63) < B; i += 64)
     n += __popcll(__ballot(i < B && cu[min(i, B - 1) + 1] <= t));
   return n;
+}
+
+// What lies at p[i], by a scalar load: i the same in every lane, and nothing that the kernel writes.
+__device__ __forceinline__ int scalar_at(const int32_t* p, int64_t i) {
+  return ((const __attribute__((address_space(4))) int32_t*)p)[i];
 }
 
 // A sequence of a step, as far as it can be served: its tokens lie in the packed ones, its request and its length in the
