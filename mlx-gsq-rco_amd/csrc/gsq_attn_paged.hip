@@ -54,6 +54,13 @@ __device__ __forceinline__ int anew(int v) {
   return v;
 }
 
+// 16 bytes a lane from base + off to LDS, 64 times 16 from `dst` on. As assembly: the compiler makes every transposing read
+// wait for all DMA that it knows of, the next tile's too. Whoever reads what it brings waits for vmcnt.
+__device__ __forceinline__ void dma16(const uint16_t* base, uint32_t off, const uint8_t* dst) {
+  const uint32_t lds = uniform((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)dst);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
+}
+
 constexpr int kRowsTile = 16;   // rows of a workgroup of attn_paged_rows_kernel: 2^4
 constexpr int kTileRows = 128;  // of attn_paged_tile_kernel: 2^7
 constexpr int kFewRows = 32;    // rows up to which a sequence takes the first
@@ -91,7 +98,7 @@ __device__ __forceinline__ T wave_scan(T v) {  // inclusive
 // fill the device. Many rows: the longest sequence in 1 .. 64 pieces, whichever ends first when workgroups of one piece each
 // fill the device in turn (kPieceCost blocks for what a piece costs besides: its partial outputs, written and merged); with
 // enough tiles of rows, or many sequences of them, none is split.
-constexpr int kPieceCost = 10;
+constexpr int kPieceCost = 10, kMostTurns = 4;
 
 __device__ __forceinline__ float over_chunk(const AttnPagedArgs& a, const PagedSched& p) {
   const int lane = threadIdx.x & 63;
@@ -102,7 +109,7 @@ __device__ __forceinline__ float over_chunk(const AttnPagedArgs& a, const PagedS
   }
   total = lanes_sum(total) * (float)a.Hkv;
   if (p.which != kMany) return __builtin_amdgcn_rcpf(fmaxf(total / (float)p.target, (float)p.least));
-  if (total >= 8.f * (float)p.target || a.B > 64) return 0.f;
+  if (total >= (float)kMostTurns * (float)p.target || a.B > 64) return 0.f;
   const SeqLane s(a, p, lane);
   uint64_t many = __ballot(s.tiles > 0);
   if (__popcll(many) > 16) return 0.f;
@@ -114,7 +121,8 @@ __device__ __forceinline__ float over_chunk(const AttnPagedArgs& a, const PagedS
     const int i = __builtin_ctzll(many);
     items += (float)__builtin_amdgcn_readlane(s.tiles, i) * ceilf((float)__builtin_amdgcn_readlane(s.blocks, i) * over);
   }
-  float cost = ceilf(items * (float)a.Hkv / (float)p.target) * (chunk + (float)(lane ? kPieceCost : 0));
+  const float turns = ceilf(items * (float)a.Hkv / (float)p.target);
+  const float cost = turns > (float)kMostTurns && lane ? FLT_MAX : turns * (chunk + (float)(lane ? kPieceCost : 0));
   const float best = lanes_reduce(cost, [](float x, float y) { return fminf(x, y); });
   const int pick = __builtin_ctzll(__ballot(cost <= best) | (1ull << 63));
   return pick ? __shfl(over, pick, 64) : 0.f;
@@ -147,10 +155,12 @@ struct PagedTask {
         rows = uniform(__shfl(s.n, at, 64)) * a.rep;
         part = uniform((int)split_before + (at ? __shfl(split, at - 1, 64) : 0)) + inside;
         const int tiles = uniform(__shfl(s.tiles, at, 64));
-        kvh = inside % a.Hkv;  // neighbours: other KV heads, then other pieces of the same rows
+        // neighbours: other KV heads, then other rows over the same positions, which an XCD's L2 then holds (pieces
+        // of the same rows beside each other: 58 of 100 reads of a chunk of 1024 missed it); the last rows see most: first
+        kvh = inside % a.Hkv;
         const int rest = inside / a.Hkv;
-        z = rest % nz;
-        r0 = (tiles - 1 - rest / nz) << p.lrt;  // the last rows see most: first
+        z = rest / tiles;
+        r0 = (tiles - 1 - (rest - z * tiles)) << p.lrt;
         const PackedSeq q(a.cu, a.rows, a.lens, b, a.N, a.R, a.W * a.P);
         t0 = uniform(min(max(q.t0, 0), a.N));
         len = uniform(q.len);
@@ -590,8 +600,8 @@ __device__ __forceinline__ void paged_tile(const AttnPagedArgs& a, const PagedSc
     for (int i = 0; i < NI; ++i) {
       const int e = i * 64 + ln, r = e / NO, key = WR * wave + r, ko = (e % NO) ^ ksw(key), vo = (e % NO) ^ vsw(key);
       uint8_t* const dst = buf + wave * WR * RB + i * 1024;
-      __builtin_amdgcn_global_load_lds(kp + (uint32_t)(min(r, left) * HD + 8 * ko), (lds_ptr_t)dst, 16, 0, 0);
-      __builtin_amdgcn_global_load_lds(vp + (uint32_t)(min(r, left) * HD + 8 * vo), (lds_ptr_t)(dst + TB), 16, 0, 0);
+      dma16(kp, (uint32_t)(min(r, left) * HD + 8 * ko) * 2, dst);
+      dma16(vp, (uint32_t)(min(r, left) * HD + 8 * vo) * 2, dst + TB);
     }
   };
   const int j_end = 32 * blk1;
@@ -661,31 +671,52 @@ __device__ __forceinline__ void paged_tile(const AttnPagedArgs& a, const PagedSc
 #pragma unroll
         for (int b = 0; b < NB; ++b) s[n][b] = (f32x4){0.f, 0.f, 0.f, 0.f};
       const uint8_t* const ks = kt + sb * RB;
+      const uint8_t* const vb = ks + TB;
       const int ln = anew(lane), g = ln >> 4, c = ln & 15;
+      // operands are read a step (K) or two (V) before the products that take them, which the scheduler would undo
+      u32x4 kf[2][NB], qs[2][NT];
+      auto k_step = [&](int st) {
 #pragma unroll
-      for (int st = 0; st < KS; ++st)
+        for (int b = 0; b < NB; ++b)  // a swizzle changes 4 bits of a piece's number, the others are constants of the step
+          kf[st & 1][b] = *reinterpret_cast<const u32x4*>(ks + c * RB + (((4 * (st & 3) + g) ^ ksw(c)) << 4) + 16 * b * RB + st / 4 * 256);
+        if (st < QL) {
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          // a swizzle changes 4 bits of a piece's number, the others are constants of the step
-          const u32x4 kf = *reinterpret_cast<const u32x4*>(ks + c * RB + (((4 * (st & 3) + g) ^ ksw(c)) << 4) + 16 * b * RB + st / 4 * 256);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) s[n][b] = E::mma(kf, st < QL ? ql[(n * QL + st) * 64] : qf[n][st < QL ? 0 : st - QL], s[n][b]);
+          for (int n = 0; n < NT; ++n) qs[st & 1][n] = ql[(n * QL + st) * 64];
         }
+      };
+      k_step(0);
+#pragma unroll
+      for (int st = 0; st < KS; ++st) {
+        if (st + 1 < KS) k_step(st + 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) s[n][b] = E::mma(kf[st & 1][b], st < QL ? qs[st & 1][n] : qf[n][st < QL ? 0 : st - QL], s[n][b]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      const int vkey = 4 * g + (c >> 2), vlane = vkey * RB + (((c & 3) >> 1) << 4) + ((c & 1) << 3);
+      u32x4 vf[3];
+      auto v_tile = [&](int i) {
+        const uint8_t* const at = vb + vlane + (((2 * (i & 7)) ^ vsw(vkey)) << 4) + i / 8 * 256;
+        const s16x4 lo = tr_read(at), hi = tr_read(at + 16 * RB);
+        vf[i % 3] = __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+      };
+      v_tile(0);
+      v_tile(1);
       int last[NT];
 #pragma unroll
       for (int n = 0; n < NT; ++n) last[n] = qpos[n] - js;
       const bool masked = js + 31 > pfirst;
       u32x4 pf[1][2][NT];
       rows.weights(s, masked, last, pf);
-      const uint8_t* const vb = kt + TB + sb * RB;
-      const int vkey = 4 * g + (c >> 2), vlane = vkey * RB + (((c & 3) >> 1) << 4) + ((c & 1) << 3);
-      auto operand = [&](int i) {
-        const uint8_t* const at = vb + vlane + (((2 * (i & 7)) ^ vsw(vkey)) << 4) + i / 8 * 256;
-        const s16x4 lo = tr_read(at), hi = tr_read(at + 16 * RB);
-        return __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-      };
 #pragma unroll
-      for (int i = 0; i < VB; ++i) rows.add(i, operand(i), pf[0]);
+      for (int i = 0; i < VB; ++i) {
+        if (i + 2 < VB) v_tile(i + 2);
+        __builtin_amdgcn_sched_barrier(0);
+        rows.add(i, vf[i % 3], pf[0]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
   }
   if (lane == 0) bad_s[wave] = bad;
@@ -788,9 +819,8 @@ __global__ void __launch_bounds__(64 * kMergeWaves) attn_paged_merge_kernel(Attn
         if (!q.fine || part + (int64_t)tiles * nz * a.Hkv > p.parts) {
           l = NAN;
         } else if (on) {
-          // pieces of the tile's rows, a.Hkv apart
-          const float* const first = a.part + p.part_at + ((part + (int64_t)(tiles - 1 - tile) * nz * a.Hkv + kvh) * p.rt() + (r - (tile << p.lrt))) * (HD + 2);
-          const int64_t next = (int64_t)a.Hkv * p.rt() * (HD + 2);
+          const float* const first = a.part + p.part_at + ((part + (int64_t)(tiles - 1 - tile) * a.Hkv + kvh) * p.rt() + (r - (tile << p.lrt))) * (HD + 2);
+          const int64_t next = (int64_t)tiles * a.Hkv * p.rt() * (HD + 2);  // the same rows' next piece
           const int z0 = shared ? wave : 0, step = shared ? kMergeWaves : 1;
           for (int z = z0; z < live; z += 8 * step) {
             vec_t x[8];
@@ -867,8 +897,8 @@ struct PagedPlan {
 };
 
 // Pieces and workspaces that a launch may need, from what the host knows. A piece of a split sequence holds more than half
-// of `target`-th of the work, so there are fewer than 2 target of them (many rows: as many as the search in over_chunk
-// may make of fewer than 8 target tiles, eight rounds of them at most).
+// of `target`-th of the work, so there are fewer than 2 target of them (many rows: at most kMostTurns target, as the search
+// in over_chunk goes).
 PagedPlan paged_plan(const AttnPagedArgs& a) {
   PagedPlan r = {};
   const int64_t blocks = (a.W * a.P + 31) / 32;
@@ -882,7 +912,7 @@ PagedPlan paged_plan(const AttnPagedArgs& a) {
   r.few.parts = pieces(r.few, ((int64_t)a.N * a.rep >> 4) + a.B, 2 * r.few.target + 64);
   r.floats = r.few.parts * kRowsTile * (a.hd + 2);
   if (r.tiles) {
-    r.many.parts = pieces(r.many, ((int64_t)a.N * a.rep >> 7) + a.B, 9 * r.many.target);
+    r.many.parts = pieces(r.many, ((int64_t)a.N * a.rep >> 7) + a.B, kMostTurns * r.many.target + 64);
     r.many.part_at = r.floats;
     r.floats += r.many.parts * kTileRows * (a.hd + 2);
   }
@@ -896,7 +926,8 @@ hipError_t launch_attn_paged_t(const AttnPagedArgs& a, hipStream_t s) {
   auto grid = [&](const PagedSched& q) {  // whole turns
     int64_t tiles = ((int64_t)a.N * a.rep >> q.lrt) + a.B;
     if (q.which == kFew) tiles = std::min<int64_t>(tiles, (int64_t)a.B * (kFewRows >> q.lrt));
-    return (int)((std::min<int64_t>(tiles * a.Hkv + q.target + 64 + (q.which == kMany ? q.parts : 0), 1 << 23) + kTurn - 1) / kTurn * kTurn);
+    const int64_t most = q.which == kMany ? std::max<int64_t>(tiles * a.Hkv, q.parts) : tiles * a.Hkv + q.target;
+    return (int)((std::min<int64_t>(most + 64, 1 << 23) + kTurn - 1) / kTurn * kTurn);
   };
   const int few = grid(p.few), many = p.tiles ? grid(p.many) : 0;
   static LdsLimit limit;
