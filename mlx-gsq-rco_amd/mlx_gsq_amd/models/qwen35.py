@@ -42,16 +42,21 @@ runs the model on the CPU with dense stand-ins for the packed layers).
 such a cache ``Qwen35Model.verify`` runs a tree of drafted tokens in one pass without advancing the
 cache, and ``accept`` keeps one path of it: the GatedDeltaNet layers run along every path from the cached
 state (``gdn_tree``) and the kept tokens' inputs advance it afterwards.
+
+``new_paged_cache`` and ``Qwen35Model.step`` serve many requests at once, of any lengths: their new tokens are packed behind
+one another, K and V lie in pages that are handed out as requests grow (packed.py, runtime/kernels/paged.py).
 """
 from __future__ import annotations
 
 import math
 from dataclasses import dataclass
+from types import SimpleNamespace
 
 import torch
 import torch.nn.functional as F
 from torch.autograd import forward_ad
 
+from .packed import PackedStep, PagedCache
 
 @dataclass(frozen=True)
 class Qwen35Args:
@@ -185,6 +190,8 @@ class GatedDeltaNet(torch.nn.Module):
         """``first``: ``in_proj_qkvz(x)`` when the caller has computed it already, or
         ``first_pre``'s (qkvz, convolution outputs). ``parents``: the tokens are a drafted tree; the cache is
         left alone, and the layer's inputs are kept for ``advance``."""
+        if isinstance(cache, PackedStep):
+            return self._packed(x, cache)
         a_ = self.args
         S = x.shape[1]
         conv_out = None
@@ -213,6 +220,23 @@ class GatedDeltaNet(torch.nn.Module):
                                         self.ssm_a, self.dt_bias, cache.rec[self.layer], self.norm_w, **self._heads)
             return self.out_proj(out)
         return self.out_proj(self._mix(qkv, z, F.linear(x, self.w_ab), cache).to(x.dtype))
+
+    def _packed(self, x, step: PackedStep):
+        """The tokens of a step, x (1, N, hidden), each request with a state of its own."""
+        n, c = self.args.conv_dim, step.cache
+        qkvz, ab = self.in_proj_qkvz(x)[0], F.linear(x, self.w_ab)[0]
+        conv, rec = c.conv[self.layer], c.rec[self.layer]
+        if x.is_cuda:
+            from ..runtime.kernels import paged
+            return self.out_proj(paged.gdn_packed(qkvz[:, :n], qkvz[:, n:], ab, conv, self.conv_w, self.ssm_a, self.dt_bias, rec,
+                                                  self.norm_w, step.plan, max_new=step.max_new, **self._heads)[None])
+        out = x.new_zeros(1, x.shape[1], self.args.value_dim)
+        for r, t0, t1, length in step.sequences():
+            if length == t1 - t0:
+                conv[r], rec[r] = 0, 0
+            one = SimpleNamespace(conv={self.layer: conv[r:r + 1]}, rec={self.layer: rec[r:r + 1]})
+            out[:, t0:t1] = self._mix(qkvz[None, t0:t1, :n], qkvz[None, t0:t1, n:], ab[None, t0:t1], one).to(x.dtype)
+        return self.out_proj(out)
 
     @property
     def _heads(self):
@@ -411,9 +435,39 @@ class FullAttention(torch.nn.Module):
         att = torch.matmul(torch.softmax(scores, dim=-1), vf).reshape(B, H, S, hd).transpose(1, 2)
         return (att * torch.sigmoid(qg[..., hd:].float())).reshape(B, S, H * hd).to(qk.dtype)
 
+    def _packed(self, x, step: PackedStep):
+        """The tokens of a step, x (1, N, hidden), over their requests' pages."""
+        a_, c, i, plan = self.args, step.cache, self.layer, step.plan
+        N, H, Hkv, hd = x.shape[1], a_.num_attention_heads, a_.num_key_value_heads, a_.head_dim
+        qk, v = self.qk_proj(x)[0], self.v_proj(x)[0].view(N, Hkv, hd)
+        qg, k = qk[:, :H * 2 * hd].view(N, H, 2 * hd), qk[:, H * 2 * hd:].view(N, Hkv, hd)
+        if x.is_cuda:
+            from ..runtime.kernels import paged
+            q = paged.paged_write(qg[..., :hd], k, v, self.q_norm_w, self.k_norm_w, self.inv_freq, c.k[i], c.v[i], plan.pos,
+                                  plan.slots, eps=a_.rms_norm_eps)
+            out = paged.attn_paged(q, c.k[i], c.v[i], c.table, plan, gate=qg[..., hd:], max_new=step.max_new)
+            return self.o_proj(out.view(1, N, H * hd))
+        q = self._rope(rms_norm(qg[..., :hd].float(), self.q_norm_w, a_.rms_norm_eps)[None], plan.pos)[0]
+        k = self._rope(rms_norm(k.float(), self.k_norm_w, a_.rms_norm_eps)[None], plan.pos)[0].to(k.dtype)
+        there, P = plan.slots >= 0, c.page_size
+        at = plan.slots[there]
+        c.k[i][at // P, :, at % P], c.v[i][at // P, :, at % P] = k[there], v[there]
+        out = x.new_zeros(N, H, hd)
+        for r, t0, t1, n in step.sequences():
+            pages = c.table[r, :-(-n // P)].long()
+            kf, vf = (t[pages].transpose(1, 2).reshape(-1, Hkv, hd)[:n].float().repeat_interleave(H // Hkv, 1).transpose(0, 1)
+                      for t in (c.k[i], c.v[i]))                                   # (H, n, hd)
+            scores = torch.matmul(q[t0:t1].float().transpose(0, 1), kf.transpose(1, 2).contiguous()) * hd ** -0.5
+            later = torch.arange(n) > torch.arange(n - (t1 - t0), n)[:, None]
+            att = torch.matmul(torch.softmax(scores.masked_fill(later, float("-inf")), -1), vf).transpose(0, 1)
+            out[t0:t1] = (att * torch.sigmoid(qg[t0:t1, :, hd:].float())).to(x.dtype)
+        return self.o_proj(out.view(1, N, H * hd))
+
     def forward(self, x, cache: Qwen35Cache, first=None, parents=None):
         """``first``: ``qk_proj(x)`` when the caller has computed it already. ``parents``: the tokens are a
         drafted tree (8-bit caches)."""
+        if isinstance(cache, PackedStep):
+            return self._packed(x, cache)
         if parents is not None and cache.kv_bits != 8:
             raise ValueError("trees of drafted tokens need an 8-bit cache (new_cache(kv_bits=8))")
         a_ = self.args
@@ -489,7 +543,7 @@ class Qwen35Layer(torch.nn.Module):
     def forward(self, x, delta, cache, parents=None):
         eps = self.args.rms_norm_eps
         # a drafted token leaves the convolution's state alone, which the fused projection would advance
-        if parents is None and _fused_row(x, self.mixer.first_proj, self.gate_up, self.down):
+        if parents is None and not isinstance(cache, PackedStep) and _fused_row(x, self.mixer.first_proj, self.gate_up, self.down):
             h = torch.empty_like(x)                 # the normalized layer input
             x1 = x if delta is None else torch.empty_like(x)
             first = self.mixer.first_pre(x, cache, pre_a=delta, pre_w=self.input_norm_w, eps=eps,
@@ -522,6 +576,54 @@ class Qwen35Model(torch.nn.Module):
     def new_cache(self, batch: int = 1, max_len: int = 4096, device=None, kv_bits: int = 16) -> Qwen35Cache:
         device = device if device is not None else self.norm_w.device
         return Qwen35Cache(self.args, batch, max_len, device, self.dtype, kv_bits)
+
+    def new_paged_cache(self, requests: int, pages: int, page_size: int = 64, max_len: int = 4096, device=None) -> PagedCache:
+        """States of up to ``requests`` requests for ``step``, ``pages`` pages of ``page_size`` positions between them."""
+        device = device if device is not None else self.norm_w.device
+        return PagedCache(self.args, requests, pages, page_size, max_len, device, self.dtype)
+
+    def step(self, ids, new, requests, cache: PagedCache, max_new=None, all_logits: bool = False):
+        """One step of many requests: request ``requests[b]`` brings the next ``new[b]`` of the tokens ``ids`` (N,), a whole
+        prompt, a piece of one or a single token, behind what the cache holds of it. Returns the logits behind each
+        sequence's last token (B, vocab), or (``all_logits``) behind every token (N, vocab).
+
+        ``new`` and ``requests`` are lists, or int32 tensors on the cache's device, which are not looked at on the host
+        (``max_new``: their most new tokens, if known). Rows of sequences that are not served (no pages left, longer than
+        ``max_len``) or bring no tokens are NaN, and those requests stay as they were."""
+        device = cache.table.device
+        if not (torch.is_tensor(new) and torch.is_tensor(requests) and new.device == device):
+            new, requests = ([int(x) for x in t] for t in (new, requests))
+            if len(new) != len(requests) or sum(new) != len(ids):
+                raise ValueError("one number of new tokens for each request, and as many tokens in all")
+            if min(new, default=1) < 1:
+                raise ValueError("a sequence brings at least one token")
+            if len(set(requests)) < len(requests) or not all(0 <= r < cache.requests for r in requests):
+                raise ValueError(f"requests are different numbers below {cache.requests}")
+            max_new = max(new, default=0)
+            new, requests = (torch.tensor(t, dtype=torch.int32).to(device) for t in (new, requests))
+        ids = torch.as_tensor(ids, device=device)
+        if ids.dim() != 1 or new.dim() != 1 or new.shape != requests.shape or not len(ids):
+            raise ValueError("ids must be (N,) with a token at least, new and requests (B,)")
+        return self._packed(ids, requests, new, cache, len(ids) if max_new is None else max_new, all_logits)[0]
+
+    def _packed(self, ids, requests, new, cache: PagedCache, max_new: int, all_logits: bool):
+        """(logits, plan) of a step."""
+        N = ids.shape[0]
+        plan = cache.plan(requests, new, N)
+        step = PackedStep(cache, plan, max_new)
+        x = self.embed(ids[None]).to(self.dtype).reshape(1, N, -1).contiguous()
+        delta = None
+        for layer in self.layers:
+            x, delta = layer(x, delta, step)
+        h = add_rms_norm(x, delta, self.norm_w, self.args.rms_norm_eps)
+        if not all_logits:
+            first, end = plan.cu[:-1], plan.cu[1:]
+            at = (end - 1).clamp(min=0).long()
+            h = h[:, at].masked_fill((end <= first)[None, :, None], float("nan"))
+        logits = self.lm_head(h)[0]
+        logits = logits.masked_fill((plan.slots if all_logits else plan.rows)[:, None] < 0, float("nan"))
+        cache.advance(plan)
+        return logits, plan
 
     def forward(self, ids, cache: Qwen35Cache):
         S = ids.shape[1]
