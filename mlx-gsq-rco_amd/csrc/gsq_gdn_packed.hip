@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(256) gdn_conv_packed_kernel(GdnPackedArgs a, b
 // The recurrence of one (sequence, value head), its state in registers from the first token to the last: a thread
 // holds 4 columns of every NG-th row. Per token two sums over the rows, across the workgroup.
 template <bool BF, int DK, int DV>
-__global__ void __launch_bounds__(256) gdn_rec_packed_kernel(GdnPackedArgs a) {
+__global__ void __launch_bounds__(256) gdn_rec_packed_kernel(GdnPackedArgs a, int long_from) {
   using E = Half<BF>;
   constexpr int CG = DV / 4, NG = 256 / CG, NR = DK / NG;  // threads of a row, row groups, rows of a thread
   __shared__ __attribute__((aligned(16))) float red[2][4][DV];
@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(256) gdn_rec_packed_kernel(GdnPackedArgs a) {
     fill(a.cu[b], a.cu[b + 1], E::mk(__builtin_nanf("")));
     return;
   }
-  if (sq.n == 0) return;
+  if (sq.n == 0 || sq.n >= long_from) return;
   float* const Sp = a.rec + (((int64_t)sq.row * a.Hv + h) * DK + rg) * DV + col;
   f32x4 st[NR];
 #pragma unroll
@@ -204,7 +204,373 @@ __global__ void __launch_bounds__(256) gdn_rec_packed_kernel(GdnPackedArgs a) {
   for (int i = 0; i < NR; ++i) *reinterpret_cast<f32x4*>(Sp + (int64_t)i * NG * DV) = st[i];
 }
 
-int64_t gdn_packed_work(const GdnPackedArgs& a) { return (int64_t)a.N * (2 * a.Hk * a.dk + a.Hv * a.dv); }
+// ---- long sequences: chunks of 64 tokens ----------------------------------------------------------
+// With G the running sum of a chunk's logarithms of decays, S the state before it, and row vectors q_t, k_t, v_t:
+//   u_t = beta_t (v_t - e^(G_t) k_t S - sum_(s<t) e^(G_t - G_s) (k_t . k_s) u_s)          u = T r, T = (1 + M)^-1
+//   o_t = e^(G_t) q_t S + sum_(s<=t) e^(G_t - G_s) (q_t . k_s) u_s                        o = e^G (q S) + P u
+//   S' = e^(G_C) S + sum_s e^(G_C - G_s) k_s^T u_s
+// T and P depend on no state: gdn_chunk_kernel forms them for all chunks at once. What is left is a chain of products
+// over the chunks (gdn_scan_kernel), split over the state's columns, which do not meet. All products are float32 matrix
+// instructions; G is summed in float64, as e^(G_t - G_s) would lose bits behind tokens that forget nearly everything, and a
+// token's logarithm is at least -1000.
+//
+// Matrix instruction j of four takes element j of 16-byte pieces: lane (g, c) = (lane / 16, lane % 16) holds A[c][4 g + j] and
+// B[4 g + j][c], and C[4 g + r][c] in register r, so that a product's result is the next one's B operand as it lies.
+constexpr int kChunk = 64;
+
+__device__ __forceinline__ f32x4 mma4(f32x4 a, f32x4 b, f32x4 c) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+  return c;
+}
+
+// lane t: token t of a chunk of n
+struct ChunkGate {
+  float beta;
+  double sum;  // G
+  __device__ ChunkGate(const uint16_t* ab, int64_t stride, int n, int h, int Hv, float dtb, float sa, bool bf) {
+    const int lane = threadIdx.x & 63;
+    const uint16_t* const p = ab + (int64_t)min(lane, n - 1) * stride;
+    const float av = (bf ? Half<true>::ld(p[h]) : Half<false>::ld(p[h])) + dtb;
+    const float bv = bf ? Half<true>::ld(p[Hv + h]) : Half<false>::ld(p[Hv + h]);
+    const float sp = av > 20.f ? av : log1pf(expf(av));  // softplus (torch's threshold 20)
+    const float g = sa * sp;
+    beta = lane < n ? 1.f / (1.f + expf(-bv)) : 0.f;
+    sum = lane < n ? (g < -1000.f ? -1000.0 : (double)g) : 0.0;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const double u = __shfl_up(sum, o, 64);
+      if (lane >= o) sum += u;
+    }
+  }
+};
+
+// The chunk that slot i of the workspaces belongs to: those of sequence b begin at slot (cu[b] / 64) + b.
+struct ChunkAt {
+  int b, c;
+  __device__ ChunkAt(const GdnPackedArgs& a, int slot) {
+    const int lane = threadIdx.x & 63;
+    int n = 0;
+    for (int i = lane; i - lane < a.B; i += 64) n += __popcll(__ballot(i < a.B && (max(a.cu[min(i, a.B - 1)], 0) >> 6) + i <= slot));
+    b = __builtin_amdgcn_readfirstlane(n) - 1;
+    c = b < 0 ? 0 : slot - ((max(a.cu[b], 0) >> 6) + b);
+  }
+};
+
+// T and P of one chunk, for the value heads of one key head. The ten 16 x 16 blocks of the lower triangles of k k^T and q k^T
+// are shared out over the waves; T by blocks: forward substitution in the diagonal ones, then T_ij = -T_ii (sum over
+// i > l >= j of M_il T_lj), three levels of them.
+template <bool BF, int DK>
+__global__ void __launch_bounds__(256) gdn_chunk_kernel(GdnPackedArgs a, float* tp, int long_from) {
+  constexpr int LD = kChunk + 4;
+  __shared__ __attribute__((aligned(16))) float M[kChunk * LD], T[kChunk * LD], beta_s[kChunk];
+  __shared__ double sum_s[kChunk];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
+  const ChunkAt at(a, blockIdx.x);
+  if (at.b < 0 || at.c < 0) return;
+  const PackedSeq sq(a.cu, a.rows, a.lens, at.b, a.N, a.R, 0x7FFFFFFF);
+  if (!sq.fine || sq.n < long_from || at.c * kChunk >= sq.n) return;
+  const int n = min(kChunk, sq.n - at.c * kChunk), kh = blockIdx.y, key_dim = a.Hk * DK, conv_dim = 2 * key_dim + a.Hv * a.dv;
+  const int64_t t0 = sq.t0 + at.c * kChunk;
+  // block (bi, bj) p of this wave: (3,0) (3,1) (3,2) | (3,3) (2,0) (2,1) | (2,2) (1,0) | (1,1) (0,0)
+  constexpr int BI[4][3] = {{3, 3, 3}, {3, 2, 2}, {2, 1, -1}, {1, 0, -1}}, BJ[4][3] = {{0, 1, 2}, {3, 0, 1}, {2, 0, -1}, {1, 0, -1}};
+  int bi[3], bj[3];
+  f32x4 kk[3], qk[3];
+#pragma unroll
+  for (int p = 0; p < 3; ++p) {
+    bi[p] = wave == 0 ? BI[0][p] : wave == 1 ? BI[1][p] : wave == 2 ? BI[2][p] : BI[3][p];
+    bj[p] = wave == 0 ? BJ[0][p] : wave == 1 ? BJ[1][p] : wave == 2 ? BJ[2][p] : BJ[3][p];
+    kk[p] = qk[p] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    if (bi[p] < 0) continue;
+    const float* const qi = a.work + (t0 + min(16 * bi[p] + c, n - 1)) * conv_dim + kh * DK + 4 * g;
+    const float* const kj = a.work + (t0 + min(16 * bj[p] + c, n - 1)) * conv_dim + key_dim + kh * DK + 4 * g;
+#pragma unroll
+    for (int s = 0; s < DK / 16; ++s) {
+      const f32x4 b = *reinterpret_cast<const f32x4*>(kj + 16 * s);
+      qk[p] = mma4(*reinterpret_cast<const f32x4*>(qi + 16 * s), b, qk[p]);
+      kk[p] = mma4(*reinterpret_cast<const f32x4*>(qi + key_dim + 16 * s), b, kk[p]);
+    }
+  }
+  for (int h = kh; h < a.Hv; h += a.Hk) {
+    if (wave == 0) {
+      const ChunkGate gate(static_cast<const uint16_t*>(a.ab) + t0 * a.ab_stride, a.ab_stride, n, h, a.Hv, a.dt_bias[h], a.ssm_a[h], BF);
+      beta_s[lane] = gate.beta;
+      sum_s[lane] = gate.sum;
+    }
+    __syncthreads();
+    float* const Tg = tp + ((int64_t)blockIdx.x * a.Hv + h) * 2 * kChunk * kChunk;
+    float* const Pg = Tg + kChunk * kChunk;
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      if (bi[p] < 0) continue;
+      const int s = 16 * bj[p] + c;
+      const double gs = sum_s[s];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int t = 16 * bi[p] + 4 * g + r;
+        const float ratio = s <= t ? expf((float)(sum_s[t] - gs)) : 0.f;
+        M[t * LD + s] = s < t ? beta_s[t] * ratio * kk[p][r] : 0.f;
+        Pg[t * kChunk + s] = s <= t ? ratio * qk[p][r] : 0.f;
+      }
+    }
+    __syncthreads();
+    {  // column c of the inverse of diagonal block `wave`, in every lane group
+      const float* const D = M + 16 * wave * LD + 16 * wave;
+      float x[16];
+#pragma unroll
+      for (int t = 0; t < 16; ++t) {
+        float v = t == c ? 1.f : 0.f;
+#pragma unroll
+        for (int s = 0; s < t; ++s) v -= D[t * LD + s] * x[s];
+        x[t] = v;
+      }
+#pragma unroll
+      for (int t = 0; t < 16; ++t)
+        if ((t >> 2) == g) T[(16 * wave + t) * LD + 16 * wave + c] = x[t];
+    }
+#pragma unroll
+    for (int level = 1; level < 4; ++level) {
+      __syncthreads();
+      const int i = level + wave, j = wave;  // block (i, j)
+      if (i < 4) {
+        f32x4 y = {0.f, 0.f, 0.f, 0.f};
+        for (int l = j; l < i; ++l) {
+          f32x4 b;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) b[r] = T[(16 * l + 4 * g + r) * LD + 16 * j + c];
+          y = mma4(*reinterpret_cast<const f32x4*>(M + (16 * i + c) * LD + 16 * l + 4 * g), b, y);
+        }
+        const f32x4 z = mma4(*reinterpret_cast<const f32x4*>(T + (16 * i + c) * LD + 16 * i + 4 * g), y, (f32x4){0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+        for (int r = 0; r < 4; ++r) T[(16 * i + 4 * g + r) * LD + 16 * j + c] = -z[r];
+      }
+    }
+    __syncthreads();
+    for (int i = tid; i < kChunk * kChunk / 4; i += 256) {
+      const int t = i / 16, s = 4 * (i % 16);
+      if (s < (t | 15)) *reinterpret_cast<f32x4*>(Tg + t * kChunk + s) = *reinterpret_cast<const f32x4*>(T + t * LD + s);
+    }
+    __syncthreads();
+  }
+}
+
+// The chain over a sequence's chunks, for 32 columns of a value head's state: its tiles stay in registers (rows of wave w:
+// the blocks of 16 w, w + 4, ..), a copy in LDS is the products' operand. Wave w holds tokens 16 w .. of a chunk.
+constexpr int kScanCols = 32;
+
+template <bool BF, int DK>
+__global__ void __launch_bounds__(256) gdn_scan_kernel(GdnPackedArgs a, const float* tp, float* ow, int long_from) {
+  constexpr int LS = DK + 4, LT = kChunk + 4, NB = (DK / 16 + 3) / 4, CT = kScanCols / 16;
+  __shared__ __attribute__((aligned(16))) float Sl[kScanCols * LS], rl[kScanCols * LT], ul[kScanCols * LT];
+  __shared__ __attribute__((aligned(16))) float grown_s[2][kChunk], left_s[2][kChunk], beta_s[2][kChunk];
+  __shared__ int odd_s;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
+  const int ns = a.dv / kScanCols, h = blockIdx.x / ns, col0 = blockIdx.x % ns * kScanCols, kh = h % a.Hk, b = blockIdx.y;
+  const PackedSeq sq(a.cu, a.rows, a.lens, b, a.N, a.R, 0x7FFFFFFF);
+  if (!sq.fine || sq.n < long_from) return;
+  const int key_dim = a.Hk * DK, conv_dim = 2 * key_dim + a.Hv * a.dv, vdim = a.Hv * a.dv, n = sq.n;
+  const float* const wq = a.work + (int64_t)sq.t0 * conv_dim + kh * DK;
+  const float* const wk = wq + key_dim;
+  const float* const wv = a.work + (int64_t)sq.t0 * conv_dim + 2 * key_dim + h * a.dv + col0;
+  float* const o_at = ow + (int64_t)sq.t0 * vdim + h * a.dv + col0;
+  const uint16_t* const ab = static_cast<const uint16_t*>(a.ab) + (int64_t)sq.t0 * a.ab_stride;
+  const float* tg = tp + ((int64_t)((sq.t0 >> 6) + b) * a.Hv + h) * 2 * kChunk * kChunk;
+  float* const Sg = a.rec + (((int64_t)sq.row * a.Hv + h) * DK) * a.dv + col0;
+  const bool fresh = sq.len == n;
+  if (tid == 0) odd_s = 0;
+  auto gates = [&](int t0, int buf) {  // one wave
+    const ChunkGate x(ab + (int64_t)t0 * a.ab_stride, a.ab_stride, min(kChunk, n - t0), h, a.Hv, a.dt_bias[h], a.ssm_a[h], BF);
+    grown_s[buf][lane] = expf((float)x.sum);
+    left_s[buf][lane] = expf((float)(__shfl(x.sum, 63, 64) - x.sum));
+    beta_s[buf][lane] = x.beta;
+  };
+  f32x4 st[NB][CT];
+#pragma unroll
+  for (int i = 0; i < NB; ++i)
+#pragma unroll
+    for (int t = 0; t < CT; ++t) {
+      const int row = 16 * (wave + 4 * i);
+      st[i][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      if (row >= DK) continue;
+      if (!fresh)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) st[i][t][r] = Sg[(int64_t)(row + 4 * g + r) * a.dv + 16 * t + c];
+      *reinterpret_cast<f32x4*>(Sl + (16 * t + c) * LS + row + 4 * g) = st[i][t];
+    }
+  if (wave == 0) gates(0, 0);
+  bool odd = false;
+  int buf = 0;
+  __syncthreads();
+  for (int t0 = 0; t0 < n; t0 += kChunk, buf ^= 1, tg += (int64_t)a.Hv * 2 * kChunk * kChunk) {
+    const int m = min(kChunk, n - t0), row = t0 + min(16 * wave + c, m - 1);  // tokens behind the last repeat it
+    f32x4 qs[CT], ks[CT];
+#pragma unroll
+    for (int t = 0; t < CT; ++t) qs[t] = ks[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < DK / 16; ++s) {
+      const f32x4 q = *reinterpret_cast<const f32x4*>(wq + (int64_t)row * conv_dim + 16 * s + 4 * g);
+      const f32x4 k = *reinterpret_cast<const f32x4*>(wk + (int64_t)row * conv_dim + 16 * s + 4 * g);
+#pragma unroll
+      for (int t = 0; t < CT; ++t) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(Sl + (16 * t + c) * LS + 16 * s + 4 * g);
+        ks[t] = mma4(k, x, ks[t]);
+        qs[t] = mma4(q, x, qs[t]);
+      }
+    }
+    const f32x4 grown = *reinterpret_cast<const f32x4*>(&grown_s[buf][16 * wave + 4 * g]);
+    const f32x4 beta = *reinterpret_cast<const f32x4*>(&beta_s[buf][16 * wave + 4 * g]);
+#pragma unroll
+    for (int t = 0; t < CT; ++t) {
+      f32x4 r4;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float v = wv[(int64_t)(t0 + min(16 * wave + 4 * g + r, m - 1)) * conv_dim + 16 * t + c];
+        r4[r] = beta[r] * (v - grown[r] * ks[t][r]);
+      }
+      *reinterpret_cast<f32x4*>(rl + (16 * t + c) * LT + 16 * wave + 4 * g) = r4;
+    }
+    __syncthreads();
+    f32x4 u[CT];
+#pragma unroll
+    for (int t = 0; t < CT; ++t) u[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    for (int l = 0; l <= wave; ++l) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(tg + (16 * wave + c) * kChunk + 16 * l + 4 * g);
+#pragma unroll
+      for (int t = 0; t < CT; ++t) u[t] = mma4(x, *reinterpret_cast<const f32x4*>(rl + (16 * t + c) * LT + 16 * l + 4 * g), u[t]);
+    }
+#pragma unroll
+    for (int t = 0; t < CT; ++t) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) odd |= !(fabsf(u[t][r]) <= 3.4028235e38f);
+      *reinterpret_cast<f32x4*>(ul + (16 * t + c) * LT + 16 * wave + 4 * g) = u[t];
+    }
+    if (wave == 0 && t0 + kChunk < n) gates(t0 + kChunk, buf ^ 1);
+    __syncthreads();
+    f32x4 o[CT];
+#pragma unroll
+    for (int t = 0; t < CT; ++t) o[t] = qs[t] * grown;
+    for (int l = 0; l <= wave; ++l) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(tg + kChunk * kChunk + (16 * wave + c) * kChunk + 16 * l + 4 * g);
+#pragma unroll
+      for (int t = 0; t < CT; ++t) o[t] = mma4(x, *reinterpret_cast<const f32x4*>(ul + (16 * t + c) * LT + 16 * l + 4 * g), o[t]);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (16 * wave + 4 * g + r < m)
+#pragma unroll
+        for (int t = 0; t < CT; ++t) o_at[(int64_t)(t0 + 16 * wave + 4 * g + r) * vdim + 16 * t + c] = o[t][r];
+    const float all = grown_s[buf][kChunk - 1];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const int row0 = 16 * (wave + 4 * i);
+      if (row0 >= DK) continue;
+#pragma unroll
+      for (int t = 0; t < CT; ++t) st[i][t] *= all;
+#pragma unroll
+      for (int l = 0; l < 4; ++l) {
+        f32x4 x;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = wk[(int64_t)(t0 + min(16 * l + 4 * g + r, m - 1)) * conv_dim + row0 + c];
+        const f32x4 left = *reinterpret_cast<const f32x4*>(&left_s[buf][16 * l + 4 * g]);
+#pragma unroll
+        for (int t = 0; t < CT; ++t) st[i][t] = mma4(x, *reinterpret_cast<const f32x4*>(ul + (16 * t + c) * LT + 16 * l + 4 * g) * left, st[i][t]);
+      }
+#pragma unroll
+      for (int t = 0; t < CT; ++t) *reinterpret_cast<f32x4*>(Sl + (16 * t + c) * LS + row0 + 4 * g) = st[i][t];
+    }
+    __syncthreads();
+  }
+  if (odd) odd_s = 1;
+  __syncthreads();
+  if (!odd_s) {
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int t = 0; t < CT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (16 * (wave + 4 * i) < DK) Sg[(int64_t)(16 * (wave + 4 * i) + 4 * g + r) * a.dv + 16 * t + c] = st[i][t][r];
+    return;
+  }
+  // A value that is not finite has reached tokens before its own through the products: once more, token by token. Thread
+  // (x, y) = (tid / 32, tid % 32) holds rows x, x + 8, .. of column y.
+  {
+    constexpr int NR = DK / 8;
+    const int x = tid >> 5, y = tid & 31;
+    float s[NR];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) s[i] = fresh ? 0.f : Sg[(int64_t)(x + 8 * i) * a.dv + y];
+    auto total = [&](float v) {  // over x
+      __syncthreads();
+      rl[x * 32 + y] = v;
+      __syncthreads();
+      float r = 0.f;
+      for (int i = 0; i < 8; ++i) r += rl[i * 32 + y];
+      return r;
+    };
+    for (int t = 0; t < n; ++t) {
+      const float av = Half<BF>::ld(ab[(int64_t)t * a.ab_stride + h]) + a.dt_bias[h], bv = Half<BF>::ld(ab[(int64_t)t * a.ab_stride + a.Hv + h]);
+      const float sp = av > 20.f ? av : log1pf(expf(av)), decay = expf(a.ssm_a[h] * sp), beta = 1.f / (1.f + expf(-bv));
+      float p = 0.f;
+#pragma unroll
+      for (int i = 0; i < NR; ++i) {
+        s[i] *= decay;
+        p += s[i] * wk[(int64_t)t * conv_dim + x + 8 * i];
+      }
+      const float d = (wv[(int64_t)t * conv_dim + y] - total(p)) * beta;
+      p = 0.f;
+#pragma unroll
+      for (int i = 0; i < NR; ++i) {
+        s[i] += d * wk[(int64_t)t * conv_dim + x + 8 * i];
+        p += s[i] * wq[(int64_t)t * conv_dim + x + 8 * i];
+      }
+      const float o = total(p);
+      if (x == 0) o_at[(int64_t)t * vdim + y] = o;
+    }
+#pragma unroll
+    for (int i = 0; i < NR; ++i) Sg[(int64_t)(x + 8 * i) * a.dv + y] = s[i];
+  }
+}
+
+// Gated RMSNorm of the long sequences' outputs: a wave per (token, head).
+template <bool BF>
+__global__ void __launch_bounds__(256) gdn_out_packed_kernel(GdnPackedArgs a, const float* ow, int long_from) {
+  using E = Half<BF>;
+  const int lane = threadIdx.x & 63, nj = a.dv >> 6;
+  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (i >= (int64_t)a.N * a.Hv) return;
+  const int t = (int)(i / a.Hv), h = (int)(i - (int64_t)t * a.Hv), b = seq_of(a.cu, a.B, t);
+  if (b >= a.B) return;
+  const PackedSeq sq(a.cu, a.rows, a.lens, b, a.N, a.R, 0x7FFFFFFF);
+  if (!sq.fine || sq.n < long_from || t < sq.t0 || t - sq.t0 >= sq.n) return;
+  const float* const o = ow + i * a.dv + lane;
+  const uint16_t* const z = static_cast<const uint16_t*>(a.z) + (int64_t)t * a.z_stride + h * a.dv + lane;
+  const uint16_t* const w = static_cast<const uint16_t*>(a.norm_w) + lane;
+  float ov[4], zv[4], wv[4], ss = 0.f;  // dv <= 256
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    ov[j] = j < nj ? o[64 * j] : 0.f;
+    zv[j] = j < nj ? E::ld(z[64 * j]) : 0.f;
+    wv[j] = j < nj ? E::ld(w[64 * j]) : 0.f;
+    ss += ov[j] * ov[j];
+  }
+  const float rn = 1.f / sqrtf(lanes_sum(ss) / (float)a.dv + a.eps);
+  uint16_t* const out = static_cast<uint16_t*>(a.out) + (int64_t)t * a.out_stride + h * a.dv + lane;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (j < nj) out[64 * j] = E::mk(ov[j] * rn * wv[j] * silu_f(zv[j]));
+}
+
+// Sequences from kLongFrom tokens on go by chunks.
+constexpr int kLongFrom = 24;
+
+static int64_t gdn_slots(const GdnPackedArgs& a) { return (int64_t)(a.N >> 6) + a.B + 1; }
+
+// convolution outputs; if there may be long sequences, T and P of their chunks and the recurrence's outputs
+int64_t gdn_packed_work(const GdnPackedArgs& a) {
+  const int64_t rows = (int64_t)a.N * (2 * a.Hk * a.dk + a.Hv * a.dv);
+  return a.max_new < kLongFrom ? rows : rows + gdn_slots(a) * a.Hv * 2 * kChunk * kChunk + (int64_t)a.N * a.Hv * a.dv;
+}
 
 template <bool BF>
 static hipError_t launch_gdn_packed_t(const GdnPackedArgs& a, hipStream_t s) {
@@ -212,8 +578,18 @@ static hipError_t launch_gdn_packed_t(const GdnPackedArgs& a, hipStream_t s) {
   const bool pair = ((a.qkv_stride & 1) | (reinterpret_cast<uintptr_t>(a.qkv) & 3)) == 0;
   const dim3 cgrid((unsigned)((conv_dim + 511) / 512), (unsigned)((a.N + 7) / 8)), rgrid((unsigned)a.Hv, (unsigned)a.B + 1);
   hipLaunchKernelGGL((gdn_conv_packed_kernel<BF, 8>), cgrid, dim3(256), 0, s, a, pair);
+  const bool chunks = a.max_new >= kLongFrom;
+  const int long_from = chunks ? kLongFrom : 0x7FFFFFFF;
   auto rec = [&](auto dk, auto dv) {
-    hipLaunchKernelGGL((gdn_rec_packed_kernel<BF, decltype(dk)::value, decltype(dv)::value>), rgrid, dim3(256), 0, s, a);
+    if (chunks) {
+      float* const tp = a.work + (int64_t)a.N * conv_dim;
+      float* const ow = tp + gdn_slots(a) * a.Hv * 2 * kChunk * kChunk;
+      hipLaunchKernelGGL((gdn_chunk_kernel<BF, decltype(dk)::value>), dim3((unsigned)gdn_slots(a), (unsigned)a.Hk), dim3(256), 0, s, a, tp, long_from);
+      hipLaunchKernelGGL((gdn_scan_kernel<BF, decltype(dk)::value>), dim3((unsigned)(a.Hv * (a.dv / kScanCols)), (unsigned)a.B), dim3(256), 0, s, a,
+                         (const float*)tp, ow, long_from);
+      hipLaunchKernelGGL(gdn_out_packed_kernel<BF>, dim3((unsigned)(((int64_t)a.N * a.Hv + 3) / 4)), dim3(256), 0, s, a, (const float*)ow, long_from);
+    }
+    hipLaunchKernelGGL((gdn_rec_packed_kernel<BF, decltype(dk)::value, decltype(dv)::value>), rgrid, dim3(256), 0, s, a, long_from);
     return hipGetLastError();
   };
   auto dims = [&](auto dk) -> hipError_t {

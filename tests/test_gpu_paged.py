@@ -411,6 +411,28 @@ def test_gdn_packed_pieces_of_a_prompt():
     assert float((torch.cat(outs).double() - whole[0].double()).norm() / whole[0].double().norm()) <= 2 * 2.0 ** -11
 
 
+@pytest.mark.parametrize("where", ["k", "v", "q", "decay"])
+def test_gdn_packed_values_that_are_not_finite(where):
+    """They reach their own token and what follows it in its request, as in the recurrence, and nothing else."""
+    case = ([0, 9, 3], [150, 70, 2], 1, 2, 64, 64, 4, F16)
+    t, plan = _gdn_inputs(case)
+    at = 100  # of the first sequence
+    if where == "decay":
+        t[2][at, 1] = -float("inf")  # softplus 0: nothing is forgotten
+        t[2][at + 30, 0] = float("inf")  # everything is
+    else:
+        t[0][at, {"q": 3, "k": 64 + 5, "v": 128 + 64 + 7}[where]] = float("nan") if where == "k" else float("inf")
+    out, conv, rec = _run_gdn(case, t, plan)
+    want, want_conv, want_rec, scale = R.gdn(*t, *plan[:3], 1, 2, 64, 64, 1e-6)
+    assert torch.equal(torch.isnan(out), torch.isnan(want)) and bool(torch.isfinite(out[:at]).all())
+    assert torch.equal(torch.isnan(rec), torch.isnan(want_rec))
+    assert bool(torch.isfinite(out[150:]).all()) and (where == "decay") == bool(torch.isfinite(out).all())
+    err, fine = (out.double() - want).abs(), torch.isfinite(want)
+    assert bool((err <= 2.0 ** -11 * want.abs() + 2.0 ** -9 * scale + 2.0 ** -25)[fine].all())
+    fine = torch.isfinite(want_rec)
+    assert float((rec.double() - want_rec)[fine].norm() / want_rec[fine].norm()) <= 2e-6
+
+
 def test_gdn_packed_begins_from_zeros():
     """A request's first tokens do not see what its states held."""
     case = ([0, 5], [70, 3], 1, 2, 128, 128, 4, BF16)
