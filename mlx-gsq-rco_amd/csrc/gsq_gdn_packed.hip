@@ -13,29 +13,30 @@ namespace gsq {
 
 constexpr int kConvMax = 8;  // inputs of a convolution window at most
 
-// Convolution + SiLU of 128 channels (2 per lane) over the packed tokens TPB blockIdx.y .. + TPB - 1, the window
-// sliding in registers from one token of a sequence to the next; q and k channels are RMS-normalized over their head
-// (dk / 2 lanes, a power of two) and scaled, so that `work` holds [q | k | v] rows ready for the recurrence. The thread
-// that meets a sequence's first token has read its state by then, and writes the new one.
-template <bool BF, int TPB>
+// Convolution + SiLU of 128 channels (2 per lane) over the packed tokens TPB blockIdx.y .. + TPB - 1, whose inputs are all
+// asked for at once; the window slides in registers from one token of a sequence to the next. q and k channels are
+// RMS-normalized over their head (dk / 2 lanes, a power of two) and scaled, so that `work` holds [q | k | v] rows ready
+// for the recurrence. The thread that meets a sequence's first token has read its state by then, and writes the new one.
+// KW: window of the convolution (kConvMax: any up to it).
+template <bool BF, int TPB, int KW>
 __global__ void __launch_bounds__(256) gdn_conv_packed_kernel(GdnPackedArgs a, bool pair) {
   using E = Half<BF>;
-  const int key_dim = a.Hk * a.dk, conv_dim = 2 * key_dim + a.Hv * a.dv, K = a.K;
+  const int key_dim = a.Hk * a.dk, conv_dim = 2 * key_dim + a.Hv * a.dv, K = KW < kConvMax ? KW : a.K;
   const int lane = threadIdx.x & 63, wave = blockIdx.x * 4 + (threadIdx.x >> 6);
   const int cc = wave * 128 + 2 * lane, c = min(cc, conv_dim - 2);  // conv_dim is even
   const bool on = cc < conv_dim;
   const uint16_t* const q = static_cast<const uint16_t*>(a.qkv) + c;
-  auto ld2 = [&](const uint16_t* p, float& x, float& y) {
-    const uint32_t w = pair ? *reinterpret_cast<const uint32_t*>(p) : (uint32_t)p[0] | ((uint32_t)p[1] << 16);
-    x = E::ld((uint16_t)w);
-    y = E::ld((uint16_t)(w >> 16));
-  };
-  // window and weights right-aligned: slot kConvMax - 1 is the current token
-  float w0[kConvMax], w1[kConvMax], in0[kConvMax], in1[kConvMax];
+  auto ld2 = [&](const uint16_t* p) { return pair ? *reinterpret_cast<const uint32_t*>(p) : (uint32_t)p[0] | ((uint32_t)p[1] << 16); };
+  const int half = a.dk >> 1, first = blockIdx.y * TPB;
+  uint32_t x[TPB];
+#pragma unroll
+  for (int i = 0; i < TPB; ++i) x[i] = ld2(q + (int64_t)min(first + i, a.N - 1) * a.qkv_stride);
+  // window and weights right-aligned: slot KW - 1 is the current token
+  float w0[KW], w1[KW], in0[KW], in1[KW];
   const uint16_t* const cw = static_cast<const uint16_t*>(a.conv_w) + (int64_t)c * K;
 #pragma unroll
-  for (int i = 0; i < kConvMax; ++i) {
-    const int j = i - (kConvMax - K);
+  for (int i = 0; i < KW; ++i) {
+    const int j = i - (KW - K);
     w0[i] = w1[i] = in0[i] = in1[i] = 0.f;
     if (j >= 0) {
       w0[i] = E::ld(cw[j]);
@@ -43,7 +44,6 @@ __global__ void __launch_bounds__(256) gdn_conv_packed_kernel(GdnPackedArgs a, b
     }
   }
   const float sc = c < key_dim ? 1.f / (float)a.dk : 1.f / sqrtf((float)a.dk);
-  const int half = a.dk >> 1, first = blockIdx.y * TPB;
   int b = -1, t0 = 0, end = 0;  // the sequence of the token before
   bool fine = false;
 #pragma unroll
@@ -59,59 +59,64 @@ __global__ void __launch_bounds__(256) gdn_conv_packed_kernel(GdnPackedArgs a, b
       fine = sq.fine && t >= t0 && t < end;
       if (!fine) end = t + 1;
       const bool fresh = sq.len == sq.n;
-      uint16_t* const cst = static_cast<uint16_t*>(a.conv) + (int64_t)(fine ? sq.row : 0) * (K - 1) * conv_dim + c;
+      uint16_t* const cst = static_cast<uint16_t*>(a.conv) + (int64_t)(fine ? sq.row : 0) * (K - 1) * conv_dim + c;  // conv_dim is even
+      uint32_t old[KW];  // the window of token t - 1, oldest first; slot KW - K is shifted out
 #pragma unroll
-      for (int s = 0; s < kConvMax; ++s) {
-        const int j = s - (kConvMax - K);  // the window of token t - 1, oldest 0
-        in0[s] = in1[s] = 0.f;
-        if (j < 0 || !fine) continue;
-        const int u = t - t0 - K + j;
-        if (u >= 0) ld2(q + (int64_t)(t0 + u) * a.qkv_stride, in0[s], in1[s]);
-        else if (u >= -(K - 1) && !fresh) {
-          in0[s] = E::ld(cst[(int64_t)(K - 1 + u) * conv_dim]);
-          in1[s] = E::ld(cst[(int64_t)(K - 1 + u) * conv_dim + 1]);
-        }
+      for (int s = 0; s < KW; ++s) {
+        const int j = s - (KW - K), u = t - t0 - K + j;
+        old[s] = 0;
+        if (j < 1 || !fine) continue;
+        if (u >= 0) old[s] = ld2(q + (int64_t)(t0 + u) * a.qkv_stride);
+        else if (!fresh) old[s] = (uint32_t)cst[(int64_t)(K - 1 + u) * conv_dim] | ((uint32_t)cst[(int64_t)(K - 1 + u) * conv_dim + 1] << 16);
+      }
+#pragma unroll
+      for (int s = 0; s < KW; ++s) {
+        in0[s] = E::ld((uint16_t)old[s]);
+        in1[s] = E::ld((uint16_t)(old[s] >> 16));
       }
       if (fine && on && t == t0) {  // slots ascending: a shift in place reads before it writes
         for (int j = 0; j < K - 1; ++j) {
           const int u = sq.n - (K - 1) + j;
-          uint16_t x = 0, y = 0;
+          uint16_t y0 = 0, y1 = 0;
           if (u >= 0) {
-            x = q[(int64_t)(t0 + u) * a.qkv_stride];
-            y = q[(int64_t)(t0 + u) * a.qkv_stride + 1];
+            y0 = q[(int64_t)(t0 + u) * a.qkv_stride];
+            y1 = q[(int64_t)(t0 + u) * a.qkv_stride + 1];
           } else if (!fresh) {
-            x = cst[(int64_t)(K - 1 + u) * conv_dim];
-            y = cst[(int64_t)(K - 1 + u) * conv_dim + 1];
+            y0 = cst[(int64_t)(K - 1 + u) * conv_dim];
+            y1 = cst[(int64_t)(K - 1 + u) * conv_dim + 1];
           }
-          cst[(int64_t)j * conv_dim] = x;
-          cst[(int64_t)j * conv_dim + 1] = y;
+          cst[(int64_t)j * conv_dim] = y0;
+          cst[(int64_t)j * conv_dim + 1] = y1;
         }
       }
     }
     if (!fine) continue;
 #pragma unroll
-    for (int s = 0; s + 1 < kConvMax; ++s) {
+    for (int s = 0; s + 1 < KW; ++s) {
       in0[s] = in0[s + 1];
       in1[s] = in1[s + 1];
     }
-    ld2(q + (int64_t)t * a.qkv_stride, in0[kConvMax - 1], in1[kConvMax - 1]);
-    float x = 0.f, y = 0.f;
+    in0[KW - 1] = E::ld((uint16_t)x[i]);
+    in1[KW - 1] = E::ld((uint16_t)(x[i] >> 16));
+    float y0 = 0.f, y1 = 0.f;
 #pragma unroll
-    for (int s = 0; s < kConvMax; ++s)
-      if (s >= kConvMax - K) {
-        x += in0[s] * w0[s];
-        y += in1[s] * w1[s];
-      }
-    x = silu_f(x);
-    y = silu_f(y);
-    float ss = x * x + y * y;
-    for (int o = 1; o < half; o <<= 1) ss += __shfl_xor(ss, o, 64);
-    if (c < 2 * key_dim) {
-      const float rn = 1.f / sqrtf(ss / (float)a.dk + 1e-6f);
-      x = x * rn * sc;
-      y = y * rn * sc;
+    for (int s = 0; s < KW; ++s) {
+      if (KW == kConvMax && s < KW - K) continue;  // weights of 0 times anything
+      y0 += in0[s] * w0[s];
+      y1 += in1[s] * w1[s];
     }
-    if (on) *reinterpret_cast<float2*>(a.work + (int64_t)t * conv_dim + c) = make_float2(x, y);
+    y0 *= sigmoid_raw(y0);
+    y1 *= sigmoid_raw(y1);
+    if (wave * 128 < 2 * key_dim) {  // a wave with q or k channels
+      float ss = y0 * y0 + y1 * y1;
+      for (int o = 1; o < half; o <<= 1) ss += __shfl_xor(ss, o, 64);
+      if (c < 2 * key_dim) {
+        const float rn = 1.f / sqrtf(ss / (float)a.dk + 1e-6f);
+        y0 = y0 * rn * sc;
+        y1 = y1 * rn * sc;
+      }
+    }
+    if (on) *reinterpret_cast<float2*>(a.work + (int64_t)t * conv_dim + c) = make_float2(y0, y1);
   }
 }
 
@@ -359,7 +364,7 @@ __global__ void __launch_bounds__(256) gdn_chunk_kernel(GdnPackedArgs a, float* 
 constexpr int kScanCols = 32;
 
 template <bool BF, int DK>
-__global__ void __launch_bounds__(256) gdn_scan_kernel(GdnPackedArgs a, const float* tp, float* ow, int long_from) {
+__global__ void __launch_bounds__(256, 2) gdn_scan_kernel(GdnPackedArgs a, const float* tp, float* ow, int long_from) {
   constexpr int LS = DK + 4, LT = kChunk + 4, NB = (DK / 16 + 3) / 4, CT = kScanCols / 16;
   __shared__ __attribute__((aligned(16))) float Sl[kScanCols * LS], rl[kScanCols * LT], ul[kScanCols * LT];
   __shared__ __attribute__((aligned(16))) float grown_s[2][kChunk], left_s[2][kChunk], beta_s[2][kChunk];
@@ -398,45 +403,68 @@ __global__ void __launch_bounds__(256) gdn_scan_kernel(GdnPackedArgs a, const fl
       *reinterpret_cast<f32x4*>(Sl + (16 * t + c) * LS + row + 4 * g) = st[i][t];
     }
   if (wave == 0) gates(0, 0);
+  // what a chunk reads from memory is asked for a phase or more before it is used: q and k rows a chunk ahead, T, P, v and
+  // the transposed k at its beginning
+  constexpr int KQ = DK / 16;
+  f32x4 q4[KQ], k4[KQ];
+  auto load_qk = [&](int t0) {
+    const int64_t row = t0 + min(16 * wave + c, min(kChunk, n - t0) - 1);  // tokens behind the last repeat it
+#pragma unroll
+    for (int s = 0; s < KQ; ++s) {
+      q4[s] = *reinterpret_cast<const f32x4*>(wq + row * conv_dim + 16 * s + 4 * g);
+      k4[s] = *reinterpret_cast<const f32x4*>(wk + row * conv_dim + 16 * s + 4 * g);
+    }
+  };
   bool odd = false;
   int buf = 0;
+  load_qk(0);
   __syncthreads();
   for (int t0 = 0; t0 < n; t0 += kChunk, buf ^= 1, tg += (int64_t)a.Hv * 2 * kChunk * kChunk) {
-    const int m = min(kChunk, n - t0), row = t0 + min(16 * wave + c, m - 1);  // tokens behind the last repeat it
+    const int m = min(kChunk, n - t0);
+    f32x4 v4[CT], t4[4], p4[4], kt[NB][4];
+#pragma unroll
+    for (int t = 0; t < CT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v4[t][r] = wv[(int64_t)(t0 + min(16 * wave + 4 * g + r, m - 1)) * conv_dim + 16 * t + c];
+#pragma unroll
+    for (int l = 0; l < 4; ++l) {
+      if (l > wave) break;
+      t4[l] = *reinterpret_cast<const f32x4*>(tg + (16 * wave + c) * kChunk + 16 * l + 4 * g);
+      p4[l] = *reinterpret_cast<const f32x4*>(tg + kChunk * kChunk + (16 * wave + c) * kChunk + 16 * l + 4 * g);
+    }
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int l = 0; l < 4; ++l)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          kt[i][l][r] = wk[(int64_t)(t0 + min(16 * l + 4 * g + r, m - 1)) * conv_dim + min(16 * (wave + 4 * i), DK - 16) + c];
     f32x4 qs[CT], ks[CT];
 #pragma unroll
     for (int t = 0; t < CT; ++t) qs[t] = ks[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int s = 0; s < DK / 16; ++s) {
-      const f32x4 q = *reinterpret_cast<const f32x4*>(wq + (int64_t)row * conv_dim + 16 * s + 4 * g);
-      const f32x4 k = *reinterpret_cast<const f32x4*>(wk + (int64_t)row * conv_dim + 16 * s + 4 * g);
+    for (int s = 0; s < KQ; ++s)
 #pragma unroll
       for (int t = 0; t < CT; ++t) {
         const f32x4 x = *reinterpret_cast<const f32x4*>(Sl + (16 * t + c) * LS + 16 * s + 4 * g);
-        ks[t] = mma4(k, x, ks[t]);
-        qs[t] = mma4(q, x, qs[t]);
+        ks[t] = mma4(k4[s], x, ks[t]);
+        qs[t] = mma4(q4[s], x, qs[t]);
       }
-    }
+    if (t0 + kChunk < n) load_qk(t0 + kChunk);
     const f32x4 grown = *reinterpret_cast<const f32x4*>(&grown_s[buf][16 * wave + 4 * g]);
     const f32x4 beta = *reinterpret_cast<const f32x4*>(&beta_s[buf][16 * wave + 4 * g]);
 #pragma unroll
-    for (int t = 0; t < CT; ++t) {
-      f32x4 r4;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float v = wv[(int64_t)(t0 + min(16 * wave + 4 * g + r, m - 1)) * conv_dim + 16 * t + c];
-        r4[r] = beta[r] * (v - grown[r] * ks[t][r]);
-      }
-      *reinterpret_cast<f32x4*>(rl + (16 * t + c) * LT + 16 * wave + 4 * g) = r4;
-    }
-    __syncthreads();
+    for (int t = 0; t < CT; ++t)
+      *reinterpret_cast<f32x4*>(rl + (16 * t + c) * LT + 16 * wave + 4 * g) = beta * (v4[t] - grown * ks[t]);
+    lds_sync();
     f32x4 u[CT];
 #pragma unroll
     for (int t = 0; t < CT; ++t) u[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    for (int l = 0; l <= wave; ++l) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(tg + (16 * wave + c) * kChunk + 16 * l + 4 * g);
 #pragma unroll
-      for (int t = 0; t < CT; ++t) u[t] = mma4(x, *reinterpret_cast<const f32x4*>(rl + (16 * t + c) * LT + 16 * l + 4 * g), u[t]);
+    for (int l = 0; l < 4; ++l) {
+      if (l > wave) break;
+#pragma unroll
+      for (int t = 0; t < CT; ++t) u[t] = mma4(t4[l], *reinterpret_cast<const f32x4*>(rl + (16 * t + c) * LT + 16 * l + 4 * g), u[t]);
     }
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
@@ -444,15 +472,16 @@ __global__ void __launch_bounds__(256) gdn_scan_kernel(GdnPackedArgs a, const fl
       for (int r = 0; r < 4; ++r) odd |= !(fabsf(u[t][r]) <= 3.4028235e38f);
       *reinterpret_cast<f32x4*>(ul + (16 * t + c) * LT + 16 * wave + 4 * g) = u[t];
     }
-    if (wave == 0 && t0 + kChunk < n) gates(t0 + kChunk, buf ^ 1);
-    __syncthreads();
+    if (wave == 0 && t0 + kChunk < n) gates(t0 + kChunk, buf ^ 1);  // the wave with the fewest blocks
+    lds_sync();
     f32x4 o[CT];
 #pragma unroll
     for (int t = 0; t < CT; ++t) o[t] = qs[t] * grown;
-    for (int l = 0; l <= wave; ++l) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(tg + kChunk * kChunk + (16 * wave + c) * kChunk + 16 * l + 4 * g);
 #pragma unroll
-      for (int t = 0; t < CT; ++t) o[t] = mma4(x, *reinterpret_cast<const f32x4*>(ul + (16 * t + c) * LT + 16 * l + 4 * g), o[t]);
+    for (int l = 0; l < 4; ++l) {
+      if (l > wave) break;
+#pragma unroll
+      for (int t = 0; t < CT; ++t) o[t] = mma4(p4[l], *reinterpret_cast<const f32x4*>(ul + (16 * t + c) * LT + 16 * l + 4 * g), o[t]);
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r)
@@ -468,17 +497,15 @@ __global__ void __launch_bounds__(256) gdn_scan_kernel(GdnPackedArgs a, const fl
       for (int t = 0; t < CT; ++t) st[i][t] *= all;
 #pragma unroll
       for (int l = 0; l < 4; ++l) {
-        f32x4 x;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) x[r] = wk[(int64_t)(t0 + min(16 * l + 4 * g + r, m - 1)) * conv_dim + row0 + c];
         const f32x4 left = *reinterpret_cast<const f32x4*>(&left_s[buf][16 * l + 4 * g]);
 #pragma unroll
-        for (int t = 0; t < CT; ++t) st[i][t] = mma4(x, *reinterpret_cast<const f32x4*>(ul + (16 * t + c) * LT + 16 * l + 4 * g) * left, st[i][t]);
+        for (int t = 0; t < CT; ++t)
+          st[i][t] = mma4(kt[i][l], *reinterpret_cast<const f32x4*>(ul + (16 * t + c) * LT + 16 * l + 4 * g) * left, st[i][t]);
       }
 #pragma unroll
       for (int t = 0; t < CT; ++t) *reinterpret_cast<f32x4*>(Sl + (16 * t + c) * LS + row0 + 4 * g) = st[i][t];
     }
-    __syncthreads();
+    lds_sync();
   }
   if (odd) odd_s = 1;
   __syncthreads();
@@ -532,33 +559,49 @@ __global__ void __launch_bounds__(256) gdn_scan_kernel(GdnPackedArgs a, const fl
   }
 }
 
-// Gated RMSNorm of the long sequences' outputs: a wave per (token, head).
+// Gated RMSNorm of the long sequences' outputs: a workgroup per token, dv / 8 lanes to a head, eight values each.
 template <bool BF>
-__global__ void __launch_bounds__(256) gdn_out_packed_kernel(GdnPackedArgs a, const float* ow, int long_from) {
+__global__ void __launch_bounds__(256) gdn_out_packed_kernel(GdnPackedArgs a, const float* ow, int long_from, bool wide) {
   using E = Half<BF>;
-  const int lane = threadIdx.x & 63, nj = a.dv >> 6;
-  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (i >= (int64_t)a.N * a.Hv) return;
-  const int t = (int)(i / a.Hv), h = (int)(i - (int64_t)t * a.Hv), b = seq_of(a.cu, a.B, t);
+  const int t = blockIdx.x, b = seq_of(a.cu, a.B, t), vdim = a.Hv * a.dv, lanes = a.dv >> 3;
   if (b >= a.B) return;
   const PackedSeq sq(a.cu, a.rows, a.lens, b, a.N, a.R, 0x7FFFFFFF);
   if (!sq.fine || sq.n < long_from || t < sq.t0 || t - sq.t0 >= sq.n) return;
-  const float* const o = ow + i * a.dv + lane;
-  const uint16_t* const z = static_cast<const uint16_t*>(a.z) + (int64_t)t * a.z_stride + h * a.dv + lane;
-  const uint16_t* const w = static_cast<const uint16_t*>(a.norm_w) + lane;
-  float ov[4], zv[4], wv[4], ss = 0.f;  // dv <= 256
+  const float* const o = ow + (int64_t)t * vdim;
+  const uint16_t* const z = static_cast<const uint16_t*>(a.z) + (int64_t)t * a.z_stride;
+  uint16_t* const out = static_cast<uint16_t*>(a.out) + (int64_t)t * a.out_stride;
+  const int d = 8 * (threadIdx.x & (lanes - 1));
+  float w[8];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    ov[j] = j < nj ? o[64 * j] : 0.f;
-    zv[j] = j < nj ? E::ld(z[64 * j]) : 0.f;
-    wv[j] = j < nj ? E::ld(w[64 * j]) : 0.f;
-    ss += ov[j] * ov[j];
+  for (int e = 0; e < 8; ++e) w[e] = E::ld(static_cast<const uint16_t*>(a.norm_w)[d + e]);
+  for (int i = 8 * threadIdx.x; i < vdim; i += 2048) {  // whole heads to a wave: dv divides 512
+    const f32x4 lo = *reinterpret_cast<const f32x4*>(o + i), hi = *reinterpret_cast<const f32x4*>(o + i + 4);
+    u32x4 zw;
+    if (wide) {
+      zw = *reinterpret_cast<const u32x4*>(z + i);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) zw[e] = (uint32_t)z[i + 2 * e] | ((uint32_t)z[i + 2 * e + 1] << 16);
+    }
+    const float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
+    for (int m = 1; m < lanes; m <<= 1) ss += __shfl_xor(ss, m, 64);
+    const float rn = 1.f / sqrtf(ss / (float)a.dv + a.eps);
+    u32x4 r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float z0 = E::ld((uint16_t)zw[e]), z1 = E::ld((uint16_t)(zw[e] >> 16));
+      r[e] = E::pack((f32x2){x[2 * e] * rn * w[2 * e] * (z0 * sigmoid_raw(z0)), x[2 * e + 1] * rn * w[2 * e + 1] * (z1 * sigmoid_raw(z1))});
+    }
+    if (wide) {
+      *reinterpret_cast<u32x4*>(out + i) = r;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) out[i + e] = (uint16_t)(r[e >> 1] >> (16 * (e & 1)));
+    }
   }
-  const float rn = 1.f / sqrtf(lanes_sum(ss) / (float)a.dv + a.eps);
-  uint16_t* const out = static_cast<uint16_t*>(a.out) + (int64_t)t * a.out_stride + h * a.dv + lane;
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (j < nj) out[64 * j] = E::mk(ov[j] * rn * wv[j] * silu_f(zv[j]));
 }
 
 // Sequences from kLongFrom tokens on go by chunks.
@@ -576,8 +619,18 @@ template <bool BF>
 static hipError_t launch_gdn_packed_t(const GdnPackedArgs& a, hipStream_t s) {
   const int conv_dim = 2 * a.Hk * a.dk + a.Hv * a.dv;
   const bool pair = ((a.qkv_stride & 1) | (reinterpret_cast<uintptr_t>(a.qkv) & 3)) == 0;
-  const dim3 cgrid((unsigned)((conv_dim + 511) / 512), (unsigned)((a.N + 7) / 8)), rgrid((unsigned)a.Hv, (unsigned)a.B + 1);
-  hipLaunchKernelGGL((gdn_conv_packed_kernel<BF, 8>), cgrid, dim3(256), 0, s, a, pair);
+  const dim3 rgrid((unsigned)a.Hv, (unsigned)a.B + 1);
+  auto conv = [&](auto tpb, auto kw) {
+    constexpr int TPB = decltype(tpb)::value;
+    hipLaunchKernelGGL((gdn_conv_packed_kernel<BF, TPB, decltype(kw)::value>), dim3((unsigned)((conv_dim + 511) / 512), (unsigned)((a.N + TPB - 1) / TPB)),
+                       dim3(256), 0, s, a, pair);
+  };
+  auto width = [&](auto tpb) {
+    if (a.K == 4) conv(tpb, std::integral_constant<int, 4>{});
+    else conv(tpb, std::integral_constant<int, kConvMax>{});
+  };
+  if (a.N <= 512) width(std::integral_constant<int, 1>{});
+  else width(std::integral_constant<int, 8>{});
   const bool chunks = a.max_new >= kLongFrom;
   const int long_from = chunks ? kLongFrom : 0x7FFFFFFF;
   auto rec = [&](auto dk, auto dv) {
@@ -587,7 +640,8 @@ static hipError_t launch_gdn_packed_t(const GdnPackedArgs& a, hipStream_t s) {
       hipLaunchKernelGGL((gdn_chunk_kernel<BF, decltype(dk)::value>), dim3((unsigned)gdn_slots(a), (unsigned)a.Hk), dim3(256), 0, s, a, tp, long_from);
       hipLaunchKernelGGL((gdn_scan_kernel<BF, decltype(dk)::value>), dim3((unsigned)(a.Hv * (a.dv / kScanCols)), (unsigned)a.B), dim3(256), 0, s, a,
                          (const float*)tp, ow, long_from);
-      hipLaunchKernelGGL(gdn_out_packed_kernel<BF>, dim3((unsigned)(((int64_t)a.N * a.Hv + 3) / 4)), dim3(256), 0, s, a, (const float*)ow, long_from);
+      const bool wide = ((reinterpret_cast<uintptr_t>(a.z) | reinterpret_cast<uintptr_t>(a.out)) & 15) == 0 && ((a.z_stride | a.out_stride) & 7) == 0;
+      hipLaunchKernelGGL(gdn_out_packed_kernel<BF>, dim3((unsigned)a.N), dim3(256), 0, s, a, (const float*)ow, long_from, wide);
     }
     hipLaunchKernelGGL((gdn_rec_packed_kernel<BF, decltype(dk)::value, decltype(dv)::value>), rgrid, dim3(256), 0, s, a, long_from);
     return hipGetLastError();
