@@ -16,7 +16,8 @@ constexpr int kConvMax = 8;  // inputs of a convolution window at most
 // Convolution + SiLU of 128 channels (2 per lane) over the packed tokens TPB blockIdx.y .. + TPB - 1, whose inputs are all
 // asked for at once; the window slides in registers from one token of a sequence to the next. q and k channels are
 // RMS-normalized over their head (dk / 2 lanes, a power of two) and scaled, so that `work` holds [q | k | v] rows ready
-// for the recurrence. The thread that meets a sequence's first token has read its state by then, and writes the new one.
+// for the recurrence. The states are
+// read only: tokens of one window lie in different workgroups, so the launch behind this one advances them.
 // KW: window of the convolution (kConvMax: any up to it).
 template <bool BF, int TPB, int KW>
 __global__ void __launch_bounds__(256) gdn_conv_packed_kernel(GdnPackedArgs a, bool pair) {
@@ -59,7 +60,7 @@ __global__ void __launch_bounds__(256) gdn_conv_packed_kernel(GdnPackedArgs a, b
       fine = sq.fine && t >= t0 && t < end;
       if (!fine) end = t + 1;
       const bool fresh = sq.len == sq.n;
-      uint16_t* const cst = static_cast<uint16_t*>(a.conv) + (int64_t)(fine ? sq.row : 0) * (K - 1) * conv_dim + c;  // conv_dim is even
+      const uint16_t* const cst = static_cast<const uint16_t*>(a.conv) + (int64_t)(fine ? sq.row : 0) * (K - 1) * conv_dim + c;  // conv_dim is even
       uint32_t old[KW];  // the window of token t - 1, oldest first; slot KW - K is shifted out
 #pragma unroll
       for (int s = 0; s < KW; ++s) {
@@ -73,21 +74,6 @@ __global__ void __launch_bounds__(256) gdn_conv_packed_kernel(GdnPackedArgs a, b
       for (int s = 0; s < KW; ++s) {
         in0[s] = E::ld((uint16_t)old[s]);
         in1[s] = E::ld((uint16_t)(old[s] >> 16));
-      }
-      if (fine && on && t == t0) {  // slots ascending: a shift in place reads before it writes
-        for (int j = 0; j < K - 1; ++j) {
-          const int u = sq.n - (K - 1) + j;
-          uint16_t y0 = 0, y1 = 0;
-          if (u >= 0) {
-            y0 = q[(int64_t)(t0 + u) * a.qkv_stride];
-            y1 = q[(int64_t)(t0 + u) * a.qkv_stride + 1];
-          } else if (!fresh) {
-            y0 = cst[(int64_t)(K - 1 + u) * conv_dim];
-            y1 = cst[(int64_t)(K - 1 + u) * conv_dim + 1];
-          }
-          cst[(int64_t)j * conv_dim] = y0;
-          cst[(int64_t)j * conv_dim + 1] = y1;
-        }
       }
     }
     if (!fine) continue;
@@ -144,7 +130,24 @@ __global__ void __launch_bounds__(256) gdn_rec_packed_kernel(GdnPackedArgs a, in
     fill(a.cu[b], a.cu[b + 1], E::mk(__builtin_nanf("")));
     return;
   }
-  if (sq.n == 0 || sq.n >= long_from) return;
+  if (sq.n == 0) return;
+  {  // this head's share of the convolution state: every input of the step's windows has been read
+    const int conv_dim = 2 * a.Hk * DK + a.Hv * DV, K = a.K;
+    const uint16_t* const q = static_cast<const uint16_t*>(a.qkv) + (int64_t)sq.t0 * a.qkv_stride;
+    uint16_t* const cst = static_cast<uint16_t*>(a.conv) + (int64_t)sq.row * (K - 1) * conv_dim;
+    for (int c = h * 256 + tid; c < conv_dim; c += a.Hv * 256) {
+      uint16_t y[kConvMax - 1];
+#pragma unroll
+      for (int j = 0; j < kConvMax - 1; ++j) {
+        const int u = sq.n - (K - 1) + j;
+        y[j] = j >= K - 1 ? 0 : u >= 0 ? q[(int64_t)u * a.qkv_stride + c] : sq.len == sq.n ? 0 : cst[(int64_t)(K - 1 + u) * conv_dim + c];
+      }
+#pragma unroll
+      for (int j = 0; j < kConvMax - 1; ++j)
+        if (j < K - 1) cst[(int64_t)j * conv_dim + c] = y[j];
+    }
+  }
+  if (sq.n >= long_from) return;
   float* const Sp = a.rec + (((int64_t)sq.row * a.Hv + h) * DK + rg) * DV + col;
   f32x4 st[NR];
 #pragma unroll

@@ -433,6 +433,20 @@ def test_gdn_packed_values_that_are_not_finite(where):
     assert float((rec.double() - want_rec)[fine].norm() / want_rec[fine].norm()) <= 2e-6
 
 
+@pytest.mark.parametrize("conv_kernel,new", [(4, 3), (8, 7), (8, 30)])
+def test_gdn_packed_windows_read_the_state_before_the_step(conv_kernel, new):
+    """All tokens whose window begins before the step see the convolution state that the step before left."""
+    case = ([5] * 40, [new - i % 3 for i in range(40)], 4, 8, 128, 128, conv_kernel, F16)
+    t, plan = _gdn_inputs(case)
+    first = None
+    for _ in range(6):
+        got = _run_gdn(case, t, plan)
+        if first is None:
+            first = got
+            _check_gdn(case, t, plan, got)
+        assert all(torch.equal(x, y) for x, y in zip(got, first))
+
+
 def test_gdn_packed_begins_from_zeros():
     """A request's first tokens do not see what its states held."""
     case = ([0, 5], [70, 3], 1, 2, 128, 128, 4, BF16)
