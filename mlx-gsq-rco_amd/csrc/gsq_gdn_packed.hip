@@ -11,12 +11,40 @@
 
 namespace gsq {
 
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+
+// q and k values, at most 1, are held as two fp16 numbers of 2^12 times them (22 bits, down to 2^-37): what the matrix
+// cores take, in float32's room. The low half of a word is the first, the high half the rest.
+__device__ __forceinline__ uint32_t split22(float x) {
+  const float v = x * 4096.f;
+  const _Float16 h = (_Float16)v, l = (_Float16)(v - (float)h);
+  return (uint32_t)__builtin_bit_cast(uint16_t, h) | ((uint32_t)__builtin_bit_cast(uint16_t, l) << 16);
+}
+__device__ __forceinline__ float join22(uint32_t w) {
+  return (Half<false>::ld((uint16_t)w) + Half<false>::ld((uint16_t)(w >> 16))) * (1.f / 4096.f);
+}
+// eight words to operands of first halves and of rests
+__device__ __forceinline__ void halves8(u32x4 a, u32x4 b, u32x4& hi, u32x4& lo) {
+  const uint32_t w[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    hi[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x05040100u);
+    lo[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x07060302u);
+  }
+}
+// a product of 22-bit operands, without the rests' product (2^-22 of it)
+__device__ __forceinline__ f32x4 mma22(u32x4 ah, u32x4 al, u32x4 bh, u32x4 bl, f32x4 c) {
+  c = Half<false>::mma(al, bh, c);
+  c = Half<false>::mma(ah, bl, c);
+  return Half<false>::mma(ah, bh, c);
+}
+
 constexpr int kConvMax = 8;  // inputs of a convolution window at most
 
 // Convolution + SiLU of 128 channels (2 per lane) over the packed tokens TPB blockIdx.y .. + TPB - 1, whose inputs are all
 // asked for at once; the window slides in registers from one token of a sequence to the next. q and k channels are
 // RMS-normalized over their head (dk / 2 lanes, a power of two) and scaled, so that `work` holds [q | k | v] rows ready
-// for the recurrence. The states are
+// for the recurrence (q and k as split22 words). The states are
 // read only: tokens of one window lie in different workgroups, so the launch behind this one advances them.
 // KW: window of the convolution (kConvMax: any up to it).
 template <bool BF, int TPB, int KW>
@@ -102,7 +130,8 @@ __global__ void __launch_bounds__(256) gdn_conv_packed_kernel(GdnPackedArgs a, b
         y1 = y1 * rn * sc;
       }
     }
-    if (on) *reinterpret_cast<float2*>(a.work + (int64_t)t * conv_dim + c) = make_float2(y0, y1);
+    float2* const to = reinterpret_cast<float2*>(a.work + (int64_t)t * conv_dim + c);
+    if (on) *to = c < 2 * key_dim ? make_float2(__builtin_bit_cast(float, split22(y0)), __builtin_bit_cast(float, split22(y1))) : make_float2(y0, y1);
   }
 }
 
@@ -177,8 +206,8 @@ __global__ void __launch_bounds__(256) gdn_rec_packed_kernel(GdnPackedArgs a, in
     float k[NR], q[NR];
 #pragma unroll
     for (int j = 0; j < NR; ++j) {
-      q[j] = row[kh * DK + rg + j * NG];
-      k[j] = row[key_dim + kh * DK + rg + j * NG];
+      q[j] = join22(__builtin_bit_cast(uint32_t, row[kh * DK + rg + j * NG]));
+      k[j] = join22(__builtin_bit_cast(uint32_t, row[key_dim + kh * DK + rg + j * NG]));
     }
     const f32x4 v = *reinterpret_cast<const f32x4*>(row + 2 * key_dim + h * DV + col);
     const float av = E::ld(abr[h]) + dtb, bv = E::ld(abr[a.Hv + h]);
@@ -225,6 +254,7 @@ __global__ void __launch_bounds__(256) gdn_rec_packed_kernel(GdnPackedArgs a, in
 // Matrix instruction j of four takes element j of 16-byte pieces: lane (g, c) = (lane / 16, lane % 16) holds A[c][4 g + j] and
 // B[4 g + j][c], and C[4 g + r][c] in register r, so that a product's result is the next one's B operand as it lies.
 constexpr int kChunk = 64;
+constexpr int kChunkFloats = 2 * kChunk * kChunk + 3 * kChunk;  // T, P, e^G, e^(G_C - G), beta of a chunk and head
 
 __device__ __forceinline__ f32x4 mma4(f32x4 a, f32x4 b, f32x4 c) {
 #pragma unroll
@@ -290,14 +320,23 @@ __global__ void __launch_bounds__(256) gdn_chunk_kernel(GdnPackedArgs a, float* 
     bj[p] = wave == 0 ? BJ[0][p] : wave == 1 ? BJ[1][p] : wave == 2 ? BJ[2][p] : BJ[3][p];
     kk[p] = qk[p] = (f32x4){0.f, 0.f, 0.f, 0.f};
     if (bi[p] < 0) continue;
-    const float* const qi = a.work + (t0 + min(16 * bi[p] + c, n - 1)) * conv_dim + kh * DK + 4 * g;
-    const float* const kj = a.work + (t0 + min(16 * bj[p] + c, n - 1)) * conv_dim + key_dim + kh * DK + 4 * g;
+    const uint32_t* const words = reinterpret_cast<const uint32_t*>(a.work);
+    const uint32_t* const qi = words + (t0 + min(16 * bi[p] + c, n - 1)) * conv_dim + kh * DK + 8 * g;
+    const uint32_t* const kj = words + (t0 + min(16 * bj[p] + c, n - 1)) * conv_dim + key_dim + kh * DK + 8 * g;
+    auto load = [&](const uint32_t* at, u32x4& hi, u32x4& lo) {
+      halves8(*reinterpret_cast<const u32x4*>(at), *reinterpret_cast<const u32x4*>(at + 4), hi, lo);
+    };
 #pragma unroll
-    for (int s = 0; s < DK / 16; ++s) {
-      const f32x4 b = *reinterpret_cast<const f32x4*>(kj + 16 * s);
-      qk[p] = mma4(*reinterpret_cast<const f32x4*>(qi + 16 * s), b, qk[p]);
-      kk[p] = mma4(*reinterpret_cast<const f32x4*>(qi + key_dim + 16 * s), b, kk[p]);
+    for (int s = 0; s < DK / 32; ++s) {
+      u32x4 bh, bl, ah, al;
+      load(kj + 32 * s, bh, bl);
+      load(qi + 32 * s, ah, al);
+      qk[p] = mma22(ah, al, bh, bl, qk[p]);
+      load(qi + key_dim + 32 * s, ah, al);
+      kk[p] = mma22(ah, al, bh, bl, kk[p]);
     }
+    qk[p] *= 0x1p-24f;
+    kk[p] *= 0x1p-24f;
   }
   for (int h = kh; h < a.Hv; h += a.Hk) {
     if (wave == 0) {
@@ -306,8 +345,15 @@ __global__ void __launch_bounds__(256) gdn_chunk_kernel(GdnPackedArgs a, float* 
       sum_s[lane] = gate.sum;
     }
     __syncthreads();
-    float* const Tg = tp + ((int64_t)blockIdx.x * a.Hv + h) * 2 * kChunk * kChunk;
+    float* const Tg = tp + ((int64_t)blockIdx.x * a.Hv + h) * kChunkFloats;
     float* const Pg = Tg + kChunk * kChunk;
+    if (wave == 1) {
+      const double sum = sum_s[lane];
+      float* const gates = Pg + kChunk * kChunk + lane;
+      gates[0] = expf((float)sum);
+      gates[kChunk] = expf((float)(sum_s[kChunk - 1] - sum));
+      gates[2 * kChunk] = beta_s[lane];
+    }
 #pragma unroll
     for (int p = 0; p < 3; ++p) {
       if (bi[p] < 0) continue;
@@ -362,103 +408,173 @@ __global__ void __launch_bounds__(256) gdn_chunk_kernel(GdnPackedArgs a, float* 
   }
 }
 
-// The chain over a sequence's chunks, for 32 columns of a value head's state: its tiles stay in registers (rows of wave w:
-// the blocks of 16 w, w + 4, ..), a copy in LDS is the products' operand. Wave w holds tokens 16 w .. of a chunk.
-constexpr int kScanCols = 32;
+// The chain over a sequence's chunks, for 32 columns of a value head's state: its tiles stay in registers (32 rows to each
+// of the first waves), a copy in LDS is the products' operand. Wave w holds tokens 16 w .. of a chunk. What goes into the
+// state's products is held in two fp16 numbers (22 bits: the state and left u times a power of two for each 32 rows, 16
+// tokens; q and k as split22 words), for the 16-bit matrix instructions; u and the outputs inside the chunk are float32
+// products. Bound by the chain: a chunk's operands come from L2 a chunk ahead, two workgroups to a CU.
+// Columns: 64 read q, k, T and P half as often but leave one workgroup to a CU (3 prompts of 2047, 48 heads: 691 against
+// 635 us for the whole call).
+
+constexpr int kScanColumns = 32;
 
 template <bool BF, int DK>
 __global__ void __launch_bounds__(256, 2) gdn_scan_kernel(GdnPackedArgs a, const float* tp, float* ow, int long_from) {
-  constexpr int LS = DK + 4, LT = kChunk + 4, NB = (DK / 16 + 3) / 4, CT = kScanCols / 16;
-  __shared__ __attribute__((aligned(16))) float Sl[kScanCols * LS], rl[kScanCols * LT], ul[kScanCols * LT];
-  __shared__ __attribute__((aligned(16))) float grown_s[2][kChunk], left_s[2][kChunk], beta_s[2][kChunk];
+  static_assert(kScanColumns == 32);
+  constexpr int LS = DK + 8, LT = kChunk + 4, LU = kChunk + 8, COLS = kScanColumns, CT = COLS / 16;
+  // the state's copy and left u as two fp16 numbers, by column: of a power of two times them for each 32 rows, 16 tokens
+  __shared__ __attribute__((aligned(16))) uint16_t Sh[2][COLS * LS], uh[2][COLS * LU];
+  __shared__ __attribute__((aligned(16))) float rl[COLS * LT], ul[COLS * LT];
+  __shared__ float sunit_s[4], uunit_s[4];
   __shared__ int odd_s;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
-  const int ns = a.dv / kScanCols, h = blockIdx.x / ns, col0 = blockIdx.x % ns * kScanCols, kh = h % a.Hk, b = blockIdx.y;
+  const int ns = a.dv / COLS, h = blockIdx.x / ns, col0 = blockIdx.x % ns * COLS, kh = h % a.Hk, b = blockIdx.y;
   const PackedSeq sq(a.cu, a.rows, a.lens, b, a.N, a.R, 0x7FFFFFFF);
   if (!sq.fine || sq.n < long_from) return;
   const int key_dim = a.Hk * DK, conv_dim = 2 * key_dim + a.Hv * a.dv, vdim = a.Hv * a.dv, n = sq.n;
-  const float* const wq = a.work + (int64_t)sq.t0 * conv_dim + kh * DK;
-  const float* const wk = wq + key_dim;
+  const uint32_t* const wq = reinterpret_cast<const uint32_t*>(a.work) + (int64_t)sq.t0 * conv_dim + kh * DK;
+  const uint32_t* const wk = wq + key_dim;
   const float* const wv = a.work + (int64_t)sq.t0 * conv_dim + 2 * key_dim + h * a.dv + col0;
   float* const o_at = ow + (int64_t)sq.t0 * vdim + h * a.dv + col0;
   const uint16_t* const ab = static_cast<const uint16_t*>(a.ab) + (int64_t)sq.t0 * a.ab_stride;
-  const float* tg = tp + ((int64_t)((sq.t0 >> 6) + b) * a.Hv + h) * 2 * kChunk * kChunk;
+  const float* tg = tp + ((int64_t)((sq.t0 >> 6) + b) * a.Hv + h) * kChunkFloats;
+  const int64_t next = (int64_t)a.Hv * kChunkFloats;
   float* const Sg = a.rec + (((int64_t)sq.row * a.Hv + h) * DK) * a.dv + col0;
   const bool fresh = sq.len == n;
   if (tid == 0) odd_s = 0;
-  auto gates = [&](int t0, int buf) {  // one wave
-    const ChunkGate x(ab + (int64_t)t0 * a.ab_stride, a.ab_stride, min(kChunk, n - t0), h, a.Hv, a.dt_bias[h], a.ssm_a[h], BF);
-    grown_s[buf][lane] = expf((float)x.sum);
-    left_s[buf][lane] = expf((float)(__shfl(x.sum, 63, 64) - x.sum));
-    beta_s[buf][lane] = x.beta;
-  };
-  f32x4 st[NB][CT];
-#pragma unroll
-  for (int i = 0; i < NB; ++i)
-#pragma unroll
-    for (int t = 0; t < CT; ++t) {
-      const int row = 16 * (wave + 4 * i);
-      st[i][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
-      if (row >= DK) continue;
-      if (!fresh)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) st[i][t][r] = Sg[(int64_t)(row + 4 * g + r) * a.dv + 16 * t + c];
-      *reinterpret_cast<f32x4*>(Sl + (16 * t + c) * LS + row + 4 * g) = st[i][t];
-    }
-  if (wave == 0) gates(0, 0);
-  // what a chunk reads from memory is asked for a phase or more before it is used: q and k rows a chunk ahead, T, P, v and
-  // the transposed k at its beginning
-  constexpr int KQ = DK / 16;
-  f32x4 q4[KQ], k4[KQ];
-  auto load_qk = [&](int t0) {
-    const int64_t row = t0 + min(16 * wave + c, min(kChunk, n - t0) - 1);  // tokens behind the last repeat it
-#pragma unroll
-    for (int s = 0; s < KQ; ++s) {
-      q4[s] = *reinterpret_cast<const f32x4*>(wq + row * conv_dim + 16 * s + 4 * g);
-      k4[s] = *reinterpret_cast<const f32x4*>(wk + row * conv_dim + 16 * s + 4 * g);
-    }
-  };
   bool odd = false;
-  int buf = 0;
-  load_qk(0);
-  __syncthreads();
-  for (int t0 = 0; t0 < n; t0 += kChunk, buf ^= 1, tg += (int64_t)a.Hv * 2 * kChunk * kChunk) {
+  auto largest = [&](const f32x4 (&v)[CT]) {  // of the lane's values; what is not finite is odd
+    float top = 0.f;
+#pragma unroll
+    for (int t = 0; t < CT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        odd |= !(fabsf(v[t][r]) <= 3.4028235e38f);
+        top = fmaxf(top, fabsf(v[t][r]));
+      }
+    return top;
+  };
+  auto power = [&](float top, float& back) {  // 2^x that brings the wave's largest below 2^7, and 2^-x
+    top = lanes_reduce(top, [](float x, float y) { return fmaxf(x, y); });
+    const int e = top > 0.f && top <= 3.4028235e38f ? min(max(6 - ilogbf(top), -120), 120) : 0;
+    back = ldexpf(1.f, -e);
+    return ldexpf(1.f, e);
+  };
+  // four values of a column, at 2^x times them, to the two arrays
+  auto put_split = [&](uint16_t (*to)[COLS * LS], uint16_t (*tu)[COLS * LU], int at, f32x4 v, float f) {
+    f16x4 h, l;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float x = v[r] * f;
+      h[r] = (_Float16)x;
+      l[r] = (_Float16)(x - (float)h[r]);
+    }
+    if (to) {
+      *reinterpret_cast<f16x4*>(&to[0][at]) = h;
+      *reinterpret_cast<f16x4*>(&to[1][at]) = l;
+    } else {
+      *reinterpret_cast<f16x4*>(&tu[0][at]) = h;
+      *reinterpret_cast<f16x4*>(&tu[1][at]) = l;
+    }
+  };
+  const bool owner = 32 * wave < DK;  // of rows 32 wave .. + 31 of the state
+  f32x4 st[2][CT];
+  auto copy_state = [&]() {
+    float back;
+    const float f = power(fmaxf(largest(st[0]), largest(st[1])), back);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int t = 0; t < CT; ++t) put_split(Sh, nullptr, (16 * t + c) * LS + 32 * wave + 16 * i + 4 * g, st[i][t], f);
+    if (lane == 0) sunit_s[wave] = back * (1.f / 4096.f);  // k and q are 2^12 times themselves
+  };
+  if (owner) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int t = 0; t < CT; ++t) {
+        st[i][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        if (!fresh)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) st[i][t][r] = Sg[(int64_t)(32 * wave + 16 * i + 4 * g + r) * a.dv + 16 * t + c];
+      }
+    copy_state();
+  }
+  // what a chunk reads from memory is asked for a chunk before it is used, when its registers have been read
+  constexpr int KQ = DK / 32;
+  u32x4 q4[KQ][2], k4[KQ][2], kt[2][4];
+  f32x4 v4[CT], t4[4], p4[4], grown, left, beta;
+  float all;
+  auto load_rows = [&](int t0) {  // tokens behind the last repeat it
     const int m = min(kChunk, n - t0);
-    f32x4 v4[CT], t4[4], p4[4], kt[NB][4];
+    const int64_t row = t0 + min(16 * wave + c, m - 1);
+#pragma unroll
+    for (int s = 0; s < KQ; ++s)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        q4[s][e] = *reinterpret_cast<const u32x4*>(wq + row * conv_dim + 32 * s + 8 * g + 4 * e);
+        k4[s][e] = *reinterpret_cast<const u32x4*>(wk + row * conv_dim + 32 * s + 8 * g + 4 * e);
+      }
 #pragma unroll
     for (int t = 0; t < CT; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) v4[t][r] = wv[(int64_t)(t0 + min(16 * wave + 4 * g + r, m - 1)) * conv_dim + 16 * t + c];
+  };
+  auto load_block = [&](f32x4 (&x)[4], const float* at) {
 #pragma unroll
-    for (int l = 0; l < 4; ++l) {
-      if (l > wave) break;
-      t4[l] = *reinterpret_cast<const f32x4*>(tg + (16 * wave + c) * kChunk + 16 * l + 4 * g);
-      p4[l] = *reinterpret_cast<const f32x4*>(tg + kChunk * kChunk + (16 * wave + c) * kChunk + 16 * l + 4 * g);
-    }
+    for (int l = 0; l < 4; ++l)
+      x[l] = *reinterpret_cast<const f32x4*>(at + (16 * wave + c) * kChunk + 16 * min(l, wave) + 4 * g);
+  };
+  auto load_columns = [&](int t0) {
+    const int m = min(kChunk, n - t0);
 #pragma unroll
-    for (int i = 0; i < NB; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int l = 0; l < 4; ++l)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          kt[i][l][r] = wk[(int64_t)(t0 + min(16 * l + 4 * g + r, m - 1)) * conv_dim + min(16 * (wave + 4 * i), DK - 16) + c];
+        for (int r = 0; r < 4; ++r) kt[i][l][r] = wk[(int64_t)(t0 + min(16 * l + 4 * g + r, m - 1)) * conv_dim + min(32 * wave, DK - 32) + 16 * i + c];
+  };
+  auto load_gates = [&](const float* at) {
+    at += 2 * kChunk * kChunk;
+    grown = *reinterpret_cast<const f32x4*>(at + 16 * wave + 4 * g);
+    left = *reinterpret_cast<const f32x4*>(at + kChunk + 16 * wave + 4 * g);
+    beta = *reinterpret_cast<const f32x4*>(at + 2 * kChunk + 16 * wave + 4 * g);
+    all = at[kChunk - 1];
+  };
+  load_rows(0);
+  load_gates(tg);
+  load_block(t4, tg);
+  load_block(p4, tg + kChunk * kChunk);
+  load_columns(0);
+  __syncthreads();
+  for (int t0 = 0; t0 < n; t0 += kChunk, tg += next) {
+    const int m = min(kChunk, n - t0);
+    // the last chunk asks for its own again: a load that some turn of the loop leaves out would be waited for at once
+    const bool more = t0 + kChunk < n;
+    const int tn = more ? t0 + kChunk : t0;
+    const float* const tgn = more ? tg + next : tg;
     f32x4 qs[CT], ks[CT];
 #pragma unroll
     for (int t = 0; t < CT; ++t) qs[t] = ks[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int s = 0; s < KQ; ++s)
+    for (int s = 0; s < KQ; ++s) {
+      const float back = sunit_s[s];
+      u32x4 qh, ql, kh_, kl;
+      halves8(q4[s][0], q4[s][1], qh, ql);
+      halves8(k4[s][0], k4[s][1], kh_, kl);
 #pragma unroll
       for (int t = 0; t < CT; ++t) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(Sl + (16 * t + c) * LS + 16 * s + 4 * g);
-        ks[t] = mma4(k4[s], x, ks[t]);
-        qs[t] = mma4(q4[s], x, qs[t]);
+        const u32x4 xh = *reinterpret_cast<const u32x4*>(&Sh[0][(16 * t + c) * LS + 32 * s + 8 * g]);
+        const u32x4 xl = *reinterpret_cast<const u32x4*>(&Sh[1][(16 * t + c) * LS + 32 * s + 8 * g]);
+        const f32x4 none = {0.f, 0.f, 0.f, 0.f};
+        ks[t] += mma22(kh_, kl, xh, xl, none) * back;
+        qs[t] += mma22(qh, ql, xh, xl, none) * back;
       }
-    if (t0 + kChunk < n) load_qk(t0 + kChunk);
-    const f32x4 grown = *reinterpret_cast<const f32x4*>(&grown_s[buf][16 * wave + 4 * g]);
-    const f32x4 beta = *reinterpret_cast<const f32x4*>(&beta_s[buf][16 * wave + 4 * g]);
+    }
 #pragma unroll
     for (int t = 0; t < CT; ++t)
       *reinterpret_cast<f32x4*>(rl + (16 * t + c) * LT + 16 * wave + 4 * g) = beta * (v4[t] - grown * ks[t]);
+    load_rows(tn);
     lds_sync();
     f32x4 u[CT];
 #pragma unroll
@@ -469,13 +585,17 @@ __global__ void __launch_bounds__(256, 2) gdn_scan_kernel(GdnPackedArgs a, const
 #pragma unroll
       for (int t = 0; t < CT; ++t) u[t] = mma4(t4[l], *reinterpret_cast<const f32x4*>(rl + (16 * t + c) * LT + 16 * l + 4 * g), u[t]);
     }
+    load_block(t4, tgn);
+    {
+      float back;
+      const float f = power(largest(u), back);  // left is at most 1
 #pragma unroll
-    for (int t = 0; t < CT; ++t) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) odd |= !(fabsf(u[t][r]) <= 3.4028235e38f);
-      *reinterpret_cast<f32x4*>(ul + (16 * t + c) * LT + 16 * wave + 4 * g) = u[t];
+      for (int t = 0; t < CT; ++t) {
+        *reinterpret_cast<f32x4*>(ul + (16 * t + c) * LT + 16 * wave + 4 * g) = u[t];
+        put_split(nullptr, uh, (16 * t + c) * LU + 16 * wave + 4 * g, u[t] * left, f);
+      }
+      if (lane == 0) uunit_s[wave] = back * (1.f / 4096.f);
     }
-    if (wave == 0 && t0 + kChunk < n) gates(t0 + kChunk, buf ^ 1);  // the wave with the fewest blocks
     lds_sync();
     f32x4 o[CT];
 #pragma unroll
@@ -491,35 +611,52 @@ __global__ void __launch_bounds__(256, 2) gdn_scan_kernel(GdnPackedArgs a, const
       if (16 * wave + 4 * g + r < m)
 #pragma unroll
         for (int t = 0; t < CT; ++t) o_at[(int64_t)(t0 + 16 * wave + 4 * g + r) * vdim + 16 * t + c] = o[t][r];
-    const float all = grown_s[buf][kChunk - 1];
+    load_block(p4, tgn + kChunk * kChunk);
+    if (owner) {
 #pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      const int row0 = 16 * (wave + 4 * i);
-      if (row0 >= DK) continue;
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int t = 0; t < CT; ++t) st[i][t] *= all;
+        for (int t = 0; t < CT; ++t) st[i][t] *= all;
 #pragma unroll
       for (int l = 0; l < 4; ++l) {
-        const f32x4 left = *reinterpret_cast<const f32x4*>(&left_s[buf][16 * l + 4 * g]);
+        const float back = uunit_s[l];
+        f16x4 bh[CT], bl[CT];
 #pragma unroll
-        for (int t = 0; t < CT; ++t)
-          st[i][t] = mma4(kt[i][l], *reinterpret_cast<const f32x4*>(ul + (16 * t + c) * LT + 16 * l + 4 * g) * left, st[i][t]);
+        for (int t = 0; t < CT; ++t) {
+          bh[t] = *reinterpret_cast<const f16x4*>(&uh[0][(16 * t + c) * LU + 16 * l + 4 * g]);
+          bl[t] = *reinterpret_cast<const f16x4*>(&uh[1][(16 * t + c) * LU + 16 * l + 4 * g]);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const u32x4 w = kt[i][l];
+          const uint2 hw = make_uint2(__builtin_amdgcn_perm(w[1], w[0], 0x05040100u), __builtin_amdgcn_perm(w[3], w[2], 0x05040100u));
+          const uint2 lw = make_uint2(__builtin_amdgcn_perm(w[1], w[0], 0x07060302u), __builtin_amdgcn_perm(w[3], w[2], 0x07060302u));
+          const f16x4 ah = __builtin_bit_cast(f16x4, hw), al = __builtin_bit_cast(f16x4, lw);
+#pragma unroll
+          for (int t = 0; t < CT; ++t) {
+            f32x4 x = __builtin_amdgcn_mfma_f32_16x16x16f16(al, bh[t], (f32x4){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+            x = __builtin_amdgcn_mfma_f32_16x16x16f16(ah, bl[t], x, 0, 0, 0);
+            x = __builtin_amdgcn_mfma_f32_16x16x16f16(ah, bh[t], x, 0, 0, 0);
+            st[i][t] += x * back;
+          }
+        }
       }
-#pragma unroll
-      for (int t = 0; t < CT; ++t) *reinterpret_cast<f32x4*>(Sl + (16 * t + c) * LS + row0 + 4 * g) = st[i][t];
+      copy_state();
     }
+    load_columns(tn);
+    load_gates(tgn);
     lds_sync();
   }
   if (odd) odd_s = 1;
   __syncthreads();
   if (!odd_s) {
+    if (owner)
 #pragma unroll
-    for (int i = 0; i < NB; ++i)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int t = 0; t < CT; ++t)
+        for (int t = 0; t < CT; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (16 * (wave + 4 * i) < DK) Sg[(int64_t)(16 * (wave + 4 * i) + 4 * g + r) * a.dv + 16 * t + c] = st[i][t][r];
+          for (int r = 0; r < 4; ++r) Sg[(int64_t)(32 * wave + 16 * i + 4 * g + r) * a.dv + 16 * t + c] = st[i][t][r];
     return;
   }
   // A value that is not finite has reached tokens before its own through the products: once more, token by token. Thread
@@ -545,14 +682,14 @@ __global__ void __launch_bounds__(256, 2) gdn_scan_kernel(GdnPackedArgs a, const
 #pragma unroll
       for (int i = 0; i < NR; ++i) {
         s[i] *= decay;
-        p += s[i] * wk[(int64_t)t * conv_dim + x + 8 * i];
+        p += s[i] * join22(wk[(int64_t)t * conv_dim + x + 8 * i]);
       }
       const float d = (wv[(int64_t)t * conv_dim + y] - total(p)) * beta;
       p = 0.f;
 #pragma unroll
       for (int i = 0; i < NR; ++i) {
-        s[i] += d * wk[(int64_t)t * conv_dim + x + 8 * i];
-        p += s[i] * wq[(int64_t)t * conv_dim + x + 8 * i];
+        s[i] += d * join22(wk[(int64_t)t * conv_dim + x + 8 * i]);
+        p += s[i] * join22(wq[(int64_t)t * conv_dim + x + 8 * i]);
       }
       const float o = total(p);
       if (x == 0) o_at[(int64_t)t * vdim + y] = o;
@@ -607,15 +744,16 @@ __global__ void __launch_bounds__(256) gdn_out_packed_kernel(GdnPackedArgs a, co
   }
 }
 
-// Sequences from kLongFrom tokens on go by chunks.
-constexpr int kLongFrom = 24;
+// Sequences from kLongFrom tokens on go by chunks (us for the whole call, one sequence of 48 heads of 128, token by token
+// and by chunks: 16 tokens 50 and 43, 24 tokens 71 and 44, 64 tokens 176 and 48; 15 tokens token by token 48).
+constexpr int kLongFrom = 16;
 
 static int64_t gdn_slots(const GdnPackedArgs& a) { return (int64_t)(a.N >> 6) + a.B + 1; }
 
 // convolution outputs; if there may be long sequences, T and P of their chunks and the recurrence's outputs
 int64_t gdn_packed_work(const GdnPackedArgs& a) {
   const int64_t rows = (int64_t)a.N * (2 * a.Hk * a.dk + a.Hv * a.dv);
-  return a.max_new < kLongFrom ? rows : rows + gdn_slots(a) * a.Hv * 2 * kChunk * kChunk + (int64_t)a.N * a.Hv * a.dv;
+  return a.max_new < kLongFrom ? rows : rows + gdn_slots(a) * a.Hv * kChunkFloats + (int64_t)a.N * a.Hv * a.dv;
 }
 
 template <bool BF>
@@ -639,9 +777,9 @@ static hipError_t launch_gdn_packed_t(const GdnPackedArgs& a, hipStream_t s) {
   auto rec = [&](auto dk, auto dv) {
     if (chunks) {
       float* const tp = a.work + (int64_t)a.N * conv_dim;
-      float* const ow = tp + gdn_slots(a) * a.Hv * 2 * kChunk * kChunk;
+      float* const ow = tp + gdn_slots(a) * a.Hv * kChunkFloats;
       hipLaunchKernelGGL((gdn_chunk_kernel<BF, decltype(dk)::value>), dim3((unsigned)gdn_slots(a), (unsigned)a.Hk), dim3(256), 0, s, a, tp, long_from);
-      hipLaunchKernelGGL((gdn_scan_kernel<BF, decltype(dk)::value>), dim3((unsigned)(a.Hv * (a.dv / kScanCols)), (unsigned)a.B), dim3(256), 0, s, a,
+      hipLaunchKernelGGL((gdn_scan_kernel<BF, decltype(dk)::value>), dim3((unsigned)(a.Hv * (a.dv / kScanColumns)), (unsigned)a.B), dim3(256), 0, s, a,
                          (const float*)tp, ow, long_from);
       const bool wide = ((reinterpret_cast<uintptr_t>(a.z) | reinterpret_cast<uintptr_t>(a.out)) & 15) == 0 && ((a.z_stride | a.out_stride) & 7) == 0;
       hipLaunchKernelGGL(gdn_out_packed_kernel<BF>, dim3((unsigned)a.N), dim3(256), 0, s, a, (const float*)ow, long_from, wide);
