@@ -5,6 +5,8 @@
 // One workgroup, a thread to a sequence: need_b = max(0, ceil((len + new) / P) - held) and its prefix sums decide who is
 // served, in the order of the sequences; pages come off the end of the list of free ones, and go back to it in the
 // opposite order. Whole numbers throughout, every sum in 64 bits, no atomics: the result is the definition's.
+// Bound by its chain of three prefix sums and the reads before them: 6 us for 16 single tokens, one workgroup for at most
+// 1024 sequences being less than a second launch for a sum across workgroups.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -14,6 +16,10 @@
 namespace gsq {
 
 constexpr int kPlanThreads = 1024;  // sequences of a step at most
+// Tokens that the one workgroup lays out as well; those of larger steps have a launch of their own (us, without and with:
+// one sequence of 512 5.6 and 7.4, of 4096 7.6 and 7.4, of 8191 9.9 and 7.6; four of up to 8191 beside 250 tokens, and
+// their release: 46 and 32).
+constexpr int kPlanTokens = 4096;
 
 // Inclusive prefix sums over the workgroup; red: 16 values of LDS.
 __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* red) {
@@ -33,7 +39,13 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* red) {
 // Whether an earlier sequence names the request of this thread's. req: every sequence's, in LDS.
 __device__ __forceinline__ bool named_before(const int* req, int r, int b) {
   bool again = false;
-  for (int i = 0; i < b; ++i) again |= req[i] == r;
+  const int4* const four = reinterpret_cast<const int4*>(req);
+#pragma unroll 4
+  for (int i = 0; i < b / 4; ++i) {
+    const int4 v = four[i];
+    again |= v.x == r || v.y == r || v.z == r || v.w == r;
+  }
+  for (int i = b & ~3; i < b; ++i) again |= req[i] == r;
   return again;
 }
 
@@ -48,8 +60,11 @@ __device__ __forceinline__ int find_end(const int64_t* end, int n, int64_t i) {
   return lo;
 }
 
+// TOKENS: positions and slots of the tokens too.
+template <bool TOKENS>
 __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PagePlanArgs a) {
-  __shared__ int req[kPlanThreads], base[kPlanThreads], old[kPlanThreads], row[kPlanThreads];
+  __shared__ __attribute__((aligned(16))) int req[kPlanThreads];
+  __shared__ int base[kPlanThreads], old[kPlanThreads], row[kPlanThreads];
   __shared__ int64_t end[kPlanThreads], take[kPlanThreads], red[16];
   const int b = threadIdx.x;
   const bool on = b < a.B;
@@ -86,15 +101,15 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PagePlanArgs a)
     const int64_t first = s ? take[s - 1] : 0;
     a.table[(int64_t)row[s] * a.W + old[s] + (i - first)] = a.free[avail - 1 - i];
   }
-  for (int64_t t = b; t < a.N; t += kPlanThreads) {
+  for (int64_t t = b; TOKENS && t < a.N; t += kPlanThreads) {
     const int s = find_end(end, a.B, t);
     int64_t p = -1, slot = -1;
     if (s < a.B && row[s] >= 0) {
       p = base[s] + (t - (s ? end[s - 1] : 0));
-      const int64_t j = p / a.P;
+      const int j = (int)p / a.P;  // positions fit in 32 bits, as lens does
       // a page of this step comes from the list: the table may not hold it yet
       const int page = j < old[s] ? a.table[(int64_t)row[s] * a.W + j] : a.free[avail - 1 - ((s ? take[s - 1] : 0) + j - old[s])];
-      slot = page >= 0 && page < a.n_pages ? (int64_t)page * a.P + p % a.P : -1;
+      slot = page >= 0 && page < a.n_pages ? (int64_t)page * a.P + (p - j * a.P) : -1;
     }
     a.pos[t] = p;
     a.slots[t] = slot;
@@ -103,6 +118,27 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PagePlanArgs a)
     a.cu[0] = 0;
     a.n_free[0] = (int)(avail - all);
   }
+}
+
+// Positions and slots of the tokens of a step that has been laid out, a thread to each.
+__global__ void __launch_bounds__(256) page_tokens_kernel(PagePlanArgs a) {
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (t >= a.N) return;
+  int lo = 0, hi = a.B;  // first sequence that ends behind t
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (a.cu[mid + 1] <= t) lo = mid + 1;
+    else hi = mid;
+  }
+  int64_t p = -1, slot = -1;
+  if (lo < a.B && a.rows[lo] >= 0) {
+    p = a.lens[lo] - (a.cu[lo + 1] - (int)t);
+    const int j = (int)p / a.P;
+    const int page = a.table[(int64_t)a.rows[lo] * a.W + j];
+    slot = page >= 0 && page < a.n_pages ? (int64_t)page * a.P + (p - j * a.P) : -1;
+  }
+  a.pos[t] = p;
+  a.slots[t] = slot;
 }
 
 __global__ void __launch_bounds__(kPlanThreads) page_advance_kernel(const int32_t* rows, const int32_t* lens, int32_t* lengths,
@@ -114,7 +150,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_advance_kernel(const int32_
 // Pages of the requests back to the list, so that the first page of the first request ends on top: what page_plan took
 // last for these requests, in this order, lies there as before.
 __global__ void __launch_bounds__(kPlanThreads) page_release_kernel(PageReleaseArgs a) {
-  __shared__ int req[kPlanThreads];
+  __shared__ __attribute__((aligned(16))) int req[kPlanThreads];
   __shared__ int64_t back[kPlanThreads], red[16];
   const int b = threadIdx.x;
   const int r = b < a.B ? a.requests[b] : -1;
@@ -142,7 +178,12 @@ __global__ void __launch_bounds__(kPlanThreads) page_release_kernel(PageReleaseA
 }
 
 hipError_t launch_page_plan(const PagePlanArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL(page_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a);
+  if (a.N <= kPlanTokens) {
+    hipLaunchKernelGGL(page_plan_kernel<true>, dim3(1), dim3(kPlanThreads), 0, s, a);
+    return hipGetLastError();
+  }
+  hipLaunchKernelGGL(page_plan_kernel<false>, dim3(1), dim3(kPlanThreads), 0, s, a);
+  hipLaunchKernelGGL(page_tokens_kernel, dim3((unsigned)((a.N + 255) / 256)), dim3(256), 0, s, a);
   return hipGetLastError();
 }
 
