@@ -351,7 +351,8 @@ int64_t gsq_attn_paged_work(int64_t tokens, int64_t sequences, int64_t heads, in
 /* out = round(softmax(q K^T / sqrt(head_dim)) V [* sigmoid(gate)]) of every packed token and head (kv head h / (heads /
  * kv_heads)) over positions 0 .. its own. q and out [tokens, heads, head_dim], 16-byte aligned as the pages and work; gate
  * NULL, or with strides in elements between tokens and heads. max_new: most new tokens that a sequence is expected to
- * bring; it chooses kernels, longer ones are served too. */
+ * bring; it chooses kernels, longer ones are served too. Steps of
+ * 2^24 workgroups and more (about tokens * heads / 16 of them, / 128 with many new tokens) are refused. */
 int gsq_attn_paged(const void* q, const void* gate, int64_t gate_stride, int64_t gate_head_stride, const void* k_pages,
                    const void* v_pages, const int32_t* table, const int32_t* cu, const int32_t* rows, const int32_t* lens,
                    void* out, float* work, int64_t tokens, int64_t sequences, int64_t n_requests, int64_t max_pages,

@@ -927,14 +927,15 @@ hipError_t launch_attn_paged_t(const AttnPagedArgs& a, hipStream_t s) {
     int64_t tiles = ((int64_t)a.N * a.rep >> q.lrt) + a.B;
     if (q.which == kFew) tiles = std::min<int64_t>(tiles, (int64_t)a.B * (kFewRows >> q.lrt));
     const int64_t most = q.which == kMany ? std::max<int64_t>(tiles * a.Hkv, q.parts) : tiles * a.Hkv + q.target;
-    return (int)((std::min<int64_t>(most + 64, 1 << 23) + kTurn - 1) / kTurn * kTurn);
+    return (most + 64 + kTurn - 1) / kTurn * kTurn;
   };
-  const int few = grid(p.few), many = p.tiles ? grid(p.many) : 0;
+  const int64_t few = grid(p.few), many = p.tiles ? grid(p.many) : 0;
+  if (few + many >= 1 << 24) return hipErrorInvalidConfiguration;  // threads along x are counted in 32 bits
   static LdsLimit limit;
   const hipError_t e = limit.raise((const void*)attn_paged_kernel<BF, HD>, most_lds);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL((attn_paged_kernel<BF, HD>), dim3((unsigned)(few + many)), dim3(256), p.tiles ? most_lds : rows_lds, s, a,
-                     p.few, p.many, few, many);
+                     p.few, p.many, (int)few, (int)many);
   if (p.few.parts || p.many.parts) {
     const unsigned most = (unsigned)std::min<int64_t>((int64_t)a.N * a.H, 4 * a.cus);
     hipLaunchKernelGGL((attn_paged_merge_kernel<BF, HD>), dim3(most), dim3(64 * kMergeWaves), 0, s, a, p.few, p.many, (int)p.tiles);
