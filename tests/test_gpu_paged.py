@@ -520,3 +520,93 @@ def test_a_step_as_it_is_used():
         # q and k may each take the other neighbour of 16 bits, which moves a score by 2^-11 of the sum of its terms' sizes twice
         bound = R.attention_bound(want, size, score, dtype, hd, n) + 2 * 2 * 2.0 ** -11 * score * size
         assert bool(((torch.cat(outs[r]).cpu().double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("tokens", [4096, 4097, 9001])
+def test_page_plan_of_many_tokens(tokens):
+    """Sequences that are not served and rows behind the last among thousands of tokens."""
+    case = ([2, 0, 2, 4, 1, 3], [3000, 1, 9, 500, 400, 190], [70, 31, 5, 0, 900], [2, 1, 1, 0, 29], 130, 111, tokens, 32)
+    requests, new, lengths, held, table, free, n_free, tokens, page = _plan_state(case, R.gen(case))
+    d = _on_gpu(requests, new, lengths, held, table, free, n_free)
+    got = _paged().page_plan(*d, tokens=tokens, page_size=page)
+    want, n_free = R.plan(requests, new, lengths, held, table, free, n_free, tokens, page)
+    assert [x >= 0 for x in want[1]] == [True, True, False, True, False, False]
+    for name, x, y in zip(got._fields, got, want):
+        assert x.tolist() == y, name
+    assert d[4].tolist() == table and d[6].tolist() == [n_free]
+
+
+def test_caches_past_32_bits():
+    """Pages whose first element lies past 2^31 and past 2^32 bytes: as in a small cache."""
+    P = _paged()
+    H, G, hd, page, N = 8, 8, 256, 256, 300
+    g = R.gen("far")
+    x = torch.randn(N, H + 2 * G, hd, generator=g).to(BF16).cuda()
+    w = torch.ones(hd, dtype=BF16, device="cuda")
+    freq = (1e4 ** (-torch.arange(0, hd, 2).double() / hd)).cuda()
+    i32 = dict(dtype=torch.int32, device="cuda")
+    n_pages = 2 ** 31 // (G * page * hd) + 3
+    outs = []
+    for pages in (3, n_pages):
+        kp, vp = (torch.empty(pages, G, page, hd, dtype=BF16, device="cuda") for _ in range(2))
+        for c in (kp, vp):
+            c[-3:].zero_()
+        table = torch.tensor([[pages - 1, pages - 3]], **i32)
+        pos = torch.arange(N, device="cuda")
+        slots = table[0][pos // page].long() * page + pos % page
+        plan = P.PagePlan(torch.tensor([0, N], **i32), torch.tensor([0], **i32), torch.tensor([N], **i32), pos, slots)
+        q = P.paged_write(x[:, :H], x[:, H:H + G], x[:, H + G:], w, w, freq, kp, vp, pos, slots, eps=1e-6)
+        one = P.PagePlan(torch.tensor([0, 1], **i32), *plan[1:3], pos[-1:], slots[-1:])
+        outs.append((q, kp[-3:].clone(), vp[-3:].clone(), P.attn_paged(q, kp, vp, table, plan), P.attn_paged(q[-1:], kp, vp, table, one, max_new=1)))
+        del kp, vp
+    for a, b in zip(*outs):
+        assert torch.equal(a, b) and bool(torch.isfinite(a).all())
+
+
+def test_a_captured_step_of_all_kinds():
+    """Plan, write, attend, recur and advance in one graph: every replay as the eager calls, which run between them on
+    states of their own."""
+    P = _paged()
+    H, G, hd, page, N, hk, hv, dk = 6, 2, 64, 16, 100, 2, 4, 64
+    g = R.gen("captured")
+    conv_dim = 2 * hk * dk + hv * dk
+    x, z, ab = (torch.randn(N, n, generator=g).to(F16).cuda() for n in ((H + 2 * G) * hd + conv_dim, hv * dk, 2 * hv))
+    qkv = x[:, :(H + 2 * G) * hd].view(N, H + 2 * G, hd)
+    w, nw = torch.ones(hd, dtype=F16, device="cuda"), torch.ones(dk, dtype=F16, device="cuda")
+    freq = (1e4 ** (-torch.arange(0, 32, 2).double() / 32)).cuda()
+    conv_w = (0.5 * torch.randn(conv_dim, 4, generator=g)).to(F16).cuda()
+    ssm_a, dt_bias = -torch.ones(hv, device="cuda"), torch.zeros(hv, device="cuda")
+    i32 = dict(dtype=torch.int32, device="cuda")
+    new = torch.zeros(3, **i32)
+    requests = torch.tensor([3, 0, 1], **i32)
+
+    def state():
+        kp, vp = (torch.zeros(40, G, page, hd, dtype=F16, device="cuda") for _ in range(2))
+        return dict(kp=kp, vp=vp, lengths=torch.zeros(4, **i32), held=torch.zeros(4, **i32), table=torch.full((4, 12), -1, **i32),
+                    free=torch.arange(40, **i32), n_free=torch.tensor([40], **i32),
+                    conv=torch.zeros(4, 3, conv_dim, dtype=F16, device="cuda"), rec=torch.zeros(4, hv, dk, dk, device="cuda"))
+
+    def step(s):
+        plan = P.page_plan(requests, new, s["lengths"], s["held"], s["table"], s["free"], s["n_free"], tokens=N, page_size=page)
+        q = P.paged_write(qkv[:, :H], qkv[:, H:H + G], qkv[:, H + G:], w, w, freq, s["kp"], s["vp"], plan.pos, plan.slots, eps=1e-6)
+        a = P.attn_paged(q, s["kp"], s["vp"], s["table"], plan)
+        o = P.gdn_packed(x[:, -conv_dim:], z, ab, s["conv"], conv_w, ssm_a, dt_bias, s["rec"], nw, plan, key_heads=hk, value_heads=hv,
+                         head_k_dim=dk, head_v_dim=dk, eps=1e-6)
+        P.page_advance(plan, s["lengths"])
+        return [*plan, a, o]
+    captured, eager = state(), state()
+    step(state())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(captured)
+    for i, n in enumerate(([30, 0, 1], [1, 70, 20], [1, 1, 1], [80, 3, 17], [500, 1, 1])):
+        new.copy_(torch.tensor(n, **i32))
+        graph.replay()
+        want = step(eager)
+        torch.cuda.synchronize()
+        for j, (a, b) in enumerate(zip(got, want)):
+            assert torch.equal(a.nan_to_num(nan=7.), b.nan_to_num(nan=7.)), (i, j)
+        for name in eager:
+            assert torch.equal(captured[name], eager[name]), (i, name)
+    assert eager["lengths"].tolist() == [74, 39, 0, 112]
