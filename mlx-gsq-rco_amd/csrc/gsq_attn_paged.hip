@@ -234,15 +234,16 @@ __device__ __forceinline__ void clear_tail(const AttnPagedArgs& a) {
 
 // The softmax and the sums of a wave's 16 NT rows over the positions it has seen. Weights are powers of two over a
 // reference m that moves only when a score passes it by 2^kLazy, for all rows of the wave at once: mostly no rescaling
-// and no exchange between lanes in the loop. They are held in two 16-bit values, cut off and the rest: fp16 times
-// 2^kScale (22 bits; 2^15 at most), bf16 16 bits (2^-17 of a weight; with one value of 8 bits outputs would be off by 1.4
-// times their rounding), small enough that sums of V rows next to float32's largest number stay finite.
+// and no exchange between lanes in the loop. They are held in kTerms 16-bit values, cut off and the rests: two of fp16 times
+// 2^kScale (22 bits; 2^15 at most), three of bf16 (all 24 bits; two are 2^-17 of a weight off, which moved one output in
+// some hundreds to its rounding's other neighbour; prompts of 2001 249 us with two and 280 with three), small enough that
+// sums of V rows next to float32's largest number stay finite.
 constexpr float kLazy = 6.f;
 
 template <bool BF, int HD, int NT>
 struct PagedRows {
   using E = Half<BF>;
-  static constexpr int VB = HD / 16;
+  static constexpr int VB = HD / 16, kTerms = BF ? 3 : 2;
   static constexpr float kScale = BF ? -24.f : 9.f;  // log2
   float m[NT], l[NT];  // l: this lane's share of the sum
   f32x4 acc[NT][VB];
@@ -259,7 +260,7 @@ struct PagedRows {
   // scores s of 16 NB positions to weights pf (and, in s, as float32); last[n]: the last position that the lane's row
   // n sees, as an offset from the first of these
   template <int NB>
-  __device__ void weights(f32x4 (&s)[NT][NB], bool masked, const int (&last)[NT], u32x4 (&pf)[NB / 2][2][NT]) {
+  __device__ void weights(f32x4 (&s)[NT][NB], bool masked, const int (&last)[NT], u32x4 (&pf)[NB / 2][kTerms][NT]) {
     const int g = (threadIdx.x & 63) >> 4;
     const float c = 1.44269504088896340736f / sqrtf((float)HD);
     float mx[NT];
@@ -308,19 +309,27 @@ struct PagedRows {
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const f32x2 p = j ? s[n][b].zw : s[n][b].xy;
-          const uint32_t hi = E::chop(p);
-          pf[b / 2][0][n][2 * (b & 1) + j] = hi;
-          pf[b / 2][1][n][2 * (b & 1) + j] =
-              __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, E::rest(p, hi)), least));
+          f32x2 p = j ? s[n][b].zw : s[n][b].xy;
+          uint32_t w = E::chop(p);
+          pf[b / 2][0][n][2 * (b & 1) + j] = w;
+#pragma unroll
+          for (int t = 1; t < kTerms; ++t) {
+            if (t + 1 < kTerms) {
+              p -= E::unpack(w);
+              w = E::chop(p);
+            } else {
+              w = E::rest(p, w);
+            }
+            pf[b / 2][t][n][2 * (b & 1) + j] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, w), least));
+          }
         }
       }
     }
   }
   // output tile i += V's operand times the weights
-  __device__ void add(int i, u32x4 vf, const u32x4 (&pf)[2][NT]) {
+  __device__ void add(int i, u32x4 vf, const u32x4 (&pf)[kTerms][NT]) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < kTerms; ++t)
 #pragma unroll
       for (int n = 0; n < NT; ++n) acc[n][i] = E::mma(vf, pf[t][n], acc[n][i]);
   }
@@ -476,7 +485,7 @@ __device__ __forceinline__ void paged_rows(const AttnPagedArgs& a, const PagedSc
     }
     const int last[1] = {qpos - 32 * blk};
     const bool masked = 32 * blk + 31 > k.pos + tfirst;
-    u32x4 pf[1][2][1];
+    u32x4 pf[1][decltype(rows)::kTerms][1];
     rows.weights(s, masked, last, pf);
 #pragma unroll
     for (int h = 0; h < NP; ++h) {
@@ -715,7 +724,7 @@ __device__ __forceinline__ void paged_tile(const AttnPagedArgs& a, const PagedSc
 #pragma unroll
       for (int n = 0; n < NT; ++n) last[n] = qpos[n] - js;
       const bool masked = js + 31 > pfirst;
-      u32x4 pf[1][2][NT];
+      u32x4 pf[1][decltype(rows)::kTerms][NT];
       rows.weights(s, masked, last, pf);
 #pragma unroll
       for (int i = 0; i < VB; ++i) {
