@@ -236,7 +236,7 @@ __device__ __forceinline__ void clear_tail(const AttnPagedArgs& a) {
 // reference m that moves only when a score passes it by 2^kLazy, for all rows of the wave at once: mostly no rescaling
 // and no exchange between lanes in the loop. They are held in kTerms 16-bit values, cut off and the rests: two of fp16 times
 // 2^kScale (22 bits; 2^15 at most), three of bf16 (all 24 bits; two are 2^-17 of a weight off, which moved one output in
-// some hundreds to its rounding's other neighbour; prompts of 2001 249 us with two and 280 with three), small enough that
+// some hundreds to its rounding's other neighbour; prompts of 2001 249 us with two and 283 with three), small enough that
 // sums of V rows next to float32's largest number stay finite.
 constexpr float kLazy = 6.f;
 
@@ -294,7 +294,8 @@ struct PagedRows {
         for (int i = 0; i < VB; ++i) acc[n][i] *= alpha;
       }
     }
-    // a rest of 0 times a visible V of infinity would be NaN, where its weight is not 0 and the sum is infinite
+    // a rest of 0 times a visible V of infinity would be NaN, where its weight is not 0 and the sum is infinite. Weights that
+    // are 0 stay 0: below 2^-34 of the reference's in fp16, which thousands of positions would otherwise all weigh
     const uint16_t one = masked ? 0 : E::kLeast;
     const u16x2 least = {one, one};
 #pragma unroll
@@ -312,6 +313,7 @@ struct PagedRows {
           f32x2 p = j ? s[n][b].zw : s[n][b].xy;
           uint32_t w = E::chop(p);
           pf[b / 2][0][n][2 * (b & 1) + j] = w;
+          const u16x2 floor = __builtin_elementwise_min(__builtin_bit_cast(u16x2, w), least);
 #pragma unroll
           for (int t = 1; t < kTerms; ++t) {
             if (t + 1 < kTerms) {
@@ -320,7 +322,7 @@ struct PagedRows {
             } else {
               w = E::rest(p, w);
             }
-            pf[b / 2][t][n][2 * (b & 1) + j] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, w), least));
+            pf[b / 2][t][n][2 * (b & 1) + j] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, w), floor));
           }
         }
       }

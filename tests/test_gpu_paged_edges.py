@@ -8,7 +8,7 @@ if not torch.cuda.is_available():
     pytest.skip("no GPU", allow_module_level=True)
 
 import paged_ref as R  # noqa: E402
-from test_gpu_paged import _attend, _attn_inputs  # noqa: E402
+from test_gpu_paged import _attend, _attn_inputs, _paged  # noqa: E402
 
 F16, BF16 = torch.float16, torch.bfloat16
 
@@ -39,3 +39,20 @@ def test_weights_keep_22_bits(dtype, hd, rep):
     if dtype is BF16:
         bound -= (2.0 ** -16 - 2.0 ** -22) * size
     assert bool(((got.double() - want).abs() <= bound).all()), float(((got.double() - want).abs() - bound).max())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["fp16", "bf16"])
+def test_positions_of_no_weight_add_nothing(dtype):
+    """A first position that everybody looks at, 60000 behind it with weights e^-40 of its own and a large V: nothing of
+    that V reaches the outputs. 512 single tokens, then a prompt, each enough to leave the positions in long pieces; the
+    sequences share their pages."""
+    L, hd, P = 60000, 64, _paged()
+    kp, vp = torch.full((235, 1, 256, hd), -2.5, dtype=dtype, device="cuda"), torch.full((235, 1, 256, hd), 1000.0, dtype=dtype, device="cuda")
+    kp[0, 0, 0], vp[0, 0, 0] = 2.5, 0.0
+    i32 = dict(dtype=torch.int32, device="cuda")
+    for B, n, heads in ((512, 1, 4), (1, 8192, 64)):
+        table = torch.arange(235, **i32).expand(B, -1).contiguous()
+        cu, rows, lens = torch.arange(B + 1, **i32) * n, torch.arange(B, **i32), torch.full((B,), L, **i32)
+        q = torch.ones(B * n, heads, hd, dtype=dtype, device="cuda")
+        # 60000 * 1000 * e^-40 = 3e-10; a V of 1000 at 2^-33 of the first one's weight for each position would be 7e-3
+        assert float(P.attn_paged(q, kp, vp, table, P.PagePlan(cu, rows, lens, rows, rows), max_new=n).abs().max()) <= 1e-6
