@@ -491,7 +491,7 @@ __device__ __forceinline__ void paged_rows(const AttnPagedArgs& a, const PagedSc
     rows.weights(s, masked, last, pf);
 #pragma unroll
     for (int h = 0; h < NP; ++h) {
-      if (masked && tfirst != tlast) {
+      if (masked) {  // a single token too: places behind its position repeat its row with a weight of 0
         bool odd = false;
 #pragma unroll
         for (int i = 0; i < 8; ++i)

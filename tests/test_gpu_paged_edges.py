@@ -11,6 +11,7 @@ import paged_ref as R  # noqa: E402
 from test_gpu_paged import _attend, _attn_inputs, _paged  # noqa: E402
 
 F16, BF16 = torch.float16, torch.bfloat16
+INF, NAN = float("inf"), float("nan")
 
 
 # ---- attention: bits of the weights ----------------------------------------------------------------
@@ -56,3 +57,23 @@ def test_positions_of_no_weight_add_nothing(dtype):
         q = torch.ones(B * n, heads, hd, dtype=dtype, device="cuda")
         # 60000 * 1000 * e^-40 = 3e-10; a V of 1000 at 2^-33 of the first one's weight for each position would be 7e-3
         assert float(P.attn_paged(q, kp, vp, table, P.PagePlan(cu, rows, lens, rows, rows), max_new=n).abs().max()) <= 1e-6
+
+
+# ---- attention: values that are not finite ---------------------------------------------------------
+
+@pytest.mark.parametrize("at", [0, 20, 34, 40], ids=["block before", "middle", "last block", "own"])
+@pytest.mark.parametrize("cached", [40, 300])
+@pytest.mark.parametrize("value", [INF, -INF, NAN])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_a_single_token_sees_what_is_not_finite(hd, value, cached, at):
+    """V of infinity at a position that a single token sees is its output, wherever in its blocks that is."""
+    at += cached - 40
+    for dtype in (F16, BF16):
+        q, kp, vp, table, plan, gate = _attn_inputs([cached, 3], [1, 1], 16, 6, 2, hd, dtype, key=("one", hd, cached), k_size=0.1)
+        row = int(plan[1][0])
+        vp[table[row, at // 16], :, at % 16, 5] = value
+        for g in (None, gate):
+            got = _attend(q, kp, vp, table, plan, g)
+            keep = torch.arange(hd) != 5
+            assert bool(torch.isfinite(got[0][:, keep]).all()) and bool(torch.isfinite(got[1]).all())
+            assert bool((torch.isnan(got[0][:, 5]) if value != value else got[0][:, 5] == value).all())
