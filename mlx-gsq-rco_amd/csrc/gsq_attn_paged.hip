@@ -344,8 +344,8 @@ struct PagedRows {
 };
 
 // V rows that some of a tile's rows do not see would reach those as 0 x NaN if they are not finite. Blocks with such
-// positions are looked at: values that are not finite are taken out of the product, and put into the outputs that see them
-// when the sums are done (odd_sum).
+// positions are looked at: values that are not finite are taken out of the product, and added to the sums that see them
+// at the end (odd_sum).
 template <bool BF>
 __device__ __forceinline__ bool odd_pair(uint32_t w) {  // whether a pair of values holds one that is not finite
   const uint32_t e = BF ? 0x7F80u : 0x7C00u;
@@ -740,6 +740,27 @@ __device__ __forceinline__ void paged_tile(const AttnPagedArgs& a, const PagedSc
   if (lane == 0) bad_s[wave] = bad;
   __syncthreads();
   bad = bad_s[0] | bad_s[1] | bad_s[2] | bad_s[3];
+  if (any_odd) {  // of the piece's positions in blocks that were looked at, to the sums: through the wave's share of LDS
+    constexpr int DW = HD < 128 ? HD : 128;  // dims at a time
+    static_assert(32 * DW * 4 <= TB);
+    float* const x = reinterpret_cast<float*>(paged_lds + wave * TB);
+    const int ln = anew(lane), g = ln >> 4, c = ln & 15;
+    const int from = max(32 * blk0, wfirst + 1 - KT);
+#pragma unroll
+    for (int d0 = 0; d0 < HD; d0 += DW) {
+#pragma unroll 1
+      for (int i = ln; i < 32 * DW; i += 64) {
+        const int r = rw + i / DW;
+        x[i] = r < k.rows ? odd_sum<BF, HD>(a, table, k.kvh, d0 + i % DW, from, min(j_end - 1, k.pos + token_of(a, r))) : 0.f;
+      }
+      __builtin_amdgcn_wave_barrier();  // a wave's LDS operations complete in order
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < DW / 16; ++i) rows.acc[n][d0 / 16 + i] += *reinterpret_cast<const f32x4*>(x + (16 * n + c) * DW + 16 * i + 4 * g);
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
   // a lane's outputs: row rw + 16 n + c, dims 16 i + 4 g + e
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
@@ -758,19 +779,6 @@ __device__ __forceinline__ void paged_tile(const AttnPagedArgs& a, const PagedSc
       } else {
         put<BF, 4>(a, i0, g0, 16 * i + 4 * g, v);
       }
-    }
-  }
-  if (any_odd) {  // over what was stored: the piece's positions in blocks that were looked at
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    const int from = max(32 * blk0, wfirst + 1 - KT);
-#pragma unroll 1
-    for (int i = lane; i < 32 * HD; i += 64) {
-      const int r = rw + i / HD, d = i % HD;
-      if (r >= k.rows) break;
-      const float x = odd_sum<BF, HD>(a, table, k.kvh, d, from, min(j_end - 1, k.pos + token_of(a, r)));
-      if (x == 0.f) continue;
-      if (k.nz > 1) a.part[p.part_at + (k.part * kTileRows + (r - k.r0)) * (HD + 2) + d] = x;
-      else static_cast<uint16_t*>(a.out)[k.at(a, r) * HD + d] = E::mk(x);
     }
   }
 }

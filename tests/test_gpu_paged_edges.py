@@ -77,3 +77,41 @@ def test_a_single_token_sees_what_is_not_finite(hd, value, cached, at):
             keep = torch.arange(hd) != 5
             assert bool(torch.isfinite(got[0][:, keep]).all()) and bool(torch.isfinite(got[1]).all())
             assert bool((torch.isnan(got[0][:, 5]) if value != value else got[0][:, 5] == value).all())
+
+
+@pytest.mark.parametrize("cached", [0, 700])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["fp16", "bf16"])
+def test_prompts_add_up_what_is_not_finite(dtype, hd, cached):
+    """A prompt's rows that see a V of infinity among places that others do not see: NaN where the row is NaN for another
+    reason (a score, a gate, an infinity of the other sign), infinite elsewhere; the gate's sign and NaN count."""
+    n = 60
+    q, kp, vp, table, plan, gate = _attn_inputs([cached], [n], 16, 6, 1, hd, dtype, key=("sum", hd, cached), k_size=0.1)
+    row = int(plan[1][0])
+
+    def at(t, p=cached):
+        return table[row, (p + t) // 16], 0, (p + t) % 16
+    vp[at(30)][5] = INF
+    vp[at(40)][5] = -INF
+    vp[at(20)][7] = -INF
+    q[50, 2, 0] = NAN
+    gate[25, 1, hd + 7], gate[33, 0, hd + 5], gate[34, 0, hd + 5] = NAN, NAN, -INF
+    if cached:  # seen by all
+        vp[at(0, 100)][9] = INF
+        vp[at(45)][9] = -INF
+    want = torch.zeros(n, 6, hd)
+    want[30:, :, 5] = INF
+    want[40:, :, 5] = NAN
+    want[20:, :, 7] = -INF
+    if cached:
+        want[:, :, 9] = INF
+        want[45:, :, 9] = NAN
+    want[50, 2] = NAN
+    for g in (None, gate):
+        w = want.clone()
+        if g is not None:
+            w[25, 1, 7] = w[33, 0, 5] = w[34, 0, 5] = NAN
+        got = _attend(q, kp, vp, table, plan, g)
+        odd = ~torch.isfinite(w)
+        assert torch.equal(torch.isfinite(got), ~odd)
+        assert torch.equal(got[odd].float().nan_to_num(nan=7.0), w[odd].nan_to_num(nan=7.0))
