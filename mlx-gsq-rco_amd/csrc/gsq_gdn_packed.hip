@@ -13,19 +13,16 @@ namespace gsq {
 
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
-// q and k values, at most 1, are held as two fp16 numbers of 2^12 times them (22 bits, down to 2^-37): what the matrix
-// cores take, in float32's room. The low half of a word is the first, the high half the rest.
+// q and k values, at most 1, enter the scan's products as two fp16 numbers of 2^12 times them (22 bits, down to 2^-37). The
+// low half of a word is the first, the high half the rest.
 __device__ __forceinline__ uint32_t split22(float x) {
   const float v = x * 4096.f;
   const _Float16 h = (_Float16)v, l = (_Float16)(v - (float)h);
   return (uint32_t)__builtin_bit_cast(uint16_t, h) | ((uint32_t)__builtin_bit_cast(uint16_t, l) << 16);
 }
-__device__ __forceinline__ float join22(uint32_t w) {
-  return (Half<false>::ld((uint16_t)w) + Half<false>::ld((uint16_t)(w >> 16))) * (1.f / 4096.f);
-}
-// eight words to operands of first halves and of rests
-__device__ __forceinline__ void halves8(u32x4 a, u32x4 b, u32x4& hi, u32x4& lo) {
-  const uint32_t w[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+// eight values to operands of first halves and of rests
+__device__ __forceinline__ void halves8(f32x4 a, f32x4 b, u32x4& hi, u32x4& lo) {
+  const uint32_t w[8] = {split22(a[0]), split22(a[1]), split22(a[2]), split22(a[3]), split22(b[0]), split22(b[1]), split22(b[2]), split22(b[3])};
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     hi[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x05040100u);
@@ -44,7 +41,7 @@ constexpr int kConvMax = 8;  // inputs of a convolution window at most
 // Convolution + SiLU of 128 channels (2 per lane) over the packed tokens TPB blockIdx.y .. + TPB - 1, whose inputs are all
 // asked for at once; the window slides in registers from one token of a sequence to the next. q and k channels are
 // RMS-normalized over their head (dk / 2 lanes, a power of two) and scaled, so that `work` holds [q | k | v] rows ready
-// for the recurrence (q and k as split22 words). The states are
+// for the recurrence, in float32. The states are
 // read only: tokens of one window lie in different workgroups, so the launch behind this one advances them.
 // KW: window of the convolution (kConvMax: any up to it). Bound by its bytes where tokens are many (5118 of 10240 channels:
 // 314 MB in 72 us, 4.4 TB/s), by its latencies where they are few (32: 4 us).
@@ -131,8 +128,7 @@ __global__ void __launch_bounds__(256) gdn_conv_packed_kernel(GdnPackedArgs a, b
         y1 = y1 * rn * sc;
       }
     }
-    float2* const to = reinterpret_cast<float2*>(a.work + (int64_t)t * conv_dim + c);
-    if (on) *to = c < 2 * key_dim ? make_float2(__builtin_bit_cast(float, split22(y0)), __builtin_bit_cast(float, split22(y1))) : make_float2(y0, y1);
+    if (on) *reinterpret_cast<float2*>(a.work + (int64_t)t * conv_dim + c) = make_float2(y0, y1);
   }
 }
 
@@ -208,8 +204,8 @@ __global__ void __launch_bounds__(256) gdn_rec_packed_kernel(GdnPackedArgs a, in
     float k[NR], q[NR];
 #pragma unroll
     for (int j = 0; j < NR; ++j) {
-      q[j] = join22(__builtin_bit_cast(uint32_t, row[kh * DK + rg + j * NG]));
-      k[j] = join22(__builtin_bit_cast(uint32_t, row[key_dim + kh * DK + rg + j * NG]));
+      q[j] = row[kh * DK + rg + j * NG];
+      k[j] = row[key_dim + kh * DK + rg + j * NG];
     }
     const f32x4 v = *reinterpret_cast<const f32x4*>(row + 2 * key_dim + h * DV + col);
     const float av = E::ld(abr[h]) + dtb, bv = E::ld(abr[a.Hv + h]);
@@ -323,23 +319,14 @@ __global__ void __launch_bounds__(256) gdn_chunk_kernel(GdnPackedArgs a, float* 
     bj[p] = wave == 0 ? BJ[0][p] : wave == 1 ? BJ[1][p] : wave == 2 ? BJ[2][p] : BJ[3][p];
     kk[p] = qk[p] = (f32x4){0.f, 0.f, 0.f, 0.f};
     if (bi[p] < 0) continue;
-    const uint32_t* const words = reinterpret_cast<const uint32_t*>(a.work);
-    const uint32_t* const qi = words + (t0 + min(16 * bi[p] + c, n - 1)) * conv_dim + kh * DK + 8 * g;
-    const uint32_t* const kj = words + (t0 + min(16 * bj[p] + c, n - 1)) * conv_dim + key_dim + kh * DK + 8 * g;
-    auto load = [&](const uint32_t* at, u32x4& hi, u32x4& lo) {
-      halves8(*reinterpret_cast<const u32x4*>(at), *reinterpret_cast<const u32x4*>(at + 4), hi, lo);
-    };
+    const float* const qi = a.work + (t0 + min(16 * bi[p] + c, n - 1)) * conv_dim + kh * DK + 4 * g;
+    const float* const kj = a.work + (t0 + min(16 * bj[p] + c, n - 1)) * conv_dim + key_dim + kh * DK + 4 * g;
 #pragma unroll
-    for (int s = 0; s < DK / 32; ++s) {
-      u32x4 bh, bl, ah, al;
-      load(kj + 32 * s, bh, bl);
-      load(qi + 32 * s, ah, al);
-      qk[p] = mma22(ah, al, bh, bl, qk[p]);
-      load(qi + key_dim + 32 * s, ah, al);
-      kk[p] = mma22(ah, al, bh, bl, kk[p]);
+    for (int s = 0; s < DK / 16; ++s) {
+      const f32x4 b = *reinterpret_cast<const f32x4*>(kj + 16 * s);
+      qk[p] = mma4(*reinterpret_cast<const f32x4*>(qi + 16 * s), b, qk[p]);
+      kk[p] = mma4(*reinterpret_cast<const f32x4*>(qi + key_dim + 16 * s), b, kk[p]);
     }
-    qk[p] *= 0x1p-24f;
-    kk[p] *= 0x1p-24f;
   }
   for (int h = kh; h < a.Hv; h += a.Hk) {
     if (wave == 0) {
@@ -414,7 +401,7 @@ __global__ void __launch_bounds__(256) gdn_chunk_kernel(GdnPackedArgs a, float* 
 // The chain over a sequence's chunks, for 32 columns of a value head's state: its tiles stay in registers (32 rows to each
 // of the first waves), a copy in LDS is the products' operand. Wave w holds tokens 16 w .. of a chunk. What goes into the
 // state's products is held in two fp16 numbers (22 bits: the state and left u times a power of two for each 32 rows, 16
-// tokens; q and k as split22 words), for the 16-bit matrix instructions; u and the outputs inside the chunk are float32
+// tokens; q and k by split22), for the 16-bit matrix instructions; u and the outputs inside the chunk are float32
 // products. Bound by the chain: a chunk's operands come from L2 a chunk ahead, two workgroups to a CU.
 // Columns: 64 read q, k, T and P half as often but leave one workgroup to a CU (3 prompts of 2047, 48 heads: 691 against
 // 635 us for the whole call).
@@ -435,8 +422,8 @@ __global__ void __launch_bounds__(256, 2) gdn_scan_kernel(GdnPackedArgs a, const
   const PackedSeq sq(a.cu, a.rows, a.lens, b, a.N, a.R, 0x7FFFFFFF);
   if (!sq.fine || sq.n < long_from) return;
   const int key_dim = a.Hk * DK, conv_dim = 2 * key_dim + a.Hv * a.dv, vdim = a.Hv * a.dv, n = sq.n;
-  const uint32_t* const wq = reinterpret_cast<const uint32_t*>(a.work) + (int64_t)sq.t0 * conv_dim + kh * DK;
-  const uint32_t* const wk = wq + key_dim;
+  const float* const wq = a.work + (int64_t)sq.t0 * conv_dim + kh * DK;
+  const float* const wk = wq + key_dim;
   const float* const wv = a.work + (int64_t)sq.t0 * conv_dim + 2 * key_dim + h * a.dv + col0;
   float* const o_at = ow + (int64_t)sq.t0 * vdim + h * a.dv + col0;
   const uint16_t* const ab = static_cast<const uint16_t*>(a.ab) + (int64_t)sq.t0 * a.ab_stride;
@@ -505,8 +492,7 @@ __global__ void __launch_bounds__(256, 2) gdn_scan_kernel(GdnPackedArgs a, const
   }
   // what a chunk reads from memory is asked for a chunk before it is used, when its registers have been read
   constexpr int KQ = DK / 32;
-  u32x4 q4[KQ][2], k4[KQ][2], kt[2][4];
-  f32x4 v4[CT], t4[4], p4[4], grown, left, beta;
+  f32x4 q4[KQ][2], k4[KQ][2], kt[2][4], v4[CT], t4[4], p4[4], grown, left, beta;
   float all;
   auto load_rows = [&](int t0) {  // tokens behind the last repeat it
     const int m = min(kChunk, n - t0);
@@ -515,8 +501,8 @@ __global__ void __launch_bounds__(256, 2) gdn_scan_kernel(GdnPackedArgs a, const
     for (int s = 0; s < KQ; ++s)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        q4[s][e] = *reinterpret_cast<const u32x4*>(wq + row * conv_dim + 32 * s + 8 * g + 4 * e);
-        k4[s][e] = *reinterpret_cast<const u32x4*>(wk + row * conv_dim + 32 * s + 8 * g + 4 * e);
+        q4[s][e] = *reinterpret_cast<const f32x4*>(wq + row * conv_dim + 32 * s + 8 * g + 4 * e);
+        k4[s][e] = *reinterpret_cast<const f32x4*>(wk + row * conv_dim + 32 * s + 8 * g + 4 * e);
       }
 #pragma unroll
     for (int t = 0; t < CT; ++t)
@@ -631,7 +617,7 @@ __global__ void __launch_bounds__(256, 2) gdn_scan_kernel(GdnPackedArgs a, const
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const u32x4 w = kt[i][l];
+          const u32x4 w = {split22(kt[i][l][0]), split22(kt[i][l][1]), split22(kt[i][l][2]), split22(kt[i][l][3])};
           const uint2 hw = make_uint2(__builtin_amdgcn_perm(w[1], w[0], 0x05040100u), __builtin_amdgcn_perm(w[3], w[2], 0x05040100u));
           const uint2 lw = make_uint2(__builtin_amdgcn_perm(w[1], w[0], 0x07060302u), __builtin_amdgcn_perm(w[3], w[2], 0x07060302u));
           const f16x4 ah = __builtin_bit_cast(f16x4, hw), al = __builtin_bit_cast(f16x4, lw);
@@ -685,14 +671,14 @@ __global__ void __launch_bounds__(256, 2) gdn_scan_kernel(GdnPackedArgs a, const
 #pragma unroll
       for (int i = 0; i < NR; ++i) {
         s[i] *= decay;
-        p += s[i] * join22(wk[(int64_t)t * conv_dim + x + 8 * i]);
+        p += s[i] * wk[(int64_t)t * conv_dim + x + 8 * i];
       }
       const float d = (wv[(int64_t)t * conv_dim + y] - total(p)) * beta;
       p = 0.f;
 #pragma unroll
       for (int i = 0; i < NR; ++i) {
-        s[i] += d * join22(wk[(int64_t)t * conv_dim + x + 8 * i]);
-        p += s[i] * join22(wq[(int64_t)t * conv_dim + x + 8 * i]);
+        s[i] += d * wk[(int64_t)t * conv_dim + x + 8 * i];
+        p += s[i] * wq[(int64_t)t * conv_dim + x + 8 * i];
       }
       const float o = total(p);
       if (x == 0) o_at[(int64_t)t * vdim + y] = o;

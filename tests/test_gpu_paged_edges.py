@@ -8,7 +8,7 @@ if not torch.cuda.is_available():
     pytest.skip("no GPU", allow_module_level=True)
 
 import paged_ref as R  # noqa: E402
-from test_gpu_paged import _attend, _attn_inputs, _paged  # noqa: E402
+from test_gpu_paged import _attend, _attn_inputs, _gdn_inputs, _paged, _run_gdn  # noqa: E402
 
 F16, BF16 = torch.float16, torch.bfloat16
 INF, NAN = float("inf"), float("nan")
@@ -115,3 +115,59 @@ def test_prompts_add_up_what_is_not_finite(dtype, hd, cached):
         odd = ~torch.isfinite(w)
         assert torch.equal(torch.isfinite(got), ~odd)
         assert torch.equal(got[odd].float().nan_to_num(nan=7.0), w[odd].nan_to_num(nan=7.0))
+
+
+# ---- GatedDeltaNet: small rows and columns ---------------------------------------------------------
+
+def _one_head(n, K=4, dv=64, dk=128):
+    """One head of n tokens from a cached state, its convolution the current token's input alone, so that its outputs have
+    their inputs' bits. Returns the call's tensors (test_gpu_paged._gdn_inputs) and the plan."""
+    case = ([5], [n], 1, 1, dk, dv, K, BF16)
+    t, plan = _gdn_inputs(case)
+    t = [x.clone() for x in t]
+    t[4].zero_()
+    t[4][:, -1] = 1
+    t[5][:], t[6][:] = -0.05, 0.0
+    return case, t, plan
+
+
+@pytest.mark.parametrize("size", [1e-5, 1e-7, 1e-9, 1e-15])
+@pytest.mark.parametrize("which", ["q", "k"])
+@pytest.mark.parametrize("n", [1, 9])
+def test_small_rows_keep_their_bits(n, which, size):
+    """q or k rows far below the norm's epsilon enter the recurrence with float32's bits: with small q the outputs, with
+    small k what the state gains from zero, relative to what they are."""
+    case, t, plan = _one_head(n)
+    dk, dv = 128, 64
+    cols = slice(0, dk) if which == "q" else slice(dk, 2 * dk)
+    t[0][:, cols] = (t[0][:, cols].float() * size).bfloat16()
+    if which == "k":
+        plan = list(plan)
+        plan[2] = torch.tensor([n], dtype=torch.int32)  # from zeros
+    out, conv, rec = _run_gdn(case, t, plan)
+    want, _, want_rec, scale = R.gdn(*t, *plan[:3], 1, 1, dk, dv, 1e-6)
+    r = int(plan[1][0])
+    # float32: 16 roundings on the way to q and k, sums of 128 rows and of up to n tokens. Matrix cores truncate:
+    # 2^-22 for every 8 terms
+    rel = (16 + dk / 8 + n / 4) * 2.0 ** -22
+    if which == "k":
+        # rows of the state are sums of k_t u_t, u_t at most 2 |v_t| (k is small: what the state gives back is smaller still)
+        x = t[0].double()
+        k = x[:, cols]
+        k = (k * torch.sigmoid(k)).abs()
+        k = k / (k.square().mean(-1, keepdim=True) + 1e-6).sqrt() / dk ** 0.5
+        v = x[:, 2 * dk:]
+        terms = k.T @ (2 * (v * torch.sigmoid(v)).abs())
+        err = (rec[r, 0].double() - want_rec[r, 0]).abs()
+        assert bool((err <= rel * terms).all()), float((err / terms).max())
+        assert float(want_rec[r].abs().max()) > 0
+    else:
+        # an output is a sum over rows of q_i S_i: sizes from the largest entry of the state on its way
+        x = t[0].double()[:, cols]
+        q = (x * torch.sigmoid(x)).abs()
+        q = q / (q.square().mean(-1, keepdim=True) + 1e-6).sqrt() / dk
+        top = float(t[7][r].abs().max()) + 2 * float(t[0][:, 2 * dk:].abs().max()) * n ** 0.5
+        # o over the norm's root, which is at least 1e-3
+        terms = q.sum(-1, keepdim=True) * top * 1e3 * scale
+        err = (out.double() - want).abs()
+        assert bool((err <= torch.finfo(BF16).eps / 2 * want.abs() + rel * terms).all()), float(((err - 2.0 ** -8 * want.abs()) / terms).max())
