@@ -11,29 +11,43 @@
 
 namespace gsq {
 
-typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-
-// q and k values, at most 1, enter the scan's products as two fp16 numbers of 2^12 times them (22 bits, down to 2^-37). The
-// low half of a word is the first, the high half the rest.
-__device__ __forceinline__ uint32_t split22(float x) {
-  const float v = x * 4096.f;
-  const _Float16 h = (_Float16)v, l = (_Float16)(v - (float)h);
-  return (uint32_t)__builtin_bit_cast(uint16_t, h) | ((uint32_t)__builtin_bit_cast(uint16_t, l) << 16);
+// Eight float32 values as three bf16 numbers each, cut off one after the other: exactly their 24 bits, of any size.
+struct Three {
+  u32x4 h, m, l;
+};
+__device__ __forceinline__ float cut16(float x) { return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & 0xFFFF0000u); }
+__device__ __forceinline__ uint32_t upper16(float x, float y) {
+  return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, y), __builtin_bit_cast(uint32_t, x), 0x07060302u);
 }
-// eight values to operands of first halves and of rests
-__device__ __forceinline__ void halves8(f32x4 a, f32x4 b, u32x4& hi, u32x4& lo) {
-  const uint32_t w[8] = {split22(a[0]), split22(a[1]), split22(a[2]), split22(a[3]), split22(b[0]), split22(b[1]), split22(b[2]), split22(b[3])};
+// a pair of values
+__device__ __forceinline__ void split3(float x, float y, uint32_t& h, uint32_t& m, uint32_t& l) {
+  h = upper16(x, y);
+  x -= cut16(x);
+  y -= cut16(y);
+  m = upper16(x, y);
+  l = upper16(x - cut16(x), y - cut16(y));
+}
+__device__ __forceinline__ Three split3(f32x4 a, f32x4 b) {
+  Three r;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    hi[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x05040100u);
-    lo[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x07060302u);
+    const f32x4 v = j < 2 ? a : b;
+    uint32_t h, m, l;
+    split3(v[2 * (j & 1)], v[2 * (j & 1) + 1], h, m, l);
+    r.h[j] = h;
+    r.m[j] = m;
+    r.l[j] = l;
   }
+  return r;
 }
-// a product of 22-bit operands, without the rests' product (2^-22 of it)
-__device__ __forceinline__ f32x4 mma22(u32x4 ah, u32x4 al, u32x4 bh, u32x4 bl, f32x4 c) {
-  c = Half<false>::mma(al, bh, c);
-  c = Half<false>::mma(ah, bl, c);
-  return Half<false>::mma(ah, bh, c);
+// their product; left out: what is 2^-24 of it and less
+__device__ __forceinline__ f32x4 mma_three(const Three& a, const Three& b, f32x4 c) {
+  c = Half<true>::mma(a.l, b.h, c);
+  c = Half<true>::mma(a.h, b.l, c);
+  c = Half<true>::mma(a.m, b.m, c);
+  c = Half<true>::mma(a.m, b.h, c);
+  c = Half<true>::mma(a.h, b.m, c);
+  return Half<true>::mma(a.h, b.h, c);
 }
 
 constexpr int kConvMax = 8;  // inputs of a convolution window at most
@@ -399,10 +413,11 @@ __global__ void __launch_bounds__(256) gdn_chunk_kernel(GdnPackedArgs a, float* 
 }
 
 // The chain over a sequence's chunks, for 32 columns of a value head's state: its tiles stay in registers (32 rows to each
-// of the first waves), a copy in LDS is the products' operand. Wave w holds tokens 16 w .. of a chunk. What goes into the
-// state's products is held in two fp16 numbers (22 bits: the state and left u times a power of two for each 32 rows, 16
-// tokens; q and k by split22), for the 16-bit matrix instructions; u and the outputs inside the chunk are float32
-// products. Bound by the chain: a chunk's operands come from L2 a chunk ahead, two workgroups to a CU.
+// of the first waves), a copy in LDS is the products' operand. Wave w holds tokens 16 w .. of a chunk. The products with
+// the state, and those that advance it, take their operands as three bf16 numbers (Three): float32's bits for every row and
+// column whatever its neighbours are, in six 16-bit matrix instructions, 96 cycles where float32 ones would take 256; u and
+// the outputs inside the chunk are float32 products. Bound by the chain: a chunk's operands come from L2 a chunk ahead, two
+// workgroups to a CU.
 // Columns: 64 read q, k, T and P half as often but leave one workgroup to a CU (3 prompts of 2047, 48 heads: 691 against
 // 635 us for the whole call).
 
@@ -412,10 +427,8 @@ template <bool BF, int DK>
 __global__ void __launch_bounds__(256, 2) gdn_scan_kernel(GdnPackedArgs a, const float* tp, float* ow, int long_from) {
   static_assert(kScanColumns == 32);
   constexpr int LS = DK + 8, LT = kChunk + 4, LU = kChunk + 8, COLS = kScanColumns, CT = COLS / 16;
-  // the state's copy and left u as two fp16 numbers, by column: of a power of two times them for each 32 rows, 16 tokens
-  __shared__ __attribute__((aligned(16))) uint16_t Sh[2][COLS * LS], uh[2][COLS * LU];
+  __shared__ __attribute__((aligned(16))) uint16_t Sh[3][COLS * LS], uh[3][COLS * LU];  // the state's copy and left u, by column
   __shared__ __attribute__((aligned(16))) float rl[COLS * LT], ul[COLS * LT];
-  __shared__ float sunit_s[4], uunit_s[4];
   __shared__ int odd_s;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
   const int ns = a.dv / COLS, h = blockIdx.x / ns, col0 = blockIdx.x % ns * COLS, kh = h % a.Hk, b = blockIdx.y;
@@ -432,51 +445,21 @@ __global__ void __launch_bounds__(256, 2) gdn_scan_kernel(GdnPackedArgs a, const
   float* const Sg = a.rec + (((int64_t)sq.row * a.Hv + h) * DK) * a.dv + col0;
   const bool fresh = sq.len == n;
   if (tid == 0) odd_s = 0;
-  bool odd = false;
-  auto largest = [&](const f32x4 (&v)[CT]) {  // of the lane's values; what is not finite is odd
-    float top = 0.f;
+  // four values of a column, and where the other terms of them are
+  auto put_split = [&](uint16_t* to, int term, f32x4 v) {
+    uint32_t w[3][2];
 #pragma unroll
-    for (int t = 0; t < CT; ++t)
+    for (int j = 0; j < 2; ++j) split3(v[2 * j], v[2 * j + 1], w[0][j], w[1][j], w[2][j]);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        odd |= !(fabsf(v[t][r]) <= 3.4028235e38f);
-        top = fmaxf(top, fabsf(v[t][r]));
-      }
-    return top;
-  };
-  auto power = [&](float top, float& back) {  // 2^x that brings the wave's largest below 2^7, and 2^-x
-    top = lanes_reduce(top, [](float x, float y) { return fmaxf(x, y); });
-    const int e = top > 0.f && top <= 3.4028235e38f ? min(max(6 - ilogbf(top), -120), 120) : 0;
-    back = ldexpf(1.f, -e);
-    return ldexpf(1.f, e);
-  };
-  // four values of a column, at 2^x times them, to the two arrays
-  auto put_split = [&](uint16_t (*to)[COLS * LS], uint16_t (*tu)[COLS * LU], int at, f32x4 v, float f) {
-    f16x4 h, l;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const float x = v[r] * f;
-      h[r] = (_Float16)x;
-      l[r] = (_Float16)(x - (float)h[r]);
-    }
-    if (to) {
-      *reinterpret_cast<f16x4*>(&to[0][at]) = h;
-      *reinterpret_cast<f16x4*>(&to[1][at]) = l;
-    } else {
-      *reinterpret_cast<f16x4*>(&tu[0][at]) = h;
-      *reinterpret_cast<f16x4*>(&tu[1][at]) = l;
-    }
+    for (int i = 0; i < 3; ++i) *reinterpret_cast<uint2*>(to + i * term) = make_uint2(w[i][0], w[i][1]);
   };
   const bool owner = 32 * wave < DK;  // of rows 32 wave .. + 31 of the state
   f32x4 st[2][CT];
   auto copy_state = [&]() {
-    float back;
-    const float f = power(fmaxf(largest(st[0]), largest(st[1])), back);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int t = 0; t < CT; ++t) put_split(Sh, nullptr, (16 * t + c) * LS + 32 * wave + 16 * i + 4 * g, st[i][t], f);
-    if (lane == 0) sunit_s[wave] = back * (1.f / 4096.f);  // k and q are 2^12 times themselves
+      for (int t = 0; t < CT; ++t) put_split(&Sh[0][(16 * t + c) * LS + 32 * wave + 16 * i + 4 * g], COLS * LS, st[i][t]);
   };
   if (owner) {
 #pragma unroll
@@ -547,17 +530,14 @@ __global__ void __launch_bounds__(256, 2) gdn_scan_kernel(GdnPackedArgs a, const
     for (int t = 0; t < CT; ++t) qs[t] = ks[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int s = 0; s < KQ; ++s) {
-      const float back = sunit_s[s];
-      u32x4 qh, ql, kh_, kl;
-      halves8(q4[s][0], q4[s][1], qh, ql);
-      halves8(k4[s][0], k4[s][1], kh_, kl);
+      const Three q = split3(q4[s][0], q4[s][1]), k = split3(k4[s][0], k4[s][1]);
 #pragma unroll
       for (int t = 0; t < CT; ++t) {
-        const u32x4 xh = *reinterpret_cast<const u32x4*>(&Sh[0][(16 * t + c) * LS + 32 * s + 8 * g]);
-        const u32x4 xl = *reinterpret_cast<const u32x4*>(&Sh[1][(16 * t + c) * LS + 32 * s + 8 * g]);
-        const f32x4 none = {0.f, 0.f, 0.f, 0.f};
-        ks[t] += mma22(kh_, kl, xh, xl, none) * back;
-        qs[t] += mma22(qh, ql, xh, xl, none) * back;
+        const uint16_t* const at = &Sh[0][(16 * t + c) * LS + 32 * s + 8 * g];
+        const Three x = {*reinterpret_cast<const u32x4*>(at), *reinterpret_cast<const u32x4*>(at + COLS * LS),
+                         *reinterpret_cast<const u32x4*>(at + 2 * COLS * LS)};
+        ks[t] = mma_three(k, x, ks[t]);
+        qs[t] = mma_three(q, x, qs[t]);
       }
     }
 #pragma unroll
@@ -575,15 +555,10 @@ __global__ void __launch_bounds__(256, 2) gdn_scan_kernel(GdnPackedArgs a, const
       for (int t = 0; t < CT; ++t) u[t] = mma4(t4[l], *reinterpret_cast<const f32x4*>(rl + (16 * t + c) * LT + 16 * l + 4 * g), u[t]);
     }
     load_block(t4, tgn);
-    {
-      float back;
-      const float f = power(largest(u), back);  // left is at most 1
 #pragma unroll
-      for (int t = 0; t < CT; ++t) {
-        *reinterpret_cast<f32x4*>(ul + (16 * t + c) * LT + 16 * wave + 4 * g) = u[t];
-        put_split(nullptr, uh, (16 * t + c) * LU + 16 * wave + 4 * g, u[t] * left, f);
-      }
-      if (lane == 0) uunit_s[wave] = back * (1.f / 4096.f);
+    for (int t = 0; t < CT; ++t) {
+      *reinterpret_cast<f32x4*>(ul + (16 * t + c) * LT + 16 * wave + 4 * g) = u[t];
+      put_split(&uh[0][(16 * t + c) * LU + 16 * wave + 4 * g], COLS * LU, u[t] * left);
     }
     lds_sync();
     f32x4 o[CT];
@@ -607,27 +582,22 @@ __global__ void __launch_bounds__(256, 2) gdn_scan_kernel(GdnPackedArgs a, const
 #pragma unroll
         for (int t = 0; t < CT; ++t) st[i][t] *= all;
 #pragma unroll
-      for (int l = 0; l < 4; ++l) {
-        const float back = uunit_s[l];
-        f16x4 bh[CT], bl[CT];
+      for (int l = 0; l < 4; l += 2) {  // tokens 16 l + 4 g .. + 3 and 16 more on, of both operands
+        Three x[CT];
 #pragma unroll
         for (int t = 0; t < CT; ++t) {
-          bh[t] = *reinterpret_cast<const f16x4*>(&uh[0][(16 * t + c) * LU + 16 * l + 4 * g]);
-          bl[t] = *reinterpret_cast<const f16x4*>(&uh[1][(16 * t + c) * LU + 16 * l + 4 * g]);
+          auto both = [&](int term) {
+            const uint16_t* const at = &uh[term][(16 * t + c) * LU + 16 * l + 4 * g];
+            const uint2 lo = *reinterpret_cast<const uint2*>(at), hi = *reinterpret_cast<const uint2*>(at + 16);
+            return (u32x4){lo.x, lo.y, hi.x, hi.y};
+          };
+          x[t] = {both(0), both(1), both(2)};
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const u32x4 w = {split22(kt[i][l][0]), split22(kt[i][l][1]), split22(kt[i][l][2]), split22(kt[i][l][3])};
-          const uint2 hw = make_uint2(__builtin_amdgcn_perm(w[1], w[0], 0x05040100u), __builtin_amdgcn_perm(w[3], w[2], 0x05040100u));
-          const uint2 lw = make_uint2(__builtin_amdgcn_perm(w[1], w[0], 0x07060302u), __builtin_amdgcn_perm(w[3], w[2], 0x07060302u));
-          const f16x4 ah = __builtin_bit_cast(f16x4, hw), al = __builtin_bit_cast(f16x4, lw);
+          const Three k = split3(kt[i][l], kt[i][l + 1]);
 #pragma unroll
-          for (int t = 0; t < CT; ++t) {
-            f32x4 x = __builtin_amdgcn_mfma_f32_16x16x16f16(al, bh[t], (f32x4){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-            x = __builtin_amdgcn_mfma_f32_16x16x16f16(ah, bl[t], x, 0, 0, 0);
-            x = __builtin_amdgcn_mfma_f32_16x16x16f16(ah, bh[t], x, 0, 0, 0);
-            st[i][t] += x * back;
-          }
+          for (int t = 0; t < CT; ++t) st[i][t] = mma_three(k, x[t], st[i][t]);
         }
       }
       copy_state();
@@ -636,6 +606,15 @@ __global__ void __launch_bounds__(256, 2) gdn_scan_kernel(GdnPackedArgs a, const
     load_gates(tgn);
     lds_sync();
   }
+  // a u that is not finite leaves a state that is not
+  bool odd = false;
+  if (owner)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int t = 0; t < CT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) odd |= !(fabsf(st[i][t][r]) <= 3.4028235e38f);
   if (odd) odd_s = 1;
   __syncthreads();
   if (!odd_s) {

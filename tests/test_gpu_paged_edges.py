@@ -133,7 +133,7 @@ def _one_head(n, K=4, dv=64, dk=128):
 
 @pytest.mark.parametrize("size", [1e-5, 1e-7, 1e-9, 1e-15])
 @pytest.mark.parametrize("which", ["q", "k"])
-@pytest.mark.parametrize("n", [1, 9])
+@pytest.mark.parametrize("n", [1, 9, 16, 130])
 def test_small_rows_keep_their_bits(n, which, size):
     """q or k rows far below the norm's epsilon enter the recurrence with float32's bits: with small q the outputs, with
     small k what the state gains from zero, relative to what they are."""
@@ -171,3 +171,21 @@ def test_small_rows_keep_their_bits(n, which, size):
         terms = q.sum(-1, keepdim=True) * top * 1e3 * scale
         err = (out.double() - want).abs()
         assert bool((err <= torch.finfo(BF16).eps / 2 * want.abs() + rel * terms).all()), float(((err - 2.0 ** -8 * want.abs()) / terms).max())
+
+
+@pytest.mark.parametrize("n", [2, 16, 64, 200])
+def test_columns_of_a_state_do_not_meet(n):
+    """Columns of the state, and of v, from 1 down to 1e-7 of their neighbours: each keeps the bits of its own size."""
+    case, t, plan = _one_head(n)
+    dk, dv = 128, 64
+    size = 10.0 ** -(torch.arange(dv) % 8).float()
+    size = size[torch.randperm(dv, generator=R.gen("columns"))]
+    t[0][:, 2 * dk:] = (t[0][:, 2 * dk:].float() * size).bfloat16()
+    t[7] = t[7] * size
+    out, conv, rec = _run_gdn(case, t, plan)
+    want, _, want_rec, scale = R.gdn(*t, *plan[:3], 1, 1, dk, dv, 1e-6)
+    r = int(plan[1][0])
+    # as test_gpu_paged._check_gdn's bound, each column by itself: its largest entry, of v too
+    top = torch.maximum(want_rec[r, 0].abs().amax(0), t[7][r, 0].double().abs().amax(0)) + 2 * t[0][:, 2 * dk:].double().abs().amax(0)
+    err = (rec[r, 0].double() - want_rec[r, 0]).abs()
+    assert bool((err <= (n + 16) * 2.0 ** -21 * top).all()), float((err / top).max())
