@@ -717,12 +717,15 @@ __global__ void __launch_bounds__(256) gdn_out_packed_kernel(GdnPackedArgs a, co
 // and by chunks: 16 tokens 50 and 43, 24 tokens 71 and 44, 64 tokens 176 and 48; 15 tokens token by token 48).
 constexpr int kLongFrom = 16;
 
+// whether a step may have long sequences, which take launches and memory of their own
+static bool gdn_may_chunk(const GdnPackedArgs& a) { return a.max_new >= kLongFrom && a.B > 0; }
+
 static int64_t gdn_slots(const GdnPackedArgs& a) { return (int64_t)(a.N >> 6) + a.B + 1; }
 
 // convolution outputs; if there may be long sequences, T and P of their chunks and the recurrence's outputs
 int64_t gdn_packed_work(const GdnPackedArgs& a) {
   const int64_t rows = (int64_t)a.N * (2 * a.Hk * a.dk + a.Hv * a.dv);
-  return a.max_new < kLongFrom ? rows : rows + gdn_slots(a) * a.Hv * kChunkFloats + (int64_t)a.N * a.Hv * a.dv;
+  return !gdn_may_chunk(a) ? rows : rows + gdn_slots(a) * a.Hv * kChunkFloats + (int64_t)a.N * a.Hv * a.dv;
 }
 
 template <bool BF>
@@ -742,7 +745,7 @@ static hipError_t launch_gdn_packed_t(const GdnPackedArgs& a, hipStream_t s) {
   // tokens of a thread (us for the whole call, 1 and 8: 64 tokens 50 and 54, 256 77 and 79, 512 104 and 102, 2048 294 and 275)
   if (a.N <= 512) width(std::integral_constant<int, 1>{});
   else width(std::integral_constant<int, 8>{});
-  const bool chunks = a.max_new >= kLongFrom;
+  const bool chunks = gdn_may_chunk(a);
   const int long_from = chunks ? kLongFrom : 0x7FFFFFFF;
   auto rec = [&](auto dk, auto dv) {
     if (chunks) {

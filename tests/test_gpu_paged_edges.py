@@ -117,6 +117,26 @@ def test_prompts_add_up_what_is_not_finite(dtype, hd, cached):
         assert torch.equal(got[odd].float().nan_to_num(nan=7.0), w[odd].nan_to_num(nan=7.0))
 
 
+# ---- steps of many sequences, and of none ----------------------------------------------------------
+
+@pytest.mark.parametrize("N", [1, 16, 100])
+def test_steps_without_sequences(N):
+    """No sequence at all: every row lies behind the last."""
+    P = _paged()
+    i32, i64 = torch.int32, torch.int64
+    none = P.PagePlan(torch.zeros(1, dtype=i32).cuda(), torch.zeros(0, dtype=i32).cuda(), torch.zeros(0, dtype=i32).cuda(),
+                      torch.full((N,), -1, dtype=i64).cuda(), torch.full((N,), -1, dtype=i64).cuda())
+    for hint in ({}, {"max_new": 1}):
+        pages = torch.ones(3, 2, 16, 64, dtype=F16, device="cuda")
+        got = P.attn_paged(torch.ones(N, 4, 64, dtype=F16, device="cuda"), pages, pages, torch.zeros(2, 4, dtype=i32, device="cuda"), none, **hint)
+        assert got.shape == (N, 4, 64) and not bool(got.any())
+        case = ([], [], 2, 4, 64, 64, 4, F16)
+        t, _ = _gdn_inputs(case)
+        t = tuple(torch.ones(N, x.shape[1], dtype=F16) for x in t[:3]) + t[3:]
+        out, conv, rec = _run_gdn(case, t, none, **hint)
+        assert out.shape == (N, 256) and not bool(out.any()) and torch.equal(conv, t[3]) and torch.equal(rec, t[7])
+
+
 # ---- GatedDeltaNet: small rows and columns ---------------------------------------------------------
 
 def _one_head(n, K=4, dv=64, dk=128):
