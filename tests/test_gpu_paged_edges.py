@@ -8,7 +8,7 @@ if not torch.cuda.is_available():
     pytest.skip("no GPU", allow_module_level=True)
 
 import paged_ref as R  # noqa: E402
-from test_gpu_paged import _attend, _attn_inputs, _gdn_inputs, _paged, _run_gdn  # noqa: E402
+from test_gpu_paged import _attend, _attn_inputs, _check_gdn, _gdn_inputs, _name, _paged, _run_gdn  # noqa: E402
 
 F16, BF16 = torch.float16, torch.bfloat16
 INF, NAN = float("inf"), float("nan")
@@ -135,6 +135,62 @@ def test_steps_without_sequences(N):
         t = tuple(torch.ones(N, x.shape[1], dtype=F16) for x in t[:3]) + t[3:]
         out, conv, rec = _run_gdn(case, t, none, **hint)
         assert out.shape == (N, 256) and not bool(out.any()) and torch.equal(conv, t[3]) and torch.equal(rec, t[7])
+
+
+def _crowd(B, longest, seed):
+    """(cached, new, sequences that are not served) of a step of B sequences: single tokens, some without any, some of a few,
+    some prompts; one that is not served among each 64; long ones on both sides of each border of 64."""
+    g = R.gen("crowd", B, seed)
+    cached = torch.randint(0, 200, (B,), generator=g).tolist()
+    new = [1] * B
+    for b in torch.randperm(B, generator=g)[:B // 4].tolist():
+        new[b] = int(torch.randint(0, 30, (1,), generator=g))
+    for b in range(0, B, 64):
+        for at, c, n in ((b - 2, longest, 1), (b + 1, longest // 2, 1), (b + 3, longest, 45), (b + 5, 0, 70)):
+            if 0 <= at < B:
+                cached[at], new[at] = c, n
+    return cached, new, [b for b in (7, 71, 135, 199, 263, 1000) if b < B]
+
+
+@pytest.mark.parametrize("case", CROWDS, ids=_name)
+def test_attention_of_many_sequences(case):
+    B, longest, page, H, G, hd, dtype = case
+    cached, new, gone = _crowd(B, longest, 0)
+    q, kp, vp, table, plan, gate = _attn_inputs(cached, new, page, H, G, hd, dtype, key=case, tail=2)
+    plan = [x.clone() for x in plan]
+    plan[1][gone] = -1
+    cu, N = plan[0].tolist(), q.shape[0] - 2
+    lost = torch.zeros(N, dtype=torch.bool)
+    for b in gone:
+        lost[cu[b]:cu[b + 1]] = True
+    want, size, score = R.attention(q[:N], kp, vp, table, *plan[:3], gate[:N, :, hd:])
+    bound = R.attention_bound(want, size, score, dtype, hd, longest + 70)
+    for hint in ({}, {"max_new": 1}):  # in both kinds of workgroups, and in one
+        got = _attend(q, kp, vp, table, plan, gate, **hint)
+        assert not bool(got[N:].any()) and bool(torch.isnan(got[:N][lost]).all())
+        err = (got[:N].double() - want).abs()
+        assert bool((err <= bound)[~lost].all()), float((err - bound)[~lost].max())
+
+
+@pytest.mark.parametrize("B", [64, 65, 130, 300, 1024])
+def test_recurrence_of_many_sequences(B):
+    cached, new, gone = _crowd(B, 500, 1)
+    case = (cached, new, 1, 2, 32, 64, 4, F16 if B % 2 else BF16)
+    t, plan = _gdn_inputs(case, tail=2)
+    plan = [x.clone() for x in plan]
+    rows = plan[1].clone()
+    plan[1][gone] = -1
+    cu, N = plan[0].tolist(), t[0].shape[0] - 2
+    lost = torch.zeros(N, dtype=torch.bool)
+    for b in gone:
+        lost[cu[b]:cu[b + 1]] = True
+    cut = tuple(x[:-2] for x in t[:3]) + t[3:]
+    for hint in ({}, {"max_new": 1}):  # long ones by chunks, and all token by token
+        out, conv, rec = _run_gdn(case, t, plan, **hint)
+        assert not bool(out[N:].any()) and bool(torch.isnan(out[:N][lost]).all())
+        kept = [int(rows[b]) for b in gone]
+        assert torch.equal(conv[kept], t[3][kept]) and torch.equal(rec[kept], t[7][kept])
+        _check_gdn(case, cut, plan, (out[:N].masked_fill(lost[:, None], 0), conv, rec))
 
 
 # ---- GatedDeltaNet: small rows and columns ---------------------------------------------------------
