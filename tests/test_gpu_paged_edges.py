@@ -152,6 +152,11 @@ def _crowd(B, longest, seed):
     return cached, new, [b for b in (7, 71, 135, 199, 263, 1000) if b < B]
 
 
+# (sequences, longest context, page, heads, kv heads, head dim, dtype)
+CROWDS = [(64, 3000, 16, 4, 2, 64, F16), (65, 3000, 16, 4, 2, 64, BF16), (130, 5000, 64, 6, 1, 128, F16), (300, 2000, 32, 4, 1, 256, BF16),
+          (1024, 700, 16, 2, 1, 64, F16)]
+
+
 @pytest.mark.parametrize("case", CROWDS, ids=_name)
 def test_attention_of_many_sequences(case):
     B, longest, page, H, G, hd, dtype = case
