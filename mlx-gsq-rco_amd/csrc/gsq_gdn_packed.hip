@@ -295,15 +295,39 @@ struct ChunkGate {
   }
 };
 
-// The chunk that slot i of the workspaces belongs to: those of sequence b begin at slot (cu[b] / 64) + b.
+// Slots of the workspaces that hold T, P and gates of a chunk: those of a long sequence begin at slot (its first token / 64)
+// + (long sequences before it), of which there are at most one for every long_from tokens.
+__host__ __device__ __forceinline__ int64_t gdn_slots(int64_t N, int64_t B, int long_from) {
+  const int64_t most = N / long_from;
+  return N / 64 + (B < most ? B : most) + 1;
+}
+// whether sequences base + lane are long, and below n
+__device__ __forceinline__ uint64_t long_ones(const GdnPackedArgs& a, int base, int n, int long_from) {
+  const int i = base + (threadIdx.x & 63), at = min(i, a.B - 1);
+  return __ballot(i < n && a.cu[at + 1] - a.cu[at] >= long_from);
+}
+__device__ __forceinline__ int first_slot(const GdnPackedArgs& a, int b, int long_from) {
+  int n = max(a.cu[b], 0) >> 6;
+  for (int base = 0; base < b; base += 64) n += __popcll(long_ones(a, base, b, long_from));
+  return n;
+}
+// The chunk that a slot belongs to.
 struct ChunkAt {
-  int b, c;
-  __device__ ChunkAt(const GdnPackedArgs& a, int slot) {
+  int b = -1, c = -1;
+  __device__ ChunkAt(const GdnPackedArgs& a, int slot, int long_from) {
     const int lane = threadIdx.x & 63;
-    int n = 0;
-    for (int i = lane; i - lane < a.B; i += 64) n += __popcll(__ballot(i < a.B && (max(a.cu[min(i, a.B - 1)], 0) >> 6) + i <= slot));
-    b = __builtin_amdgcn_readfirstlane(n) - 1;
-    c = b < 0 ? 0 : slot - ((max(a.cu[b], 0) >> 6) + b);
+    int before = 0;
+    for (int base = 0; base < a.B; base += 64) {
+      const uint64_t those = long_ones(a, base, a.B, long_from);
+      const int first = (max(a.cu[min(base + lane, a.B - 1)], 0) >> 6) + before + __popcll(those & ((1ull << lane) - 1));
+      const uint64_t here = __ballot(first <= slot) & those;
+      if (here) {  // the last of them
+        const int at = 63 - __builtin_clzll(here);
+        b = base + at;
+        c = slot - __builtin_amdgcn_readlane(first, at);
+      }
+      before += __popcll(those);
+    }
   }
 };
 
@@ -317,7 +341,7 @@ __global__ void __launch_bounds__(256) gdn_chunk_kernel(GdnPackedArgs a, float* 
   __shared__ __attribute__((aligned(16))) float M[kChunk * LD], T[kChunk * LD], beta_s[kChunk];
   __shared__ double sum_s[kChunk];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
-  const ChunkAt at(a, blockIdx.x);
+  const ChunkAt at(a, blockIdx.x, long_from);
   if (at.b < 0 || at.c < 0) return;
   const PackedSeq sq(a.cu, a.rows, a.lens, at.b, a.N, a.R, 0x7FFFFFFF);
   if (!sq.fine || sq.n < long_from || at.c * kChunk >= sq.n) return;
@@ -440,7 +464,12 @@ __global__ void __launch_bounds__(256, 2) gdn_scan_kernel(GdnPackedArgs a, const
   const float* const wv = a.work + (int64_t)sq.t0 * conv_dim + 2 * key_dim + h * a.dv + col0;
   float* const o_at = ow + (int64_t)sq.t0 * vdim + h * a.dv + col0;
   const uint16_t* const ab = static_cast<const uint16_t*>(a.ab) + (int64_t)sq.t0 * a.ab_stride;
-  const float* tg = tp + ((int64_t)((sq.t0 >> 6) + b) * a.Hv + h) * kChunkFloats;
+  const int slot = first_slot(a, b, long_from);
+  if (slot + (n + kChunk - 1) / kChunk > gdn_slots(a.N, a.B, long_from)) {  // sequences that lie over one another
+    for (int i = tid; i < n * COLS; i += 256) o_at[(int64_t)(i / COLS) * vdim + i % COLS] = NAN;
+    return;
+  }
+  const float* tg = tp + ((int64_t)slot * a.Hv + h) * kChunkFloats;
   const int64_t next = (int64_t)a.Hv * kChunkFloats;
   float* const Sg = a.rec + (((int64_t)sq.row * a.Hv + h) * DK) * a.dv + col0;
   const bool fresh = sq.len == n;
@@ -720,12 +749,10 @@ constexpr int kLongFrom = 16;
 // whether a step may have long sequences, which take launches and memory of their own
 static bool gdn_may_chunk(const GdnPackedArgs& a) { return a.max_new >= kLongFrom && a.B > 0; }
 
-static int64_t gdn_slots(const GdnPackedArgs& a) { return (int64_t)(a.N >> 6) + a.B + 1; }
-
 // convolution outputs; if there may be long sequences, T and P of their chunks and the recurrence's outputs
 int64_t gdn_packed_work(const GdnPackedArgs& a) {
   const int64_t rows = (int64_t)a.N * (2 * a.Hk * a.dk + a.Hv * a.dv);
-  return !gdn_may_chunk(a) ? rows : rows + gdn_slots(a) * a.Hv * kChunkFloats + (int64_t)a.N * a.Hv * a.dv;
+  return !gdn_may_chunk(a) ? rows : rows + gdn_slots(a.N, a.B, kLongFrom) * a.Hv * kChunkFloats + (int64_t)a.N * a.Hv * a.dv;
 }
 
 template <bool BF>
@@ -750,8 +777,9 @@ static hipError_t launch_gdn_packed_t(const GdnPackedArgs& a, hipStream_t s) {
   auto rec = [&](auto dk, auto dv) {
     if (chunks) {
       float* const tp = a.work + (int64_t)a.N * conv_dim;
-      float* const ow = tp + gdn_slots(a) * a.Hv * kChunkFloats;
-      hipLaunchKernelGGL((gdn_chunk_kernel<BF, decltype(dk)::value>), dim3((unsigned)gdn_slots(a), (unsigned)a.Hk), dim3(256), 0, s, a, tp, long_from);
+      const int64_t slots = gdn_slots(a.N, a.B, kLongFrom);
+      float* const ow = tp + slots * a.Hv * kChunkFloats;
+      hipLaunchKernelGGL((gdn_chunk_kernel<BF, decltype(dk)::value>), dim3((unsigned)slots, (unsigned)a.Hk), dim3(256), 0, s, a, tp, long_from);
       hipLaunchKernelGGL((gdn_scan_kernel<BF, decltype(dk)::value>), dim3((unsigned)(a.Hv * (a.dv / kScanColumns)), (unsigned)a.B), dim3(256), 0, s, a,
                          (const float*)tp, ow, long_from);
       const bool wide = ((reinterpret_cast<uintptr_t>(a.z) | reinterpret_cast<uintptr_t>(a.out)) & 15) == 0 && ((a.z_stride | a.out_stride) & 7) == 0;

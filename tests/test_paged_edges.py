@@ -15,3 +15,35 @@ for tokens in (1, 16, 100, 5000):
     assert lib.gsq_gdn_packed_work(tokens, 0, 16, 48, 128, 128, 4, tokens) == lib.gsq_gdn_packed_work(tokens, 0, 16, 48, 128, 128, 4, 1)
     assert attn(tokens, 0, 80) == 0
 """)
+
+
+def test_workspaces_do_not_grow_with_single_tokens(stub):  # noqa: F811
+    """T, P and gates of a chunk are kept for sequences that go by chunks, of which a step of N tokens has N / 16 at most:
+    what 251 sequences with one turn of 16 among them take is what 16 take, and their own rows."""
+    run(stub, SIGNATURES + """
+def floats(tokens, sequences, most=None):
+    return lib.gsq_gdn_packed_work(tokens, sequences, 16, 48, 128, 128, 4, tokens if most is None else most)
+rows = 10240 + 48 * 128  # of a token: convolution and recurrence outputs
+chunk = 48 * (2 * 64 * 64 + 3 * 64)  # of a chunk
+for tokens, sequences in ((266, 251), (1050, 1024), (1024, 1024), (16, 1), (64, 4), (2047 * 3, 3), (524280, 1024)):
+    got = floats(tokens, sequences)
+    assert got == tokens * rows + (tokens // 64 + min(sequences, tokens // 16) + 1) * chunk, (tokens, sequences, got)
+assert floats(266, 251) * 4 < 60 << 20
+assert floats(1050, 1024) * 4 < 230 << 20
+# what the chunks of any step take: sequences of 16 and more and shorter ones in all orders
+import random
+rng = random.Random(5)
+for _ in range(2000):
+    new = [rng.choice([0, 1, 15, 16, 17, 63, 64, 65, 80, 200]) for _ in range(rng.randint(1, 40))]
+    tokens, at, longs, last = sum(new), 0, 0, -1
+    if not tokens:
+        continue
+    for n in new:
+        if n >= 16:
+            first, chunks = at // 64 + longs, -(-n // 64)
+            assert first > last  # no two chunks share a slot
+            last = first + chunks - 1
+            longs += 1
+        at += n
+    assert last < tokens // 64 + min(len(new), tokens // 16) + 1
+""")
