@@ -318,7 +318,8 @@ int gsq_attn_kv8(const void* q, int64_t q_stride, const void* qg, int64_t qg_str
  * *n_free are free): sequence by sequence, need_b = max(0, ceil((lengths[r] + new_tokens[b]) / page_size) - held[r]). A
  * sequence is served unless its request is out of range or named by an earlier sequence, it does not fit its table row or
  * the `tokens` rows, or it needs pages and the running sum of the needs passes *n_free. table, held and n_free are
- * updated; lengths are not (gsq_page_advance), so that the same call again gives the same step. Out: cu (sequences + 1), rows and
+ * updated; lengths are not (gsq_page_advance), so that the same call again gives the same step (recurrent states that
+ * gsq_gdn_packed has advanced for it are not taken back: a step that failed behind one cannot be repeated). Out: cu (sequences + 1), rows and
  * lens (-1 and 0 if not served), pos and slots (page * page_size + row) of each of the `tokens` rows, -1 where there is none. */
 int gsq_page_plan(const int32_t* requests, const int32_t* new_tokens, const int32_t* lengths, int32_t* held, int32_t* table,
                   const int32_t* free_pages, int32_t* n_free, int64_t sequences, int64_t n_requests, int64_t max_pages,

@@ -15,6 +15,10 @@ class PagedCache:
 
     All bookkeeping is on the device: ``table`` (requests, max_pages), ``lengths`` and ``held`` (requests,), ``free`` and
     ``n_free``, int32. A request begins with its first tokens at length 0 and ends with ``release``.
+
+    A step that fails part way has advanced the recurrent states of some layers and no lengths: run again, it would
+    advance them twice. ``torn`` then holds the requests that it served and that are not released yet, and no step is taken
+    until there are none.
     """
 
     def __init__(self, args, requests: int, pages: int, page_size: int, max_len: int, device, dtype):
@@ -35,6 +39,7 @@ class PagedCache:
         self.table = torch.full((requests, -(-max_len // page_size)), -1, **i32)
         self.lengths, self.held = torch.zeros(requests, **i32), torch.zeros(requests, **i32)
         self.free, self.n_free = torch.arange(pages, **i32), torch.tensor([pages], **i32)
+        self.torn = None
         self.conv, self.rec, self.k, self.v = {}, {}, {}, {}
         for i in range(args.num_hidden_layers):
             if args.is_linear(i):
@@ -44,6 +49,13 @@ class PagedCache:
             else:
                 shape = (pages, args.num_key_value_heads, page_size, args.head_dim)
                 self.k[i], self.v[i] = (torch.zeros(shape, device=device, dtype=dtype) for _ in range(2))
+
+    def whole(self):
+        """Refuses a cache that a failed step has left torn."""
+        if self.torn is not None and not bool((self.torn >= 0).any()):
+            self.torn = None  # it served nobody
+        if self.torn is not None:
+            raise ValueError("a step over this cache failed part way: release its requests (torn) before the next one")
 
     def plan(self, requests, new, tokens: int):
         """The layout of a step (``page_plan``) over ``tokens`` rows; takes the pages it needs."""
@@ -69,7 +81,15 @@ class PagedCache:
             from ..runtime.kernels import paged
             for some in requests.split(paged.MAX_SEQUENCES):
                 paged.page_release(some.contiguous(), self.lengths, self.held, self.table, self.free, self.n_free)
-            return
+        else:
+            self._release_host(requests)
+        if self.torn is not None:
+            gone = set(requests.tolist())
+            left = [r for r in self.torn.tolist() if 0 <= r < self.requests and r not in gone]
+            self.torn = torch.tensor(left, dtype=torch.int32) if left else None
+
+    def _release_host(self, requests):
+        """``page_release`` for a cache on the CPU."""
         back = []
         for r in dict.fromkeys(requests.tolist()):
             if 0 <= r < self.requests:
@@ -155,12 +175,14 @@ class PackedGraphDecoder:
         self.capture_stream = side  # the graph's QMM launches use its workspace
 
     def _run(self):
-        return self.model._packed(self.ids, self.requests, self.new, self.cache, 1, False)
+        plan = self.cache.plan(self.requests, self.new, self.batch)
+        return self.model._packed(self.ids, plan, self.cache, 1, False), plan
 
     def step(self, ids, requests):
         n = len(requests)
         if len(ids) != n or n > self.batch:
             raise ValueError(f"one token for each of at most {self.batch} requests")
+        self.cache.whole()
         self.ids[:n].copy_(torch.as_tensor(ids, dtype=torch.int64))
         self.requests.fill_(-1)
         self.requests[:n].copy_(torch.as_tensor(requests, dtype=torch.int32))

@@ -589,7 +589,9 @@ class Qwen35Model(torch.nn.Module):
 
         ``new`` and ``requests`` are lists, or int32 tensors on the cache's device, which are not looked at on the host
         (``max_new``: their most new tokens, if known). Rows of sequences that are not served (no pages left, longer than
-        ``max_len``) or bring no tokens are NaN, and those requests stay as they were."""
+        ``max_len``) or bring no tokens are NaN, and those requests stay as they were. A step that fails part way leaves its
+        requests to ``cache.release``; the next one is refused until then."""
+        cache.whole()
         device = cache.table.device
         if not (torch.is_tensor(new) and torch.is_tensor(requests) and new.device == device):
             new, requests = ([int(x) for x in t] for t in (new, requests))
@@ -604,12 +606,16 @@ class Qwen35Model(torch.nn.Module):
         ids = torch.as_tensor(ids, device=device)
         if ids.dim() != 1 or new.dim() != 1 or new.shape != requests.shape or not len(ids):
             raise ValueError("ids must be (N,) with a token at least, new and requests (B,)")
-        return self._packed(ids, requests, new, cache, len(ids) if max_new is None else max_new, all_logits)[0]
+        plan = cache.plan(requests, new, len(ids))
+        try:
+            return self._packed(ids, plan, cache, len(ids) if max_new is None else max_new, all_logits)
+        except BaseException:
+            cache.torn = plan.rows  # some layers' states may have moved on
+            raise
 
-    def _packed(self, ids, requests, new, cache: PagedCache, max_new: int, all_logits: bool):
-        """(logits, plan) of a step."""
+    def _packed(self, ids, plan, cache: PagedCache, max_new: int, all_logits: bool):
+        """Logits of a step that has been laid out."""
         N = ids.shape[0]
-        plan = cache.plan(requests, new, N)
         step = PackedStep(cache, plan, max_new)
         x = self.embed(ids[None]).to(self.dtype).reshape(1, N, -1).contiguous()
         delta = None
@@ -623,7 +629,7 @@ class Qwen35Model(torch.nn.Module):
         logits = self.lm_head(h)[0]
         logits = logits.masked_fill((plan.slots if all_logits else plan.rows)[:, None] < 0, float("nan"))
         cache.advance(plan)
-        return logits, plan
+        return logits
 
     def forward(self, ids, cache: Qwen35Cache):
         S = ids.shape[1]

@@ -56,7 +56,8 @@ def page_plan(requests, new_tokens, lengths, held, table, free, n_free, *, token
     ones, over ``tokens`` rows. Pages that it needs beyond the ``held[r]`` it has are taken from the end of ``free``
     ((n_pages,), the first ``n_free[0]`` of them free), sequence by sequence; ``table``, ``held`` and ``n_free`` are updated.
     A sequence is not served if its request is out of range or named before, if it does not fit its table row or the
-    rows, or if the pages run out before it. Lengths stay (``page_advance``): the same call again gives the same step."""
+    rows, or if the pages run out before it. Lengths stay (``page_advance``): the same call again gives the same step,
+    before ``gdn_packed`` has advanced a recurrent state for it."""
     dev = _one_gpu(requests, new_tokens, lengths, held, table, free, n_free)
     B = requests.shape[0] if requests.dim() == 1 else -1
     _int32((B,), requests, new_tokens)

@@ -1,7 +1,15 @@
 """The host side of steps of packed requests where it can go wrong, without a GPU: launches of empty steps, sizes of
 workspaces, and the decoder's bookkeeping."""
+import pytest
+import torch
+
+from mlx_gsq_amd.models import PackedGraphDecoder, build_qwen35
+from qwen35_fixture import ARGS, TinyStore, dense_factories
 from test_host_launches import run, stub  # noqa: F401  (a fixture)
 from test_paged_launches import SIGNATURES
+
+
+# ---- launches and workspaces ---------------------------------------------------------------------
 
 
 def test_no_launch_is_empty(stub):  # noqa: F811
@@ -47,3 +55,64 @@ for _ in range(2000):
         at += n
     assert last < tokens // 64 + min(len(new), tokens // 16) + 1
 """)
+
+
+# ---- the decoder ---------------------------------------------------------------------------------
+
+@pytest.fixture(scope="module")
+def model():
+    store = TinyStore("cpu", seed=1)
+    linear, fused, embedding = dense_factories(store)
+    return build_qwen35(store, dtype=torch.float32, args=ARGS, linear=linear, fused=fused, embedding=embedding)
+
+
+def test_a_step_that_fails_part_way_cannot_be_repeated(model, monkeypatch):
+    """Layers before the failure have advanced their requests' states: every step is refused until those are released."""
+    with torch.no_grad():
+        cache = model.new_paged_cache(4, pages=8, page_size=16, max_len=32)
+        model.step([5, 6, 7, 8], [3, 1], [2, 0], cache)
+        want = model.new_paged_cache(4, pages=8, page_size=16, max_len=32)
+        want = model.step([9, 10, 11], [2, 1], [3, 2], want)
+        before = {i: t.clone() for i, t in cache.rec.items()}
+
+        def fail(*_):
+            raise MemoryError("no room")
+        for last in (model.layers[-1], model.lm_head):
+            with monkeypatch.context() as m:
+                m.setattr(last, "forward", fail)
+                with pytest.raises(MemoryError):
+                    model.step([9, 10], [1, 1], [2, 0], cache)
+            assert any(not torch.equal(t, before[i]) for i, t in cache.rec.items()) and cache.lengths.tolist() == [1, 0, 3, 0]
+            decoder = object.__new__(PackedGraphDecoder)
+            decoder.cache, decoder.batch = cache, 4
+            for _ in range(2):
+                for call in (lambda: model.step([9, 10], [1, 1], [2, 0], cache), lambda: model.step([9], [1], [3], cache),
+                             lambda: decoder.step([9], [2])):
+                    with pytest.raises(ValueError, match="failed part way"):
+                        call()
+                cache.release([0])
+            cache.release([1, 2])
+            assert int(cache.n_free) == 8
+            got = model.step([9, 10, 11], [2, 1], [3, 2], cache)  # new requests begin from zeros
+            assert torch.equal(got, want)
+            cache.release(torch.arange(4))
+            model.step([5, 6, 7, 8], [3, 1], [2, 0], cache)
+
+
+def test_a_step_that_is_refused_leaves_a_cache_whole(model):
+    with torch.no_grad():
+        cache = model.new_paged_cache(2, pages=2, page_size=16, max_len=32)
+        for args in (([1, 2], [1], [0]), ([], [], []), ([1], [1], [5])):
+            with pytest.raises(ValueError):
+                model.step(*args, cache)
+        assert cache.torn is None and bool(torch.isfinite(model.step([1, 2], [2], [0], cache)).all())
+
+
+def test_a_step_that_served_nobody_leaves_a_cache_whole(model, monkeypatch):
+    with torch.no_grad():
+        cache = model.new_paged_cache(2, pages=2, page_size=16, max_len=32)
+        with monkeypatch.context() as m:
+            m.setattr(model.lm_head, "forward", lambda *_: 1 / 0)
+            with pytest.raises(ZeroDivisionError):
+                model.step([1] * 33, [33], [0], cache)  # longer than max_len
+        assert bool(torch.isfinite(model.step([1, 2], [2], [0], cache)).all())
