@@ -9,6 +9,14 @@ from __future__ import annotations
 import torch
 
 
+def _numbers(requests):
+    """Requests as int32; what does not fit is out of range there too."""
+    t = torch.as_tensor(requests)
+    if t.is_floating_point() and t.numel():
+        raise ValueError("requests are whole numbers")
+    return t.to(torch.int64).clamp(-1, 2 ** 31 - 1).to(torch.int32)
+
+
 class PagedCache:
     """States of up to ``requests`` requests. K and V of the attention layers lie in ``pages`` pages of ``page_size`` positions,
     handed out as requests grow (up to ``max_len`` positions each); the GatedDeltaNet layers keep a state for each request.
@@ -76,7 +84,7 @@ class PagedCache:
 
     def release(self, requests):
         """Ends requests: their pages are free again. Numbers out of range, or named before, are passed over."""
-        requests = torch.as_tensor(requests, dtype=torch.int32).reshape(-1).to(self.table.device)
+        requests = _numbers(requests).reshape(-1).to(self.table.device)
         if self.table.is_cuda:
             from ..runtime.kernels import paged
             for some in requests.split(paged.MAX_SEQUENCES):
@@ -185,7 +193,7 @@ class PackedGraphDecoder:
         self.cache.whole()
         self.ids[:n].copy_(torch.as_tensor(ids, dtype=torch.int64))
         self.requests.fill_(-1)
-        self.requests[:n].copy_(torch.as_tensor(requests, dtype=torch.int32))
+        self.requests[:n].copy_(_numbers(requests))
         self.new.zero_()
         self.new[:n].fill_(1)
         self.graph.replay()

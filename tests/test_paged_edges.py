@@ -1,5 +1,7 @@
 """The host side of steps of packed requests where it can go wrong, without a GPU: launches of empty steps, sizes of
 workspaces, and the decoder's bookkeeping."""
+from types import SimpleNamespace
+
 import pytest
 import torch
 
@@ -116,3 +118,24 @@ def test_a_step_that_served_nobody_leaves_a_cache_whole(model, monkeypatch):
             with pytest.raises(ZeroDivisionError):
                 model.step([1] * 33, [33], [0], cache)  # longer than max_len
         assert bool(torch.isfinite(model.step([1, 2], [2], [0], cache)).all())
+
+
+def test_request_numbers_past_32_bits_are_out_of_range(model):
+    """2^32 + 1 is not request 1."""
+    far = [2 ** 32 + 1, 2 ** 31 + 1, -2 ** 32 + 1, -2 ** 40]
+    with torch.no_grad():
+        cache = model.new_paged_cache(2, pages=2, page_size=16, max_len=32)
+        model.step([1, 2], [2], [1], cache)
+        for some in (torch.tensor(far), far, torch.tensor(far[:1])):
+            cache.release(some)
+            assert cache.lengths.tolist() == [0, 2] and int(cache.n_free) == 1
+        with pytest.raises(ValueError, match="whole numbers"):
+            cache.release([1.0])
+        decoder = object.__new__(PackedGraphDecoder)
+        decoder.cache, decoder.batch, decoder.logits, decoder.graph = cache, 4, torch.zeros(4, 8), SimpleNamespace(replay=lambda: None)
+        decoder.ids, decoder.requests, decoder.new = torch.zeros(4, dtype=torch.int64), torch.zeros(4, dtype=torch.int32), torch.zeros(4)
+        decoder.step([5] * 4, torch.tensor(far))
+        assert all(r < 0 or r >= cache.requests for r in decoder.requests.tolist())
+        cache.release(torch.tensor([1], dtype=torch.int16))
+        assert cache.lengths.tolist() == [0, 0] and int(cache.n_free) == 2
+        cache.release([])
