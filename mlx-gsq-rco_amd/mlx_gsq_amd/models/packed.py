@@ -19,7 +19,8 @@ def _numbers(requests):
 
 class PagedCache:
     """States of up to ``requests`` requests. K and V of the attention layers lie in ``pages`` pages of ``page_size`` positions,
-    handed out as requests grow (up to ``max_len`` positions each); the GatedDeltaNet layers keep a state for each request.
+    handed out as requests grow (up to ``max_len`` positions each, which is rounded up to whole pages); the GatedDeltaNet
+    layers keep a state for each request.
 
     All bookkeeping is on the device: ``table`` (requests, max_pages), ``lengths`` and ``held`` (requests,), ``free`` and
     ``n_free``, int32. A request begins with its first tokens at length 0 and ends with ``release``.
@@ -42,9 +43,10 @@ class PagedCache:
             if (args.head_dim not in (64, 128, 256) or args.linear_key_head_dim not in (32, 64, 128)
                     or args.linear_value_head_dim not in (64, 128, 256)):
                 raise ValueError("head dims must be 64, 128 or 256 (GatedDeltaNet keys 32, 64 or 128)")
+        max_len = -(-max_len // page_size) * page_size
         self.args, self.requests, self.page_size, self.max_len = args, requests, page_size, max_len
         i32 = dict(dtype=torch.int32, device=device)
-        self.table = torch.full((requests, -(-max_len // page_size)), -1, **i32)
+        self.table = torch.full((requests, max_len // page_size), -1, **i32)
         self.lengths, self.held = torch.zeros(requests, **i32), torch.zeros(requests, **i32)
         self.free, self.n_free = torch.arange(pages, **i32), torch.tensor([pages], **i32)
         self.torn = None

@@ -578,7 +578,8 @@ class Qwen35Model(torch.nn.Module):
         return Qwen35Cache(self.args, batch, max_len, device, self.dtype, kv_bits)
 
     def new_paged_cache(self, requests: int, pages: int, page_size: int = 64, max_len: int = 4096, device=None) -> PagedCache:
-        """States of up to ``requests`` requests for ``step``, ``pages`` pages of ``page_size`` positions between them."""
+        """States of up to ``requests`` requests for ``step``, ``pages`` pages of ``page_size`` positions between them, up to
+        ``max_len`` positions each (rounded up to whole pages: the cache's ``max_len``)."""
         device = device if device is not None else self.norm_w.device
         return PagedCache(self.args, requests, pages, page_size, max_len, device, self.dtype)
 
@@ -589,7 +590,7 @@ class Qwen35Model(torch.nn.Module):
 
         ``new`` and ``requests`` are lists, or int32 tensors on the cache's device, which are not looked at on the host
         (``max_new``: their most new tokens, if known). Rows of sequences that are not served (no pages left, longer than
-        ``max_len``) or bring no tokens are NaN, and those requests stay as they were. A step that fails part way leaves its
+        ``cache.max_len``) or bring no tokens are NaN, and those requests stay as they were. A step that fails part way leaves its
         requests to ``cache.release``; the next one is refused until then."""
         cache.whole()
         device = cache.table.device

@@ -139,3 +139,12 @@ def test_request_numbers_past_32_bits_are_out_of_range(model):
         cache.release(torch.tensor([1], dtype=torch.int16))
         assert cache.lengths.tolist() == [0, 0] and int(cache.n_free) == 2
         cache.release([])
+
+
+def test_max_len_is_what_a_request_may_have(model):
+    """Whole pages: 17 positions in pages of 16 are 32, and a 33rd is not served."""
+    with torch.no_grad():
+        cache = model.new_paged_cache(1, pages=4, page_size=16, max_len=17)
+        assert cache.max_len == 32 and cache.table.shape == (1, 2)
+        assert bool(torch.isfinite(model.step([3] * 32, [32], [0], cache)).all())
+        assert bool(torch.isnan(model.step([3], [1], [0], cache)).all()) and cache.lengths.tolist() == [32]
