@@ -99,31 +99,41 @@ __device__ __forceinline__ T wave_scan(T v) {  // inclusive
 
 // One over the blocks of a piece. Few rows: the step's work (tiles of rows times blocks) over as many workgroups as
 // fill the device. Many rows: the longest sequence in 1 .. 64 pieces, whichever ends first when workgroups of one piece each
-// fill the device in turn (kPieceCost blocks for what a piece costs besides: its partial outputs, written and merged); with
-// enough tiles of rows, or many sequences of them, none is split.
-constexpr int kPieceCost = 10, kMostTurns = 4;
+// fill the device in turn (kPieceCost blocks for what a piece costs besides: its partial outputs, written and merged); of more
+// than kSearched sequences, which the search would take too long for, in proportion to the work as few rows; with
+// enough tiles of rows none is split. Only sequences of many rows count here: what runs beside them is another kind's (fp16,
+// 24 heads of 256 over 4 KV heads, us, in pieces and not: 64 tokens behind 131071 beside 64 single ones 406 and 7650, 1024 behind
+// 30000 1100 and 2168; in proportion and not: 17 turns of 64 behind 15000 to 30000 1097 and 1883 (16, searched: 844), 40 of 8
+// behind 8000 to 16000 486 and 1046, 20 of 150 to 300 behind 4000 to 8000 1051 and 1042).
+constexpr int kPieceCost = 10, kMostTurns = 4, kSearched = 16;
 
 __device__ __forceinline__ float over_chunk(const AttnPagedArgs& a, const PagedSched& p) {
   const int lane = threadIdx.x & 63;
-  float total = 0.f;
+  float work = 0.f, workgroups = 0.f;
+  int count = 0, tiles = 0, blocks = 0;  // sequences of many rows; lane i: tiles and blocks of the i-th
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const SeqLane s(a, p, b0 + lane);
-    total += (float)s.tiles * (float)(p.which == kMany ? 1 : s.blocks);
+    work = __builtin_fmaf((float)s.tiles, (float)s.blocks, work);  // the same bits in both kernels
+    if (p.which != kMany) continue;
+    workgroups += (float)s.tiles;
+    for (uint64_t some = __ballot(s.tiles > 0); some && count <= kSearched; some &= some - 1, ++count) {
+      const int i = __builtin_ctzll(some), t = __builtin_amdgcn_readlane(s.tiles, i), n = __builtin_amdgcn_readlane(s.blocks, i);
+      tiles = lane == count ? t : tiles;
+      blocks = lane == count ? n : blocks;
+    }
   }
-  total = lanes_sum(total) * (float)a.Hkv;
-  if (p.which != kMany) return __builtin_amdgcn_rcpf(fmaxf(total / (float)p.target, (float)p.least));
-  if (total >= (float)kMostTurns * (float)p.target || a.B > 64) return 0.f;
-  const SeqLane s(a, p, lane);
-  uint64_t many = __ballot(s.tiles > 0);
-  if (__popcll(many) > 16) return 0.f;
-  int longest = s.tiles > 0 ? s.blocks : 0;
-  longest = (int)lanes_reduce((float)longest, [](float x, float y) { return fmaxf(x, y); });
-  const float chunk = fmaxf((float)longest / (float)(lane + 1), (float)p.least), over = 0.99999f * __builtin_amdgcn_rcpf(chunk);  // not one piece more by its rounding
+  work = lanes_sum(work) * (float)a.Hkv;
+  const float share = __builtin_amdgcn_rcpf(fmaxf(work / (float)p.target, (float)p.least));
+  if (p.which != kMany) return share;
+  workgroups = lanes_sum(workgroups) * (float)a.Hkv;
+  if (workgroups >= (float)kMostTurns * (float)p.target) return 0.f;
+  // pieces are fewer than the workgroups and `target` together
+  if (count > kSearched) return workgroups < (float)(kMostTurns - 1) * (float)p.target ? share : 0.f;
+  const float longest = lanes_reduce(lane < count ? (float)blocks : 0.f, [](float x, float y) { return fmaxf(x, y); });
+  const float chunk = fmaxf(longest / (float)(lane + 1), (float)p.least), over = 0.99999f * __builtin_amdgcn_rcpf(chunk);  // not one piece more by its rounding
   float items = 0.f;
-  for (; many; many &= many - 1) {
-    const int i = __builtin_ctzll(many);
-    items += (float)__builtin_amdgcn_readlane(s.tiles, i) * ceilf((float)__builtin_amdgcn_readlane(s.blocks, i) * over);
-  }
+  for (int i = 0; i < count; ++i)
+    items += (float)__builtin_amdgcn_readlane(tiles, i) * ceilf((float)__builtin_amdgcn_readlane(blocks, i) * over);
   const float turns = ceilf(items * (float)a.Hkv / (float)p.target);
   const float cost = turns > (float)kMostTurns && lane ? FLT_MAX : turns * (chunk + (float)(lane ? kPieceCost : 0));
   const float best = lanes_reduce(cost, [](float x, float y) { return fminf(x, y); });
@@ -924,7 +934,7 @@ struct PagedPlan {
 
 // Pieces and workspaces that a launch may need, from what the host knows. A piece of a split sequence holds more than half
 // of `target`-th of the work, so there are fewer than 2 target of them (many rows: at most kMostTurns target, as the search
-// in over_chunk goes).
+// in over_chunk goes, and fewer than 2 target in proportion).
 PagedPlan paged_plan(const AttnPagedArgs& a) {
   PagedPlan r = {};
   const int64_t blocks = (a.W * a.P + 31) / 32;

@@ -8,7 +8,7 @@ if not torch.cuda.is_available():
     pytest.skip("no GPU", allow_module_level=True)
 
 import paged_ref as R  # noqa: E402
-from test_gpu_paged import _attend, _attn_inputs, _check_gdn, _gdn_inputs, _name, _paged, _run_gdn  # noqa: E402
+from test_gpu_paged import _attend, _attn_inputs, _check_attn, _check_gdn, _gdn_inputs, _name, _paged, _run_gdn  # noqa: E402
 
 F16, BF16 = torch.float16, torch.bfloat16
 INF, NAN = float("inf"), float("nan")
@@ -175,6 +175,37 @@ def test_attention_of_many_sequences(case):
         assert not bool(got[N:].any()) and bool(torch.isnan(got[:N][lost]).all())
         err = (got[:N].double() - want).abs()
         assert bool((err <= bound)[~lost].all()), float((err - bound)[~lost].max())
+
+
+def test_a_prompt_is_cut_alike_beside_any_number_of_single_tokens():
+    """How a chunk of a prompt behind many positions is cut into pieces follows from the sequences of many rows: its bits are
+    the same beside 3 single tokens and beside 100."""
+    P, H, G, hd, page, long, n = _paged(), 6, 1, 128, 64, 20000, 50
+    g = R.gen("alike")
+    pages = -(-(long + n) // page)
+    kp, vp = (torch.randn(pages, G, page, hd, generator=g).half().cuda() for _ in range(2))
+    q = torch.randn(n + 1100, H, hd, generator=g).half().cuda()
+    i32 = dict(dtype=torch.int32, device="cuda")
+    got = []
+    for singles, at in ((3, 0), (62, 30), (63, 63), (64, 64), (100, 5), (1023, 1000)):  # the chunk behind `at` of them
+        new = [1] * at + [n] + [1] * (singles - at)
+        cu = torch.tensor([0] + new).cumsum(0).int().cuda()
+        lens = torch.tensor([200] * at + [long + n] + [200] * (singles - at), **i32)
+        table = torch.arange(pages, **i32).expand(singles + 1, -1).contiguous()
+        plan = P.PagePlan(cu, torch.arange(singles + 1, **i32), lens, None, None)
+        x = torch.cat([q[n:n + at], q[:n], q[n + at:n + singles]])
+        got.append(P.attn_paged(x, kp, vp, table, plan)[at:at + n])
+    for x in got[1:]:
+        assert torch.equal(x, got[0])
+
+
+@pytest.mark.parametrize("turns", [16, 17, 70])
+def test_attention_of_many_turns(turns):
+    """Turns of some tokens behind long contexts, more than the search for pieces takes, between single tokens."""
+    new, cached = [1, 9] * turns, [40, 0] * turns
+    cached[1::2] = [1500 + 61 * i % 900 for i in range(turns)]
+    q, kp, vp, table, plan, gate = _attn_inputs(cached, new, 32, 4, 1, 64, F16, key=("turns", turns))
+    _check_attn(_attend(q, kp, vp, table, plan, gate), q, kp, vp, table, plan, gate)
 
 
 @pytest.mark.parametrize("B", [64, 65, 130, 300, 1024])
