@@ -245,16 +245,15 @@ __device__ __forceinline__ void clear_tail(const AttnPagedArgs& a) {
 // The softmax and the sums of a wave's 16 NT rows over the positions it has seen. Weights are powers of two over a
 // reference m that moves only when a score passes it by 2^kLazy, for all rows of the wave at once: mostly no rescaling
 // and no exchange between lanes in the loop. They are held in kTerms 16-bit values, cut off and the rests: two of fp16 times
-// 2^kScale (22 bits; 2^15 at most), three of bf16 (all 24 bits; two are 2^-17 of a weight off, which moved one output in
-// some hundreds to its rounding's other neighbour; prompts of 2001 249 us with two and 283 with three), small enough that
-// sums of V rows next to float32's largest number stay finite.
-constexpr float kLazy = 6.f;
-
+// 2^kScale (22 bits, down to 2^-38 of the reference's: what the attention over one sequence keeps; 2^15 at most, which
+// leaves 2^1 to kLazy: 1024 tokens behind 30000 1182 us, 1138 with 2^6 and 2^-33), three of bf16 (all 24 bits; two are 2^-17
+// of a weight off, which moved one output in some hundreds to its rounding's other neighbour; prompts of 2001 249 us with two
+// and 279 with three), small enough that sums of V rows next to float32's largest number stay finite.
 template <bool BF, int HD, int NT>
 struct PagedRows {
   using E = Half<BF>;
   static constexpr int VB = HD / 16, kTerms = BF ? 3 : 2;
-  static constexpr float kScale = BF ? -24.f : 9.f;  // log2
+  static constexpr float kLazy = BF ? 6.f : 1.f, kScale = BF ? -24.f : 14.f;  // log2
   float m[NT], l[NT];  // l: this lane's share of the sum
   f32x4 acc[NT][VB];
 
@@ -305,7 +304,7 @@ struct PagedRows {
       }
     }
     // a rest of 0 times a visible V of infinity would be NaN, where its weight is not 0 and the sum is infinite. Weights that
-    // are 0 stay 0: below 2^-34 of the reference's in fp16, which thousands of positions would otherwise all weigh
+    // are 0 stay 0: below 2^-39 of the reference's in fp16, which thousands of positions would otherwise all weigh
     const uint16_t one = masked ? 0 : E::kLeast;
     const u16x2 least = {one, one};
 #pragma unroll

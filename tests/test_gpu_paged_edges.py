@@ -59,6 +59,27 @@ def test_positions_of_no_weight_add_nothing(dtype):
         assert float(P.attn_paged(q, kp, vp, table, P.PagePlan(cu, rows, lens, rows, rows), max_new=n).abs().max()) <= 1e-6
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["fp16", "bf16"])
+def test_small_weights_behind_a_large_one(dtype):
+    """A first position that takes nearly all weight and has no V, 60000 behind it with 2^-29.4 of its weight each, which
+    make the output. In fp16 a weight's last place is 2^-38 of the largest, as in the attention over one sequence."""
+    L, hd, P = 60000, 64, _paged()
+    kp, vp = torch.full((235, 1, 256, hd), -0.0435, dtype=dtype, device="cuda"), torch.full((235, 1, 256, hd), 1000.0, dtype=dtype, device="cuda")
+    kp[0, 0, 0], vp[0, 0, 0] = 2.5, 0.0
+    small = torch.exp((kp[0, 0, 1].double() - 2.5).sum() / 8)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    for B, n, heads in ((512, 1, 4), (1, 8192, 64)):
+        table = torch.arange(235, **i32).expand(B, -1).contiguous()
+        cu, rows, lens = torch.arange(B + 1, **i32) * n, torch.arange(B, **i32), torch.full((B,), L, **i32)
+        q = torch.ones(B * n, heads, hd, dtype=dtype, device="cuda")
+        got = P.attn_paged(q, kp, vp, table, P.PagePlan(cu, rows, lens, rows, rows), max_new=n)[0].double()
+        seen = L - n  # by the first token
+        want = seen * small * 1000 / (1 + seen * small)
+        # half a last place of each, 22 bits, the sums' roundings (2^-23 for 8 terms), one rounding of the output
+        bound = 2.0 ** -39 * seen * 1000 + (2.0 ** -22 + (seen / 8 + 100) * 2.0 ** -23 + torch.finfo(dtype).eps / 2) * want
+        assert bool(((got - want).abs() <= bound).all()), float((got - want).abs().max() / bound)
+
+
 # ---- attention: values that are not finite ---------------------------------------------------------
 
 @pytest.mark.parametrize("at", [0, 20, 34, 40], ids=["block before", "middle", "last block", "own"])
