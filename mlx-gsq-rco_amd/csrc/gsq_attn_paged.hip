@@ -2,8 +2,8 @@
 // (the reference runs mlx-lm's attention over one sequence, mlx_gsq/models/qwen35.py:114-152).
 //
 // The rows of a (sequence, KV head) are its rep = heads / kv_heads query heads of every new token, row t rep + r for
-// head r of token t. Two kernels share the arithmetic: attn_paged_rows_kernel for few rows, whose waves share a tile of
-// 16 rows and take its positions in turn, attn_paged_tile_kernel for many, whose waves share tiles of K and V in LDS.
+// head r of token t. Two kinds of workgroups share the arithmetic and a launch: paged_rows for few rows, whose waves share a
+// tile of 16 rows and take its positions in turn, paged_tile for many, whose waves share tiles of K and V in LDS.
 // Both products run on the 16-bit matrix cores, transposed: S^T = K Q^T puts a row on each lane column, lane % 16, and
 // positions 16 b + 4 (lane / 16) + e of a block of 32 on its registers, which is the layout of the B operand of
 // O^T = V^T P^T: weights never leave their lane.
@@ -61,8 +61,8 @@ __device__ __forceinline__ void dma16(const uint16_t* base, uint32_t off, const 
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
 }
 
-constexpr int kRowsTile = 16;   // rows of a workgroup of attn_paged_rows_kernel: 2^4
-constexpr int kTileRows = 128;  // of attn_paged_tile_kernel: 2^7
+constexpr int kRowsTile = 16;   // rows of a workgroup of paged_rows: 2^4
+constexpr int kTileRows = 128;  // of paged_tile: 2^7
 // Rows up to which a sequence takes the first (us, six heads to a KV head of 256, first and second: 36 rows behind 30000 62
 // and 55, 96 rows 91 and 62; 36 rows of 16 sequences behind 3000 74 and 68; one sequence of 36 behind 2000 20 and 30, a
 // latency that steps of few tokens and short contexts pay).
@@ -396,7 +396,8 @@ __device__ __forceinline__ void nan_rows(const AttnPagedArgs& a, const PagedTask
 // ahead: no LDS and no barrier in the loop. K's lanes read 8 dims of one position, V's PW neighbouring dims of eight
 // positions, each dim of another output tile, so that two rows give a pair of a tile's operand by one permute. The
 // waves are merged at the end. Heads of 256, four KV heads: 32 tokens behind 8447 to 16383 301 us, 1.63 GB at 5.4 TB/s; one
-// behind 131071 99 us, 537 MB at the same; one behind 300 12 us, its chain of lengths, page numbers, K, V and the merge.
+// behind 131071 97 us, 537 MB at 5.5; one behind 300 13 us, its chain of lengths, page numbers, K, V and the merge (1 of it the
+// look at the last block's V).
 template <bool BF, int HD>
 __device__ __forceinline__ void paged_rows(const AttnPagedArgs& a, const PagedSched& p, int item, uint8_t* lds) {
   using E = Half<BF>;
@@ -581,8 +582,8 @@ __device__ __forceinline__ void paged_rows(const AttnPagedArgs& a, const PagedSc
 // buffers, one barrier a tile). K's operand is read as it lies, V's by transposing reads (four positions x 16
 // dims per 16 lanes); 16-byte pieces of a row are XOR-swizzled by position so that reads are free of bank conflicts.
 // Bound by matrix instructions and the softmax's vector ones, which overlap between the two workgroups of a CU in part: 1024
-// tokens of 24 heads of 256 behind 30000 (and 23 single ones beside them) 1035 us, 740 TFLOP/s by the definition's products,
-// half as many again with the weights' second term.
+// tokens of 24 heads of 256 behind 30000 (and 23 single ones beside them) 1184 us at least, 650 TFLOP/s by the definition's
+// products, half as many again with the weights' second term (bf16: twice as many with three).
 constexpr int tile_keys(int hd) { return hd == 256 ? 32 : 64; }
 // steps of a wave's queries that it reads from LDS, as its registers do not hold them
 constexpr int tile_lds_steps(int hd) { return hd == 256 ? 1 : 0; }

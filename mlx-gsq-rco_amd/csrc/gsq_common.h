@@ -255,7 +255,8 @@ struct Kv8AttnArgs {
   int B, S, H, Hkv, hd, nsplit;
 };
 
-// Arguments of the operators on paged caches (kernels in gsq_paged.hip, gsq_gdn_packed.hip). A step packs the new
+// Arguments of the operators on paged caches (kernels in gsq_page_plan.hip, gsq_paged_write.hip, gsq_attn_paged.hip and
+// gsq_gdn_packed.hip). A step packs the new
 // tokens of B sequences behind one another: sequence b's are tokens cu[b] .. cu[b + 1] - 1 of N, it belongs to request
 // rows[b] (none: not served) of R, and has lens[b] positions, the new ones among them. Position p of request r lies
 // in page table[r * W + p / P] at row p % P.

@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(256) gdn_rec_packed_kernel(GdnPackedArgs a, in
   }
   if (sq.n == 0) return;
   {  // this head's share of the convolution state: every input of the step's windows has been read
-    const int conv_dim = 2 * a.Hk * DK + a.Hv * DV, K = a.K;
+    const int K = a.K;
     const uint16_t* const q = static_cast<const uint16_t*>(a.qkv) + (int64_t)sq.t0 * a.qkv_stride;
     uint16_t* const cst = static_cast<uint16_t*>(a.conv) + (int64_t)sq.row * (K - 1) * conv_dim;
     for (int c = h * 256 + tid; c < conv_dim; c += a.Hv * 256) {
@@ -259,8 +259,8 @@ __global__ void __launch_bounds__(256) gdn_rec_packed_kernel(GdnPackedArgs a, in
 //   o_t = e^(G_t) q_t S + sum_(s<=t) e^(G_t - G_s) (q_t . k_s) u_s                        o = e^G (q S) + P u
 //   S' = e^(G_C) S + sum_s e^(G_C - G_s) k_s^T u_s
 // T and P depend on no state: gdn_chunk_kernel forms them for all chunks at once. What is left is a chain of products
-// over the chunks (gdn_scan_kernel), split over the state's columns, which do not meet. All products are float32 matrix
-// instructions; G is summed in float64, as e^(G_t - G_s) would lose bits behind tokens that forget nearly everything, and a
+// over the chunks (gdn_scan_kernel), split over the state's columns, which do not meet. Products are float32 matrix
+// instructions, those of the state as Three; G is summed in float64, as e^(G_t - G_s) would lose bits behind tokens that forget nearly everything, and a
 // token's logarithm is at least -1000.
 //
 // Matrix instruction j of four takes element j of 16-byte pieces: lane (g, c) = (lane / 16, lane % 16) holds A[c][4 g + j] and
@@ -334,7 +334,7 @@ struct ChunkAt {
 // T and P of one chunk, for the value heads of one key head. The ten 16 x 16 blocks of the lower triangles of k k^T and q k^T
 // are shared out over the waves; T by blocks: forward substitution in the diagonal ones, then T_ij = -T_ii (sum over
 // i > l >= j of M_il T_lj), three levels of them. Bound by the stages' latencies, two workgroups to a CU: 24 us for one chunk of
-// 48 heads, 97 us for 81.
+// 48 heads, 104 us for 81.
 template <bool BF, int DK>
 __global__ void __launch_bounds__(256) gdn_chunk_kernel(GdnPackedArgs a, float* tp, int long_from) {
   constexpr int LD = kChunk + 4;
@@ -442,8 +442,8 @@ __global__ void __launch_bounds__(256) gdn_chunk_kernel(GdnPackedArgs a, float* 
 // column whatever its neighbours are, in six 16-bit matrix instructions, 96 cycles where float32 ones would take 256; u and
 // the outputs inside the chunk are float32 products. Bound by the chain: a chunk's operands come from L2 a chunk ahead, two
 // workgroups to a CU.
-// Columns: 64 read q, k, T and P half as often but leave one workgroup to a CU (3 prompts of 2047, 48 heads: 691 against
-// 635 us for the whole call).
+// Columns: 64 read q, k, T and P half as often but leave one workgroup to a CU (3 prompts of 2047, 48 heads, operands of two
+// fp16 numbers: 691 against 635 us for the whole call).
 
 constexpr int kScanColumns = 32;
 
@@ -743,7 +743,8 @@ __global__ void __launch_bounds__(256) gdn_out_packed_kernel(GdnPackedArgs a, co
 }
 
 // Sequences from kLongFrom tokens on go by chunks (us for the whole call, one sequence of 48 heads of 128, token by token
-// and by chunks: 16 tokens 50 and 43, 24 tokens 71 and 44, 64 tokens 176 and 48; 15 tokens token by token 48).
+// and by chunks: 16 tokens 47 and 44, 24 tokens 66 and 46, 64 tokens 176 and 48; 15 tokens token by token 45. Several short
+// ones beside each other would be quicker token by token: eight of 16 53 and 88, eight of 24 75 and 116).
 constexpr int kLongFrom = 16;
 
 // whether a step may have long sequences, which take launches and memory of their own

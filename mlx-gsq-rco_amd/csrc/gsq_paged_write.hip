@@ -15,8 +15,8 @@ namespace gsq {
 // 512 / HD rows at once, kRows times before the first is used. The rotary factors of the position are formed once per
 // workgroup: turns in double, reduced to half a turn, sine and cosine in float32 (2^-22 of a radian off at any position).
 // Everything up to the one rounding of the result is float32.
-// Bound by memory: 4445 tokens of 24 + 2 x 4 rows of 256, 146 MB in 36 us (4.1 TB/s; a large copy moves 5.1). Few tokens
-// are one latency: 3.3 us up to 32 of them.
+// Bound by memory: 4445 tokens of 24 + 2 x 4 rows of 256, 146 MB in 40 us (3.7 TB/s; a large copy moves 5.1). Few tokens
+// are one latency: 3.6 us for 8 of them.
 constexpr int kWholeFrom = 512;  // tokens from which a workgroup takes all rows of its token (us, shares and whole: 128 tokens
                                  // 3.9 and 6.0, 300 5.4 and 7.0, 600 8.7 and 8.5, 2048 22 and 18)
 
