@@ -11,7 +11,8 @@
 
 namespace gsq {
 
-// Eight float32 values as three bf16 numbers each, cut off one after the other: exactly their 24 bits, of any size.
+// Eight float32 values as three bf16 numbers each, cut off one after the other: exactly their 24 bits, from 2^-102 on (terms
+// below 2^-126 are 0 to the matrix instructions).
 struct Three {
   u32x4 h, m, l;
 };
@@ -260,8 +261,8 @@ __global__ void __launch_bounds__(256) gdn_rec_packed_kernel(GdnPackedArgs a, in
 //   S' = e^(G_C) S + sum_s e^(G_C - G_s) k_s^T u_s
 // T and P depend on no state: gdn_chunk_kernel forms them for all chunks at once. What is left is a chain of products
 // over the chunks (gdn_scan_kernel), split over the state's columns, which do not meet. Products are float32 matrix
-// instructions, those of the state as Three; G is summed in float64, as e^(G_t - G_s) would lose bits behind tokens that forget nearly everything, and a
-// token's logarithm is at least -1000.
+// instructions, those of the state as Three; G is summed in float64, as e^(G_t - G_s) would lose bits behind tokens that forget
+// nearly everything, and a token's logarithm is at least -1000.
 //
 // Matrix instruction j of four takes element j of 16-byte pieces: lane (g, c) = (lane / 16, lane % 16) holds A[c][4 g + j] and
 // B[4 g + j][c], and C[4 g + r][c] in register r, so that a product's result is the next one's B operand as it lies.
